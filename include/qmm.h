@@ -298,6 +298,73 @@ int qmm_linear(qmm_array *res, qmm_array x, qmm_array w, qmm_stream s);
 int qmm_mlp_forward_q(qmm_array *res, qmm_weight_map m, qmm_array x, const char *gate_name, const char *down_name,
                       const char *up_name, qmm_stream s);
 
+/* ---- attention layers: block tables, rotary positions, paged cache (attentionForward,
+ * src/model.zig:918-979, between its projections) ----
+ * A cache holds keys (and another values) as pages [pages, Hkv, block, D] bfloat16; a token's
+ * slot is page * block + its place in the page.  A request's pages in order are a row of the
+ * block table [R, W] int32; -1 (or any id that is no page) stands for a page it does not have.
+ * Lengths, tables and slots stay on the GPU: no call waits for them, and all of them can be
+ * captured into a graph.  Head dimensions D are multiples of 8 from 8 to 256; arrays of
+ * vectors must be 16-byte aligned. */
+
+/* The tables of one step.  cached_lens [R] tokens are in the cache, new_lens [R] come in this
+ * step (negative: none), together at most n_tokens, the rows of the step's x (what is over is
+ * left out; fewer is fine).  Each request gets the pages it lacks, at most W in all, from
+ * free_blocks [F], starting at index head[0], in the order of the requests.  Results, int32:
+ *  table_out [R, W]: the table with the new pages (-1 where free_blocks ran out);
+ *  head_out [1]: head plus the pages taken (past F: some were missing);
+ *  q_starts [R + 1]: the first row of each request's new tokens, then their number;
+ *  kv_lens [R]: cached plus new; positions, slots [n_tokens]: each row's position in its
+ *  request and its cache slot (0 and -1 for rows of no request; -1 without a page).
+ * table_out, head_out and kv_lens may be the handles of table, head and cached_lens (the update
+ * is then in place).  R is at most 4096. */
+int qmm_block_tables(qmm_array *table_out, qmm_array *head_out, qmm_array *q_starts, qmm_array *kv_lens,
+                     qmm_array *positions, qmm_array *slots, qmm_array table, qmm_array head, qmm_array cached_lens,
+                     qmm_array new_lens, qmm_array free_blocks, int block_size, int n_tokens, qmm_stream s);
+
+/* Frequencies of the rotation, host-only: out[i] = base^(-2 i / rotary_dim) for i < rotary_dim / 2,
+ * scaled for contexts longer than original_len by `factor`; *amplitude (if not NULL) receives the
+ * factor of cos and sin that goes with them.
+ *  LINEAR: all divided by factor.  BASE: base * factor^(rotary_dim / (rotary_dim - 2)).
+ *  RAMP: divided where a pair turns less than `slow` times over original_len, kept where more
+ *  than `fast` times, a linear ramp over the pairs between; amplitude 1 + 0.1 ln(factor).
+ *  BANDS: the same with the ramp linear in the turns, amplitude 1. */
+typedef enum { QMM_ROPE_PLAIN = 0, QMM_ROPE_LINEAR = 1, QMM_ROPE_BASE = 2, QMM_ROPE_RAMP = 3, QMM_ROPE_BANDS = 4 } qmm_rope_kind;
+typedef struct { qmm_rope_kind kind; double factor, original_len, slow, fast; } qmm_rope_scaling;
+int qmm_rope_frequencies(float *out, float *amplitude, int rotary_dim, double base, qmm_rope_scaling scaling);
+
+/* Rotary positions of x [..., T, H, D], bfloat16 or float32: the first 2 n values of each head,
+ * n = freqs' size (float32), in pairs (i, i + n), or (2 i, 2 i + 1) when interleaved, turned by
+ * positions[t] * freqs[i] and multiplied by amplitude; the others are copied.  positions: int32,
+ * one for each of the leading indices.  Angles are exact to f32 at any position.  transpose: the
+ * transposed rotation (the gradient, or the way back when amplitude is 1).  *res may be x's own
+ * handle. */
+int qmm_rope(qmm_array *res, qmm_array x, qmm_array positions, qmm_array freqs, float amplitude, bool interleaved,
+             bool transpose, qmm_stream s);
+
+/* What a layer does between its projections and its attention: q [T, Hq, Dq] (the first D <= Dq
+ * values of each head; a gate may follow them) and k [T, Hkv, D] through their head norms
+ * (x * rsqrt(mean(x^2) + norm_eps) * w over each head; w [D], bfloat16 or float32, or the null
+ * handle for none) and the rotation of qmm_rope, q into *q_out [T, Hq, D], k and v [T, Hkv, D] into
+ * the rows slots[t] of k_cache and v_cache (slots that are none, as -1, are left out).  q, k and v
+ * all bfloat16 or all float32; results bfloat16, rounded once.  Two rows of one slot race. */
+int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_array q, qmm_array k, qmm_array v,
+                   qmm_array positions, qmm_array slots, qmm_array freqs, float amplitude, bool interleaved,
+                   qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s);
+
+/* Attention of each request's new tokens over its pages: rows q_starts[r] .. q_starts[r + 1] - 1 of
+ * q [T, Hq, D] bfloat16 are the last of request r's kv_lens[r] positions.  A row at position p
+ * (below 0: before the first key) sees the keys j <= p, with a window (> 0) only j > p - window;
+ * keys on missing pages are not seen.  Query head h reads key head h / (Hq / Hkv).
+ *  res [T, Hq, D] = softmax(scale q . k) v, zero for a row that sees nothing and for the rows
+ *  from q_starts[R] on; times sigmoid(gate), if given: gate [T, Hq, Dg >= D] bfloat16, the last
+ *  D values of each head (so the q projection's own array, where the gate lies beside the query).
+ * Stale contents of pages past kv_lens do not reach the result, whatever they are.  R is at most
+ * 4096.  Partial sums of contexts that several workgroups share lie in the stream's workspace
+ * (see qmm_gdn_recurrence). */
+int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array table,
+                        qmm_array q_starts, qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s);
+
 /* Library / device info. */
 const char *qmm_version(void);
 int qmm_device_info(char *buf, size_t len);

@@ -180,4 +180,47 @@ size_t linear_bf16_workspace(int M, int N, int K);
 hipError_t launch_linear_bf16(const uint16_t *x, const uint16_t *w, uint16_t *y, int M, int N, int K, void *ws,
                               hipStream_t st);
 
+// ---- attention over a paged cache
+
+// Block tables, slots and positions of a step's tokens (formulas at block_tables_kernel).
+constexpr int BLOCK_TABLES_MAX_R = 4096;  // requests of a call
+struct BlockTableArgs {
+  int R, W, T, F, block;
+  const int *table, *head, *cached, *fresh, *free_blocks;
+  int *table_out, *head_out, *q_starts, *kv_lens, *positions, *slots;
+};
+hipError_t launch_block_tables(const BlockTableArgs &a, hipStream_t st);
+
+// Head norm, rotation and cache write of up to three sets of heads of T tokens.
+struct RopeHeads {
+  const void *in;      // [T, heads, in_stride]: the first D values of each
+  void *out;           // [T, heads, D], or cache pages [NB, heads, block, D]
+  const void *norm;    // [D] weights of the head's RMS norm, or null
+  int heads, in_stride;
+  int norm_f32, rotate, cache;
+};
+constexpr int ROPE_MAX_SETS = 3;
+struct RopeArgs {
+  RopeHeads set[ROPE_MAX_SETS];
+  int sets, T, D, half;      // half: rotated pairs of a head
+  int in_f32, out_f32, interleaved;
+  float amplitude, sign, eps;
+  const int *positions, *slots;
+  const float *freqs;
+  int NB, block;
+};
+hipError_t launch_rope(const RopeArgs &a, hipStream_t st);
+
+// Attention of the requests' new tokens over their pages.
+constexpr int ATTN_MAX_R = 4096;
+struct AttnArgs {
+  const uint16_t *q, *k, *v, *gate;  // q [T, Hq, D]; pages [NB, Hkv, block, D]; gate [T, Hq, Dg] (its last D) or null
+  uint16_t *o;
+  const int *table, *q_starts, *kv_lens;
+  int T, R, W, Hq, Hkv, D, Dg, NB, block, window;
+  float scale;
+};
+size_t attention_workspace(const AttnArgs &a);
+hipError_t launch_attention(const AttnArgs &a, void *workspace, hipStream_t st);
+
 }  // namespace qmm

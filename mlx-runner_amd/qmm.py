@@ -11,7 +11,7 @@ fallback path.
 from __future__ import annotations
 
 import ctypes
-from ctypes import POINTER, byref, c_bool, c_char_p, c_int, c_size_t, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, byref, c_bool, c_char_p, c_double, c_float, c_int, c_size_t, c_uint32, c_uint64, c_void_p
 from pathlib import Path
 
 import numpy as np
@@ -50,6 +50,11 @@ class qmm_optional_dtype(ctypes.Structure):
 
 class qmm_quant_spec(ctypes.Structure):
     _fields_ = [("mode", c_int), ("group_size", c_uint32), ("bits", c_uint32)]
+
+
+class qmm_rope_scaling(ctypes.Structure):
+    _fields_ = [("kind", c_int), ("factor", c_double), ("original_len", c_double), ("slow", c_double),
+                ("fast", c_double)]
 
 
 UINT8, UINT16, UINT32, INT32, FLOAT16, FLOAT32, BFLOAT16 = 1, 2, 3, 7, 9, 10, 12
@@ -135,6 +140,12 @@ _SIGS = {
     "qmm_quantized_matmul_group": (c_int, [POINTER(qmm_array), c_size_t, qmm_array, POINTER(qmm_array),
                                            POINTER(qmm_array), qmm_optional_int, qmm_optional_int, c_char_p,
                                            qmm_stream]),
+    "qmm_block_tables": (c_int, [POINTER(qmm_array)] * 6 + [qmm_array] * 5 + [c_int, c_int, qmm_stream]),
+    "qmm_rope_frequencies": (c_int, [POINTER(c_float), POINTER(c_float), c_int, c_double, qmm_rope_scaling]),
+    "qmm_rope": (c_int, [POINTER(qmm_array), qmm_array, qmm_array, qmm_array, c_float, c_bool, c_bool, qmm_stream]),
+    "qmm_rope_cache": (c_int, [POINTER(qmm_array)] + [qmm_array] * 8 + [c_float, c_bool, qmm_array, qmm_array, c_float,
+                                                                        qmm_stream]),
+    "qmm_paged_attention": (c_int, [POINTER(qmm_array)] + [qmm_array] * 7 + [c_float, c_int, qmm_stream]),
     "qmm_named_linear_q_group": (c_int, [POINTER(qmm_array), c_size_t, qmm_weight_map, qmm_array,
                                          POINTER(c_char_p), qmm_stream]),
 }
@@ -240,7 +251,7 @@ class Array:
         return lib.qmm_array_data_device(self.h) or 0
 
     def numpy(self, stream: Stream | None = None) -> np.ndarray:
-        npdt = {UINT8: np.uint8, UINT32: np.uint32, FLOAT32: np.float32, BFLOAT16: np.uint16}[self.dtype]
+        npdt = {UINT8: np.uint8, UINT32: np.uint32, INT32: np.int32, FLOAT32: np.float32, BFLOAT16: np.uint16}[self.dtype]
         out = np.empty(self.shape, dtype=npdt)
         s = stream or Stream()
         check(lib.qmm_array_to_host(c_void_p(out.ctypes.data), out.nbytes, self.h, s.h), "array_to_host")
@@ -376,6 +387,70 @@ def quantized_matmul_group(x: Array, ws, scales, mode: str, *, group_size=None, 
     for r, h in zip(res, hs):
         r.h = h
     check(rc, "quantized_matmul_group")
+    return res
+
+
+def block_tables(table: Array, head: Array, cached_lens: Array, new_lens: Array, free_blocks: Array, block_size: int,
+                 n_tokens: int, *, table_out: Array | None = None, head_out: Array | None = None,
+                 q_starts: Array | None = None, kv_lens: Array | None = None, positions: Array | None = None,
+                 slots: Array | None = None, stream: Stream | None = None) -> tuple:
+    """A step's (table_out, head_out, q_starts, kv_lens, positions, slots) from the requests' lengths, all int32
+    (arrays made from torch tensors: `Array.from_torch(t, INT32)`).  Pass table_out=table, head_out=head or
+    kv_lens=cached_lens to update in place."""
+    outs = [a if a is not None else Array() for a in (table_out, head_out, q_starts, kv_lens, positions, slots)]
+    s = _stream(stream)
+    check(lib.qmm_block_tables(*[byref(a.h) for a in outs], table.h, head.h, cached_lens.h, new_lens.h, free_blocks.h,
+                               block_size, n_tokens, s.h), "block_tables")
+    return tuple(outs)
+
+
+ROPE_KINDS = {"plain": 0, "linear": 1, "base": 2, "ramp": 3, "bands": 4}
+
+
+def rope_frequencies(rotary_dim: int, base: float, kind: str = "plain", *, factor: float = 1.0,
+                     original_len: float = 0.0, slow: float = 1.0, fast: float = 32.0) -> tuple[np.ndarray, float]:
+    """(float32 frequencies [rotary_dim / 2], amplitude) of a rotation, on the host."""
+    out = np.zeros(max(rotary_dim // 2, 1), dtype=np.float32)
+    amp = c_float(1.0)
+    check(lib.qmm_rope_frequencies(out.ctypes.data_as(POINTER(c_float)), byref(amp), rotary_dim, base,
+                                   qmm_rope_scaling(ROPE_KINDS[kind], factor, original_len, slow, fast)),
+          "rope_frequencies")
+    return out, amp.value
+
+
+def rope(x: Array, positions: Array, freqs: Array, *, amplitude: float = 1.0, interleaved: bool = False,
+         transpose: bool = False, out: Array | None = None, stream: Stream | None = None) -> Array:
+    """Rotary positions of x [..., T, H, D]; out=x rotates in place."""
+    res = out if out is not None else Array()
+    s = _stream(stream)
+    check(lib.qmm_rope(byref(res.h), x.h, positions.h, freqs.h, amplitude, interleaved, transpose, s.h), "rope")
+    return res
+
+
+_NULL = qmm_array(None)
+
+
+def rope_cache(q: Array, k: Array, v: Array, k_cache: Array, v_cache: Array, positions: Array, slots: Array,
+               freqs: Array, *, amplitude: float = 1.0, interleaved: bool = False, q_norm: Array | None = None,
+               k_norm: Array | None = None, norm_eps: float = 1e-6, q_out: Array | None = None,
+               stream: Stream | None = None) -> Array:
+    """Head norms and rotation of q and k; k and v go to their cache rows, q [T, Hq, D] is returned."""
+    res = q_out if q_out is not None else Array()
+    s = _stream(stream)
+    check(lib.qmm_rope_cache(byref(res.h), k_cache.h, v_cache.h, q.h, k.h, v.h, positions.h, slots.h, freqs.h,
+                             amplitude, interleaved, q_norm.h if q_norm else _NULL, k_norm.h if k_norm else _NULL,
+                             norm_eps, s.h), "rope_cache")
+    return res
+
+
+def paged_attention(q: Array, k_cache: Array, v_cache: Array, table: Array, q_starts: Array, kv_lens: Array, *,
+                    gate: Array | None = None, scale: float, window: int = 0, out: Array | None = None,
+                    stream: Stream | None = None) -> Array:
+    """Attention of each request's new tokens over its pages (times sigmoid(gate))."""
+    res = out if out is not None else Array()
+    s = _stream(stream)
+    check(lib.qmm_paged_attention(byref(res.h), q.h, k_cache.h, v_cache.h, table.h, q_starts.h, kv_lens.h,
+                                  gate.h if gate else _NULL, scale, window, s.h), "paged_attention")
     return res
 
 
