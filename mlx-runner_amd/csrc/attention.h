@@ -1,0 +1,271 @@
+// Pieces shared by the paged-attention kernels: what a tile of query rows sees, how the work is
+// shared among workgroups, where partial results go.
+//
+// The g = Hq / Hkv query heads of a key head and the n new tokens of a request make n g rows
+// (row = token * g + head) that read the same keys; a tile is TR of them, for one key head.  Its
+// keys run from the first that any of its rows sees to the last; their cost is counted in units
+// of KT keys.  All (head, tile, unit) in a line are cut into equal shares, one per workgroup, so
+// requests of any lengths fill the chip evenly; a tile cut between workgroups leaves its partial
+// sums (unnormalised, with the rows' maxima and sums) in the workspace, and a second kernel joins
+// them.  Which workgroup runs what follows from the lengths alone: every workgroup scans them
+// itself, nothing is planned on the host.
+#pragma once
+
+#include "qmm_device.h"
+#include "qmm_launch.h"
+
+namespace qmm {
+
+constexpr int ATTN_THREADS = 256;
+
+// A launch over the requests of min_rows < n g <= max_rows rows.
+struct AttnShare {
+  int min_rows, max_rows;
+  int first;        // this launch writes the rows of no request (zeros)
+  int *count;       // [1]: tiles per head
+  int *desc;        // [tiles][8] by head * count + tile: first and last workgroup (or -1: written whole), q0, row0, rows
+  float *ml;        // [2 workgroups][TR][2]: maximum and sum of a partial's rows
+  float *acc;       // [2 workgroups][TR][DP]
+};
+
+struct AttnReq {
+  int q0, n, base;  // first row of q, tokens, position of the first
+  int rows;
+};
+
+__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int r, int g) {
+  AttnReq q;
+  const int s0 = a.q_starts[r], s1 = a.q_starts[r + 1], kv = a.kv_lens[r];
+  q.q0 = s0 < 0 ? 0 : s0 < a.T ? s0 : a.T;
+  const int q1 = s1 < q.q0 ? q.q0 : s1 < a.T ? s1 : a.T;
+  q.n = q1 - q.q0;
+  q.base = (kv < 0 ? 0 : kv) - q.n;
+  q.rows = q.n * g;
+  return q;
+}
+
+// The keys of a tile: [b, e) are seen by some row, [full_b, full_e) by all.
+struct AttnTile {
+  int row0, rows;  // of the request; rows of the tile
+  int b, e, full_b, full_e;
+};
+
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs &a, const AttnReq &q, int j, int tr, int g) {
+  AttnTile t;
+  t.row0 = j * tr;
+  t.rows = q.rows - t.row0 < tr ? q.rows - t.row0 : tr;
+  const int p0 = q.base + t.row0 / g, p1 = q.base + (t.row0 + t.rows - 1) / g;  // positions of the ends
+  const int64_t cap64 = (int64_t)a.W * a.block;
+  const int cap = cap64 < 0x7FFF0000 ? (int)cap64 : 0x7FFF0000;  // (ends rounded up stay in range)
+  t.e = p1 < cap ? p1 + 1 : cap;
+  t.full_e = p0 < cap ? p0 + 1 : cap;
+  t.b = 0, t.full_b = 0;
+  if (a.window) {
+    t.b = p0 - a.window + 1;
+    t.full_b = p1 - a.window + 1;
+    t.b = t.b < 0 ? 0 : t.b;
+    t.full_b = t.full_b < 0 ? 0 : t.full_b;
+  }
+  if (t.e < t.b) t.e = t.b;  // (also no key at all: e <= 0)
+  return t;
+}
+
+template <int KT>
+__device__ __forceinline__ int attn_units(const AttnTile &t) {
+  return t.e > t.b ? (t.e + KT - 1) / KT - t.b / KT : 0;
+}
+
+// Inclusive sum over the workgroup; the total too.
+__device__ __forceinline__ uint32_t attn_scan(uint32_t v, uint32_t *waves, uint32_t *total) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const uint32_t u = __shfl_up(v, off, 64);
+    if (lane >= off) v += u;
+  }
+  __syncthreads();
+  if (lane == 63) waves[wave] = v;
+  __syncthreads();
+  uint32_t before = 0, all = 0;
+#pragma unroll
+  for (int w = 0; w < ATTN_THREADS / 64; ++w) {
+    if (w == wave) before = all;
+    all += waves[w];
+  }
+  *total = all;
+  return before + v;
+}
+
+// The first r with ends[r] > i.
+__device__ __forceinline__ int attn_find(const int *ends, int n, int i) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi) >> 1;
+    if (ends[mid] > i)
+      hi = mid;
+    else
+      lo = mid + 1;
+  }
+  return lo;
+}
+
+// A workgroup's share: `left` units from unit `u` of (head, tile) on.
+struct AttnWork {
+  int g, groups;        // this workgroup, of how many with work
+  int tiles;            // per head
+  uint32_t per_head;    // units
+  int64_t total, at;    // units in all; the place of unit `u` in the line
+  int head, tile;
+  int u, left;
+};
+
+constexpr int ATTN_SCAN_LDS = 64;  // bytes of LDS beside ends[R]
+
+// EXTRA units a tile costs beside its keys'.  ends: LDS, [R]; scratch: ATTN_SCAN_LDS bytes of LDS.
+template <int TR, int KT, int EXTRA>
+__device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShare &s, int *ends, uint32_t *scratch) {
+  const int tid = threadIdx.x, g = a.Hq / a.Hkv;
+  uint32_t *waves = scratch, *found = scratch + 8;
+  AttnWork w;
+  uint32_t run = 0, all = 0;
+  for (int r0 = 0; r0 < a.R; r0 += ATTN_THREADS) {
+    const int r = r0 + tid;
+    uint32_t nt = 0;
+    if (r < a.R) {
+      const AttnReq q = attn_req(a, r, g);
+      if (q.rows > s.min_rows && q.rows <= s.max_rows) nt = (uint32_t)(q.rows + TR - 1) / TR;
+    }
+    const uint32_t end = run + attn_scan(nt, waves, &all);
+    if (r < a.R) ends[r] = (int)end;
+    run += all;
+  }
+  __syncthreads();
+  w.tiles = (int)run;
+  auto units_of = [&](int i) -> uint32_t {
+    if (i >= w.tiles) return 0;
+    const int r = attn_find(ends, a.R, i);
+    const AttnReq q = attn_req(a, r, g);
+    return (uint32_t)(attn_units<KT>(attn_tile(a, q, i - (r ? ends[r - 1] : 0), TR, g)) + EXTRA);
+  };
+  uint32_t mine = 0, end = 0;  // of the last turn
+  run = 0;
+  for (int i0 = 0; i0 < w.tiles; i0 += ATTN_THREADS) {
+    mine = units_of(i0 + tid);
+    end = run + attn_scan(mine, waves, &all);
+    run += all;
+  }
+  w.per_head = run;
+  w.total = (int64_t)run * a.Hkv;
+  w.left = 0;
+  w.g = 0;
+  const int64_t most = gridDim.x;
+  w.groups = (int)(w.total < most ? w.total : most);
+  if (w.total == 0) return w;
+  // consecutive shares, which read the same keys, on one XCD (workgroups go to the 8 in turn)
+  const int per = (w.groups + 7) >> 3, y = blockIdx.x >> 3;
+  w.g = (blockIdx.x & 7) * per + y;
+  if (y >= per || w.g >= w.groups) return w;
+  w.at = w.g * w.total / w.groups;
+  w.left = (int)((w.g + 1) * w.total / w.groups - w.at);
+  w.head = (int)(w.at / w.per_head);
+  const uint32_t x = (uint32_t)(w.at - (int64_t)w.head * w.per_head);
+  if (w.tiles > ATTN_THREADS) run = 0;  // (else the one turn's values are still here)
+  for (int i0 = 0; i0 < w.tiles; i0 += ATTN_THREADS) {
+    if (w.tiles > ATTN_THREADS) {
+      mine = units_of(i0 + tid);
+      end = run + attn_scan(mine, waves, &all);
+      run += all;
+    }
+    if (x < end && x >= end - mine) found[0] = (uint32_t)(i0 + tid), found[1] = x - (end - mine);
+  }
+  __syncthreads();
+  w.tile = (int)found[0];
+  w.u = (int)found[1];
+  return w;
+}
+
+// Zeros for the rows of no request, by all workgroups of a launch.
+__device__ __forceinline__ void attn_zero_rest(const AttnArgs &a) {
+  const int lo = a.R ? a.q_starts[0] : a.T, hi = a.R ? a.q_starts[a.R] : a.T;
+  const int cpr = a.D / 8;
+  const int64_t per_row = (int64_t)a.Hq * cpr;
+  auto fill = [&](int t0, int t1) {
+    for (int64_t i = t0 * per_row + (int64_t)blockIdx.x * ATTN_THREADS + threadIdx.x; i < t1 * per_row;
+         i += (int64_t)gridDim.x * ATTN_THREADS)
+      ((uint4 *)a.o)[i] = make_uint4(0, 0, 0, 0);
+  };
+  fill(0, a.R ? (lo < 0 ? 0 : lo < a.T ? lo : a.T) : a.T);
+  if (a.R) fill(hi < 0 ? 0 : hi < a.T ? hi : a.T, a.T);
+}
+
+// Eight values of a finished row (already divided by its sum), d0 a multiple of 8 below D.
+__device__ __forceinline__ void attn_store8(const AttnArgs &a, int q0, int row, int head, int g, int d0,
+                                            float (&v)[8]) {
+  const int tok = row / g;
+  const int64_t at = ((int64_t)(q0 + tok) * a.Hq + head * g + (row - tok * g));
+  if (a.gate) {
+    const uint4 d = *(const uint4 *)(a.gate + at * a.Dg + (a.Dg - a.D) + d0);
+    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      v[2 * i] /= 1.f + expf(-__uint_as_float(w[i] << 16));
+      v[2 * i + 1] /= 1.f + expf(-__uint_as_float(w[i] & 0xFFFF0000u));
+    }
+  }
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_rne(v[2 * i]) | (uint32_t)f32_to_bf16_rne(v[2 * i + 1]) << 16;
+  *(uint4 *)(a.o + at * a.D + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// bf16 values in pairs, those that are not finite replaced by zero.
+__device__ __forceinline__ uint32_t attn_finite(uint32_t x) {
+  x = (x & 0x7F80u) == 0x7F80u ? x & 0xFFFF0000u : x;
+  return (x & 0x7F800000u) == 0x7F800000u ? x & 0xFFFFu : x;
+}
+__device__ __forceinline__ uint4 attn_finite(uint4 x) {
+  return make_uint4(attn_finite(x.x), attn_finite(x.y), attn_finite(x.z), attn_finite(x.w));
+}
+
+// Adds to 8 sums of a row the values that are not finite of the keys in [ks, ke) that it sees: what was
+// left out where the rows of a tile see different keys.  Slow, and only where there are any.
+__device__ __forceinline__ void attn_poison(const AttnArgs &a, const AttnReq &q, const int *tabrow, int head,
+                                                      int row, int g, int ks, int ke, int d0, float (&o)[8]) {
+  const int pos = q.base + row / g;
+  const int hi = pos < ke - 1 ? pos : ke - 1;
+  int lo = a.window && pos - a.window + 1 > ks ? pos - a.window + 1 : ks;
+#pragma unroll 1
+  for (int key = lo; key <= hi; ++key) {
+    const int blk = tabrow[(uint32_t)key / (uint32_t)a.block];
+    if ((uint32_t)blk >= (uint32_t)a.NB) continue;
+    const uint64_t r = ((uint64_t)blk * a.Hkv + head) * a.block + (uint32_t)key % (uint32_t)a.block;
+    const uint16_t *v = a.v + r * a.D + d0;
+#pragma unroll 1
+    for (int e = 0; e < 8; ++e)
+      if ((v[e] & 0x7F80) == 0x7F80) o[e] += bf16_to_f32(v[e]);
+  }
+}
+
+// LDS rows of keys or values are DP bf16 in 16-byte chunks; chunk c of row r lies at c ^ attn_swz(r), so that
+// the reads of one chunk (or pair) of 16 rows touch every bank once.
+template <int DP>
+__device__ __forceinline__ int attn_swz(int row) {
+  return DP >= 128 ? row & 15 : (row >> 1) & 7;
+}
+
+__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+typedef short i16x4_t __attribute__((ext_vector_type(4)));
+typedef short i16x8_t __attribute__((ext_vector_type(8)));
+
+// 4 x 16 values read across: the 16 lanes of a group give the addresses of four rows of 32 bytes,
+// lane i that of bytes 8 (i % 4) of row i / 4; lane i gets column i of the four rows.
+__device__ __forceinline__ i16x4_t attn_read_tr(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t *)(uintptr_t)at);
+}
+
+// Launches of the kernels (the workspace's parts in s).
+size_t attn_rows_lds(int DP, int R);
+hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st);
+
+}  // namespace qmm

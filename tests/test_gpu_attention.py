@@ -344,6 +344,41 @@ def test_attention_with_a_negative_scale_and_infinite_keys(new):
     assert (attention(c, q, [0, new], [L], scale=0.1) == 0).all()
 
 
+@pytest.mark.parametrize("new,window", [(1, 0), (3, 0), (90, 0), (5, 40), (150, 70)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_attention_of_values_that_are_not_finite(new, window, D):
+    """They reach the rows that see their keys, in their columns, and no other."""
+    L = 400
+    c = ref.Cache([L], 2, D, 16, seed=20)
+    bad = [(L - 1, 0, 3, math.inf), (L - 2, 1, 0, math.nan), (L - 60, 0, 9, -math.inf), (L - 75, 1, 63, math.inf),
+           (L - 76, 1, 63, -math.inf), (7, 0, 5, math.nan)]
+    for j, h, d, x in bad:
+        c.values[0][j, h, d] = x
+        c.v[int(c.table[0, j // 16]), h, j % 16, d] = x
+    q = torch.randn(new, 4, D, generator=torch.Generator().manual_seed(21)).to(torch.bfloat16)
+    want, bound = ref.attend(q, c.keys, c.values, [0, new], [L], D ** -0.5, window)
+    got = attention(c, q, [0, new], [L], window=window).double()
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(got[~fine & ~torch.isnan(want)],
+                                                                            want[~fine & ~torch.isnan(want)])
+    assert ((got - want).abs() <= bound)[fine].all() and not fine.all()
+
+
+def test_attention_of_keys_that_are_not_finite_and_not_seen():
+    """NaN keys after a row's position, or before its window, do not reach it."""
+    D, L, new, window = 64, 300, 100, 50
+    c = ref.Cache([L], 1, D, 16, seed=22)
+    for j in (L - 1, L - 2, L - 30):
+        c.k[int(c.table[0, j // 16]), :, j % 16] = math.nan
+    c.k[int(c.table[0, 0]), :, 0] = math.nan
+    q = torch.randn(new, 2, D, generator=torch.Generator().manual_seed(23)).to(torch.bfloat16)
+    want, bound = ref.attend(q, c.keys, c.values, [0, new], [L], 0.125, window)
+    got = attention(c, q, [0, new], [L], window=window).double()
+    sees = slice(0, new - 30)
+    assert ((got - want).abs() <= bound)[sees].all()
+    assert torch.isnan(got[new - 30:]).all()
+
+
 @pytest.mark.parametrize("new", [1, 3, 90])
 def test_attention_of_a_cache_past_32_bit_offsets(new):
     """Pages at both ends of a cache of 2^31 values and more."""
