@@ -17,7 +17,7 @@ CSRC = HERE / "csrc"
 BUILD = HERE / "_build"
 LIB = HERE / "libqmm.so"
 SOURCES = ["qmv.hip", "qmv_any.hip", "qmv_mfma.hip", "gdn.hip", "gdn_chunk.hip", "gemm.hip", "gemm_dense.hip", "gemm_fp8.hip", "gemm_nvfp4.hip", "quant.hip",
-           "block_tables.hip", "rope.hip", "attention.hip", "attention_rows.hip", "qmm_api.cpp", "attention_api.cpp", "weights.cpp", "checkpoint.cpp"]
+           "block_tables.hip", "rope.hip", "attention.hip", "attention_rows.hip", "attention_chunk.hip", "qmm_api.cpp", "attention_api.cpp", "weights.cpp", "checkpoint.cpp"]
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
 FLAGS = [

@@ -255,6 +255,13 @@ __device__ __forceinline__ int attn_swz(int row) {
 
 __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A value that the compiler takes as new here: what follows from it (swizzled addresses) is formed
+// again where it is used, a few xors, instead of being kept in registers through the loop.
+__device__ __forceinline__ int attn_opaque(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
+
 typedef short i16x4_t __attribute__((ext_vector_type(4)));
 typedef short i16x8_t __attribute__((ext_vector_type(8)));
 
@@ -266,6 +273,8 @@ __device__ __forceinline__ i16x4_t attn_read_tr(uint32_t at) {
 
 // Launches of the kernels (the workspace's parts in s).
 size_t attn_rows_lds(int DP, int R);
+size_t attn_chunk_lds(int DP, int R);
+hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st);
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st);
 
 }  // namespace qmm

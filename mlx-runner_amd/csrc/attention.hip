@@ -74,28 +74,112 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
   }
 }
 
+// Tiles of many rows, cut in few parts: one wave per row.
+template <int DP>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const AttnArgs a, const AttnShare s, int tr) {
+  __shared__ __attribute__((aligned(16))) float part[4][DP];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int tiles = s.count[0];
+  if ((int64_t)blockIdx.x >= (int64_t)tiles * a.Hkv) return;
+  const int *d = s.desc + (int64_t)blockIdx.x * 8;
+  const int g0 = d[0], row = blockIdx.y * 4 + wave;
+  if (g0 < 0 || row >= d[4]) return;
+  const int np = d[1] - g0 + 1, d0 = lane * 4;
+  auto place = [&](int p) -> int64_t { return (int64_t)((g0 + p) * 2 + (p == 0)) * tr + row; };
+  float top = -__builtin_inff(), sum = 0.f;
+  for (int p = 0; p < np; ++p) top = fmaxf(top, s.ml[place(p) * 2]);
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 2
+  for (int p = 0; p < np; ++p) {
+    const float2 ml = *(const float2 *)(s.ml + place(p) * 2);
+    const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
+    sum += f * ml.y;
+    if (d0 < a.D) {
+      const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
+      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+    }
+  }
+  const float inv = sum != 0.f ? 1.f / sum : 0.f;
+  if (d0 < DP) *(float4 *)&part[wave][d0] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  if (lane * 8 < a.D) {
+    float v[8];
+    *(float4 *)&v[0] = *(const float4 *)&part[wave][lane * 8];
+    *(float4 *)&v[4] = *(const float4 *)&part[wave][lane * 8 + 4];
+    attn_store8(a, d[2], d[3] + row, (int)(blockIdx.x / tiles), a.Hq / a.Hkv, lane * 8, v);
+  }
+}
+
+// The kernels of a call: requests of up to 32 rows per key head (tokens x query heads that share
+// it) on the kernel that streams, the others on the one for many rows.  Lengths are known on the
+// GPU only, so both are launched where both kinds can be there.
+constexpr int ROWS_MOST = 32;
+
+struct Part {
+  int tr = 0, grid = 0, min_rows = 0, max_rows = 0;
+  int64_t tiles = 0;  // at most, per head
+  size_t at = 0, desc = 0, ml = 0, acc = 0;
+};
 struct Route {
-  int DP, g, tr, grid;
-  int64_t tiles;  // at most, per head
-  size_t desc, ml, acc, bytes;
+  int DP, g;
+  Part rows, chunk;  // (tr 0: not launched)
+  size_t bytes;
 };
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
+
+size_t lay_out(Part &p, const AttnArgs &a, int DP, int g, size_t at) {
+  p.tiles = (int64_t)a.T * g / p.tr + a.R;
+  p.at = at;
+  p.desc = at + 256;
+  p.ml = p.desc + up256((size_t)p.tiles * a.Hkv * 32);
+  p.acc = p.ml + up256((size_t)p.grid * 2 * p.tr * 8);
+  return p.acc + (size_t)p.grid * 2 * p.tr * DP * 4;
+}
 
 Route route_of(const AttnArgs &a) {
   Route r;
   r.DP = a.D <= 64 ? 64 : a.D <= 128 ? 128 : 256;
   r.g = a.Hq / a.Hkv;
-  r.tr = a.T <= a.R && r.g <= 16 ? 16 : 32;
-  const int cus = device_cu_count();
-  r.grid = 2 * (cus > 0 ? cus : 256) / 8 * 8;
-  if (r.grid > AC_MOST) r.grid = AC_MOST;
-  r.tiles = (int64_t)a.T * r.g / r.tr + a.R;
-  r.desc = 256;
-  r.ml = r.desc + up256((size_t)r.tiles * a.Hkv * 32);
-  r.acc = r.ml + up256((size_t)r.grid * 2 * r.tr * 8);
-  r.bytes = r.acc + (size_t)r.grid * 2 * r.tr * r.DP * 4;
+  int cus = device_cu_count();
+  cus = (cus > 0 ? cus : 256) / 8 * 8;
+  cus = cus < 8 ? 8 : cus < AC_MOST / 2 ? cus : AC_MOST / 2;
+  const bool single = a.T <= a.R && r.g <= ROWS_MOST;            // a token each
+  const bool few = (int64_t)(a.T - a.R + 1) * r.g <= 2 * ROWS_MOST;  // no request of more (if each has a token)
+  const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
+  if (!one) {
+    r.rows.tr = single && r.g <= 16 ? 16 : 32;
+    r.rows.grid = 2 * cus;
+    r.rows.min_rows = 0, r.rows.max_rows = single || few ? INT32_MAX : ROWS_MOST;
+  }
+  if (one || !(single || few)) {
+    r.chunk.tr = 256;
+    r.chunk.grid = r.DP == 64 ? 2 * cus : cus;
+    r.chunk.min_rows = one ? 0 : ROWS_MOST, r.chunk.max_rows = INT32_MAX;
+  }
+  r.bytes = 0;
+  if (r.rows.tr) r.bytes = up256(lay_out(r.rows, a, r.DP, r.g, r.bytes));
+  if (r.chunk.tr) r.bytes = lay_out(r.chunk, a, r.DP, r.g, r.bytes);
   return r;
+}
+
+AttnShare share_of(const Part &p, void *workspace) {
+  char *w = (char *)workspace;
+  AttnShare s;
+  s.min_rows = p.min_rows, s.max_rows = p.max_rows, s.first = 0;
+  s.count = (int *)(w + p.at), s.desc = (int *)(w + p.desc);
+  s.ml = (float *)(w + p.ml), s.acc = (float *)(w + p.acc);
+  return s;
+}
+
+template <int DP>
+void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) {
+  const unsigned tiles = (unsigned)(p.tiles * a.Hkv);
+  if (p.tr > 32)
+    hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(tiles, p.tr / 4), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<DP>), dim3(tiles, p.tr), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
 }
 
 }  // namespace
@@ -106,22 +190,19 @@ hipError_t launch_attention(const AttnArgs &a, void *workspace, hipStream_t st) 
   if (a.R == 0 || a.W == 0 || a.NB == 0)  // no keys at all
     return launch_fill_zero(a.o, (size_t)a.T * a.Hq * a.D * 2, st);
   const Route r = route_of(a);
-  if (r.tiles * a.Hkv > INT32_MAX) return hipErrorInvalidValue;
-  AttnShare s;
-  s.min_rows = 0, s.max_rows = INT32_MAX, s.first = 1;
-  s.count = (int *)workspace;
-  s.desc = (int *)((char *)workspace + r.desc);
-  s.ml = (float *)((char *)workspace + r.ml);
-  s.acc = (float *)((char *)workspace + r.acc);
-  hipError_t e = launch_attn_rows(a, s, r.DP, r.tr, r.grid, st);
-  if (e != hipSuccess) return e;
-  const dim3 grid((unsigned)(r.tiles * a.Hkv), (unsigned)r.tr), block(ATTN_THREADS);
-  if (r.DP == 64)
-    hipLaunchKernelGGL((attn_join_kernel<64>), grid, block, 0, st, a, s, r.tr);
-  else if (r.DP == 128)
-    hipLaunchKernelGGL((attn_join_kernel<128>), grid, block, 0, st, a, s, r.tr);
-  else
-    hipLaunchKernelGGL((attn_join_kernel<256>), grid, block, 0, st, a, s, r.tr);
+  for (const Part *p : {&r.rows, &r.chunk})
+    if (p->tiles * a.Hkv > INT32_MAX) return hipErrorInvalidValue;
+  bool first = true;
+  for (const Part *p : {&r.rows, &r.chunk}) {
+    if (!p->tr) continue;
+    AttnShare s = share_of(*p, workspace);
+    s.first = first;
+    first = false;
+    const hipError_t e = p == &r.rows ? launch_attn_rows(a, s, r.DP, p->tr, p->grid, st)
+                                      : launch_attn_chunk(a, s, r.DP, p->grid, st);
+    if (e != hipSuccess) return e;
+    r.DP == 64 ? join<64>(a, *p, s, st) : r.DP == 128 ? join<128>(a, *p, s, st) : join<256>(a, *p, s, st);
+  }
   return hipGetLastError();
 }
 

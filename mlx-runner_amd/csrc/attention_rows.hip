@@ -41,13 +41,6 @@ __device__ __forceinline__ void ar_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// A value that the compiler takes as new here: what follows from it (swizzled addresses) is formed
-// again where it is used, a few xors, instead of being kept in registers through the loop.
-__device__ __forceinline__ int opaque(int x) {
-  asm volatile("" : "+v"(x));
-  return x;
-}
-
 // FULL: D = DP (else the lanes of chunks past D stay out of the DMA).
 template <int DP, int NQ, bool FULL>
 __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnArgs a, const AttnShare s) {
@@ -148,7 +141,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
       for (int i = 0; i < OPS; ++i) rows[i] = __shfl(mine, (i * 64 + lane) / CPR, 64);
     };
     auto move = [&](const uint16_t *cache, uint32_t to) __attribute__((always_inline)) {
-      const int here = opaque(lane);
+      const int here = attn_opaque(lane);
 #pragma unroll
       for (int i = 0; i < OPS; ++i) {
         const int row = (i * 64 + here) / CPR, c = (i * 64 + here) % CPR ^ attn_swz<DP>(row);
@@ -176,7 +169,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
         for (int b = 0; b < KB; ++b) {
 #pragma unroll
           for (int n = 0; n < NQ; ++n) sv[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-          const int row = b * 16 + lr, from = opaque(row * (2 * DP) + (lg ^ attn_swz<DP>(row)) * 16);
+          const int row = b * 16 + lr, from = attn_opaque(row * (2 * DP) + (lg ^ attn_swz<DP>(row)) * 16);
 #pragma unroll
           for (int st = 0; st < ST; ++st) {
             const bf16x8_t kf = *(const bf16x8_t *)(kl + (from ^ st * 64));
@@ -266,7 +259,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
 #pragma unroll
         for (int b = 0; b < KB; ++b) {
           const int row = b * 16 + lg * 4 + (lr >> 2);
-          from[b] = opaque(row * (2 * DP) + ((lane >> 1 & 1) ^ attn_swz<DP>(row)) * 16 + (lane & 1) * 8);
+          from[b] = attn_opaque(row * (2 * DP) + ((lane >> 1 & 1) ^ attn_swz<DP>(row)) * 16 + (lane & 1) * 8);
         }
 #pragma unroll
         for (int d = 0; d < DT; ++d) {

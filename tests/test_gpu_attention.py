@@ -215,6 +215,8 @@ ATTEND = [  # Hq, Hkv, D, block, [(cached, new)], window
     (64, 1, 64, 16, [(100, 3), (33, 1)], 0),
     (2, 2, 32, 16, [(2500, 1), (100, 70)], 1),
     (5, 1, 72, 3, [(11, 6)] * 40, 4),
+    (2, 2, 56, 16, [(0, 130)], 0),
+    (3, 1, 120, 16, [(64, 64)], 1),
 ]
 
 
