@@ -11,8 +11,10 @@
 //
 // The products of one half tile's weights with the values are issued together with the
 // exponentials of the next one's scores, so that the vector unit works while the matrix unit does.
-// Weights are rounded to bf16 for the product (see attention_rows.hip), the reference maximum
-// follows only when it is passed by 2^8.
+// Weights are rounded to bf16 for the product (see attention_rows.hip).  They are relative to the
+// row's first maximum, not to the running one: bf16 and f32 hold weights of 2^60 as exactly as
+// those below 1, and nothing is left to multiply the sums with in the loop.  A tile with a score
+// past 2^60 times its reference is run again from the maxima that the first time has found.
 #include "attention.h"
 #include "gemm_pipe.h"
 
@@ -63,7 +65,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
   uint8_t *tab = lds + 4 * TILE;
   uint32_t *vm = (uint32_t *)(tab + 4 * 2 * 256);  // [2][4]
   uint32_t *scratch = (uint32_t *)(tab + CH_TAB);
-  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS), *poison = (int *)scratch + 15;
+  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS), *poison = (int *)scratch + 15, *redo = (int *)scratch + 14;
 
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 31, lh = lane >> 5;
@@ -86,7 +88,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     const int ks = (t.b / CH_KT + u0) * CH_KT, nt = u1 - u0;
 
     __syncthreads();
-    if (tid == 0) *poison = 0;
+    if (tid == 0) *poison = 0, *redo = 0;
     const int *tabrow = a.table + (int64_t)r * a.W;
     auto page_at = [&](int k0) -> const int * {
       int key = k0 + wv * 16 + (lane & 15);
@@ -106,7 +108,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       const int tok = on ? row / g : 0, hh = on ? row - tok * g : 0;
       const int pos = rq.base + tok;
       seen_e[u] = on ? pos : -1;
-      seen_b[u] = a.window ? pos - a.window + 1 : 0;
+      seen_b[u] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
       const uint16_t *qp = a.q + (((int64_t)(rq.q0 + tok) * a.Hq) + w.head * g + hh) * a.D;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
@@ -121,14 +123,17 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
 
     f32x16_t acc[DT][2];
-    float m[2] = {-__builtin_inff(), -__builtin_inff()}, l[2] = {0.f, 0.f};
+    float m[2] = {-__builtin_inff(), -__builtin_inff()}, l[2];
+    bool again = false;
+    do {
 #pragma unroll
     for (int d = 0; d < DT; ++d)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
 #pragma unroll
         for (int i = 0; i < 16; ++i) acc[d][u][i] = 0.f;
-
+    l[0] = l[1] = 0.f;
+    bool passed = false;
     if (nt > 0) {
       f32x16_t sv[2];
       bf16x8_t p[2][2];  // [16 keys][half]
@@ -148,6 +153,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           const uint32_t from = __shfl(mine, row, 64);  // (by all lanes)
           if (FULL || c * 8 < a.D)
             gp_dma16(a.k + (uint64_t)from * (uint32_t)a.D + c * 8, la + set * TILE + wv * 16 * PITCH + i * 1024);
+          __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
         }
       };
       auto move_v = [&](int set) __attribute__((always_inline)) {
@@ -158,6 +164,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           const uint32_t from = __shfl(mine, row, 64);
           if (FULL || c * 8 < a.D)
             gp_dma16(a.v + (uint64_t)from * (uint32_t)a.D + c * 8, la + (2 + set) * TILE + wv * 16 * PITCH + i * 1024);
+          __builtin_amdgcn_sched_barrier(0);
         }
       };
       // S^T of 32 keys
@@ -185,31 +192,31 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         }
         ch_mfma_done(sv[0], sv[1]);
       };
-      // masks, the maxima; f: what the sums so far are to be multiplied by; true: some f is not 1
-      float f[2];
-      auto maxima = [&](int k0, uint64_t valid, bool edge) __attribute__((always_inline)) -> bool {
-        bool moved = false;
+      // masks, the references
+      auto maxima = [&](int k0, uint64_t valid, bool edge) __attribute__((always_inline)) {
+        if (edge) {
+          const int h4 = attn_opaque(4 * lh);
+          const uint32_t bits = (uint32_t)valid >> h4;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          if (edge) {
+          for (int u = 0; u < 2; ++u) {
+            const int lo = seen_b[u] - k0 - h4, hi = seen_e[u] - k0 - h4;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int o = 8 * (i / 4) + 4 * lh + i % 4, key = k0 + o;
-              if (!(key <= seen_e[u] && key >= seen_b[u] && (valid >> o & 1))) sv[u][i] = -__builtin_inff();
+              const int o = 8 * (i / 4) + i % 4;
+              if (!(o <= hi && o >= lo && (bits >> o & 1))) sv[u][i] = -__builtin_inff();
             }
           }
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
           float top = sv[u][0];
 #pragma unroll
           for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[u][i]);
           top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
-          f[u] = 1.f;
-          if (top > m[u] + 8.f) {
-            f[u] = attn_exp2(m[u] - top);  // (top is finite or +inf here)
-            m[u] = top;
-          }
-          moved |= f[u] != 1.f;
+          passed |= top > m[u] + 60.f && m[u] != -__builtin_inff();
+          // (before its first key a row has no sums)
+          m[u] = m[u] == -__builtin_inff() || top > m[u] + 60.f ? top : m[u];
         }
-        return __any(moved);
       };
       // Step n of N: its part of the weights of sv into np, their sums into ls
       bf16x8_t np[2][2];
@@ -286,64 +293,54 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       maxima(ks, valid, edge);
       weights(0, 1);
       const int steps = 2 * nt;
-      int h = 0;
-      bool moved;
-      do {
-        // (the loop that runs is the inner one, and only products write the sums in it)
-        do {
+      for (int h = 1;; ++h) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            l[u] += ls[u];
+        for (int u = 0; u < 2; ++u) {
+          l[u] += ls[u];
 #pragma unroll
-            for (int c = 0; c < 2; ++c) p[c][u] = np[c][u];
-          }
-          if (++h == steps) break;
-          const int i = h >> 1, set = i & 1, half = h & 1;
-          const bool more = i + 1 < nt;
-          if (half == 0) {
-            gp_wait_barrier<OPS>();  // keys of tile i (its values are still on their way)
-            valid = valid_of(set);
-            edge = edge_at(ks + i * CH_KT, valid);
-            if (more) next_keys(i);
-          }
-          scores(set, half);
-          moved = maxima(ks + i * CH_KT + half * 32, valid >> half * 32, edge);
-          if (half == 1) {
-            // values of tile i
-            if (more)
-              asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
-            else
-              asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-            if (edge) {  // (see attention_rows.hip)
-              bool odd = false;
-#pragma unroll 1
-              for (int j = 0; j < OPS; ++j) {
-                uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + lane * 16);
-                const uint4 x = *at, y = attn_finite(x);
-                const bool in = valid >> (wv * 16 + (j * 64 + lane) / CPR) & 1;
-                odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
-                *at = in ? y : make_uint4(0, 0, 0, 0);
-              }
-              if (__any(odd)) *poison = 1;
-            }
-            gp_lds_barrier();
-            if (more) move_v(set ^ 1);
-          }
-          product(((h - 1) >> 1) & 1, (h - 1) & 1, true);
-        } while (!moved);
-        if (h < steps) {
-#pragma unroll
-          for (int u = 0; u < 2; ++u) {
-            l[u] *= f[u];
-#pragma unroll
-            for (int d = 0; d < DT; ++d)
-#pragma unroll
-              for (int i = 0; i < 16; ++i) acc[d][u][i] *= f[u];
-          }
+          for (int c = 0; c < 2; ++c) p[c][u] = np[c][u];
         }
-      } while (h < steps);
+        if (h == steps) break;
+        const int i = h >> 1, set = i & 1, half = h & 1;
+        const bool more = i + 1 < nt;
+        if (half == 0) {
+          gp_wait_barrier<OPS>();  // keys of tile i (its values are still on their way)
+          valid = valid_of(set);
+          edge = edge_at(ks + i * CH_KT, valid);
+          if (more) next_keys(i);
+        }
+        scores(set, half);
+        maxima(ks + i * CH_KT + half * 32, valid >> half * 32, edge);
+        if (half == 1) {
+          // values of tile i
+          if (more)
+            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
+          else
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+          if (edge) {  // (see attention_rows.hip)
+            bool odd = false;
+#pragma unroll 1
+            for (int j = 0; j < OPS; ++j) {
+              uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + lane * 16);
+              const uint4 x = *at, y = attn_finite(x);
+              const bool in = valid >> (wv * 16 + (j * 64 + lane) / CPR) & 1;
+              odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
+              *at = in ? y : make_uint4(0, 0, 0, 0);
+            }
+            if (__any(odd)) *poison = 1;
+          }
+          gp_lds_barrier();
+          if (more) move_v(set ^ 1);
+        }
+        product(((h - 1) >> 1) & 1, (h - 1) & 1, true);
+      }
       product((nt - 1) & 1, 1, false);
     }
+    if (__any(passed)) *redo = 1;
+    __syncthreads();
+    again = !again && *redo;
+    __syncthreads();
+    } while (again);
 
     const bool whole = take == cost;
     const int part = w.g * 2 + (w.u == 0 ? 1 : 0);
@@ -354,7 +351,6 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       d[0] = whole ? -1 : w.g, d[1] = g1, d[2] = rq.q0, d[3] = t.row0, d[4] = t.rows;
     }
     // rows out, 32 of a wave and half of their columns at a time, through the wave's quarter of the LDS
-    __syncthreads();
     constexpr int HC = DP / 2, OP = HC + 4;
     float *out = (float *)(lds + wv * TILE);
     const bool bad = *poison != 0;

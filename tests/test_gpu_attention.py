@@ -217,6 +217,7 @@ ATTEND = [  # Hq, Hkv, D, block, [(cached, new)], window
     (5, 1, 72, 3, [(11, 6)] * 40, 4),
     (2, 2, 56, 16, [(0, 130)], 0),
     (3, 1, 120, 16, [(64, 64)], 1),
+    (4, 2, 64, 16, [(100, 60), (9, 3)], 2 ** 31 - 1),
 ]
 
 
@@ -303,7 +304,7 @@ def test_attention_past_the_tables_width():
     assert ((far.double() - want).abs() <= bound).all()
 
 
-@pytest.mark.parametrize("new,L", [(1, 1000), (3, 300), (200, 500)])
+@pytest.mark.parametrize("new,L", [(1, 1000), (3, 300), (200, 500), (90, 1900)])
 @pytest.mark.parametrize("kind", ["sharp", "equal", "rising", "falling", "low"])
 def test_attention_of_extreme_scores(new, L, kind):
     """One key carries a row; all keys alike; maxima that move with every key; scores far below zero."""
