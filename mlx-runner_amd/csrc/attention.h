@@ -28,6 +28,17 @@ struct AttnShare {
   float *acc;       // [2 workgroups][TR][DP]
 };
 
+// The same value in all lanes, into scalar registers.
+template <class T>
+__device__ __forceinline__ T attn_uniform(const T &x) {
+  struct Words {
+    int w[sizeof(T) / 4];
+  } v = __builtin_bit_cast(Words, x);
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) v.w[i] = __builtin_amdgcn_readfirstlane(v.w[i]);
+  return __builtin_bit_cast(T, v);
+}
+
 struct AttnReq {
   int q0, n, base;  // first row of q, tokens, position of the first
   int rows;
@@ -260,6 +271,21 @@ __device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_ex
 __device__ __forceinline__ int attn_opaque(int x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// A kernel's arguments (at `offset` of its argument block) read again where they are needed, instead of
+// holding scalar registers through the loop before.
+template <class T>
+__device__ __forceinline__ T attn_again(int offset) {
+  typedef const __attribute__((address_space(4))) uint32_t *block_t;
+  block_t p = (block_t)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  struct Words {
+    uint32_t w[sizeof(T) / 4];
+  } x;
+#pragma unroll
+  for (size_t i = 0; i < sizeof(T) / 4; ++i) x.w[i] = p[offset / 4 + i];
+  return __builtin_bit_cast(T, x);
 }
 
 typedef short i16x4_t __attribute__((ext_vector_type(4)));

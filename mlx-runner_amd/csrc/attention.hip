@@ -53,8 +53,9 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
   if (d0 < a.D) {
 #pragma unroll 8
     for (int p = set; p < np; p += SETS) {
-      const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
       const float f = wt[p];
+      if (f == 0.f) continue;  // (a part without keys has no sums)
+      const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
       o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
     }
   }
@@ -94,7 +95,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
     const float2 ml = *(const float2 *)(s.ml + place(p) * 2);
     const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
     sum += f * ml.y;
-    if (d0 < a.D) {
+    if (d0 < a.D && f != 0.f) {  // (a part without keys has no sums)
       const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
       o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
     }

@@ -55,7 +55,7 @@ __device__ __forceinline__ void ch_mfma_done(f32x16_t &c0, f32x16_t &c1) {
 }
 
 template <int DP, bool FULL>
-__global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_kernel(const AttnArgs a, const AttnShare s) {
+__global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_kernel(const AttnArgs args, const AttnShare share) {
   constexpr int CPR = DP / 8;
   constexpr int KS = DP / 16;     // k steps of S^T
   constexpr int DT = DP / 32;     // 32-column tiles of O^T
@@ -65,38 +65,81 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
   uint8_t *tab = lds + 4 * TILE;
   uint32_t *vm = (uint32_t *)(tab + 4 * 2 * 256);  // [2][4]
   uint32_t *scratch = (uint32_t *)(tab + CH_TAB);
-  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS), *poison = (int *)scratch + 15, *redo = (int *)scratch + 14;
+  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS + sizeof(AttnWork)), *poison = (int *)scratch + 15, *redo = (int *)scratch + 14;
 
   const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lq = lane & 31, lh = lane >> 5;
-  if (s.first) attn_zero_rest(a);
-  AttnWork w = attn_share<CH_TR, CH_KT, 1>(a, s, ends, scratch);
-  if (blockIdx.x == 0 && tid == 0) s.count[0] = w.tiles;
-  const int g = a.Hq / a.Hkv;
+  const int g = args.Hq / args.Hkv;
+  AttnWork *work = (AttnWork *)(scratch + ATTN_SCAN_LDS / 4);  // (this workgroup's share, out of the registers)
+  int left;
+  {
+    if (share.first) attn_zero_rest(args);
+    const AttnWork w = attn_share<CH_TR, CH_KT, 1>(args, share, ends, scratch);
+    if (blockIdx.x == 0 && tid == 0) share.count[0] = w.tiles;
+    if (tid == 0) *work = w;
+    left = attn_uniform(w.left);
+  }
   const uint32_t la = lds_addr(lds), ta = lds_addr(tab) + wv * 512;
   if constexpr (!FULL) {  // head values past D: never written by the DMA
     for (int i = tid; i < 4 * TILE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = make_uint4(0, 0, 0, 0);
   }
 
-  while (w.left > 0) {
-    const int r = attn_find(ends, a.R, w.tile);
-    const AttnReq rq = attn_req(a, r, g);
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? ends[r - 1] : 0), CH_TR, g);
+  while (left > 0) {
+    __syncthreads();
+    const AttnArgs a = attn_again<AttnArgs>(0);
+    const AttnWork w = attn_uniform(*work);
+    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
+    const AttnReq rq = attn_uniform(attn_req(a, r, g));
+    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), CH_TR, g);
     const int cost = attn_units<CH_KT>(t) + 1;
     const int take = cost - w.u < w.left ? cost - w.u : w.left;
     const int u0 = w.u > 0 ? w.u - 1 : 0, u1 = w.u + take - 1;  // (the first unit: the tile's own overhead)
     const int ks = (t.b / CH_KT + u0) * CH_KT, nt = u1 - u0;
+    const bool whole = take == cost;
+    const int part = w.g * 2 + (w.u == 0 ? 1 : 0), head = w.head;
+    {
+      const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
+      if (w.u == 0 && tid == 0) {
+        const int64_t last = w.at + cost - 1;
+        const int g1 = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
+        int *d = s.desc + ((int64_t)w.head * w.tiles + w.tile) * 8;
+        d[0] = whole ? -1 : w.g, d[1] = g1, d[2] = rq.q0, d[3] = t.row0, d[4] = t.rows;
+      }
+      left = w.left - take;
+      __syncthreads();
+      if (tid == 0) {
+        work->left = left;
+        work->at = w.at + take;
+        work->u = w.u + take;
+        if (w.u + take == cost) {
+          const bool last = w.tile + 1 == w.tiles;
+          work->u = 0;
+          work->tile = last ? 0 : w.tile + 1;
+          work->head = w.head + last;
+        }
+      }
+      if (nt == 0) {  // no keys: zeros, or a part of nothing
+        if (whole) {
+          for (int j = tid; j < t.rows * (a.D / 8); j += ATTN_THREADS) {
+            float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            attn_store8(a, rq.q0, t.row0 + j / (a.D / 8), head, g, j % (a.D / 8) * 8, o);
+          }
+        } else if (tid < t.rows) {
+          const int64_t pr = (int64_t)part * CH_TR + tid;
+          s.ml[pr * 2] = -__builtin_inff(), s.ml[pr * 2 + 1] = 0.f;
+        }
+        continue;
+      }
+    }
 
-    __syncthreads();
     if (tid == 0) *poison = 0, *redo = 0;
     const int *tabrow = a.table + (int64_t)r * a.W;
-    auto page_at = [&](int k0) -> const int * {
-      int key = k0 + wv * 16 + (lane & 15);
-      key = key < t.e ? key : t.e - 1;
-      return tabrow + (uint32_t)key / (uint32_t)a.block;
-    };
-    const int page0 = nt > 0 ? *page_at(ks) : 0;
-
+    const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
+    const uint16_t *kc = a.k, *vc = a.v;
+    const uint32_t first = ks + wv * 16 + (lane & 15);
+    const uint32_t first_page = first / (uint32_t)block, first_off = first - first_page * block;
+    const uint32_t last_page = (uint32_t)(t.e - 1) / (uint32_t)block;
+    const int page0 = tabrow[first_page < last_page ? first_page : last_page];
     // the lane's rows
     int seen_b[2], seen_e[2];
     bf16x8_t q[2][KS];
@@ -109,7 +152,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       const int pos = rq.base + tok;
       seen_e[u] = on ? pos : -1;
       seen_b[u] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
-      const uint16_t *qp = a.q + (((int64_t)(rq.q0 + tok) * a.Hq) + w.head * g + hh) * a.D;
+      const uint16_t *qp = a.q + (((int64_t)(rq.q0 + tok) * a.Hq) + head * g + hh) * a.D;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
         const int d0 = k * 16 + lh * 8;
@@ -123,7 +166,9 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
 
     f32x16_t acc[DT][2];
-    float m[2] = {-__builtin_inff(), -__builtin_inff()}, l[2];
+    float m[2], l[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) m[u] = seen_e[u] < 0 ? 0.f : -__builtin_inff();  // (a row that sees nothing)
     bool again = false;
     do {
 #pragma unroll
@@ -134,43 +179,51 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         for (int i = 0; i < 16; ++i) acc[d][u][i] = 0.f;
     l[0] = l[1] = 0.f;
     bool passed = false;
-    if (nt > 0) {
       f32x16_t sv[2];
-      bf16x8_t p[2][2];  // [16 keys][half]
-      uint32_t mine = 0;  // the row (of the whole cache) of this lane's key
-      auto rows_of = [&](int k0, int blk, int set) __attribute__((always_inline)) {
-        const int key = k0 + wv * 16 + (lane & 15);
-        const bool ok = key < t.e && (uint32_t)blk < (uint32_t)a.NB;
-        mine = ok ? ((uint32_t)blk * a.Hkv + w.head) * a.block + (uint32_t)key % (uint32_t)a.block : 0u;
+      bf16x8_t p[2][2];     // weights [16 keys][half]
+      u32x4_t np[2][2];     // the next ones
+      float ls[2], ref[2], top[2];
+
+      // Keys on their way: this lane looks up key wv * 16 + lane % 16 of each tile.  `off` is its place in
+      // its page, for the tile whose rows come next; `page` and `poff` are two tiles on.
+      const uint32_t per = CH_KT / (uint32_t)block, rest = CH_KT % (uint32_t)block;
+      uint32_t page = first_page, poff = first_off, off = first_off;
+      auto onward = [&](uint32_t &pg, uint32_t &of) __attribute__((always_inline)) {
+        pg += per, of += rest;
+        if (of >= (uint32_t)block) of -= block, ++pg;
+      };
+      auto ask = [&](int set) __attribute__((always_inline)) {  // page ids of tile `page`
+        ch_dma4(tabrow + (page < last_page ? page : last_page), ta + set * 256);
+      };
+      uint32_t mine = 0;  // the row (of the whole cache) of this lane's key, 0 where there is none
+      auto rows_of = [&](int k0, uint32_t of, int blk, int set) __attribute__((always_inline)) {
+        const bool ok = k0 + wv * 16 + (attn_opaque(lane) & 15) < t.e && (uint32_t)blk < (uint32_t)NB;
+        mine = ok ? ((uint32_t)blk * Hkv + head) * block + of : 0u;
         const uint32_t mask = (uint32_t)__ballot(ok) & 0xFFFFu;
         if (lane == 0) vm[set * 4 + wv] = mask;
       };
-      auto move_k = [&](int set) __attribute__((always_inline)) {
-        const int here = attn_opaque(lane);
-#pragma unroll
-        for (int i = 0; i < OPS; ++i) {
-          const int row = (i * 64 + here) / CPR, c = (i * 64 + here) % CPR ^ attn_swz<DP>(row);
-          const uint32_t from = __shfl(mine, row, 64);  // (by all lanes)
-          if (FULL || c * 8 < a.D)
-            gp_dma16(a.k + (uint64_t)from * (uint32_t)a.D + c * 8, la + set * TILE + wv * 16 * PITCH + i * 1024);
-          __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
-        }
+      // DMA operation n: rows RPI n .. of the wave's 16, chunk (lane % CPR) ^ swizzle of each
+      constexpr int RPI = 64 / CPR;
+      auto move = [&](const uint16_t *cache, int n, int to, auto swz) __attribute__((always_inline)) {
+        const uint32_t ln = attn_opaque(lane);
+        const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(ln / CPR * 4) + RPI * n * 4, (int)mine);
+        const uint32_t c = (ln % CPR ^ (uint32_t)swz((int)(ln / CPR)) ^ (uint32_t)swz(RPI * n)) * 16;
+        if (FULL || c < 2 * (uint32_t)D)
+          gp_dma16((const char *)cache + ((uint64_t)row * (2 * (uint32_t)D) + c), la + to + wv * 16 * PITCH + n * 1024);
       };
-      auto move_v = [&](int set) __attribute__((always_inline)) {
-        const int here = attn_opaque(lane);
-#pragma unroll
-        for (int i = 0; i < OPS; ++i) {
-          const int row = (i * 64 + here) / CPR, c = (i * 64 + here) % CPR ^ ch_swz_v<DP>(row);
-          const uint32_t from = __shfl(mine, row, 64);
-          if (FULL || c * 8 < a.D)
-            gp_dma16(a.v + (uint64_t)from * (uint32_t)a.D + c * 8, la + (2 + set) * TILE + wv * 16 * PITCH + i * 1024);
-          __builtin_amdgcn_sched_barrier(0);
-        }
+      auto move_k = [&](int set, int n) __attribute__((always_inline)) {
+        move(kc, n, set * TILE, [](int r) { return attn_swz<DP>(r); });
       };
-      // S^T of 32 keys
-      auto scores = [&](int set, int half) __attribute__((always_inline)) {
+      auto move_v = [&](int set, int n) __attribute__((always_inline)) {
+        move(vc, n, (2 + set) * TILE, [](int r) { return ch_swz_v<DP>(r); });
+      };
+
+      // S^T of 32 keys; beside it, the DMA of a tile's values
+      auto scores = [&](int set, int half, bool values) __attribute__((always_inline)) {
         // (k steps 8 apart differ by 256 bytes, which the swizzle leaves alone)
-        const int from = attn_opaque(set * TILE + half * 32 * PITCH + lq * PITCH + (lh ^ attn_swz<DP>(lq)) * 16);
+        const uint32_t ln = attn_opaque(lane);
+        const int lq = ln & 31;
+        const int from = set * TILE + half * 32 * PITCH + lq * PITCH + ((int)(ln >> 5) ^ attn_swz<DP>(lq)) * 16;
         auto load = [&](int k) __attribute__((always_inline)) {
           return *(const bf16x8_t *)(lds + (from ^ (k & 7) * 32) + (k >> 3) * 256);
         };
@@ -188,15 +241,18 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             else
               ch_mfma(sv[u], kf[k], q[u][k]);
           }
+          if (values && k % 2 == 0) move_v(set, k / 2);
           __builtin_amdgcn_sched_barrier(0);
         }
-        ch_mfma_done(sv[0], sv[1]);
       };
-      // masks, the references
-      auto maxima = [&](int k0, uint64_t valid, bool edge) __attribute__((always_inline)) {
+      // where rows see different keys, or have no reference yet
+      auto special = [&](int k0, uint32_t valid, bool edge) __attribute__((always_inline)) {
+        const bool fresh = __any(m[0] == -__builtin_inff() || m[1] == -__builtin_inff());
+        if (!edge && !fresh) return;
+        ch_mfma_done(sv[0], sv[1]);
         if (edge) {
           const int h4 = attn_opaque(4 * lh);
-          const uint32_t bits = (uint32_t)valid >> h4;
+          const uint32_t bits = valid >> h4;
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
             const int lo = seen_b[u] - k0 - h4, hi = seen_e[u] - k0 - h4;
@@ -204,43 +260,63 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             for (int i = 0; i < 16; ++i) {
               const int o = 8 * (i / 4) + i % 4;
               if (!(o <= hi && o >= lo && (bits >> o & 1))) sv[u][i] = -__builtin_inff();
+              __builtin_amdgcn_sched_barrier(0);  // (one mask at a time)
             }
           }
         }
+        if (fresh) {  // (before its first key a row has no sums: any reference will do from here)
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          float top = sv[u][0];
+          for (int u = 0; u < 2; ++u) {
+            float x = sv[u][0];
 #pragma unroll
-          for (int i = 1; i < 16; ++i) top = fmaxf(top, sv[u][i]);
-          top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
-          passed |= top > m[u] + 60.f && m[u] != -__builtin_inff();
-          // (before its first key a row has no sums)
-          m[u] = m[u] == -__builtin_inff() || top > m[u] + 60.f ? top : m[u];
+            for (int i = 1; i < 16; ++i) x = fmaxf(x, sv[u][i]);
+            x = fmaxf(x, __shfl_xor(x, 32, 64)) * sc;
+            m[u] = m[u] == -__builtin_inff() ? x : m[u];
+          }
         }
       };
-      // Step n of N: its part of the weights of sv into np, their sums into ls
-      bf16x8_t np[2][2];
-      float ls[2], ref[2];
+      // Step n of N: its part of the weights of sv into np, their sums into ls, the scores' maxima into top
       auto weights = [&](int n, int N) __attribute__((always_inline)) {
         if (n == 0) {
 #pragma unroll
-          for (int u = 0; u < 2; ++u) ls[u] = 0.f, ref[u] = m[u] == -__builtin_inff() ? 0.f : m[u];
+          for (int u = 0; u < 2; ++u)
+            ls[u] = 0.f, top[u] = -__builtin_inff(), ref[u] = m[u] == -__builtin_inff() ? 0.f : m[u];
         }
 #pragma unroll
         for (int j = n * (16 / N); j < (n + 1) * (16 / N); ++j) {
           const int u = j >> 3, c = j >> 2 & 1, e = (j & 3) * 2;
+          const float s0 = sv[u][c * 8 + e], s1 = sv[u][c * 8 + e + 1];
+          top[u] = fmaxf(top[u], fmaxf(s0, s1));
           bf16x2_t x;
-          x[0] = (__bf16)attn_exp2(__builtin_fmaf(sv[u][c * 8 + e], sc, -ref[u]));
-          x[1] = (__bf16)attn_exp2(__builtin_fmaf(sv[u][c * 8 + e + 1], sc, -ref[u]));
+          x[0] = (__bf16)attn_exp2(__builtin_fmaf(s0, sc, -ref[u]));
+          x[1] = (__bf16)attn_exp2(__builtin_fmaf(s1, sc, -ref[u]));
           ls[u] = dot2_bf16(x, 0x3F803F80u, ls[u]);
-          np[c][u][e] = x[0], np[c][u][e + 1] = x[1];
+          uint32_t pair = __builtin_bit_cast(uint32_t, x);
+          asm volatile("" : "+v"(pair));  // (here, not later: beside the product)
+          np[c][u][e / 2] = pair;
         }
       };
-      // O^T += V^T P^T over 32 keys, and with it the next weights
-      auto product = [&](int set, int half, bool with) __attribute__((always_inline)) {
-        const int row = 4 * lh + (lane >> 2 & 3);
-        const int from = attn_opaque(la + (2 + set) * TILE + (half * 32 + row) * PITCH +
-                                     (((lane >> 4 & 1) * 2 + (lane >> 1 & 1)) ^ ch_swz_v<DP>(row)) * 16 + (lane & 1) * 8);
+      // the weights become the next product's; a reference passed by 2^60: noted, and followed for the second run
+      auto settle = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          l[u] += ls[u];
+#pragma unroll
+          for (int c = 0; c < 2; ++c) p[c][u] = __builtin_bit_cast(bf16x8_t, np[c][u]);
+        }
+        const bool far = top[0] * sc > m[0] + 60.f || top[1] * sc > m[1] + 60.f;
+        if (__any(far)) {
+          passed = true;
+#pragma unroll
+          for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], top[u] * sc);
+        }
+      };
+      // O^T += V^T P^T over 32 keys; beside it the next weights and the DMA of a tile's keys
+      auto product = [&](int set, int half, bool with, int keys) __attribute__((always_inline)) {
+        const uint32_t ln = attn_opaque(lane);
+        const int row = 4 * (ln >> 5) + (ln >> 2 & 3);
+        const int from = la + (2 + set) * TILE + (half * 32 + row) * PITCH +
+                         ((int)((ln >> 4 & 1) * 2 + (ln >> 1 & 1)) ^ ch_swz_v<DP>(row)) * 16 + (ln & 1) * 8;
         constexpr int N = 2 * DT, AHEAD = 2;
         auto load = [&](int n) __attribute__((always_inline)) {
           const int d = n >> 1, c = n & 1;
@@ -257,99 +333,99 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
 #pragma unroll
           for (int u = 0; u < 2; ++u)
             acc[n >> 1][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], p[n & 1][u], acc[n >> 1][u], 0, 0, 0);
+          if (n == 0 && with) ch_mfma_done(sv[0], sv[1]);
           if (with) weights(n, N);
+          if (keys >= 0 && n % 2 == 0) move_k(keys, n / 2);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
       auto edge_at = [&](int k0, uint64_t valid) -> bool {
         return k0 < t.full_b || k0 + CH_KT > t.full_e || valid != ~0ull;
       };
-      auto valid_of = [&](int set) -> uint64_t {
-        const uint32_t *v = vm + set * 4;
-        const uint32_t lo = __builtin_amdgcn_readfirstlane(v[0] | v[1] << 16);
-        const uint32_t hi = __builtin_amdgcn_readfirstlane(v[2] | v[3] << 16);
+      auto valid_of = [&](uint4 v) -> uint64_t {
+        const uint32_t lo = __builtin_amdgcn_readfirstlane(v.x | v.y << 16);
+        const uint32_t hi = __builtin_amdgcn_readfirstlane(v.z | v.w << 16);
         return (uint64_t)hi << 32 | lo;
       };
 
-      rows_of(ks, page0, 0);
-      ch_dma4(page_at(ks + CH_KT), ta + 256);
-      move_k(0);
-      move_v(0);
-      gp_wait_barrier<OPS>();  // keys of tile 0; everyone's valid bits
-      uint64_t valid = valid_of(0);
-      bool edge = edge_at(ks, valid);
-      // the page ids of tile i + 1 are there: its keys, and the ids of tile i + 2
-      auto next_keys = [&](int i) __attribute__((always_inline)) {
-        const int set = (i + 1) & 1, blk = *(const int *)(tab + wv * 512 + set * 256 + lane * 4);
-        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        rows_of(ks + (i + 1) * CH_KT, blk, set);
-        ch_dma4(page_at(ks + (i + 2) * CH_KT), ta + (i & 1) * 256);
-        move_k(set);
+      rows_of(ks, off, page0, 0);
+      onward(page, poff);
+      ask(1);
+      off = poff;
+      onward(page, poff);
+#pragma unroll
+      for (int n = 0; n < OPS; ++n) move_k(0, n);
+      // Tile i: scores of its first half | values of tile i; weights of those with the product of tile i - 1's
+      // second half | keys of tile i + 1; the same for its second half.
+      // (what is asked for past the last tile is not used; the waits count on it)
+      uint64_t valid;
+      bool edge;
+      auto begin = [&](int i) __attribute__((always_inline)) {
+        const int set = i & 1, k0 = ks + i * CH_KT;
+        gp_wait_barrier<0>();  // keys of tile i, page ids of tile i + 1, everyone's valid bits
+        const uint4 bits = *(const uint4 *)(vm + set * 4);
+        const int blk = *(const int *)(tab + wv * 512 + (set ^ 1) * 256 + attn_opaque(lane) * 4);
+        scores(set, 0, true);
+        valid = valid_of(bits);
+        edge = edge_at(k0, valid);
+        special(k0, (uint32_t)valid, edge);
+        rows_of(k0 + CH_KT, off, blk, set ^ 1);
+        ask(set);
+        off = poff;
+        onward(page, poff);
       };
-      if (nt > 1) next_keys(0);
-      // Step h: half h % 2 of tile h / 2.  Its scores; then its weights together with the product
-      // of step h - 1.
-      scores(0, 0);
-      maxima(ks, valid, edge);
-      weights(0, 1);
-      const int steps = 2 * nt;
-      for (int h = 1;; ++h) {
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          l[u] += ls[u];
-#pragma unroll
-          for (int c = 0; c < 2; ++c) p[c][u] = np[c][u];
-        }
-        if (h == steps) break;
-        const int i = h >> 1, set = i & 1, half = h & 1;
-        const bool more = i + 1 < nt;
-        if (half == 0) {
-          gp_wait_barrier<OPS>();  // keys of tile i (its values are still on their way)
-          valid = valid_of(set);
-          edge = edge_at(ks + i * CH_KT, valid);
-          if (more) next_keys(i);
-        }
-        scores(set, half);
-        maxima(ks + i * CH_KT + half * 32, valid >> half * 32, edge);
-        if (half == 1) {
-          // values of tile i
-          if (more)
-            asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
-          else
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-          if (edge) {  // (see attention_rows.hip)
-            bool odd = false;
+      auto middle = [&](int i) __attribute__((always_inline)) {
+        const int set = i & 1;
+        scores(set, 1, false);
+        special(ks + i * CH_KT + 32, (uint32_t)(valid >> 32), edge);
+        // values of tile i (the page ids and keys asked for after them may be on their way)
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
+        if (edge) {  // (see attention_rows.hip)
+          bool odd = false;
 #pragma unroll 1
-            for (int j = 0; j < OPS; ++j) {
-              uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + lane * 16);
-              const uint4 x = *at, y = attn_finite(x);
-              const bool in = valid >> (wv * 16 + (j * 64 + lane) / CPR) & 1;
-              odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
-              *at = in ? y : make_uint4(0, 0, 0, 0);
-            }
-            if (__any(odd)) *poison = 1;
+          for (int j = 0; j < OPS; ++j) {
+            uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + lane * 16);
+            const uint4 x = *at, y = attn_finite(x);
+            const bool in = valid >> (wv * 16 + (j * 64 + lane) / CPR) & 1;
+            odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
+            *at = in ? y : make_uint4(0, 0, 0, 0);
           }
-          gp_lds_barrier();
-          if (more) move_v(set ^ 1);
+          if (__any(odd)) *poison = 1;
         }
-        product(((h - 1) >> 1) & 1, (h - 1) & 1, true);
+        gp_lds_barrier();
+      };
+      begin(0);
+      ch_mfma_done(sv[0], sv[1]);
+      weights(0, 1);
+#pragma unroll
+      for (int n = 0; n < OPS; ++n) move_k(1, n);
+      settle();
+      middle(0);
+      product(0, 0, true, -1);
+      settle();
+      for (int i = 1; i < nt; ++i) {
+        begin(i);
+        product((i + 1) & 1, 1, true, (i + 1) & 1);
+        settle();
+        middle(i);
+        product(i & 1, 0, true, -1);
+        settle();
       }
-      product((nt - 1) & 1, 1, false);
-    }
+      product((nt - 1) & 1, 1, false, -1);
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     if (__any(passed)) *redo = 1;
     __syncthreads();
     again = !again && *redo;
+    if (again) {
+#pragma unroll
+      for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor(m[u], 32, 64));
+    }
     __syncthreads();
     } while (again);
 
-    const bool whole = take == cost;
-    const int part = w.g * 2 + (w.u == 0 ? 1 : 0);
-    if (w.u == 0 && tid == 0) {
-      const int64_t last = w.at + cost - 1;
-      const int g1 = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
-      int *d = s.desc + ((int64_t)w.head * w.tiles + w.tile) * 8;
-      d[0] = whole ? -1 : w.g, d[1] = g1, d[2] = rq.q0, d[3] = t.row0, d[4] = t.rows;
-    }
+    {
+    const AttnArgs a = attn_again<AttnArgs>(0);
+    const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
     // rows out, 32 of a wave and half of their columns at a time, through the wave's quarter of the LDS
     constexpr int HC = DP / 2, OP = HC + 4;
     float *out = (float *)(lds + wv * TILE);
@@ -382,9 +458,9 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           float o[8];
           *(float4 *)&o[0] = *(const float4 *)(out + rr * OP + c0);
           *(float4 *)&o[4] = *(const float4 *)(out + rr * OP + c0 + 4);
-          if (bad) attn_poison(a, rq, tabrow, w.head, t.row0 + in, g, ks, ks + nt * CH_KT < t.e ? ks + nt * CH_KT : t.e, d0, o);
+          if (bad) attn_poison(a, rq, tabrow, head, t.row0 + in, g, ks, ks + nt * CH_KT < t.e ? ks + nt * CH_KT : t.e, d0, o);
           if (whole) {
-            attn_store8(a, rq.q0, t.row0 + in, w.head, g, d0, o);
+            attn_store8(a, rq.q0, t.row0 + in, head, g, d0, o);
           } else {
             float4 *to = (float4 *)(s.acc + ((int64_t)part * CH_TR + in) * DP + d0);
             to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
@@ -394,17 +470,10 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         __builtin_amdgcn_wave_barrier();
       }
     }
+    }
     if constexpr (!FULL) {
       __syncthreads();
       for (int j = tid; j < 4 * TILE / 16; j += ATTN_THREADS) ((uint4 *)lds)[j] = make_uint4(0, 0, 0, 0);
-    }
-
-    w.left -= take;
-    w.at += take;
-    w.u += take;
-    if (w.u == cost) {
-      w.u = 0;
-      if (++w.tile == w.tiles) w.tile = 0, ++w.head;
     }
   }
 }
@@ -426,7 +495,9 @@ hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int grid, hipStream_
 
 }  // namespace
 
-size_t attn_chunk_lds(int DP, int R) { return 4 * ch_tile(DP) + CH_TAB + ATTN_SCAN_LDS + (size_t)R * 4; }
+size_t attn_chunk_lds(int DP, int R) {
+  return 4 * ch_tile(DP) + CH_TAB + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
+}
 
 hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st) {
   return DP == 64 ? launch_dp<64>(a, s, grid, st) : DP == 128 ? launch_dp<128>(a, s, grid, st) : launch_dp<256>(a, s, grid, st);

@@ -58,7 +58,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
 
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
   if (s.first) attn_zero_rest(a);
-  AttnWork w = attn_share<TR, KT, 0 + 1>(a, s, ends, scratch);
+  AttnWork w = attn_uniform(attn_share<TR, KT, 1>(a, s, ends, scratch));
   if (blockIdx.x == 0 && tid == 0) s.count[0] = w.tiles;
   const int g = a.Hq / a.Hkv;
   const int wv = __builtin_amdgcn_readfirstlane(wave);
@@ -70,9 +70,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
   }
 
   while (w.left > 0) {
-    const int r = attn_find(ends, a.R, w.tile);
-    const AttnReq rq = attn_req(a, r, g);
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? ends[r - 1] : 0), TR, g);
+    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
+    const AttnReq rq = attn_uniform(attn_req(a, r, g));
+    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), TR, g);
     const int cost = attn_units<KT>(t) + 1;
     const int take = cost - w.u < w.left ? cost - w.u : w.left;
     // (a tile's first unit stands for its own overhead)
