@@ -22,8 +22,12 @@ constexpr int ATTN_THREADS = 256;
 struct AttnShare {
   int min_rows, max_rows;
   int first;        // this launch writes the rows of no request (zeros)
-  int *count;       // [1]: tiles per head
-  int *desc;        // [tiles][8] by head * count + tile: first and last workgroup (or -1: written whole), q0, row0, rows
+  // The tiles cut between workgroups, for the joining kernel: [.][8], first and last workgroup (first -1: none),
+  // q0, row0, rows, key head; one for each workgroup (it starts at most one such tile), or, where that is
+  // fewer, one for each tile (by head * count + tile).
+  int by_tile;
+  int *count;       // tiles per head, workgroups with work
+  int *desc;
   float *ml;        // [2 workgroups][TR][2]: maximum and sum of a partial's rows
   float *acc;       // [2 workgroups][TR][DP]
 };
@@ -195,6 +199,25 @@ __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShar
   return w;
 }
 
+// Notes the tile that this workgroup starts (by one thread).
+__device__ __forceinline__ void attn_note(const AttnShare &s, const AttnWork &w, const AttnReq &q, const AttnTile &t,
+                                          int cost, bool whole) {
+  int *d = s.desc + (s.by_tile ? (int64_t)w.head * w.tiles + w.tile : (int64_t)w.g) * 8;
+  if (whole) {
+    if (s.by_tile) d[0] = -1;
+    return;
+  }
+  const int64_t last = w.at - w.u + cost - 1;
+  d[0] = w.g, d[1] = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
+  d[2] = q.q0, d[3] = t.row0, d[4] = t.rows, d[5] = w.head;
+}
+// First of all: how many tiles and workgroups with work; no tile noted yet.
+__device__ __forceinline__ void attn_note_none(const AttnShare &s, const AttnWork &w) {
+  if (threadIdx.x != 0) return;
+  if (blockIdx.x == 0) s.count[0] = w.tiles, s.count[1] = w.groups;
+  if (!s.by_tile && w.left > 0) s.desc[w.g * 8] = -1;
+}
+
 // Zeros for the rows of no request, by all workgroups of a launch.
 __device__ __forceinline__ void attn_zero_rest(const AttnArgs &a) {
   const int lo = a.R ? a.q_starts[0] : a.T, hi = a.R ? a.q_starts[a.R] : a.T;
@@ -209,24 +232,39 @@ __device__ __forceinline__ void attn_zero_rest(const AttnArgs &a) {
   if (a.R) fill(hi < 0 ? 0 : hi < a.T ? hi : a.T, a.T);
 }
 
-// Eight values of a finished row (already divided by its sum), d0 a multiple of 8 below D.
-__device__ __forceinline__ void attn_store8(const AttnArgs &a, int q0, int row, int head, int g, int d0,
-                                            float (&v)[8]) {
+// Row `row` of a request: its (token, query head) in q, gate and o.
+__device__ __forceinline__ int64_t attn_row(const AttnArgs &a, int q0, int row, int head, int g) {
   const int tok = row / g;
-  const int64_t at = ((int64_t)(q0 + tok) * a.Hq + head * g + (row - tok * g));
-  if (a.gate) {
-    const uint4 d = *(const uint4 *)(a.gate + at * a.Dg + (a.Dg - a.D) + d0);
-    const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+  return (int64_t)(q0 + tok) * a.Hq + head * g + (row - tok * g);
+}
+// Eight values of a finished row (divided by its sum), d0 a multiple of 8 below D: the gate of them, times
+// its sigmoid, their rounding.
+__device__ __forceinline__ uint4 attn_gate8(const AttnArgs &a, int64_t row, int d0) {
+  return *(const uint4 *)(a.gate + row * a.Dg + (a.Dg - a.D) + d0);
+}
+__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ void attn_times_gate(uint4 d, float (&v)[8]) {
+  const uint32_t w[4] = {d.x, d.y, d.z, d.w};
+  constexpr float LOG2E = 1.44269504088896341f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      v[2 * i] /= 1.f + expf(-__uint_as_float(w[i] << 16));
-      v[2 * i + 1] /= 1.f + expf(-__uint_as_float(w[i] & 0xFFFF0000u));
-    }
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-LOG2E * __uint_as_float(w[i] << 16)));
+    v[2 * i + 1] *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-LOG2E * __uint_as_float(w[i] & 0xFFFF0000u)));
   }
+}
+__device__ __forceinline__ void attn_put8(const AttnArgs &a, int64_t row, int d0, const float (&v)[8]) {
   uint32_t w[4];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) w[i] = f32_to_bf16_rne(v[2 * i]) | (uint32_t)f32_to_bf16_rne(v[2 * i + 1]) << 16;
-  *(uint4 *)(a.o + at * a.D + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+  for (int i = 0; i < 4; ++i) {
+    bf16x2_t x;
+    x[0] = (__bf16)v[2 * i], x[1] = (__bf16)v[2 * i + 1];
+    w[i] = __builtin_bit_cast(uint32_t, x);
+  }
+  *(uint4 *)(a.o + row * a.D + d0) = make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void attn_store8(const AttnArgs &a, int64_t row, int d0, float (&v)[8]) {
+  if (a.gate) attn_times_gate(attn_gate8(a, row, d0), v);
+  attn_put8(a, row, d0, v);
 }
 
 // bf16 values in pairs, those that are not finite replaced by zero.
@@ -264,7 +302,6 @@ __device__ __forceinline__ int attn_swz(int row) {
   return DP >= 128 ? row & 15 : (row >> 1) & 7;
 }
 
-__device__ __forceinline__ float attn_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
 // A value that the compiler takes as new here: what follows from it (swizzled addresses) is formed
 // again where it is used, a few xors, instead of being kept in registers through the loop.

@@ -23,8 +23,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
   __shared__ float wt[AC_MOST], red[8];
   __shared__ __attribute__((aligned(16))) float part[SETS][DP];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int tiles = s.count[0];
-  if ((int64_t)blockIdx.x >= (int64_t)tiles * a.Hkv) return;
+  if ((int64_t)blockIdx.x >= (s.by_tile ? (int64_t)s.count[0] * a.Hkv : (int64_t)s.count[1])) return;
   const int *d = s.desc + (int64_t)blockIdx.x * 8;
   const int g0 = d[0], row = blockIdx.y;
   if (g0 < 0 || row >= d[4]) return;
@@ -71,54 +70,87 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
       for (int i = 0; i < SETS; ++i) v[e] += part[i][tid * 8 + e];
       v[e] *= inv;
     }
-    attn_store8(a, d[2], d[3] + row, (int)(blockIdx.x / tiles), a.Hq / a.Hkv, tid * 8, v);
+    attn_store8(a, attn_row(a, d[2], d[3] + row, d[5], a.Hq / a.Hkv), tid * 8, v);
   }
 }
 
-// Tiles of many rows, cut in few parts: one wave per row.
+// Tiles of many rows, mostly cut in few parts: 16 rows per workgroup, their weights first.
+constexpr int AJ_ROWS = 16;
 template <int DP>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const AttnArgs a, const AttnShare s, int tr) {
-  __shared__ __attribute__((aligned(16))) float part[4][DP];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int tiles = s.count[0];
-  if ((int64_t)blockIdx.x >= (int64_t)tiles * a.Hkv) return;
+  constexpr int LPR = DP / 4, RP = ATTN_THREADS / LPR, TURNS = AJ_ROWS / RP;
+  __shared__ float wt[AJ_ROWS][AC_MOST / 2], total[AJ_ROWS];
+  __shared__ __attribute__((aligned(16))) float part[AJ_ROWS][DP];
+  const int tid = threadIdx.x;
+  if ((int64_t)blockIdx.x >= (s.by_tile ? (int64_t)s.count[0] * a.Hkv : (int64_t)s.count[1])) return;
   const int *d = s.desc + (int64_t)blockIdx.x * 8;
-  const int g0 = d[0], row = blockIdx.y * 4 + wave;
-  if (g0 < 0 || row >= d[4]) return;
-  const int np = d[1] - g0 + 1, d0 = lane * 4;
-  auto place = [&](int p) -> int64_t { return (int64_t)((g0 + p) * 2 + (p == 0)) * tr + row; };
-  float top = -__builtin_inff(), sum = 0.f;
-  for (int p = 0; p < np; ++p) top = fmaxf(top, s.ml[place(p) * 2]);
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  const int g0 = d[0], row0 = blockIdx.y * AJ_ROWS, rows = d[4];
+  if (g0 < 0 || row0 >= rows) return;
+  const int np = d[1] - g0 + 1;
+  auto place = [&](int p, int row) -> int64_t { return (int64_t)((g0 + p) * 2 + (p == 0)) * tr + row0 + row; };
+  {
+    const int row = tid >> 4, l = tid & 15;
+    const bool on = row0 + row < rows;
+    float top = -__builtin_inff(), sum = 0.f;
+    for (int p = l; p < np && on; p += 16) top = fmaxf(top, s.ml[place(p, row) * 2]);
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
+    for (int p = l; p < np && on; p += 16) {
+      const float2 ml = *(const float2 *)(s.ml + place(p, row) * 2);
+      const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
+      wt[row][p] = f;
+      sum += f * ml.y;
+    }
+#pragma unroll
+    for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 16);
+    if (l == 0) total[row] = sum;
+  }
+  __syncthreads();
+  const int r0 = tid / LPR, d0 = tid % LPR * 4;
+  float4 o[TURNS];
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) o[t] = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 2
   for (int p = 0; p < np; ++p) {
-    const float2 ml = *(const float2 *)(s.ml + place(p) * 2);
-    const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
-    sum += f * ml.y;
-    if (d0 < a.D && f != 0.f) {  // (a part without keys has no sums)
-      const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
-      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
+    float4 x[TURNS];
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+      const int row = t * RP + r0;
+      x[t] = make_float4(0.f, 0.f, 0.f, 0.f);
+      // (a part without keys has no sums)
+      if (row0 + row < rows && d0 < a.D && wt[row][p] != 0.f) x[t] = *(const float4 *)(s.acc + place(p, row) * DP + d0);
+    }
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t) {
+      const int row = t * RP + r0;
+      const float f = row0 + row < rows ? wt[row][p] : 0.f;
+      o[t].x += f * x[t].x, o[t].y += f * x[t].y, o[t].z += f * x[t].z, o[t].w += f * x[t].w;
     }
   }
-  const float inv = sum != 0.f ? 1.f / sum : 0.f;
-  if (d0 < DP) *(float4 *)&part[wave][d0] = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  if (lane * 8 < a.D) {
+#pragma unroll
+  for (int t = 0; t < TURNS; ++t) *(float4 *)&part[t * RP + r0][d0] = o[t];
+  __syncthreads();
+  for (int i = tid; i < AJ_ROWS * (a.D / 8); i += ATTN_THREADS) {
+    const int row = i / (a.D / 8), c0 = i % (a.D / 8) * 8;
+    if (row0 + row >= rows) break;
+    const float inv = total[row] != 0.f ? 1.f / total[row] : 0.f;
     float v[8];
-    *(float4 *)&v[0] = *(const float4 *)&part[wave][lane * 8];
-    *(float4 *)&v[4] = *(const float4 *)&part[wave][lane * 8 + 4];
-    attn_store8(a, d[2], d[3] + row, (int)(blockIdx.x / tiles), a.Hq / a.Hkv, lane * 8, v);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = part[row][c0 + e] * inv;
+    attn_store8(a, attn_row(a, d[2], d[3] + row0 + row, d[5], a.Hq / a.Hkv), c0, v);
   }
 }
 
 // The kernels of a call: requests of up to 32 rows per key head (tokens x query heads that share
 // it) on the kernel that streams, the others on the one for many rows.  Lengths are known on the
-// GPU only, so both are launched where both kinds can be there.
+// GPU only, so both are launched where both kinds can be there (a launch without work: 5 us); where
+// no request can have over 256 rows the streaming kernel takes them all, 32 at a time.
 constexpr int ROWS_MOST = 32;
 
 struct Part {
   int tr = 0, grid = 0, min_rows = 0, max_rows = 0;
+  int rows = 0;       // of a tile at most
+  int by_tile = 0;
   int64_t tiles = 0;  // at most, per head
   size_t at = 0, desc = 0, ml = 0, acc = 0;
 };
@@ -131,10 +163,11 @@ struct Route {
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t lay_out(Part &p, const AttnArgs &a, int DP, int g, size_t at) {
-  p.tiles = (int64_t)a.T * g / p.tr + a.R;
+  p.tiles = p.max_rows <= p.tr ? a.R : (int64_t)a.T * g / p.tr + a.R;
+  p.by_tile = p.tiles * a.Hkv <= p.grid;
   p.at = at;
   p.desc = at + 256;
-  p.ml = p.desc + up256((size_t)p.tiles * a.Hkv * 32);
+  p.ml = p.desc + up256((size_t)(p.by_tile ? p.tiles * a.Hkv : p.grid) * 32);
   p.acc = p.ml + up256((size_t)p.grid * 2 * p.tr * 8);
   return p.acc + (size_t)p.grid * 2 * p.tr * DP * 4;
 }
@@ -146,16 +179,18 @@ Route route_of(const AttnArgs &a) {
   int cus = device_cu_count();
   cus = (cus > 0 ? cus : 256) / 8 * 8;
   cus = cus < 8 ? 8 : cus < AC_MOST / 2 ? cus : AC_MOST / 2;
-  const bool single = a.T <= a.R && r.g <= ROWS_MOST;            // a token each
-  const bool few = (int64_t)(a.T - a.R + 1) * r.g <= 2 * ROWS_MOST;  // no request of more (if each has a token)
+  // (most: the rows of the longest request there can be, if each has a token)
+  const int64_t most = (int64_t)(a.T > a.R ? a.T - a.R + 1 : 1) * r.g;
+  const bool few = most <= 8 * ROWS_MOST;
   const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
   if (!one) {
-    r.rows.tr = single && r.g <= 16 ? 16 : 32;
+    r.rows.tr = most <= 16 ? 16 : 32;
     r.rows.grid = 2 * cus;
-    r.rows.min_rows = 0, r.rows.max_rows = single || few ? INT32_MAX : ROWS_MOST;
+    r.rows.min_rows = 0, r.rows.max_rows = few ? INT32_MAX : ROWS_MOST;
+    r.rows.rows = (int)(a.R == 1 && a.T * r.g < r.rows.tr ? a.T * r.g : a.T <= a.R && r.g < r.rows.tr ? r.g : r.rows.tr);
   }
-  if (one || !(single || few)) {
-    r.chunk.tr = 256;
+  if (one || !few) {
+    r.chunk.tr = r.chunk.rows = 256;
     r.chunk.grid = r.DP == 64 ? 2 * cus : cus;
     r.chunk.min_rows = one ? 0 : ROWS_MOST, r.chunk.max_rows = INT32_MAX;
   }
@@ -169,6 +204,7 @@ AttnShare share_of(const Part &p, void *workspace) {
   char *w = (char *)workspace;
   AttnShare s;
   s.min_rows = p.min_rows, s.max_rows = p.max_rows, s.first = 0;
+  s.by_tile = p.by_tile;
   s.count = (int *)(w + p.at), s.desc = (int *)(w + p.desc);
   s.ml = (float *)(w + p.ml), s.acc = (float *)(w + p.acc);
   return s;
@@ -176,11 +212,11 @@ AttnShare share_of(const Part &p, void *workspace) {
 
 template <int DP>
 void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) {
-  const unsigned tiles = (unsigned)(p.tiles * a.Hkv);
+  const unsigned n = (unsigned)(p.by_tile ? p.tiles * a.Hkv : p.grid);
   if (p.tr > 32)
-    hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(tiles, p.tr / 4), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+    hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(n, p.rows / AJ_ROWS), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
   else
-    hipLaunchKernelGGL((attn_join_kernel<DP>), dim3(tiles, p.tr), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+    hipLaunchKernelGGL((attn_join_kernel<DP>), dim3(n, p.rows), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
 }
 
 }  // namespace

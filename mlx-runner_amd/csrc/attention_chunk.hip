@@ -75,7 +75,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
   {
     if (share.first) attn_zero_rest(args);
     const AttnWork w = attn_share<CH_TR, CH_KT, 1>(args, share, ends, scratch);
-    if (blockIdx.x == 0 && tid == 0) share.count[0] = w.tiles;
+    attn_note_none(share, w);
     if (tid == 0) *work = w;
     left = attn_uniform(w.left);
   }
@@ -99,12 +99,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     const int part = w.g * 2 + (w.u == 0 ? 1 : 0), head = w.head;
     {
       const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
-      if (w.u == 0 && tid == 0) {
-        const int64_t last = w.at + cost - 1;
-        const int g1 = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
-        int *d = s.desc + ((int64_t)w.head * w.tiles + w.tile) * 8;
-        d[0] = whole ? -1 : w.g, d[1] = g1, d[2] = rq.q0, d[3] = t.row0, d[4] = t.rows;
-      }
+      if (w.u == 0 && tid == 0) attn_note(s, w, rq, t, cost, whole);
       left = w.left - take;
       __syncthreads();
       if (tid == 0) {
@@ -122,7 +117,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         if (whole) {
           for (int j = tid; j < t.rows * (a.D / 8); j += ATTN_THREADS) {
             float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            attn_store8(a, rq.q0, t.row0 + j / (a.D / 8), head, g, j % (a.D / 8) * 8, o);
+            attn_store8(a, attn_row(a, rq.q0, t.row0 + j / (a.D / 8), head, g), j % (a.D / 8) * 8, o);
           }
         } else if (tid < t.rows) {
           const int64_t pr = (int64_t)part * CH_TR + tid;
@@ -427,48 +422,85 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     const AttnArgs a = attn_again<AttnArgs>(0);
     const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
     // rows out, 32 of a wave and half of their columns at a time, through the wave's quarter of the LDS
-    constexpr int HC = DP / 2, OP = HC + 4;
+    constexpr int HC = DP / 2, OP = HC + 4, IT = 32 * (HC / 8) / 64, AT_ONCE = IT < 4 ? IT : 4;
     float *out = (float *)(lds + wv * TILE);
-    const bool bad = *poison != 0;
+    const int end = ks + nt * CH_KT < t.e ? ks + nt * CH_KT : t.e;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      if (wv * 64 + u * 32 >= t.rows) break;
-      l[u] += __shfl_xor(l[u], 32, 64);
-      const float scale = !whole ? 1.f : l[u] != 0.f ? 1.f / l[u] : 0.f;
-      if (!whole && lane < 32 && wv * 64 + u * 32 + lq < t.rows) {
-        const int64_t pr = (int64_t)part * CH_TR + wv * 64 + u * 32 + lq;
-        s.ml[pr * 2] = m[u], s.ml[pr * 2 + 1] = l[u];
+    for (int u = 0; u < 2; ++u) l[u] += __shfl_xor(l[u], 32, 64);
+#pragma unroll 1
+    for (int stage = 0; stage < 4; ++stage) {
+      const int u = stage >> 1, hc = stage & 1, in0 = wv * 64 + u * 32;
+      if (in0 >= t.rows) break;
+      const float lu = u ? l[1] : l[0], scale = !whole ? 1.f : lu != 0.f ? 1.f / lu : 0.f;
+      if (!whole && hc == 0 && lane < 32 && in0 + lq < t.rows) {
+        const int64_t pr = (int64_t)part * CH_TR + in0 + lq;
+        s.ml[pr * 2] = u ? m[1] : m[0], s.ml[pr * 2 + 1] = lu;
       }
-#pragma unroll
-      for (int hc = 0; hc < 2; ++hc) {
+      auto to_lds = [&](int us, int hs) __attribute__((always_inline)) {
 #pragma unroll
         for (int d = 0; d < DT / 2; ++d)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const f32x16_t &x = acc[hc * (DT / 2) + d][u];
+            const f32x16_t &x = acc[hs * (DT / 2) + d][us];
             *(float4 *)(out + lq * OP + d * 32 + v * 8 + lh * 4) =
                 make_float4(x[4 * v] * scale, x[4 * v + 1] * scale, x[4 * v + 2] * scale, x[4 * v + 3] * scale);
           }
+      };
+      switch (stage) {
+        case 0: to_lds(0, 0); break;
+        case 1: to_lds(0, 1); break;
+        case 2: to_lds(1, 0); break;
+        default: to_lds(1, 1); break;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      auto at = [&](int it, int *in, int *d0) -> float * {
+        const int j = it * 64 + lane, rr = j / (HC / 8), c0 = j % (HC / 8) * 8;
+        *in = in0 + rr, *d0 = hc * HC + c0;
+        return out + rr * OP + c0;
+      };
+      if (*poison) {
+#pragma unroll 1
+        for (int it = 0; it < IT; ++it) {
+          int in, d0;
+          float *x = at(it, &in, &d0), o[8];
+          if (in >= t.rows || d0 >= a.D) continue;
+          *(float4 *)&o[0] = *(const float4 *)x, *(float4 *)&o[4] = *(const float4 *)(x + 4);
+          attn_poison(a, rq, tabrow, head, t.row0 + in, g, ks, end, d0, o);
+          *(float4 *)x = *(const float4 *)&o[0], *(float4 *)(x + 4) = *(const float4 *)&o[4];
+        }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+      }
 #pragma unroll 1
-        for (int j = lane; j < 32 * (HC / 8); j += 64) {
-          const int rr = j / (HC / 8), c0 = j % (HC / 8) * 8, d0 = hc * HC + c0, in = wv * 64 + u * 32 + rr;
+      for (int it0 = 0; it0 < IT; it0 += AT_ONCE) {
+        uint4 gates[AT_ONCE];  // (asked for before the first is used)
+        int64_t rows[AT_ONCE];
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          int in, d0;
+          at(it0 + i, &in, &d0);
+          rows[i] = attn_row(a, rq.q0, t.row0 + in, head, g);
+          if (whole && a.gate && in < t.rows && d0 < a.D) gates[i] = attn_gate8(a, rows[i], d0);
+        }
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+          int in, d0;
+          const float *x = at(it0 + i, &in, &d0);
           if (in >= t.rows || d0 >= a.D) continue;
           float o[8];
-          *(float4 *)&o[0] = *(const float4 *)(out + rr * OP + c0);
-          *(float4 *)&o[4] = *(const float4 *)(out + rr * OP + c0 + 4);
-          if (bad) attn_poison(a, rq, tabrow, head, t.row0 + in, g, ks, ks + nt * CH_KT < t.e ? ks + nt * CH_KT : t.e, d0, o);
+          *(float4 *)&o[0] = *(const float4 *)x, *(float4 *)&o[4] = *(const float4 *)(x + 4);
           if (whole) {
-            attn_store8(a, rq.q0, t.row0 + in, head, g, d0, o);
+            if (a.gate) attn_times_gate(gates[i], o);
+            attn_put8(a, rows[i], d0, o);
           } else {
             float4 *to = (float4 *)(s.acc + ((int64_t)part * CH_TR + in) * DP + d0);
             to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
           }
         }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
       }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
     }
     }
     if constexpr (!FULL) {

@@ -59,7 +59,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
   if (s.first) attn_zero_rest(a);
   AttnWork w = attn_uniform(attn_share<TR, KT, 1>(a, s, ends, scratch));
-  if (blockIdx.x == 0 && tid == 0) s.count[0] = w.tiles;
+  attn_note_none(s, w);
   const int g = a.Hq / a.Hkv;
   const int wv = __builtin_amdgcn_readfirstlane(wave);
   uint8_t *kl = lds + wv * 2 * AR_TILE, *vl = kl + AR_TILE;
@@ -292,12 +292,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     // the four waves' parts, 16 rows at a time through the stage's LDS
     const bool whole = take == cost;
     const int part = w.g * 2 + (w.u == 0 ? 1 : 0);
-    if (w.u == 0 && tid == 0) {
-      const int64_t last = w.at + cost - 1;
-      const int g1 = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
-      int *d = s.desc + ((int64_t)w.head * w.tiles + w.tile) * 8;
-      d[0] = whole ? -1 : w.g, d[1] = g1, d[2] = rq.q0, d[3] = t.row0, d[4] = t.rows;
-    }
+    if (w.u == 0 && tid == 0) attn_note(s, w, rq, t, cost, whole);
     float *macc = (float *)lds;                                  // [wave][16][DP + 4]
     float *mml = (float *)(lds + AR_WAVES * 16 * (DP + 4) * 4);  // [wave][16][2]
 #pragma unroll
@@ -336,7 +331,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) o[e] *= inv;
-          attn_store8(a, rq.q0, t.row0 + n * 16 + row, w.head, g, d0, o);
+          attn_store8(a, attn_row(a, rq.q0, t.row0 + n * 16 + row, w.head, g), d0, o);
         } else {
           const int64_t pr = (int64_t)part * TR + n * 16 + row;
           float4 *to = (float4 *)(s.acc + pr * DP + d0);
