@@ -18,6 +18,8 @@ namespace qmm {
 
 constexpr int ATTN_THREADS = 256;
 
+__device__ __forceinline__ uint32_t attn_div(uint32_t n, FastDiv d) { return __umulhi(n << 1, d.mul) >> d.shift; }
+
 // A launch over the requests of min_rows < n g <= max_rows rows.
 struct AttnShare {
   int min_rows, max_rows;
@@ -26,6 +28,7 @@ struct AttnShare {
   // q0, row0, rows, key head; one for each workgroup (it starts at most one such tile), or, where that is
   // fewer, one for each tile (by head * count + tile).
   int by_tile;
+  int tiles;        // per head at most (what is over, by requests that overlap, is left out)
   int *count;       // tiles per head, workgroups with work
   int *desc;
   float *ml;        // [2 workgroups][TR][2]: maximum and sum of a partial's rows
@@ -48,14 +51,14 @@ struct AttnReq {
   int rows;
 };
 
-__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int r, int g) {
+__device__ __forceinline__ AttnReq attn_req(const AttnArgs &a, int r) {
   AttnReq q;
   const int s0 = a.q_starts[r], s1 = a.q_starts[r + 1], kv = a.kv_lens[r];
   q.q0 = s0 < 0 ? 0 : s0 < a.T ? s0 : a.T;
   const int q1 = s1 < q.q0 ? q.q0 : s1 < a.T ? s1 : a.T;
   q.n = q1 - q.q0;
   q.base = (kv < 0 ? 0 : kv) - q.n;
-  q.rows = q.n * g;
+  q.rows = q.n * a.g;
   return q;
 }
 
@@ -65,11 +68,12 @@ struct AttnTile {
   int b, e, full_b, full_e;
 };
 
-__device__ __forceinline__ AttnTile attn_tile(const AttnArgs &a, const AttnReq &q, int j, int tr, int g) {
+__device__ __forceinline__ AttnTile attn_tile(const AttnArgs &a, const AttnReq &q, int j, int tr) {
   AttnTile t;
   t.row0 = j * tr;
   t.rows = q.rows - t.row0 < tr ? q.rows - t.row0 : tr;
-  const int p0 = q.base + t.row0 / g, p1 = q.base + (t.row0 + t.rows - 1) / g;  // positions of the ends
+  // positions of the ends
+  const int p0 = q.base + (int)attn_div(t.row0, a.by_g), p1 = q.base + (int)attn_div(t.row0 + t.rows - 1, a.by_g);
   const int64_t cap64 = (int64_t)a.W * a.block;
   const int cap = cap64 < 0x7FFF0000 ? (int)cap64 : 0x7FFF0000;  // (ends rounded up stay in range)
   t.e = p1 < cap ? p1 + 1 : cap;
@@ -87,7 +91,7 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs &a, const AttnReq &
 
 template <int KT>
 __device__ __forceinline__ int attn_units(const AttnTile &t) {
-  return t.e > t.b ? (t.e + KT - 1) / KT - t.b / KT : 0;
+  return t.e > t.b ? (int)(((uint32_t)t.e + KT - 1) / KT - (uint32_t)t.b / KT) : 0;
 }
 
 // Inclusive sum over the workgroup; the total too.
@@ -124,12 +128,12 @@ __device__ __forceinline__ int attn_find(const int *ends, int n, int i) {
   return lo;
 }
 
-// A workgroup's share: `left` units from unit `u` of (head, tile) on.
+// A workgroup's share: `left` units from unit `u` of (head, tile) on.  Of `groups` workgroups the first
+// `longer` have one unit more than the others.
 struct AttnWork {
-  int g, groups;        // this workgroup, of how many with work
-  int tiles;            // per head
-  uint32_t per_head;    // units
-  int64_t total, at;    // units in all; the place of unit `u` in the line
+  int g, groups, share, longer;
+  int tiles;         // per head
+  uint32_t at;       // the place of unit `u` in the line of all units
   int head, tile;
   int u, left;
 };
@@ -139,64 +143,100 @@ constexpr int ATTN_SCAN_LDS = 64;  // bytes of LDS beside ends[R]
 // EXTRA units a tile costs beside its keys'.  ends: LDS, [R]; scratch: ATTN_SCAN_LDS bytes of LDS.
 template <int TR, int KT, int EXTRA>
 __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShare &s, int *ends, uint32_t *scratch) {
-  const int tid = threadIdx.x, g = a.Hq / a.Hkv;
+  const int tid = threadIdx.x;
   uint32_t *waves = scratch, *found = scratch + 8;
   AttnWork w;
   uint32_t run = 0, all = 0;
+#pragma unroll 1
   for (int r0 = 0; r0 < a.R; r0 += ATTN_THREADS) {
     const int r = r0 + tid;
     uint32_t nt = 0;
     if (r < a.R) {
-      const AttnReq q = attn_req(a, r, g);
+      const AttnReq q = attn_req(a, r);
       if (q.rows > s.min_rows && q.rows <= s.max_rows) nt = (uint32_t)(q.rows + TR - 1) / TR;
     }
-    const uint32_t end = run + attn_scan(nt, waves, &all);
-    if (r < a.R) ends[r] = (int)end;
-    run += all;
+    const uint32_t most = (uint32_t)s.tiles, end = run + attn_scan(nt < most ? nt : most, waves, &all);
+    if (r < a.R) ends[r] = (int)(end < most ? end : most);
+    run = run + all < most ? run + all : most;
   }
   __syncthreads();
   w.tiles = (int)run;
-  auto units_of = [&](int i) -> uint32_t {
-    if (i >= w.tiles) return 0;
-    const int r = attn_find(ends, a.R, i);
-    const AttnReq q = attn_req(a, r, g);
-    return (uint32_t)(attn_units<KT>(attn_tile(a, q, i - (r ? ends[r - 1] : 0), TR, g)) + EXTRA);
-  };
-  uint32_t mine = 0, end = 0;  // of the last turn
+  w.left = 0, w.g = 0, w.groups = 0;
+  // Units of the tiles, ATTN_THREADS at a time: first all of them, for the shares; then until the tile with the
+  // share's first unit (where there are no more than that, the first turn's values still serve).
+  uint32_t mine = 0, end = 0, x = 0;
   run = 0;
-  for (int i0 = 0; i0 < w.tiles; i0 += ATTN_THREADS) {
-    mine = units_of(i0 + tid);
-    end = run + attn_scan(mine, waves, &all);
-    run += all;
-  }
-  w.per_head = run;
-  w.total = (int64_t)run * a.Hkv;
-  w.left = 0;
-  w.g = 0;
-  const int64_t most = gridDim.x;
-  w.groups = (int)(w.total < most ? w.total : most);
-  if (w.total == 0) return w;
-  // consecutive shares, which read the same keys, on one XCD (workgroups go to the 8 in turn)
-  const int per = (w.groups + 7) >> 3, y = blockIdx.x >> 3;
-  w.g = (blockIdx.x & 7) * per + y;
-  if (y >= per || w.g >= w.groups) return w;
-  w.at = w.g * w.total / w.groups;
-  w.left = (int)((w.g + 1) * w.total / w.groups - w.at);
-  w.head = (int)(w.at / w.per_head);
-  const uint32_t x = (uint32_t)(w.at - (int64_t)w.head * w.per_head);
-  if (w.tiles > ATTN_THREADS) run = 0;  // (else the one turn's values are still here)
-  for (int i0 = 0; i0 < w.tiles; i0 += ATTN_THREADS) {
-    if (w.tiles > ATTN_THREADS) {
-      mine = units_of(i0 + tid);
+  bool sought = false;
+#pragma unroll 1
+  for (int i0 = 0; i0 < w.tiles;) {
+    if (!sought || w.tiles > ATTN_THREADS) {
+      const int i = i0 + tid;
+      mine = 0;
+      if (i < w.tiles) {
+        const int r = attn_find(ends, a.R, i);
+        mine = (uint32_t)(attn_units<KT>(attn_tile(a, attn_req(a, r), i - (r ? ends[r - 1] : 0), TR)) + EXTRA);
+      }
       end = run + attn_scan(mine, waves, &all);
       run += all;
     }
-    if (x < end && x >= end - mine) found[0] = (uint32_t)(i0 + tid), found[1] = x - (end - mine);
+    if (sought && x < end && x >= end - mine) found[0] = (uint32_t)(i0 + tid), found[1] = x - (end - mine);
+    i0 += ATTN_THREADS;
+    if (!sought && i0 >= w.tiles) {
+      const uint32_t per_head = run, total = run * (uint32_t)a.Hkv;
+      w.groups = (int)(total < gridDim.x ? total : gridDim.x);
+      w.share = (int)(total / (uint32_t)w.groups);
+      w.longer = (int)(total - (uint32_t)w.share * (uint32_t)w.groups);
+      // consecutive shares, which read the same keys, on one XCD (workgroups go to the 8 in turn)
+      const int per = (w.groups + 7) >> 3, y = blockIdx.x >> 3;
+      w.g = (blockIdx.x & 7) * per + y;
+      if (y >= per || w.g >= w.groups) return w;
+      w.at = (uint32_t)w.g * (uint32_t)w.share + (uint32_t)(w.g < w.longer ? w.g : w.longer);
+      w.left = w.share + (w.g < w.longer);
+      w.head = (int)(w.at / per_head);
+      x = w.at - (uint32_t)w.head * per_head;
+      sought = true;
+      i0 = 0, run = 0;
+    }
   }
   __syncthreads();
   w.tile = (int)found[0];
   w.u = (int)found[1];
   return w;
+}
+// The workgroup whose share unit `at` of the line is in.
+__device__ __forceinline__ int attn_group_of(const AttnWork &w, uint32_t at) {
+  const uint32_t head = (uint32_t)w.longer * (uint32_t)(w.share + 1);
+  return (int)(at < head ? at / (uint32_t)(w.share + 1) : (uint32_t)w.longer + (at - head) / (uint32_t)w.share);
+}
+
+// What a workgroup does of the tile that its share has come to: the key units [u0, u1) of `units`.  A tile's first
+// EXTRA units stand for its own overhead; who has the first key unit starts it.
+struct AttnPiece {
+  int take, u0, u1;
+  bool whole, start, none;
+};
+template <int EXTRA>
+__device__ __forceinline__ AttnPiece attn_piece(const AttnWork &w, int units) {
+  AttnPiece p;
+  const int cost = units + EXTRA;
+  p.take = cost - w.u < w.left ? cost - w.u : w.left;
+  p.u0 = w.u > EXTRA ? w.u - EXTRA : 0;
+  p.u1 = w.u + p.take > EXTRA ? w.u + p.take - EXTRA : 0;
+  p.start = p.u0 == 0;
+  p.whole = p.start && p.u1 == units;
+  p.none = units ? p.u1 <= p.u0 : w.u + p.take < cost;  // (a tile without keys: its zeros with its last unit)
+  return p;
+}
+__device__ __forceinline__ void attn_move_on(AttnWork &w, int take, int cost) {
+  w.left -= take;
+  w.at += (uint32_t)take;
+  w.u += take;
+  if (w.u == cost) {
+    w.u = 0;
+    const bool last = ++w.tile == w.tiles;
+    w.tile = last ? 0 : w.tile;
+    w.head += last;
+  }
 }
 
 // Notes the tile that this workgroup starts (by one thread).
@@ -207,8 +247,7 @@ __device__ __forceinline__ void attn_note(const AttnShare &s, const AttnWork &w,
     if (s.by_tile) d[0] = -1;
     return;
   }
-  const int64_t last = w.at - w.u + cost - 1;
-  d[0] = w.g, d[1] = (int)(((last + 1) * w.groups + w.total - 1) / w.total) - 1;
+  d[0] = w.g, d[1] = attn_group_of(w, w.at - (uint32_t)w.u + (uint32_t)cost - 1u);
   d[2] = q.q0, d[3] = t.row0, d[4] = t.rows, d[5] = w.head;
 }
 // First of all: how many tiles and workgroups with work; no tile noted yet.
@@ -233,9 +272,9 @@ __device__ __forceinline__ void attn_zero_rest(const AttnArgs &a) {
 }
 
 // Row `row` of a request: its (token, query head) in q, gate and o.
-__device__ __forceinline__ int64_t attn_row(const AttnArgs &a, int q0, int row, int head, int g) {
-  const int tok = row / g;
-  return (int64_t)(q0 + tok) * a.Hq + head * g + (row - tok * g);
+__device__ __forceinline__ int64_t attn_row(const AttnArgs &a, int q0, int row, int head) {
+  const int tok = (int)attn_div(row, a.by_g);
+  return (int64_t)(q0 + tok) * a.Hq + head * a.g + (row - tok * a.g);
 }
 // Eight values of a finished row (divided by its sum), d0 a multiple of 8 below D: the gate of them, times
 // its sigmoid, their rounding.
@@ -279,19 +318,23 @@ __device__ __forceinline__ uint4 attn_finite(uint4 x) {
 // Adds to 8 sums of a row the values that are not finite of the keys in [ks, ke) that it sees: what was
 // left out where the rows of a tile see different keys.  Slow, and only where there are any.
 __device__ __forceinline__ void attn_poison(const AttnArgs &a, const AttnReq &q, const int *tabrow, int head,
-                                                      int row, int g, int ks, int ke, int d0, float (&o)[8]) {
-  const int pos = q.base + row / g;
+                                                      int row, int ks, int ke, int d0, float (&o)[8]) {
+  const int pos = q.base + (int)attn_div(row, a.by_g);
   const int hi = pos < ke - 1 ? pos : ke - 1;
   int lo = a.window && pos - a.window + 1 > ks ? pos - a.window + 1 : ks;
 #pragma unroll 1
   for (int key = lo; key <= hi; ++key) {
-    const int blk = tabrow[(uint32_t)key / (uint32_t)a.block];
+    const uint32_t page = attn_div(key, a.by_block);
+    const int blk = tabrow[page];
     if ((uint32_t)blk >= (uint32_t)a.NB) continue;
-    const uint64_t r = ((uint64_t)blk * a.Hkv + head) * a.block + (uint32_t)key % (uint32_t)a.block;
-    const uint16_t *v = a.v + r * a.D + d0;
-#pragma unroll 1
-    for (int e = 0; e < 8; ++e)
-      if ((v[e] & 0x7F80) == 0x7F80) o[e] += bf16_to_f32(v[e]);
+    const uint64_t r = ((uint64_t)blk * a.Hkv + head) * a.block + ((uint32_t)key - page * (uint32_t)a.block);
+    const uint4 v = *(const uint4 *)(a.v + r * a.D + d0);
+    const uint32_t x[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if ((x[e] & 0x7F80u) == 0x7F80u) o[2 * e] += __uint_as_float(x[e] << 16);
+      if ((x[e] & 0x7F800000u) == 0x7F800000u) o[2 * e + 1] += __uint_as_float(x[e] & 0xFFFF0000u);
+    }
   }
 }
 
@@ -308,6 +351,23 @@ __device__ __forceinline__ int attn_swz(int row) {
 __device__ __forceinline__ int attn_opaque(int x) {
   asm volatile("" : "+v"(x));
   return x;
+}
+
+// The lane's number, formed here: not kept in a register through a loop that needs all of them.
+__device__ __forceinline__ uint32_t attn_lane() {
+  uint32_t x;
+  asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(x));
+  return x;
+}
+
+__device__ __forceinline__ uint4 attn_zeros() {
+  const uint32_t z = (uint32_t)attn_opaque(0);
+  return make_uint4(z, z, z, z);
+}
+
+// x of lane ^ `other`.
+__device__ __forceinline__ float attn_across(float x, int other) {
+  return __int_as_float(__builtin_amdgcn_ds_bpermute(((int)attn_lane() ^ other) * 4, __float_as_int(x)));
 }
 
 // A kernel's arguments (at `offset` of its argument block) read again where they are needed, instead of

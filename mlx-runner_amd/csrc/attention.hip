@@ -70,7 +70,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
       for (int i = 0; i < SETS; ++i) v[e] += part[i][tid * 8 + e];
       v[e] *= inv;
     }
-    attn_store8(a, attn_row(a, d[2], d[3] + row, d[5], a.Hq / a.Hkv), tid * 8, v);
+    attn_store8(a, attn_row(a, d[2], d[3] + row, d[5]), tid * 8, v);
   }
 }
 
@@ -137,7 +137,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = part[row][c0 + e] * inv;
-    attn_store8(a, attn_row(a, d[2], d[3] + row0 + row, d[5], a.Hq / a.Hkv), c0, v);
+    attn_store8(a, attn_row(a, d[2], d[3] + row0 + row, d[5]), c0, v);
   }
 }
 
@@ -159,6 +159,13 @@ struct Route {
   Part rows, chunk;  // (tr 0: not launched)
   size_t bytes;
 };
+
+// ceil(2^(31 + l) / d), l = ceil(log2 d): exact quotients for n < 2^31
+FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while (((uint64_t)1 << l) < d) ++l;
+  return FastDiv{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), l};
+}
 
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
@@ -204,7 +211,7 @@ AttnShare share_of(const Part &p, void *workspace) {
   char *w = (char *)workspace;
   AttnShare s;
   s.min_rows = p.min_rows, s.max_rows = p.max_rows, s.first = 0;
-  s.by_tile = p.by_tile;
+  s.by_tile = p.by_tile, s.tiles = (int)p.tiles;
   s.count = (int *)(w + p.at), s.desc = (int *)(w + p.desc);
   s.ml = (float *)(w + p.ml), s.acc = (float *)(w + p.acc);
   return s;
@@ -221,14 +228,25 @@ void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) 
 
 }  // namespace
 
+// What of a call passes the kernels' 32-bit counts (NULL: nothing).
+const char *attention_limits(const AttnArgs &a) {
+  if ((double)a.T * (a.Hq / a.Hkv) > 1 << 27) return "rows per key head";
+  const Route r = route_of(a);
+  for (const Part *p : {&r.rows, &r.chunk})
+    if (p->tr && (double)p->tiles * a.Hkv * ((double)a.W * a.block / 64 + 4) > INT32_MAX) return "keys of all tiles together";
+  return nullptr;
+}
+
 size_t attention_workspace(const AttnArgs &a) { return route_of(a).bytes; }
 
-hipError_t launch_attention(const AttnArgs &a, void *workspace, hipStream_t st) {
+hipError_t launch_attention(const AttnArgs &args, void *workspace, hipStream_t st) {
+  AttnArgs a = args;
+  a.g = a.Hq / a.Hkv;
+  a.by_g = fast_div((uint32_t)a.g);
+  a.by_block = fast_div((uint32_t)a.block);
   if (a.R == 0 || a.W == 0 || a.NB == 0)  // no keys at all
     return launch_fill_zero(a.o, (size_t)a.T * a.Hq * a.D * 2, st);
   const Route r = route_of(a);
-  for (const Part *p : {&r.rows, &r.chunk})
-    if (p->tiles * a.Hkv > INT32_MAX) return hipErrorInvalidValue;
   bool first = true;
   for (const Part *p : {&r.rows, &r.chunk}) {
     if (!p->tr) continue;

@@ -41,6 +41,8 @@ int check_cache(const char *op, const char *name, const Arr *a) {
   if (a->dtype != QMM_BFLOAT16 || a->ndim != 4)
     return fail("[%s] %s must be a bfloat16 array [pages, heads, block, D]", op, name);
   if (a->shape[1] < 1 || a->shape[2] < 1) return fail("[%s] %s needs heads and a block size", op, name);
+  if ((double)a->shape[0] * a->shape[1] * a->shape[2] > UINT32_MAX)  // (they are counted in 32 bits)
+    return fail("[%s] %s has over 2^32 - 1 keys", op, name);
   if (misaligned(a)) return fail("[%s] %s must be 16-byte aligned", op, name);
   return 0;
 }
@@ -256,18 +258,20 @@ int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_arra
   if (window < 0) return finish(fail("[%s] window must not be negative, got %d", op, window));
   if (!std::isfinite(scale)) return finish(fail("[%s] scale must be finite", op));
   if (misaligned(qa)) return finish(fail("[%s] q must be 16-byte aligned", op));
+  AttnArgs a;
+  a.q = (const uint16_t *)qa->data, a.k = (const uint16_t *)kc->data, a.v = (const uint16_t *)vc->data;
+  a.gate = ga ? (const uint16_t *)ga->data : nullptr;
+  a.table = (const int *)ta->data, a.q_starts = (const int *)sa->data, a.kv_lens = (const int *)la->data;
+  a.T = T, a.R = R, a.W = W, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.Dg = ga ? ga->shape[2] : 0;
+  a.NB = NB, a.block = block, a.window = window, a.scale = scale;
+  const char *too_much = attention_limits(a);
+  if (too_much) return finish(fail("[%s] too many %s", op, too_much));
   hipStream_t st = stream_of(s);
   Arr *oa;
   if (alloc_arr(res, {T, Hq, D}, QMM_BFLOAT16, st, &oa)) return finish(1);
   if (misaligned(oa)) return finish(fail("[%s] the result must be 16-byte aligned", op));
   if (T == 0) return finish(0);
-  AttnArgs a;
-  a.q = (const uint16_t *)qa->data, a.k = (const uint16_t *)kc->data, a.v = (const uint16_t *)vc->data;
-  a.gate = ga ? (const uint16_t *)ga->data : nullptr;
   a.o = (uint16_t *)oa->data;
-  a.table = (const int *)ta->data, a.q_starts = (const int *)sa->data, a.kv_lens = (const int *)la->data;
-  a.T = T, a.R = R, a.W = W, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.Dg = ga ? ga->shape[2] : 0;
-  a.NB = NB, a.block = block, a.window = window, a.scale = scale;
   Scratch scratch;
   const size_t need = attention_workspace(a);
   if (need && scratch.take(st, need)) return finish(1);

@@ -23,6 +23,7 @@ namespace qmm {
 namespace {
 
 constexpr int CH_TR = 256, CH_KT = 64;
+constexpr int CH_EXTRA = 3;  // what a tile's own overhead (queries in, rows out) costs, in units of 64 keys
 constexpr int CH_TAB = 4 * 2 * 256 + 2 * 4 * 4;  // page ids of the tiles to come, two sets per wave; valid keys
 
 constexpr int ch_tile(int DP) { return CH_KT * DP * 2; }  // bytes of a tile of keys (or of values)
@@ -64,106 +65,100 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   uint8_t *tab = lds + 4 * TILE;
   uint32_t *vm = (uint32_t *)(tab + 4 * 2 * 256);  // [2][4]
-  uint32_t *scratch = (uint32_t *)(tab + CH_TAB);
+  int *seen_at = (int *)(tab + CH_TAB);  // [thread][2][2]: what its rows see
+  uint32_t *scratch = (uint32_t *)(seen_at + 4 * ATTN_THREADS);
   int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS + sizeof(AttnWork)), *poison = (int *)scratch + 15, *redo = (int *)scratch + 14;
 
-  const int tid = threadIdx.x, lane = tid & 63, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lq = lane & 31, lh = lane >> 5;
-  const int g = args.Hq / args.Hkv;
-  AttnWork *work = (AttnWork *)(scratch + ATTN_SCAN_LDS / 4);  // (this workgroup's share, out of the registers)
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto work = [&]() __attribute__((always_inline)) {  // this workgroup's share, out of the registers
+    return (AttnWork *)(scratch + attn_opaque(ATTN_SCAN_LDS / 4));
+  };
+  auto here = [&]() __attribute__((always_inline)) { return wv * 64 + (int)attn_lane(); };  // the thread's number
   int left;
   {
     if (share.first) attn_zero_rest(args);
-    const AttnWork w = attn_share<CH_TR, CH_KT, 1>(args, share, ends, scratch);
+    const AttnWork w = attn_uniform(attn_share<CH_TR, CH_KT, CH_EXTRA>(args, share, ends, scratch));
     attn_note_none(share, w);
-    if (tid == 0) *work = w;
+    if (tid == 0) *work() = w;
     left = attn_uniform(w.left);
   }
   const uint32_t la = lds_addr(lds), ta = lds_addr(tab) + wv * 512;
   if constexpr (!FULL) {  // head values past D: never written by the DMA
-    for (int i = tid; i < 4 * TILE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < 4 * TILE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
   }
 
   while (left > 0) {
     __syncthreads();
     const AttnArgs a = attn_again<AttnArgs>(0);
-    const AttnWork w = attn_uniform(*work);
+    const AttnWork w = attn_uniform(*work());
     const int r = attn_uniform(attn_find(ends, a.R, w.tile));
-    const AttnReq rq = attn_uniform(attn_req(a, r, g));
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), CH_TR, g);
-    const int cost = attn_units<CH_KT>(t) + 1;
-    const int take = cost - w.u < w.left ? cost - w.u : w.left;
-    const int u0 = w.u > 0 ? w.u - 1 : 0, u1 = w.u + take - 1;  // (the first unit: the tile's own overhead)
-    const int ks = (t.b / CH_KT + u0) * CH_KT, nt = u1 - u0;
-    const bool whole = take == cost;
-    const int part = w.g * 2 + (w.u == 0 ? 1 : 0), head = w.head;
+    const AttnReq rq = attn_uniform(attn_req(a, r));
+    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), CH_TR);
+    const int units = attn_units<CH_KT>(t);
+    const AttnPiece pc = attn_piece<CH_EXTRA>(w, units);
+    const int ks = (int)((uint32_t)t.b / CH_KT + pc.u0) * CH_KT, nt = pc.u1 - pc.u0;
+    const bool whole = pc.whole;
+    const int part = w.g * 2 + pc.start, head = w.head;
+    if (pc.start && !pc.none && here() == 0) attn_note(attn_again<AttnShare>(sizeof(AttnArgs)), w, rq, t, units + CH_EXTRA, whole);
+    __syncthreads();
     {
-      const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
-      if (w.u == 0 && tid == 0) attn_note(s, w, rq, t, cost, whole);
-      left = w.left - take;
-      __syncthreads();
-      if (tid == 0) {
-        work->left = left;
-        work->at = w.at + take;
-        work->u = w.u + take;
-        if (w.u + take == cost) {
-          const bool last = w.tile + 1 == w.tiles;
-          work->u = 0;
-          work->tile = last ? 0 : w.tile + 1;
-          work->head = w.head + last;
-        }
+      AttnWork on = w;
+      attn_move_on(on, pc.take, units + CH_EXTRA);
+      left = on.left;
+      if (here() == 0) *work() = on;
+    }
+    if (pc.none) continue;
+    if (units == 0) {  // no keys
+      const uint32_t per = (uint32_t)a.D / 8;
+      for (uint32_t j = here(); j < t.rows * per; j += ATTN_THREADS) {
+        const uint32_t row = j / per;
+        const float z = __int_as_float(attn_opaque(0));
+        float o[8] = {z, z, z, z, z, z, z, z};
+        attn_store8(a, attn_row(a, rq.q0, t.row0 + row, head), (j - row * per) * 8, o);
       }
-      if (nt == 0) {  // no keys: zeros, or a part of nothing
-        if (whole) {
-          for (int j = tid; j < t.rows * (a.D / 8); j += ATTN_THREADS) {
-            float o[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            attn_store8(a, attn_row(a, rq.q0, t.row0 + j / (a.D / 8), head, g), j % (a.D / 8) * 8, o);
-          }
-        } else if (tid < t.rows) {
-          const int64_t pr = (int64_t)part * CH_TR + tid;
-          s.ml[pr * 2] = -__builtin_inff(), s.ml[pr * 2 + 1] = 0.f;
-        }
-        continue;
-      }
+      continue;
     }
 
-    if (tid == 0) *poison = 0, *redo = 0;
+    if (here() == 0) *poison = attn_opaque(0), *redo = attn_opaque(0);
     const int *tabrow = a.table + (int64_t)r * a.W;
     const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
     const uint16_t *kc = a.k, *vc = a.v;
-    const uint32_t first = ks + wv * 16 + (lane & 15);
-    const uint32_t first_page = first / (uint32_t)block, first_off = first - first_page * block;
-    const uint32_t last_page = (uint32_t)(t.e - 1) / (uint32_t)block;
-    const int page0 = tabrow[first_page < last_page ? first_page : last_page];
     // the lane's rows
-    int seen_b[2], seen_e[2];
+    float m[2], l[2];
     bf16x8_t q[2][KS];
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;
 #pragma unroll
     for (int u = 0; u < 2; ++u) {
-      const int in = wv * 64 + u * 32 + lq, row = t.row0 + in;
+      const uint32_t ln = attn_lane();
+      const int in = wv * 64 + u * 32 + (int)(ln & 31), lh = (int)(ln >> 5);
       const bool on = in < t.rows;
-      const int tok = on ? row / g : 0, hh = on ? row - tok * g : 0;
-      const int pos = rq.base + tok;
-      seen_e[u] = on ? pos : -1;
-      seen_b[u] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
-      const uint16_t *qp = a.q + (((int64_t)(rq.q0 + tok) * a.Hq) + head * g + hh) * a.D;
+      const int row = t.row0 + (on ? in : 0);  // (a row past the end: the first one's queries, and no keys)
+      const int tok = (int)attn_div(row, a.by_g), pos = rq.base + tok;
+      seen_at[(wv * 64 + (int)ln) * 4 + 2 * u] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
+      seen_at[(wv * 64 + (int)ln) * 4 + 2 * u + 1] = on ? pos : -1;
+      m[u] = on && pos >= 0 ? -__builtin_inff() : 0.f;  // (a row that sees nothing needs no reference)
+      const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D + lh * 8;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {
-        const int d0 = k * 16 + lh * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (on && (FULL || d0 < a.D) && a.scale != 0.f) v = *(const uint4 *)(qp + d0);
-        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-        q[u][k] = __builtin_bit_cast(bf16x8_t, v);
+        if (FULL || k * 16 + lh * 8 < a.D)
+          q[u][k] = *(const bf16x8_t *)(qp + k * 16);
+        else
+          q[u][k] = __builtin_bit_cast(bf16x8_t, u32x4_t{0u, 0u, 0u, 0u});
       }
+    }
+    if (!(a.scale > 0.f)) {  // a negative scale: -q, so that maxima stay maxima; none: no scores
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int k = 0; k < KS; ++k) {
+          u32x4_t x = __builtin_bit_cast(u32x4_t, q[u][k]);
+          x = a.scale < 0.f ? x ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
+          q[u][k] = __builtin_bit_cast(bf16x8_t, x);
+        }
     }
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the compiler's own waits would come between the DMA's
     const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
 
     f32x16_t acc[DT][2];
-    float m[2], l[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) m[u] = seen_e[u] < 0 ? 0.f : -__builtin_inff();  // (a row that sees nothing)
     bool again = false;
     do {
 #pragma unroll
@@ -181,7 +176,11 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
 
       // Keys on their way: this lane looks up key wv * 16 + lane % 16 of each tile.  `off` is its place in
       // its page, for the tile whose rows come next; `page` and `poff` are two tiles on.
-      const uint32_t per = CH_KT / (uint32_t)block, rest = CH_KT % (uint32_t)block;
+      const uint32_t per = attn_div(CH_KT, a.by_block), rest = CH_KT - per * (uint32_t)block;
+      const uint32_t first = ks + wv * 16 + ((int)attn_lane() & 15);
+      const uint32_t first_page = attn_div(first, a.by_block), first_off = first - first_page * block;
+      const uint32_t last_page = attn_div(t.e - 1, a.by_block);
+      const int page0 = tabrow[first_page < last_page ? first_page : last_page];
       uint32_t page = first_page, poff = first_off, off = first_off;
       auto onward = [&](uint32_t &pg, uint32_t &of) __attribute__((always_inline)) {
         pg += per, of += rest;
@@ -192,15 +191,15 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       };
       uint32_t mine = 0;  // the row (of the whole cache) of this lane's key, 0 where there is none
       auto rows_of = [&](int k0, uint32_t of, int blk, int set) __attribute__((always_inline)) {
-        const bool ok = k0 + wv * 16 + (attn_opaque(lane) & 15) < t.e && (uint32_t)blk < (uint32_t)NB;
-        mine = ok ? ((uint32_t)blk * Hkv + head) * block + of : 0u;
+        const bool ok = k0 + wv * 16 + ((int)attn_lane() & 15) < t.e && (uint32_t)blk < (uint32_t)NB;
+        mine = (((uint32_t)blk * Hkv + head) * block + of) & (ok ? ~0u : 0u);
         const uint32_t mask = (uint32_t)__ballot(ok) & 0xFFFFu;
-        if (lane == 0) vm[set * 4 + wv] = mask;
+        vm[set * 4 + wv] = mask;  // (by all lanes: no branch)
       };
       // DMA operation n: rows RPI n .. of the wave's 16, chunk (lane % CPR) ^ swizzle of each
       constexpr int RPI = 64 / CPR;
       auto move = [&](const uint16_t *cache, int n, int to, auto swz) __attribute__((always_inline)) {
-        const uint32_t ln = attn_opaque(lane);
+        const uint32_t ln = attn_lane();
         const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(ln / CPR * 4) + RPI * n * 4, (int)mine);
         const uint32_t c = (ln % CPR ^ (uint32_t)swz((int)(ln / CPR)) ^ (uint32_t)swz(RPI * n)) * 16;
         if (FULL || c < 2 * (uint32_t)D)
@@ -216,7 +215,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       // S^T of 32 keys; beside it, the DMA of a tile's values
       auto scores = [&](int set, int half, bool values) __attribute__((always_inline)) {
         // (k steps 8 apart differ by 256 bytes, which the swizzle leaves alone)
-        const uint32_t ln = attn_opaque(lane);
+        const uint32_t ln = attn_lane();
         const int lq = ln & 31;
         const int from = set * TILE + half * 32 * PITCH + lq * PITCH + ((int)(ln >> 5) ^ attn_swz<DP>(lq)) * 16;
         auto load = [&](int k) __attribute__((always_inline)) {
@@ -246,16 +245,20 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         if (!edge && !fresh) return;
         ch_mfma_done(sv[0], sv[1]);
         if (edge) {
-          const int h4 = attn_opaque(4 * lh);
-          const uint32_t bits = valid >> h4;
+          const int h4 = (int)attn_lane() >> 5 << 2;
+          const int4 rows = *(const int4 *)(seen_at + (wv * 64 + (int)attn_lane()) * 4);
+          const int seen_b[2] = {rows.x, rows.z}, seen_e[2] = {rows.y, rows.w};
 #pragma unroll
           for (int u = 0; u < 2; ++u) {
-            const int lo = seen_b[u] - k0 - h4, hi = seen_e[u] - k0 - h4;
+            // bit o: key k0 + o is seen
+            const int lo = seen_b[u] - k0, hi = seen_e[u] - k0;
+            uint32_t seen = hi < 0 ? 0u : hi > 30 ? ~0u : (2u << hi) - 1u;
+            seen &= lo > 31 ? 0u : lo > 0 ? ~0u << lo : ~0u;
+            seen = (seen & valid) >> h4;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
-              const int o = 8 * (i / 4) + i % 4;
-              if (!(o <= hi && o >= lo && (bits >> o & 1))) sv[u][i] = -__builtin_inff();
-              __builtin_amdgcn_sched_barrier(0);  // (one mask at a time)
+              const int on = __builtin_amdgcn_sbfe((int)seen, 8 * (i / 4) + i % 4, 1);  // 0 or -1
+              sv[u][i] = __uint_as_float((__float_as_uint(sv[u][i]) & (uint32_t)on) | (0xFF800000u & ~(uint32_t)on));
             }
           }
         }
@@ -265,7 +268,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             float x = sv[u][0];
 #pragma unroll
             for (int i = 1; i < 16; ++i) x = fmaxf(x, sv[u][i]);
-            x = fmaxf(x, __shfl_xor(x, 32, 64)) * sc;
+            x = fmaxf(x, attn_across(x, 32)) * sc;
             m[u] = m[u] == -__builtin_inff() ? x : m[u];
           }
         }
@@ -279,7 +282,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         }
 #pragma unroll
         for (int j = n * (16 / N); j < (n + 1) * (16 / N); ++j) {
-          const int u = j >> 3, c = j >> 2 & 1, e = (j & 3) * 2;
+          const int c = j >> 3, u = j >> 2 & 1, e = (j & 3) * 2;
           const float s0 = sv[u][c * 8 + e], s1 = sv[u][c * 8 + e + 1];
           top[u] = fmaxf(top[u], fmaxf(s0, s1));
           bf16x2_t x;
@@ -308,13 +311,13 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       };
       // O^T += V^T P^T over 32 keys; beside it the next weights and the DMA of a tile's keys
       auto product = [&](int set, int half, bool with, int keys) __attribute__((always_inline)) {
-        const uint32_t ln = attn_opaque(lane);
+        const uint32_t ln = attn_lane();
         const int row = 4 * (ln >> 5) + (ln >> 2 & 3);
         const int from = la + (2 + set) * TILE + (half * 32 + row) * PITCH +
                          ((int)((ln >> 4 & 1) * 2 + (ln >> 1 & 1)) ^ ch_swz_v<DP>(row)) * 16 + (ln & 1) * 8;
         constexpr int N = 2 * DT, AHEAD = 2;
         auto load = [&](int n) __attribute__((always_inline)) {
-          const int d = n >> 1, c = n & 1;
+          const int d = n % DT, c = n / DT;  // (the first 16 keys' weights are done with half way)
           const uint32_t at = (from ^ (d & 3) * 64) + (d >> 2) * 256 + c * 16 * PITCH;
           const i16x4_t v0 = attn_read_tr(at), v1 = attn_read_tr(at + 8 * PITCH);
           return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
@@ -327,7 +330,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           if (n + AHEAD < N) vf[n + AHEAD] = load(n + AHEAD);
 #pragma unroll
           for (int u = 0; u < 2; ++u)
-            acc[n >> 1][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], p[n & 1][u], acc[n >> 1][u], 0, 0, 0);
+            acc[n % DT][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], p[n / DT][u], acc[n % DT][u], 0, 0, 0);
           if (n == 0 && with) ch_mfma_done(sv[0], sv[1]);
           if (with) weights(n, N);
           if (keys >= 0 && n % 2 == 0) move_k(keys, n / 2);
@@ -359,7 +362,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         const int set = i & 1, k0 = ks + i * CH_KT;
         gp_wait_barrier<0>();  // keys of tile i, page ids of tile i + 1, everyone's valid bits
         const uint4 bits = *(const uint4 *)(vm + set * 4);
-        const int blk = *(const int *)(tab + wv * 512 + (set ^ 1) * 256 + attn_opaque(lane) * 4);
+        const int blk = *(const int *)(tab + wv * 512 + (set ^ 1) * 256 + (int)attn_lane() * 4);
         scores(set, 0, true);
         valid = valid_of(bits);
         edge = edge_at(k0, valid);
@@ -375,30 +378,31 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         special(ks + i * CH_KT + 32, (uint32_t)(valid >> 32), edge);
         // values of tile i (the page ids and keys asked for after them may be on their way)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
-        if (edge) {  // (see attention_rows.hip)
+        const int own = ks + i * CH_KT + wv * 16;  // (the values that this wave has moved; see attention_rows.hip)
+        if (edge && (own < t.full_b || own + 16 > t.full_e || ((valid >> wv * 16) & 0xFFFFu) != 0xFFFFu)) {
+          const uint32_t ln = attn_lane();
           bool odd = false;
-#pragma unroll 1
+#pragma unroll
           for (int j = 0; j < OPS; ++j) {
-            uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + lane * 16);
+            uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 16 * PITCH + j * 1024 + ln * 16);
             const uint4 x = *at, y = attn_finite(x);
-            const bool in = valid >> (wv * 16 + (j * 64 + lane) / CPR) & 1;
+            const bool in = valid >> (wv * 16 + (j * 64 + ln) / CPR) & 1;
             odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
-            *at = in ? y : make_uint4(0, 0, 0, 0);
+            *at = in ? y : attn_zeros();
+            __builtin_amdgcn_sched_barrier(0);
           }
-          if (__any(odd)) *poison = 1;
+          if (__any(odd)) *poison = attn_opaque(1);
         }
         gp_lds_barrier();
       };
-      begin(0);
-      ch_mfma_done(sv[0], sv[1]);
-      weights(0, 1);
+      // (before the first: no weights, and no values that they could meet)
 #pragma unroll
-      for (int n = 0; n < OPS; ++n) move_k(1, n);
-      settle();
-      middle(0);
-      product(0, 0, true, -1);
-      settle();
-      for (int i = 1; i < nt; ++i) {
+      for (int u = 0; u < 2; ++u)
+#pragma unroll
+        for (int c = 0; c < 2; ++c) p[c][u] = __builtin_bit_cast(bf16x8_t, u32x4_t{0u, 0u, 0u, 0u});
+      for (int j = here(); j < TILE / 32; j += ATTN_THREADS) ((uint4 *)(lds + 3 * TILE + TILE / 2))[j] = attn_zeros();
+#pragma unroll 1
+      for (int i = 0; i < nt; ++i) {
         begin(i);
         product((i + 1) & 1, 1, true, (i + 1) & 1);
         settle();
@@ -408,12 +412,12 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       }
       product((nt - 1) & 1, 1, false, -1);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    if (__any(passed)) *redo = 1;
+    if (__any(passed)) *redo = attn_opaque(1);
     __syncthreads();
     again = !again && *redo;
     if (again) {
 #pragma unroll
-      for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], __shfl_xor(m[u], 32, 64));
+      for (int u = 0; u < 2; ++u) m[u] = fmaxf(m[u], attn_across(m[u], 32));
     }
     __syncthreads();
     } while (again);
@@ -421,91 +425,80 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     {
     const AttnArgs a = attn_again<AttnArgs>(0);
     const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
-    // rows out, 32 of a wave and half of their columns at a time, through the wave's quarter of the LDS
-    constexpr int HC = DP / 2, OP = HC + 4, IT = 32 * (HC / 8) / 64, AT_ONCE = IT < 4 ? IT : 4;
+    // Rows out, 32 of a wave and half of their columns at a time, through the wave's quarter of the LDS: sums in its
+    // first half (pairs of 16-byte chunks, swizzled by row), the 32 rows' gates in the second.
+    constexpr int HC = DP / 2, PAIRS = HC / 8, IT = 32 * PAIRS / 64;
     float *out = (float *)(lds + wv * TILE);
     const int end = ks + nt * CH_KT < t.e ? ks + nt * CH_KT : t.e;
+    const bool gated = whole && a.gate;
 #pragma unroll
-    for (int u = 0; u < 2; ++u) l[u] += __shfl_xor(l[u], 32, 64);
-#pragma unroll 1
-    for (int stage = 0; stage < 4; ++stage) {
-      const int u = stage >> 1, hc = stage & 1, in0 = wv * 64 + u * 32;
+    for (int u = 0; u < 2; ++u) {
+      const int in0 = wv * 64 + u * 32;
       if (in0 >= t.rows) break;
-      const float lu = u ? l[1] : l[0], scale = !whole ? 1.f : lu != 0.f ? 1.f / lu : 0.f;
-      if (!whole && hc == 0 && lane < 32 && in0 + lq < t.rows) {
-        const int64_t pr = (int64_t)part * CH_TR + in0 + lq;
-        s.ml[pr * 2] = u ? m[1] : m[0], s.ml[pr * 2 + 1] = lu;
-      }
-      auto to_lds = [&](int us, int hs) __attribute__((always_inline)) {
+      if (gated) {
 #pragma unroll
-        for (int d = 0; d < DT / 2; ++d)
-#pragma unroll
-          for (int v = 0; v < 4; ++v) {
-            const f32x16_t &x = acc[hs * (DT / 2) + d][us];
-            *(float4 *)(out + lq * OP + d * 32 + v * 8 + lh * 4) =
-                make_float4(x[4 * v] * scale, x[4 * v + 1] * scale, x[4 * v + 2] * scale, x[4 * v + 3] * scale);
-          }
-      };
-      switch (stage) {
-        case 0: to_lds(0, 0); break;
-        case 1: to_lds(0, 1); break;
-        case 2: to_lds(1, 0); break;
-        default: to_lds(1, 1); break;
-      }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      auto at = [&](int it, int *in, int *d0) -> float * {
-        const int j = it * 64 + lane, rr = j / (HC / 8), c0 = j % (HC / 8) * 8;
-        *in = in0 + rr, *d0 = hc * HC + c0;
-        return out + rr * OP + c0;
-      };
-      if (*poison) {
-#pragma unroll 1
-        for (int it = 0; it < IT; ++it) {
-          int in, d0;
-          float *x = at(it, &in, &d0), o[8];
-          if (in >= t.rows || d0 >= a.D) continue;
-          *(float4 *)&o[0] = *(const float4 *)x, *(float4 *)&o[4] = *(const float4 *)(x + 4);
-          attn_poison(a, rq, tabrow, head, t.row0 + in, g, ks, end, d0, o);
-          *(float4 *)x = *(const float4 *)&o[0], *(float4 *)(x + 4) = *(const float4 *)&o[4];
+        for (int i = 0; i < DP / 16; ++i) {
+          const uint32_t j = i * 64 + (int)attn_lane();
+          int in = in0 + (int)(j / CPR);
+          in = in < t.rows ? in : in0;
+          const int c = (int)(j % CPR) * 8;
+          if (FULL || c < a.D)
+            gp_dma16(a.gate + attn_row(a, rq.q0, t.row0 + in, head) * a.Dg + (a.Dg - a.D) + c,
+                     la + wv * TILE + TILE / 2 + i * 1024);
+          __builtin_amdgcn_sched_barrier(0);
         }
+      }
+      const float lu = l[u] + attn_across(l[u], 32);
+      const float scale = !whole ? 1.f : lu != 0.f ? 1.f / lu : 0.f;
+      const int l32 = (int)attn_lane();
+      if (!whole && l32 < 32 && in0 + l32 < t.rows) {
+        const int64_t pr = (int64_t)part * CH_TR + in0 + l32;
+        s.ml[pr * 2] = m[u], s.ml[pr * 2 + 1] = lu;
+      }
+#pragma unroll
+      for (int hc = 0; hc < 2; ++hc) {
+        const int ln = (int)attn_lane();  // (nothing of this is kept through the loop before)
+        float *mine = out + (ln & 31) * HC + (ln >> 5) * 4;
+        const int turn = ln & (PAIRS - 1);
+#pragma unroll
+        for (int d = 0; d < DT / 2; ++d) {
+          f32x16_t x = acc[hc * (DT / 2) + d][u];
+          asm volatile("" : "+a"(x));  // (from the accumulation registers here, not all of them at once)
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            *(float4 *)(mine + ((d * 4 + v) ^ turn) * 8) =
+                make_float4(x[4 * v] * scale, x[4 * v + 1] * scale, x[4 * v + 2] * scale, x[4 * v + 3] * scale);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        if (hc == 0 && gated) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
-      }
 #pragma unroll 1
-      for (int it0 = 0; it0 < IT; it0 += AT_ONCE) {
-        uint4 gates[AT_ONCE];  // (asked for before the first is used)
-        int64_t rows[AT_ONCE];
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          int in, d0;
-          at(it0 + i, &in, &d0);
-          rows[i] = attn_row(a, rq.q0, t.row0 + in, head, g);
-          if (whole && a.gate && in < t.rows && d0 < a.D) gates[i] = attn_gate8(a, rows[i], d0);
-        }
-#pragma unroll
-        for (int i = 0; i < AT_ONCE; ++i) {
-          int in, d0;
-          const float *x = at(it0 + i, &in, &d0);
-          if (in >= t.rows || d0 >= a.D) continue;
+        for (int it = 0; it < IT; ++it) {
+          const uint32_t j = it * 64 + ln;
+          const int rr = (int)(j / PAIRS), k = (int)(j % PAIRS), in = in0 + rr, d0 = hc * HC + k * 8;
+          if (in >= t.rows || (!FULL && d0 >= a.D)) continue;
+          const float *x = out + rr * HC + (k ^ (rr & (PAIRS - 1))) * 8;
           float o[8];
           *(float4 *)&o[0] = *(const float4 *)x, *(float4 *)&o[4] = *(const float4 *)(x + 4);
+          if (*poison) attn_poison(a, rq, tabrow, head, t.row0 + in, ks, end, d0, o);
           if (whole) {
-            if (a.gate) attn_times_gate(gates[i], o);
-            attn_put8(a, rows[i], d0, o);
+            if (gated) attn_times_gate(*(const uint4 *)(lds + wv * TILE + TILE / 2 + (rr * DP + d0) * 2), o);
+            attn_put8(a, attn_row(a, rq.q0, t.row0 + in, head), d0, o);
           } else {
             float4 *to = (float4 *)(s.acc + ((int64_t)part * CH_TR + in) * DP + d0);
             to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
           }
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");  // (the gates are read before the next ones come)
     }
     }
     if constexpr (!FULL) {
       __syncthreads();
-      for (int j = tid; j < 4 * TILE / 16; j += ATTN_THREADS) ((uint4 *)lds)[j] = make_uint4(0, 0, 0, 0);
+      for (int j = here(); j < 4 * TILE / 16; j += ATTN_THREADS) ((uint4 *)lds)[j] = attn_zeros();
     }
   }
 }
@@ -528,7 +521,7 @@ hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int grid, hipStream_
 }  // namespace
 
 size_t attn_chunk_lds(int DP, int R) {
-  return 4 * ch_tile(DP) + CH_TAB + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
+  return 4 * ch_tile(DP) + CH_TAB + 16 * ATTN_THREADS + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
 }
 
 hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st) {

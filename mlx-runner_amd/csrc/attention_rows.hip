@@ -22,6 +22,7 @@ namespace qmm {
 namespace {
 
 constexpr int AR_WAVES = 4;
+constexpr int AR_EXTRA = 1;  // a tile's own overhead, in units of its keys
 constexpr int AR_TILE = 8192;  // bytes of a wave's tile of keys (and of values)
 constexpr int AR_STAGE = AR_WAVES * 2 * AR_TILE;
 constexpr int AR_TAB = AR_WAVES * 2 * 256;  // the next tile's page ids, two sets per wave
@@ -43,179 +44,237 @@ __device__ __forceinline__ void ar_wait() {
 
 // FULL: D = DP (else the lanes of chunks past D stay out of the DMA).
 template <int DP, int NQ, bool FULL>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnArgs a, const AttnShare s) {
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnArgs args, const AttnShare share) {
   constexpr int TR = 16 * NQ;
   constexpr int KW = AR_TILE / (2 * DP);  // keys of a wave's tile: 16, 32, 64
   constexpr int KT = AR_WAVES * KW;
   constexpr int CPR = DP / 8;             // 16-byte chunks of a row
+  constexpr int RPI = 64 / CPR;           // rows of a DMA operation
   constexpr int KB = KW / 16;             // 16-key blocks of a tile
-  constexpr int ST = DP / 32, DT = DP / 16;
+  constexpr int ST = DP / 32, DT = DP / 16, PITCH = 2 * DP;
   constexpr int OPS = AR_TILE / 1024;     // DMA operations of a tile
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   uint8_t *tab = lds + ar_fixed(DP);
-  uint32_t *scratch = (uint32_t *)(tab + AR_TAB);
-  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS), *poison = (int *)scratch + 15;
+  int *seen_at = (int *)(tab + AR_TAB);  // [thread][2][2]: what its rows see
+  uint32_t *scratch = (uint32_t *)(seen_at + 4 * ATTN_THREADS);
+  AttnWork *work = (AttnWork *)(scratch + ATTN_SCAN_LDS / 4);  // (this workgroup's share, out of the registers)
+  int *ends = (int *)((uint8_t *)work + sizeof(AttnWork)), *poison = (int *)scratch + 15;
 
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lr = lane & 15, lg = lane >> 4;
-  if (s.first) attn_zero_rest(a);
-  AttnWork w = attn_uniform(attn_share<TR, KT, 1>(a, s, ends, scratch));
-  attn_note_none(s, w);
-  const int g = a.Hq / a.Hkv;
-  const int wv = __builtin_amdgcn_readfirstlane(wave);
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto here = [&]() __attribute__((always_inline)) { return wv * 64 + (int)attn_lane(); };  // the thread's number
+  int left;
+  {
+    if (share.first) attn_zero_rest(args);
+    const AttnWork w = attn_uniform(attn_share<TR, KT, AR_EXTRA>(args, share, ends, scratch));
+    attn_note_none(share, w);
+    if (tid == 0) *work = w;
+    left = w.left;
+  }
   uint8_t *kl = lds + wv * 2 * AR_TILE, *vl = kl + AR_TILE;
   const uint32_t ka = lds_addr(kl), va = lds_addr(vl), ta = lds_addr(tab) + wv * 512;
   // head values past D: never written by the DMA, zero for good
   if constexpr (!FULL) {
-    for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = make_uint4(0, 0, 0, 0);
+    for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
   }
 
-  while (w.left > 0) {
-    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
-    const AttnReq rq = attn_uniform(attn_req(a, r, g));
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), TR, g);
-    const int cost = attn_units<KT>(t) + 1;
-    const int take = cost - w.u < w.left ? cost - w.u : w.left;
-    // (a tile's first unit stands for its own overhead)
-    const int u0 = w.u > 0 ? w.u - 1 : 0, u1 = w.u + take - 1;
-    const int ks = (t.b / KT + u0) * KT;
-    int ke = (t.b / KT + u1) * KT;
-    ke = ke < t.e ? ke : t.e;
-
+#pragma unroll 1
+  while (left > 0) {
     __syncthreads();  // (the last tile's merge is read; the zeros above are written)
-    if (tid == 0) *poison = 0;
+    const AttnArgs a = attn_again<AttnArgs>(0);
+    const AttnWork w = attn_uniform(*work);
+    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
+    const AttnReq rq = attn_uniform(attn_req(a, r));
+    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), TR);
+    const int units = attn_units<KT>(t);
+    const AttnPiece pc = attn_piece<AR_EXTRA>(w, units);
+    const bool whole = pc.whole;
+    const int ks = (int)(((uint32_t)t.b / KT + pc.u0) * KT), part = w.g * 2 + pc.start, head = w.head;
+    int ke = (int)(((uint32_t)t.b / KT + pc.u1) * KT);
+    ke = ke < t.e ? ke : t.e;
+    if (pc.start && !pc.none && here() == 0)
+      attn_note(attn_again<AttnShare>(sizeof(AttnArgs)), w, rq, t, units + AR_EXTRA, whole);
     __syncthreads();
-    // this wave's tiles: keys k0 = ks + KW (wave + 4 i)
+    {
+      AttnWork on = w;
+      attn_move_on(on, pc.take, units + AR_EXTRA);
+      left = on.left;
+      if (here() == 0) *work = on, *poison = 0;
+    }
+    __syncthreads();
+    if (pc.none) continue;
+
+    // This wave's tiles are the keys k0 = ks + KW (wave + 4 i), this lane's key of them the (lane % KW)th: `page`
+    // and `off` of the tile whose page ids are asked for next (held to the last page), `at` its place in its page.
+    const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
+    const uint16_t *kc = a.k, *vc = a.v;
     const int *tabrow = a.table + (int64_t)r * a.W;
-    auto page_at = [&](int k0) -> const int * {  // of this lane's key (held below e: a page of the row)
-      int key = k0 + (lane & (KW - 1));
-      key = key < t.e ? key : t.e - 1;
-      return tabrow + (uint32_t)key / (uint32_t)a.block;
-    };
+    int k0 = ks + KW * wv;
+    const uint32_t last_page = t.e > 0 ? attn_div(t.e - 1, a.by_block) : 0u;
+    const uint32_t first = k0 + (attn_lane() & (KW - 1));
+    uint32_t page = attn_div(first, a.by_block), off = first - page * block;
+    const int page0 = k0 < ke ? tabrow[page < last_page ? page : last_page] : 0;
+
     // the rows of this lane: what they see, their queries
-    int seen_b[NQ], seen_e[NQ];
+    float m[NQ], l[NQ];
+    const int ln0 = (int)attn_lane(), lr = ln0 & 15, lg = ln0 >> 4;
     bf16x8_t q[NQ][ST];
-    const uint32_t flip = a.scale < 0.f ? 0x80008000u : 0u;  // (a negative scale: -q, so that maxima stay maxima)
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      const int row = t.row0 + n * 16 + lr;
       const bool on = n * 16 + lr < t.rows;
-      const int tok = on ? row / g : 0, hh = on ? row - tok * g : 0;
-      const int pos = rq.base + tok;
-      seen_e[n] = on ? pos : -1;
-      seen_b[n] = a.window ? pos - a.window + 1 : 0;
-      const uint16_t *qp = a.q + (((int64_t)(rq.q0 + tok) * a.Hq) + w.head * g + hh) * a.D;
+      const int row = t.row0 + (on ? n * 16 + lr : 0);  // (a row past the end: the first one's queries, and no keys)
+      const int pos = rq.base + (int)attn_div(row, a.by_g);
+      seen_at[here() * 4 + 2 * n] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
+      seen_at[here() * 4 + 2 * n + 1] = on ? pos : -1;
+      m[n] = on && pos >= 0 ? -__builtin_inff() : 0.f;  // (a row that sees nothing needs no reference)
+      const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D + lg * 8;
 #pragma unroll
       for (int st = 0; st < ST; ++st) {
-        const int d0 = st * 32 + lg * 8;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (on && d0 < a.D && a.scale != 0.f) v = *(const uint4 *)(qp + d0);
-        v.x ^= flip, v.y ^= flip, v.z ^= flip, v.w ^= flip;
-        q[n][st] = __builtin_bit_cast(bf16x8_t, v);
+        if (FULL || st * 32 + lg * 8 < a.D)
+          q[n][st] = *(const bf16x8_t *)(qp + st * 32);
+        else
+          q[n][st] = __builtin_bit_cast(bf16x8_t, u32x4_t{0u, 0u, 0u, 0u});
       }
     }
-    int k0 = ks + KW * wv;
-    const int page0 = k0 < ke ? *page_at(k0) : 0;
+    if (!(a.scale > 0.f)) {  // a negative scale: -q, so that maxima stay maxima; none: no scores
+#pragma unroll
+      for (int n = 0; n < NQ; ++n)
+#pragma unroll
+        for (int st = 0; st < ST; ++st) {
+          u32x4_t x = __builtin_bit_cast(u32x4_t, q[n][st]);
+          x = a.scale < 0.f ? x ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
+          q[n][st] = __builtin_bit_cast(bf16x8_t, x);
+        }
+    }
     // all of the loads above, now: the compiler's own waits for them would come between the DMA's
     __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0)
     const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
 
     f32x4_t acc[NQ][DT];
-    float m[NQ], l[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
-      m[n] = -__builtin_inff(), l[n] = 0.f;
+      l[n] = 0.f;
 #pragma unroll
       for (int d = 0; d < DT; ++d) acc[n][d] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     }
 
-    // the row number (of the whole cache) of this lane's key, or row 0 where there is none
-    auto row_of = [&](int k0, int blk, bool *ok) -> uint32_t {
-      const int key = k0 + (lane & (KW - 1));
-      *ok = key < t.e && (uint32_t)blk < (uint32_t)a.NB;
-      const uint32_t off = (uint32_t)key % (uint32_t)a.block;
-      return *ok ? ((uint32_t)blk * a.Hkv + w.head) * a.block + off : 0u;
-    };
-    uint32_t rows[OPS];  // of the tile in the keys' buffer, per DMA operation
-    auto spread = [&](uint32_t mine) __attribute__((always_inline)) {
-#pragma unroll
-      for (int i = 0; i < OPS; ++i) rows[i] = __shfl(mine, (i * 64 + lane) / CPR, 64);
-    };
-    auto move = [&](const uint16_t *cache, uint32_t to) __attribute__((always_inline)) {
-      const int here = attn_opaque(lane);
-#pragma unroll
-      for (int i = 0; i < OPS; ++i) {
-        const int row = (i * 64 + here) / CPR, c = (i * 64 + here) % CPR ^ attn_swz<DP>(row);
-        if (FULL || c * 8 < a.D) gp_dma16(cache + (uint64_t)rows[i] * (uint32_t)a.D + c * 8, to + i * 1024);
-      }
-    };
-
     if (k0 < ke) {
-      bool ok;
-      uint32_t mine = row_of(k0, page0, &ok);
-      uint64_t valid = __ballot(ok);
-      spread(mine);
-      if (k0 + KT < ke) ar_dma4(page_at(k0 + KT), ta + 256);
-      move(a.k, ka);
-      move(a.v, va);
+      const uint32_t per = attn_div(KT, a.by_block), rest = KT - per * block;
+      uint32_t at = off;
+      auto onward = [&]() __attribute__((always_inline)) {
+        page += per, off += rest;
+        const uint32_t over = off >= (uint32_t)block;
+        off -= over ? block : 0, page += over;
+      };
+      auto ask = [&](int buf) __attribute__((always_inline)) {
+        ar_dma4(tabrow + (page < last_page ? page : last_page), ta + buf * 256);
+      };
+      // the row (of the whole cache) of this lane's key, 0 where there is none; a bit for each key that there is
+      uint32_t mine;
+      uint64_t valid;
+      auto rows_of = [&](int k, int blk) __attribute__((always_inline)) {
+        const bool ok = k + ((int)attn_lane() & (KW - 1)) < t.e && (uint32_t)blk < (uint32_t)NB;
+        mine = (((uint32_t)blk * Hkv + head) * block + at) & (ok ? ~0u : 0u);
+        valid = __ballot(ok);
+      };
+      // DMA operations: RPI rows each, chunk (lane % CPR) ^ swizzle
+      auto move = [&](const uint16_t *cache, uint32_t to) __attribute__((always_inline)) {
+        const uint32_t ln = attn_lane(), c0 = ln % CPR ^ (uint32_t)attn_swz<DP>((int)(ln / CPR));
+#pragma unroll
+        for (int i = 0; i < OPS; ++i) {
+          const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(ln / CPR * 4) + RPI * i * 4, (int)mine);
+          const uint32_t c = (c0 ^ (uint32_t)attn_swz<DP>(RPI * i)) * 16;
+          if (FULL || c < 2 * (uint32_t)D)
+            gp_dma16((const char *)cache + ((uint64_t)row * (2 * (uint32_t)D) + c), to + i * 1024);
+          if (i % 2) __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
+        }
+      };
+
+      rows_of(k0, page0);
+      onward();
+      at = off;
+      ask(1);
+      onward();
+      move(kc, ka);
+      move(vc, va);
       int buf = 1;
+#pragma unroll 1
       while (true) {
         const bool more = k0 + KT < ke;
         ar_wait<OPS>();  // the keys are here (and the next page ids, which were asked for before them)
-        const bool edge = k0 < t.full_b || k0 + KW > t.full_e || valid != ~0ull;
         const uint64_t now = valid;
+        const bool edge = k0 < t.full_b || k0 + KW > t.full_e || now != ~0ull;
         // S^T
         f32x4_t sv[NQ][KB];
+        {
+          const uint32_t ln = attn_lane();
+          const int row = ln & 15, from = row * PITCH + ((int)(ln >> 4) ^ attn_swz<DP>(row)) * 16;
+          auto load = [&](int j) __attribute__((always_inline)) {  // k step j % ST of block j / ST
+            return *(const bf16x8_t *)(kl + (from ^ (j % ST & 3) * 64) + (j % ST >> 2) * 256 + j / ST * 16 * PITCH);
+          };
+          bf16x8_t kf[KB * ST];
+          constexpr int AHEAD = NQ == 1 ? 4 : 2;
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
+          for (int j = 0; j < AHEAD && j < KB * ST; ++j) kf[j] = load(j);
 #pragma unroll
-          for (int n = 0; n < NQ; ++n) sv[n][b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-          const int row = b * 16 + lr, from = attn_opaque(row * (2 * DP) + (lg ^ attn_swz<DP>(row)) * 16);
+          for (int j = 0; j < KB * ST; ++j) {
+            if (j + AHEAD < KB * ST) kf[j + AHEAD] = load(j + AHEAD);
 #pragma unroll
-          for (int st = 0; st < ST; ++st) {
-            const bf16x8_t kf = *(const bf16x8_t *)(kl + (from ^ st * 64));
-#pragma unroll
-            for (int n = 0; n < NQ; ++n) sv[n][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(kf, q[n][st], sv[n][b], 0, 0, 0);
+            for (int n = 0; n < NQ; ++n)
+              sv[n][j / ST] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                  kf[j], q[n][j % ST], j % ST ? sv[n][j / ST] : f32x4_t{0.f, 0.f, 0.f, 0.f}, 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
           }
         }
         if (more) {  // the next keys into the buffer just read
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-          int blk = *(const int *)(tab + wv * 512 + buf * 256 + lane * 4);
-          mine = row_of(k0 + KT, blk, &ok);
-          valid = __ballot(ok);
-        }
-        if (more) {
+          const int blk = *(const int *)(tab + wv * 512 + buf * 256 + (int)attn_lane() * 4);
+          rows_of(k0 + KT, blk);
+          at = off;
           buf ^= 1;
-          if (k0 + 2 * KT < ke)
-            ar_dma4(page_at(k0 + 2 * KT), ta + buf * 256);
-          else
-            ar_dma4(page_at(k0), ta + buf * 256);  // (not read; the waits count on it)
-          spread(mine);
-          move(a.k, ka);
+          ask(buf);  // (past the end: not read; the waits count on it)
+          onward();
+          move(kc, ka);
         }
-        // the softmax's weights
+        if (edge) {
 #pragma unroll
-        for (int n = 0; n < NQ; ++n) {
-          if (edge) {
+          for (int n = 0; n < NQ; ++n) {
+            // bit o: key k0 + o is seen
+            const int *rows = seen_at + (wv * 64 + (int)attn_lane()) * 4 + 2 * n;
+            const int lo = rows[0] - k0, hi = rows[1] - k0;
+            uint64_t seen = hi < 0 ? 0ull : hi > 62 ? ~0ull : (2ull << hi) - 1ull;
+            seen &= lo > 63 ? 0ull : lo > 0 ? ~0ull << lo : ~0ull;
+            seen = (seen & now) >> (attn_lane() >> 4 << 2);
 #pragma unroll
             for (int b = 0; b < KB; ++b)
 #pragma unroll
               for (int i = 0; i < 4; ++i) {
-                const int o = b * 16 + lg * 4 + i, key = k0 + o;
-                if (!(key <= seen_e[n] && key >= seen_b[n] && (now >> o & 1))) sv[n][b][i] = -__builtin_inff();
+                const int on = __builtin_amdgcn_sbfe((int)(seen >> (b & ~1) * 16), (b & 1) * 16 + i, 1);  // 0 or -1
+                sv[n][b][i] = __uint_as_float((__float_as_uint(sv[n][b][i]) & (uint32_t)on) | (0xFF800000u & ~(uint32_t)on));
               }
           }
-          float top = sv[n][0][0];
+        }
+        // The weights' reference is the row's first maximum; it follows (and the sums with it) when a score passes
+        // it by 2^60: bf16 and f32 hold such weights as exactly as those below 1.
+        float top[NQ];
+        bool far = false;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          top[n] = sv[n][0][0];
 #pragma unroll
           for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) top = fmaxf(top, sv[n][b][i]);
-          top = fmaxf(top, __shfl_xor(top, 16, 64));
-          top = fmaxf(top, __shfl_xor(top, 32, 64)) * sc;
-          // the reference maximum follows only when it is passed by 2^8: the weights stay in range
-          if (__any(top > m[n] + 8.f)) {
-            const float mn = fmaxf(m[n], top);
-            const float f = mn == -__builtin_inff() ? 1.f : attn_exp2(m[n] - mn);
-            m[n] = mn;
+            for (int i = 0; i < 4; ++i) top[n] = fmaxf(top[n], sv[n][b][i]);
+          top[n] *= sc;
+          far |= top[n] > m[n] + 60.f;
+        }
+        if (__any(far)) {
+#pragma unroll
+          for (int n = 0; n < NQ; ++n) {
+            top[n] = fmaxf(top[n], attn_across(top[n], 16));
+            top[n] = fmaxf(top[n], attn_across(top[n], 32));
+            const bool up = top[n] > m[n] + 60.f;
+            const float f = up ? attn_exp2(m[n] - top[n]) : 1.f;
+            m[n] = up ? top[n] : m[n];
             l[n] *= f;
 #pragma unroll
             for (int d = 0; d < DT; ++d) acc[n][d] *= f;
@@ -228,10 +287,12 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
 #pragma unroll
           for (int b = 0; b < KB; ++b)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const __bf16 e = (__bf16)attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
-              l[n] += (float)e;
-              p[n][b][i] = __builtin_bit_cast(short, e);
+            for (int i = 0; i < 4; i += 2) {
+              bf16x2_t x;
+              x[0] = (__bf16)attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
+              x[1] = (__bf16)attn_exp2(__builtin_fmaf(sv[n][b][i + 1], sc, -ref));
+              l[n] = dot2_bf16(x, 0x3F803F80u, l[n]);
+              p[n][b][i] = __builtin_bit_cast(short, (__bf16)x[0]), p[n][b][i + 1] = __builtin_bit_cast(short, (__bf16)x[1]);
             }
         }
         // the values
@@ -243,114 +304,132 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           // keys that are none: zeros, whatever was loaded; values that are not finite, which must not reach
           // the rows that do not see their keys (0 inf is NaN): zeros for now
           bool odd = false;
-#pragma unroll
+#pragma unroll 1
           for (int i = 0; i < OPS; ++i) {
-            uint4 *at = (uint4 *)(vl + i * 1024 + lane * 16);
-            uint4 x = *at;
-            const bool in = now >> ((i * 64 + lane) / CPR) & 1;
-            const uint4 y = attn_finite(x);
+            const uint32_t lane = attn_lane();
+            uint4 *x4 = (uint4 *)(vl + i * 1024 + lane * 16);
+            const uint4 x = *x4, y = attn_finite(x);
+            const bool in = now >> ((uint32_t)(i * 64 + lane) / CPR) & 1;
             odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
-            *at = in ? y : make_uint4(0, 0, 0, 0);
+            const uint32_t keep = in ? ~0u : 0u;
+            *x4 = make_uint4(y.x & keep, y.y & keep, y.z & keep, y.w & keep);
           }
           if (__any(odd)) *poison = 1;
         }
-        // (this lane's place in the 16 x 16 block (b, 0) of the values)
-        int from[KB];
+        {
+          const uint32_t ln = attn_lane();
+          const int row = (int)((ln >> 4) * 4 + (ln >> 2 & 3));
+          // this lane's place in the 16 x 16 block (b, d) of the values
+          const uint32_t from = va + row * PITCH + ((int)(ln >> 1 & 1) ^ attn_swz<DP>(row)) * 16 + (ln & 1) * 8;
+          // (16 rows on, the swizzle is the same)
+          constexpr int CB = KB == 1 ? 1 : KB / 2, N = DT * CB, AHEAD = NQ == 1 ? 2 : 1;
+          auto load = [&](int j) __attribute__((always_inline)) {  // key blocks 2 (j % CB) and the next, columns j / CB
+            const int d = j / CB, b = j % CB * 2;
+            const uint32_t x = (from ^ (d & 7) * 32) + (d >> 3) * 256 + b * 16 * PITCH;
+            i16x8_t v{};
+            const i16x4_t v0 = attn_read_tr(x);
+            if constexpr (KB > 1) {
+              const i16x4_t v1 = attn_read_tr(x + 16 * PITCH);
+              v = __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+              v = __builtin_shufflevector(v0, v0, 0, 1, 2, 3, 0, 1, 2, 3);
+            }
+            return v;
+          };
+          i16x8_t vf[N];
 #pragma unroll
-        for (int b = 0; b < KB; ++b) {
-          const int row = b * 16 + lg * 4 + (lr >> 2);
-          from[b] = attn_opaque(row * (2 * DP) + ((lane >> 1 & 1) ^ attn_swz<DP>(row)) * 16 + (lane & 1) * 8);
-        }
+          for (int j = 0; j < AHEAD; ++j) vf[j] = load(j);
 #pragma unroll
-        for (int d = 0; d < DT; ++d) {
-          auto col = [&](int b) __attribute__((always_inline)) { return attn_read_tr(va + (from[b] ^ d * 32)); };
-          if constexpr (KB == 1) {
-            const i16x4_t vf = col(0);
+          for (int j = 0; j < N; ++j) {
+            if (j + AHEAD < N) vf[j + AHEAD] = load(j + AHEAD);
+            const int d = j / CB, b = j % CB * 2;
 #pragma unroll
-            for (int n = 0; n < NQ; ++n)
-              acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(vf, p[n][0], acc[n][d], 0, 0, 0);
-          } else {
-#pragma unroll
-            for (int b = 0; b < KB; b += 2) {
-              const i16x8_t vf = __builtin_shufflevector(col(b), col(b + 1), 0, 1, 2, 3, 4, 5, 6, 7);
-#pragma unroll
-              for (int n = 0; n < NQ; ++n) {
+            for (int n = 0; n < NQ; ++n) {
+              if constexpr (KB == 1) {
+                const i16x4_t v0 = __builtin_shufflevector(vf[j], vf[j], 0, 1, 2, 3);
+                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v0, p[n][0], acc[n][d], 0, 0, 0);
+              } else {
                 const i16x8_t pf = __builtin_shufflevector(p[n][b], p[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
-                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf),
+                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[j]),
                                                                     __builtin_bit_cast(bf16x8_t, pf), acc[n][d], 0, 0, 0);
               }
             }
+            if (j % 2) __builtin_amdgcn_sched_barrier(0);
           }
         }
         if (!more) break;
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-        move(a.v, va);
+        move(vc, va);
         k0 += KT;
       }
     }
 
     // the four waves' parts, 16 rows at a time through the stage's LDS
-    const bool whole = take == cost;
-    const int part = w.g * 2 + (w.u == 0 ? 1 : 0);
-    if (w.u == 0 && tid == 0) attn_note(s, w, rq, t, cost, whole);
-    float *macc = (float *)lds;                                  // [wave][16][DP + 4]
-    float *mml = (float *)(lds + AR_WAVES * 16 * (DP + 4) * 4);  // [wave][16][2]
+    {
+      const AttnArgs a = attn_again<AttnArgs>(0);
+      const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
+      float *macc = (float *)lds;                                  // [wave][16][DP + 4]
+      float *mml = (float *)(lds + AR_WAVES * 16 * (DP + 4) * 4);  // [wave][16][2]
 #pragma unroll
-    for (int n = 0; n < NQ; ++n) {
-      if (n * 16 >= t.rows) break;
-      __syncthreads();
-      l[n] += __shfl_xor(l[n], 16, 64);
-      l[n] += __shfl_xor(l[n], 32, 64);
-      if (lg == 0) mml[(wave * 16 + lr) * 2] = m[n], mml[(wave * 16 + lr) * 2 + 1] = l[n];
+      for (int n = 0; n < NQ; ++n) {
+        if (n * 16 >= t.rows) break;
+        __syncthreads();
+        l[n] += attn_across(l[n], 16);
+        l[n] += attn_across(l[n], 32);
+        const int ln = (int)attn_lane(), lr = ln & 15, lg = ln >> 4;
+        if (lg == 0) mml[(wv * 16 + lr) * 2] = m[n], mml[(wv * 16 + lr) * 2 + 1] = l[n];
 #pragma unroll
-      for (int d = 0; d < DT; ++d) *(f32x4_t *)(macc + (wave * 16 + lr) * (DP + 4) + d * 16 + lg * 4) = acc[n][d];
-      __syncthreads();
-      for (int i = tid; i < 16 * CPR; i += ATTN_THREADS) {
-        const int row = i / CPR, d0 = i % CPR * 8;
-        if (n * 16 + row >= t.rows || d0 >= a.D) continue;
-        float top = -__builtin_inff(), f[AR_WAVES], sum = 0.f, o[8];
+        for (int d = 0; d < DT; ++d) *(f32x4_t *)(macc + (wv * 16 + lr) * (DP + 4) + d * 16 + lg * 4) = acc[n][d];
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t i = here(); i < 16 * CPR; i += ATTN_THREADS) {
+          const int row = (int)(i / CPR), d0 = (int)(i % CPR * 8);
+          if (n * 16 + row >= t.rows || d0 >= D) continue;
+          const int64_t orow = attn_row(a, rq.q0, t.row0 + n * 16 + row, head);
+          uint4 gate = attn_zeros();
+          const bool gated = whole && a.gate;
+          if (gated) gate = attn_gate8(a, orow, d0);
+          float top = -__builtin_inff(), f[AR_WAVES], sum = 0.f, o[8];
 #pragma unroll
-        for (int v = 0; v < AR_WAVES; ++v) top = fmaxf(top, mml[(v * 16 + row) * 2]);
+          for (int v = 0; v < AR_WAVES; ++v) {
+            // (a wave without keys for this row has no sums)
+            const float mv = mml[(v * 16 + row) * 2];
+            f[v] = mml[(v * 16 + row) * 2 + 1] != 0.f ? mv : -__builtin_inff();
+            top = fmaxf(top, f[v]);
+          }
 #pragma unroll
-        for (int v = 0; v < AR_WAVES; ++v) {
-          const float mv = mml[(v * 16 + row) * 2];
-          f[v] = mv == -__builtin_inff() ? 0.f : attn_exp2(mv - top);
-          sum += f[v] * mml[(v * 16 + row) * 2 + 1];
-        }
+          for (int v = 0; v < AR_WAVES; ++v) {
+            f[v] = f[v] == -__builtin_inff() ? 0.f : attn_exp2(f[v] - top);
+            sum += f[v] * mml[(v * 16 + row) * 2 + 1];
+          }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = 0.f;
+          for (int e = 0; e < 8; ++e) o[e] = 0.f;
 #pragma unroll
-        for (int v = 0; v < AR_WAVES; ++v) {
-          const float4 x = *(const float4 *)(macc + (v * 16 + row) * (DP + 4) + d0);
-          const float4 y = *(const float4 *)(macc + (v * 16 + row) * (DP + 4) + d0 + 4);
-          o[0] += f[v] * x.x, o[1] += f[v] * x.y, o[2] += f[v] * x.z, o[3] += f[v] * x.w;
-          o[4] += f[v] * y.x, o[5] += f[v] * y.y, o[6] += f[v] * y.z, o[7] += f[v] * y.w;
-        }
-        if (*poison) attn_poison(a, rq, tabrow, w.head, t.row0 + n * 16 + row, g, ks, ke, d0, o);
-        if (whole) {
-          const float inv = sum != 0.f ? 1.f / sum : 0.f;
+          for (int v = 0; v < AR_WAVES; ++v) {
+            const float4 x = *(const float4 *)(macc + (v * 16 + row) * (DP + 4) + d0);
+            const float4 y = *(const float4 *)(macc + (v * 16 + row) * (DP + 4) + d0 + 4);
+            o[0] += f[v] * x.x, o[1] += f[v] * x.y, o[2] += f[v] * x.z, o[3] += f[v] * x.w;
+            o[4] += f[v] * y.x, o[5] += f[v] * y.y, o[6] += f[v] * y.z, o[7] += f[v] * y.w;
+          }
+          if (*poison) attn_poison(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, o);
+          if (whole) {
+            const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
-          for (int e = 0; e < 8; ++e) o[e] *= inv;
-          attn_store8(a, attn_row(a, rq.q0, t.row0 + n * 16 + row, w.head, g), d0, o);
-        } else {
-          const int64_t pr = (int64_t)part * TR + n * 16 + row;
-          float4 *to = (float4 *)(s.acc + pr * DP + d0);
-          to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
-          if (d0 == 0) s.ml[pr * 2] = top, s.ml[pr * 2 + 1] = sum;
+            for (int e = 0; e < 8; ++e) o[e] *= inv;
+            if (gated) attn_times_gate(gate, o);
+            attn_put8(a, orow, d0, o);
+          } else {
+            const int64_t pr = (int64_t)part * TR + n * 16 + row;
+            float4 *to = (float4 *)(s.acc + pr * DP + d0);
+            to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
+            if (d0 == 0) s.ml[pr * 2] = top, s.ml[pr * 2 + 1] = sum;
+          }
         }
       }
     }
     if constexpr (!FULL) {  // the merge has overwritten the zeros past D
       __syncthreads();
-      for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = make_uint4(0, 0, 0, 0);
-    }
-
-    w.left -= take;
-    w.at += take;
-    w.u += take;
-    if (w.u == cost) {
-      w.u = 0;
-      if (++w.tile == w.tiles) w.tile = 0, ++w.head;
+      for (int i = here(); i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
     }
   }
 }
@@ -373,7 +452,9 @@ hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int tr, int grid, hi
 
 }  // namespace
 
-size_t attn_rows_lds(int DP, int R) { return ar_fixed(DP) + AR_TAB + ATTN_SCAN_LDS + (size_t)R * 4; }
+size_t attn_rows_lds(int DP, int R) {
+  return ar_fixed(DP) + AR_TAB + 16 * ATTN_THREADS + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
+}
 
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st) {
   return DP == 64 ? launch_dp<64>(a, s, tr, grid, st)

@@ -213,13 +213,20 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t st);
 
 // Attention of the requests' new tokens over their pages.
 constexpr int ATTN_MAX_R = 4096;
+// n / d for n < 2^31 as the high half of 2 n * mul, shifted.
+struct FastDiv {
+  uint32_t mul, shift;
+};
 struct AttnArgs {
   const uint16_t *q, *k, *v, *gate;  // q [T, Hq, D]; pages [NB, Hkv, block, D]; gate [T, Hq, Dg] (its last D) or null
   uint16_t *o;
   const int *table, *q_starts, *kv_lens;
   int T, R, W, Hq, Hkv, D, Dg, NB, block, window;
   float scale;
+  int g;                 // query heads of a key head
+  FastDiv by_g, by_block;  // (set by the launch)
 };
+const char *attention_limits(const AttnArgs &a);
 size_t attention_workspace(const AttnArgs &a);
 hipError_t launch_attention(const AttnArgs &a, void *workspace, hipStream_t st);
 

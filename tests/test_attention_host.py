@@ -1,6 +1,8 @@
 """Attention operators without a GPU: what they refuse, and the rotation's frequencies."""
 import math
+import re
 from ctypes import byref, c_int, c_void_p
+from pathlib import Path
 
 import numpy as np
 import pytest
@@ -87,6 +89,7 @@ CACHE = (NB, Hkv, BS, D)
     (dict(k=arr((T, Hkv + 1, D))), "k and v must be [4, 2, 64]"),
     (dict(v=arr((T + 1, Hkv, D))), "k and v must be [4, 2, 64]"),
     (dict(v=Q.Array()), "missing input"),
+    (dict(k_cache=arr((1 << 21, Hkv, 1 << 10, D))), "over 2^32 - 1 keys"),
     (dict(slots=ints(T - 1)), "slots must be an array of shape [4]"),
     (dict(q_norm=arr((D - 8,))), "q_norm must be [64]"),
     (dict(k_norm=arr((D,), Q.UINT8)), "k_norm must be [64]"),
@@ -115,6 +118,9 @@ def test_rope_cache_refuses_to_overwrite_a_wider_q():
     (dict(v_cache=arr((NB + 1, Hkv, BS, D))), "shapes differ"),
     (dict(k_cache=arr((NB, Hkv, BS, 12)), v_cache=arr((NB, Hkv, BS, 12))), "got 12"),
     (dict(table=ints(R)), "table must be"),
+    (dict(v_cache=arr((1 << 20, 1 << 7, 1 << 5, D))), "over 2^32 - 1 keys"),
+    (dict(table=ints(R, 2 ** 31 - 1)), "too many keys of all tiles"),
+    (dict(q=arr((1 << 27, Hq, D))), "too many rows per key head"),
     (dict(q_starts=ints(R)), "q_starts must be an array of shape [4]"),
     (dict(kv_lens=ints(R + 1)), "kv_lens must be an array of shape [3]"),
     (dict(kv_lens=arr((R,), Q.UINT32)), "kv_lens must be int32"),
@@ -138,6 +144,19 @@ def test_null_results_are_refused():
     res = Q.qmm_array(None)
     assert Q.lib.qmm_rope_cache(byref(res), *[null] * 8, 1.0, False, null, null, 1e-6, Q.qmm_stream(None)) != 0
     assert not res.ctx
+
+
+def test_no_vector_register_of_the_attention_kernels_is_spilled():
+    """hipcc has put spills before the point where a divergent region's lanes come back (the lanes that were out
+    then reload what they never stored), so these kernels are kept to their registers."""
+    lib = Path(Q.lib._name).read_bytes()
+    found = {}
+    for m in re.finditer(rb"\.symbol[\xa0-\xda](.{1,400}?)\.kd.{0,400}?\.vgpr_spill_count(.)", lib, re.S):
+        name = m.group(1).decode("latin-1")
+        if "attn_" in name:
+            found[name] = m.group(2)[0]
+    assert sum("attn_rows_kernel" in n for n in found) == 12 and sum("attn_chunk_kernel" in n for n in found) == 6
+    assert not {n: c for n, c in found.items() if c}
 
 
 # ---------------------------------------------------------------- frequencies
