@@ -18,14 +18,30 @@ namespace {
 
 constexpr int ROPE_THREADS = 256;
 
+// Eight values as they lie in memory.
 template <bool F32>
-__device__ __forceinline__ void load8(const void *p, int64_t i, float (&o)[8]) {
+struct Eight {
+  uint4 w[F32 ? 2 : 1];
+};
+template <bool F32>
+__device__ __forceinline__ Eight<F32> load8(const void *p, int64_t i) {
+  Eight<F32> x;
   if constexpr (F32) {
-    const float4 a = ((const float4 *)((const float *)p + i))[0], b = ((const float4 *)((const float *)p + i))[1];
-    o[0] = a.x, o[1] = a.y, o[2] = a.z, o[3] = a.w, o[4] = b.x, o[5] = b.y, o[6] = b.z, o[7] = b.w;
+    x.w[0] = ((const uint4 *)((const float *)p + i))[0];
+    x.w[1] = ((const uint4 *)((const float *)p + i))[1];
   } else {
-    const uint4 a = *(const uint4 *)((const uint16_t *)p + i);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+    x.w[0] = *(const uint4 *)((const uint16_t *)p + i);
+  }
+  return x;
+}
+template <bool F32>
+__device__ __forceinline__ void widen(const Eight<F32> &x, float (&o)[8]) {
+  if constexpr (F32) {
+    const uint32_t w[8] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w, x.w[1].x, x.w[1].y, x.w[1].z, x.w[1].w};
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(w[j]);
+  } else {
+    const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
       o[2 * j] = __uint_as_float(w[j] << 16);
@@ -43,116 +59,171 @@ __device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8]) 
   } else {
     uint32_t w[4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) w[j] = f32_to_bf16_rne(v[2 * j]) | (uint32_t)f32_to_bf16_rne(v[2 * j + 1]) << 16;
+    for (int j = 0; j < 4; ++j) {
+      bf16x2_t x;
+      x[0] = (__bf16)v[2 * j], x[1] = (__bf16)v[2 * j + 1];
+      w[j] = __builtin_bit_cast(uint32_t, x);
+    }
     *(uint4 *)((uint16_t *)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
   }
 }
 
-// LPH: lanes of a head, the power of two from D / 8 up (8, 16 or 32).
-template <int LPH, bool IN_F32, bool OUT_F32>
-__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(const RopeArgs a, int parts) {
-  constexpr int G = ROPE_THREADS / LPH;  // heads in flight
-  __shared__ float cs[128], sn[128];
-  __shared__ float swap[G][8][LPH];  // [value of the lane][lane]
-  const int tid = threadIdx.x, l = tid % LPH, g = tid / LPH;
+// Where the pairs of a head lie: both sides (HALVES) or all (NEXT) in a lane's 16 values, or anywhere.
+enum { HALVES, NEXT, ACROSS };
+
+// lph: log2 of a head's lanes (16 values each); a wave takes heads of one set only.
+template <int PAIRS, bool IN_F32, bool OUT_F32>
+__global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(const RopeArgs a, int lph, int parts) {
+  constexpr int WAVES = ROPE_THREADS / 64;
+  constexpr int TURNS = IN_F32 ? 1 : 2;  // loads of so many heads in flight per lane
+  __shared__ __attribute__((aligned(16))) float cs[128], sn[128], norm[ROPE_MAX_SETS][256];
+  __shared__ __attribute__((aligned(16))) float swap[PAIRS == ACROSS ? ROPE_THREADS * 16 : 4];
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l = tid & ((1 << lph) - 1), g = (tid & 63) >> lph, hpw = 64 >> lph;
   const int t = blockIdx.x / parts, part = blockIdx.x - t * parts;
-  int heads = 0;
-  for (int i = 0; i < a.sets; ++i) heads += a.set[i].heads;
-  const int d0 = l * 8;
-  const bool live = d0 < a.D;
-  const int pos = a.positions ? a.positions[t] : 0;
+  // the lane's two chunks of eight values: both sides of eight pairs, or neighbours
+  const bool turned = PAIRS != ACROSS && l < a.half / 8;
+  const int d0 = (PAIRS == HALVES && turned ? l : 2 * l) * 8, d1 = PAIRS == HALVES && turned ? d0 + a.half : d0 + 8;
+  const bool in0 = d0 < a.D, in1 = d1 < a.D;
+
+  // wave item i -> its set, its first head there
+  auto which = [&](int &i) __attribute__((always_inline)) -> int {
+    int set = 0, n;
+    while (set < a.sets && i >= (n = (a.set[set].heads + hpw - 1) >> (6 - lph))) i -= n, ++set;
+    i *= hpw;
+    return set;
+  };
+  Eight<IN_F32> raw[TURNS][2];
+  auto fetch = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+      int h = i0 + u * parts * WAVES;
+      const int set = which(h);
+      if (set == a.sets) break;
+      const RopeHeads &s = a.set[set];
+      if (h + g >= s.heads) continue;
+      const int64_t at = ((int64_t)t * s.heads + h + g) * s.in_stride;
+      if (in0) raw[u][0] = load8<IN_F32>(s.in, at + d0);
+      if (in1) raw[u][1] = load8<IN_F32>(s.in, at + d1);
+    }
+  };
+  // everything that is read on its way before the first is waited for
+  int i0 = part * WAVES + wv;
+  const int pos = a.positions[t];
   const int slot = a.slots ? a.slots[t] : -1;
+  const float freq = tid < a.half ? a.freqs[tid] : 0.f;
+  float nw[ROPE_MAX_SETS];
+#pragma unroll
+  for (int i = 0; i < ROPE_MAX_SETS; ++i) {
+    nw[i] = 0.f;
+    if (i < a.sets && a.set[i].norm && tid < a.D)
+      nw[i] = a.set[i].norm_f32 ? ((const float *)a.set[i].norm)[tid]
+                                : __uint_as_float((uint32_t)((const uint16_t *)a.set[i].norm)[tid] << 16);
+  }
+  fetch(i0);
 
   if (tid < a.half) {
     // in turns and in 64 bits: at position 2^18 an f32 product is off by up to 2^-7 rad
-    double turns = (double)pos * (double)a.freqs[tid] * 0.15915494309189533577;
+    double turns = (double)pos * (double)freq * 0.15915494309189533577;
     turns -= __builtin_rint(turns);
     float s, c;
     sincospif(2.f * (float)turns, &s, &c);
     cs[tid] = c * a.amplitude;
     sn[tid] = s * a.amplitude * a.sign;
   }
+#pragma unroll
+  for (int i = 0; i < ROPE_MAX_SETS; ++i) norm[i][tid] = nw[i];
   __syncthreads();
+  float c[8], sv[8];  // of the lane's pairs
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = sv[j] = 0.f;
+  if (turned) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4)
+      *(float4 *)&c[j] = *(const float4 *)&cs[l * 8 + j], *(float4 *)&sv[j] = *(const float4 *)&sn[l * 8 + j];
+  }
 
-  for (int h0 = part * G; h0 < heads; h0 += parts * G) {
-    const int head = h0 + g;
-    const bool on = head < heads;
-    RopeHeads s = a.set[0];
-    int h = head;
-    for (int i = 1; i < a.sets; ++i)
-      if (h >= s.heads) h -= s.heads, s = a.set[i];
-    float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-    if (on && live) load8<IN_F32>(s.in, ((int64_t)t * s.heads + h) * s.in_stride + d0, x);
-    if (s.norm) {
-      float sq = 0.f;
+  const int page = slot / a.block;
+  const bool kept = slot >= 0 && page < a.NB;
+  while (true) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) sq = __builtin_fmaf(x[j], x[j], sq);
+    for (int u = 0; u < TURNS; ++u) {
+      int h = i0 + u * parts * WAVES;
+      const int set = which(h);
+      if (set == a.sets) return;
+      const RopeHeads &s = a.set[set];
+      const bool on = h + g < s.heads;
+      float x[2][8];
 #pragma unroll
-      for (int off = LPH / 2; off >= 1; off >>= 1) sq += __shfl_xor(sq, off, LPH);
-      const float r = 1.f / sqrtf(sq / (float)a.D + a.eps);
-      float w[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-      if (live) {
-        if (s.norm_f32)
-          load8<true>(s.norm, d0, w);
-        else
-          load8<false>(s.norm, d0, w);
-      }
+      for (int k = 0; k < 2; ++k) widen<IN_F32>(raw[u][k], x[k]);
+      if (s.norm) {
+        float sq[2] = {0.f, 0.f};
 #pragma unroll
-      for (int j = 0; j < 8; ++j) x[j] = x[j] * r * w[j];
-    }
-    if (a.interleaved) {
-      if (s.rotate) {
+        for (int k = 0; k < 2; ++k)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          const int i = l * 4 + j;
-          if (i < a.half) {
-            const float c = cs[i], sv = sn[i], u = x[2 * j], v = x[2 * j + 1];
-            x[2 * j] = u * c - v * sv;
-            x[2 * j + 1] = u * sv + v * c;
+          for (int j = 0; j < 8; ++j) sq[k] = __builtin_fmaf(x[k][j], x[k][j], sq[k]);
+        float sum = (in0 ? sq[0] : 0.f) + (in1 ? sq[1] : 0.f);
+        for (int off = 1 << lph >> 1; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+        const float r = 1.f / sqrtf(sum / (float)a.D + a.eps);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) {
+            const float4 w = *(const float4 *)&norm[set][((k ? d1 : d0) & 255) + j];
+            x[k][j] *= r * w.x, x[k][j + 1] *= r * w.y, x[k][j + 2] *= r * w.z, x[k][j + 3] *= r * w.w;
           }
-        }
       }
-    } else {
-      // (the lanes of a head are lanes of one wave: no barrier, the LDS unit keeps their order)
-#pragma unroll
-      for (int j = 0; j < 8; ++j) swap[g][j][l] = x[j];
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
-      if (s.rotate) {
+      if (PAIRS != ACROSS && s.rotate && turned) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-          const int d = d0 + j;
-          if (d < 2 * a.half) {
-            const bool lo = d < a.half;
-            const int i = lo ? d : d - a.half, e = lo ? d + a.half : i;
-            const float other = swap[g][e & 7][e >> 3];
-            x[j] = lo ? x[j] * cs[i] - other * sn[i] : other * sn[i] + x[j] * cs[i];
-          }
+          float &p = PAIRS == NEXT ? x[j >> 2][(j & 3) * 2] : x[0][j], &q = PAIRS == NEXT ? x[j >> 2][(j & 3) * 2 + 1] : x[1][j];
+          const float v = p;
+          p = v * c[j] - q * sv[j], q = v * sv[j] + q * c[j];
         }
       }
-      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      __builtin_amdgcn_wave_barrier();
+      if (PAIRS == ACROSS && s.rotate) {  // (a head's lanes are lanes of one wave: no barrier)
+        float *mine = swap + (tid >> lph << lph) * 16;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; j += 4) *(float4 *)&mine[(2 * l + k) * 8 + j] = *(float4 *)&x[k][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        const bool next = a.interleaved;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            const int d = (2 * l + k) * 8 + j;
+            if (d >= 2 * a.half) continue;
+            const bool first = next ? j % 2 == 0 : d < a.half;
+            const int i = next ? d / 2 : first ? d : d - a.half;
+            const float other = mine[next ? d ^ 1 : first ? d + a.half : i];
+            x[k][j] = first ? x[k][j] * cs[i] - other * sn[i] : other * sn[i] + x[k][j] * cs[i];
+          }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+      }
+      if (!on || (s.cache && !kept)) continue;
+      const int64_t at = s.cache ? (((int64_t)page * s.heads + h + g) * a.block + (slot - page * a.block)) * a.D
+                                 : ((int64_t)t * s.heads + h + g) * a.D;
+      if (in0) store8<OUT_F32>(s.out, at + d0, x[0]);
+      if (in1) store8<OUT_F32>(s.out, at + d1, x[1]);
     }
-    if (!(on && live)) continue;
-    if (s.cache) {
-      const int page = slot / a.block;
-      if (slot >= 0 && page < a.NB)
-        store8<OUT_F32>(s.out, (((int64_t)page * s.heads + h) * a.block + (slot - page * a.block)) * a.D + d0, x);
-    } else {
-      store8<OUT_F32>(s.out, ((int64_t)t * s.heads + h) * a.D + d0, x);
-    }
+    i0 += TURNS * parts * WAVES;
+    fetch(i0);
   }
 }
 
-template <int LPH>
-void launch_lph(const RopeArgs &a, unsigned grid, int parts, hipStream_t st) {
+template <int PAIRS>
+void launch_pairs(const RopeArgs &a, unsigned grid, int lph, int parts, hipStream_t st) {
   const dim3 g(grid), b(ROPE_THREADS);
   if (a.in_f32 && a.out_f32)
-    hipLaunchKernelGGL((rope_kernel<LPH, true, true>), g, b, 0, st, a, parts);
+    hipLaunchKernelGGL((rope_kernel<PAIRS, true, true>), g, b, 0, st, a, lph, parts);
   else if (a.in_f32)
-    hipLaunchKernelGGL((rope_kernel<LPH, true, false>), g, b, 0, st, a, parts);
+    hipLaunchKernelGGL((rope_kernel<PAIRS, true, false>), g, b, 0, st, a, lph, parts);
   else
-    hipLaunchKernelGGL((rope_kernel<LPH, false, false>), g, b, 0, st, a, parts);
+    hipLaunchKernelGGL((rope_kernel<PAIRS, false, false>), g, b, 0, st, a, lph, parts);
 }
 
 }  // namespace
@@ -161,19 +232,22 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t st) {
   if (a.T <= 0 || a.D < 8 || a.D > 256 || a.D % 8 || a.half < 0 || 2 * a.half > a.D || a.sets < 1 ||
       a.sets > ROPE_MAX_SETS || (!a.in_f32 && a.out_f32) || a.block < 1)
     return hipErrorInvalidValue;
-  int64_t heads = 0;
-  for (int i = 0; i < a.sets; ++i) heads += a.set[i].heads;
-  if (heads <= 0) return hipSuccess;
-  if (heads > INT32_MAX / 2) return hipErrorInvalidValue;
-  const int lph = a.D <= 64 ? 8 : a.D <= 128 ? 16 : 32;
+  const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
+  int64_t items = 0;  // of a wave
+  for (int i = 0; i < a.sets; ++i) {
+    if (a.set[i].heads > INT32_MAX / 4) return hipErrorInvalidValue;
+    items += (a.set[i].heads + (64 >> lph) - 1) >> (6 - lph);
+  }
+  if (items == 0) return hipSuccess;
   // few tokens: a token's heads over several workgroups
-  const int64_t turns = (heads * lph + ROPE_THREADS - 1) / ROPE_THREADS;
+  const int64_t turns = (items + ROPE_THREADS / 64 - 1) / (ROPE_THREADS / 64);
   int64_t parts = 1024 / a.T;
   parts = parts < 1 ? 1 : parts > turns ? turns : parts;
   if (a.T * parts > INT32_MAX) return hipErrorInvalidValue;
   const unsigned grid = (unsigned)(a.T * parts);
-  lph == 8 ? launch_lph<8>(a, grid, (int)parts, st)
-           : lph == 16 ? launch_lph<16>(a, grid, (int)parts, st) : launch_lph<32>(a, grid, (int)parts, st);
+  a.half % 8    ? launch_pairs<ACROSS>(a, grid, lph, (int)parts, st)
+  : a.interleaved ? launch_pairs<NEXT>(a, grid, lph, (int)parts, st)
+                  : launch_pairs<HALVES>(a, grid, lph, (int)parts, st);
   return hipGetLastError();
 }
 
