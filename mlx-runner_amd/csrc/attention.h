@@ -94,16 +94,22 @@ __device__ __forceinline__ int attn_units(const AttnTile &t) {
   return t.e > t.b ? (int)(((uint32_t)t.e + KT - 1) / KT - (uint32_t)t.b / KT) : 0;
 }
 
-// Inclusive sum over the workgroup; the total too.
+// Inclusive sum over the wave's lanes: over each row of 16, then the rows before.
+__device__ __forceinline__ uint32_t attn_wave_scan(uint32_t v) {
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x111, 0xF, 0xF, false);  // row_shr:1, 2, 4, 8
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x112, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x114, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x118, 0xF, 0xF, false);
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x142, 0xA, 0xF, false);  // row_bcast:15 into rows 1, 3
+  v += (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, 0x143, 0xC, 0xF, false);  // row_bcast:31 into rows 2, 3
+  return v;
+}
+// Over the workgroup; the total too.
 __device__ __forceinline__ uint32_t attn_scan(uint32_t v, uint32_t *waves, uint32_t *total) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const uint32_t u = __shfl_up(v, off, 64);
-    if (lane >= off) v += u;
-  }
+  const int wave = threadIdx.x >> 6;
+  v = attn_wave_scan(v);
   __syncthreads();
-  if (lane == 63) waves[wave] = v;
+  if ((threadIdx.x & 63) == 63) waves[wave] = v;
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
@@ -115,12 +121,46 @@ __device__ __forceinline__ uint32_t attn_scan(uint32_t v, uint32_t *waves, uint3
   return before + v;
 }
 
-// The first r with ends[r] > i.
-__device__ __forceinline__ int attn_find(const int *ends, int n, int i) {
-  int lo = 0, hi = n - 1;
+// A workgroup's share: `left` units from unit `u` of (head, tile) on, request r's.  Of `groups` workgroups the first
+// `longer` have one unit more than the others.
+struct AttnWork {
+  int g, groups, share, longer;
+  int tiles;         // per head
+  uint32_t at;       // the place of unit `u` in the line of all units
+  int head, tile, r;
+  int u, left;
+};
+
+// A workgroup's LDS for this, [R] ends of the requests' tiles behind it: with the requests themselves up to ATTN_KEPT.
+constexpr int ATTN_KEPT = 256;
+struct __attribute__((aligned(16))) AttnPlan {
+  AttnWork work[2];     // this segment's, the next one's: out of the registers
+  uint32_t waves[4], found[3];
+  uint16_t owner[64];   // a tile's request, and its number there
+  int poison[2], redo;
+};
+inline __host__ __device__ size_t attn_plan_lds(int R) { return sizeof(AttnPlan) + (size_t)R * (R <= ATTN_KEPT ? 16 : 4); }
+
+__device__ __forceinline__ int attn_end(const AttnPlan *plan, int R, int r) {
+  return ((const int *)(plan + 1))[R <= ATTN_KEPT ? 4 * r : r];
+}
+__device__ __forceinline__ void attn_keep(AttnPlan *plan, int R, int r, uint32_t end, const AttnReq &q) {
+  if (R <= ATTN_KEPT)
+    ((int4 *)(plan + 1))[r] = make_int4((int)end, q.q0, q.n, q.base);
+  else
+    ((int *)(plan + 1))[r] = (int)end;
+}
+__device__ __forceinline__ AttnReq attn_req(const AttnPlan *plan, const AttnArgs &a, int r) {
+  if (a.R > ATTN_KEPT) return attn_req(a, r);
+  const int4 x = ((const int4 *)(plan + 1))[r];
+  return AttnReq{x.y, x.z, x.w, x.z * a.g};
+}
+// The request of tile i: the first r with end(r) > i.
+__device__ __forceinline__ int attn_find(const AttnPlan *plan, int R, int i) {
+  int lo = 0, hi = R - 1;
   while (lo < hi) {
     const int mid = (lo + hi) >> 1;
-    if (ends[mid] > i)
+    if (attn_end(plan, R, mid) > i)
       hi = mid;
     else
       lo = mid + 1;
@@ -128,43 +168,78 @@ __device__ __forceinline__ int attn_find(const int *ends, int n, int i) {
   return lo;
 }
 
-// A workgroup's share: `left` units from unit `u` of (head, tile) on.  Of `groups` workgroups the first
-// `longer` have one unit more than the others.
-struct AttnWork {
-  int g, groups, share, longer;
-  int tiles;         // per head
-  uint32_t at;       // the place of unit `u` in the line of all units
-  int head, tile;
-  int u, left;
-};
-
-constexpr int ATTN_SCAN_LDS = 64;  // bytes of LDS beside ends[R]
-
-// EXTRA units a tile costs beside its keys'.  ends: LDS, [R]; scratch: ATTN_SCAN_LDS bytes of LDS.
+// EXTRA units a tile costs beside its keys'.
 template <int TR, int KT, int EXTRA>
-__device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShare &s, int *ends, uint32_t *scratch) {
-  const int tid = threadIdx.x;
-  uint32_t *waves = scratch, *found = scratch + 8;
+__device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShare &s, AttnPlan *plan) {
+  const int tid = threadIdx.x, lane = tid & 63;
+  const uint32_t most = (uint32_t)s.tiles;
   AttnWork w;
+  w.left = 0, w.g = 0, w.groups = 0, w.r = 0;
+  // this workgroup's part of the line, of `per_head` units for each head; the place of its first unit
+  auto cut = [&](uint32_t per_head) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t total = per_head * (uint32_t)a.Hkv;
+    w.groups = (int)(total < gridDim.x ? total : gridDim.x);
+    w.share = (int)(total / (uint32_t)w.groups);
+    w.longer = (int)(total - (uint32_t)w.share * (uint32_t)w.groups);
+    // consecutive shares, which read the same keys, on one XCD (workgroups go to the 8 in turn)
+    const int per = (w.groups + 7) >> 3, y = blockIdx.x >> 3;
+    w.g = (blockIdx.x & 7) * per + y;
+    if (y >= per || w.g >= w.groups) return 0;
+    w.at = (uint32_t)w.g * (uint32_t)w.share + (uint32_t)(w.g < w.longer ? w.g : w.longer);
+    w.left = w.share + (w.g < w.longer);
+    w.head = (int)(w.at / per_head);
+    return w.at - (uint32_t)w.head * per_head;
+  };
+  auto tiles_of = [&](const AttnReq &q) __attribute__((always_inline)) -> uint32_t {
+    const uint32_t n = q.rows > s.min_rows && q.rows <= s.max_rows ? (uint32_t)(q.rows + TR - 1) / TR : 0u;
+    return n < most ? n : most;
+  };
   uint32_t run = 0, all = 0;
-#pragma unroll 1
-  for (int r0 = 0; r0 < a.R; r0 += ATTN_THREADS) {
-    const int r = r0 + tid;
-    uint32_t nt = 0;
-    if (r < a.R) {
-      const AttnReq q = attn_req(a, r);
-      if (q.rows > s.min_rows && q.rows <= s.max_rows) nt = (uint32_t)(q.rows + TR - 1) / TR;
+  if (a.R <= 64) {  // every wave for itself, a request per lane, no barrier (all write the same)
+    AttnReq q{0, 0, 0, 0};
+    if (lane < a.R) q = attn_req(a, lane);
+    const uint32_t nt = tiles_of(q), end = attn_wave_scan(nt);
+    if (lane < a.R) attn_keep(plan, a.R, lane, end < most ? end : most, q);
+    run = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+    run = run < most ? run : most;
+    w.tiles = (int)run;
+    if (run == 0) return w;
+    if (run <= 64) {  // and a tile per lane
+      for (uint32_t j = 0; __any(j < nt); ++j)
+        if (j < nt && end - nt + j < 64) plan->owner[end - nt + j] = (uint16_t)(lane | j << 8);
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      __builtin_amdgcn_wave_barrier();
+      uint32_t mine = 0, r = 0;
+      if (lane < (int)run) {
+        const uint32_t o = plan->owner[lane];
+        r = o & 255;
+        mine = (uint32_t)(attn_units<KT>(attn_tile(a, attn_req(plan, a, (int)r), (int)(o >> 8), TR)) + EXTRA);
+      }
+      const uint32_t to = attn_wave_scan(mine);
+      const uint32_t x = cut((uint32_t)__builtin_amdgcn_readlane((int)to, 63));
+      if (!w.left) return w;
+      w.tile = __builtin_ctzll(__ballot(x < to && x >= to - mine) | 1ull << 63);
+      w.u = (int)(x - (uint32_t)__builtin_amdgcn_readlane((int)(to - mine), w.tile));
+      w.r = __builtin_amdgcn_readlane((int)r, w.tile);
+      return w;
     }
-    const uint32_t most = (uint32_t)s.tiles, end = run + attn_scan(nt < most ? nt : most, waves, &all);
-    if (r < a.R) ends[r] = (int)(end < most ? end : most);
-    run = run + all < most ? run + all : most;
+  } else {
+#pragma unroll 1
+    for (int r0 = 0; r0 < a.R; r0 += ATTN_THREADS) {
+      const int r = r0 + tid;
+      AttnReq q{0, 0, 0, 0};
+      if (r < a.R) q = attn_req(a, r);
+      const uint32_t end = run + attn_scan(tiles_of(q), plan->waves, &all);
+      if (r < a.R) attn_keep(plan, a.R, r, end < most ? end : most, q);
+      run = run + all < most ? run + all : most;
+    }
+    w.tiles = (int)run;
   }
   __syncthreads();
-  w.tiles = (int)run;
-  w.left = 0, w.g = 0, w.groups = 0;
   // Units of the tiles, ATTN_THREADS at a time: first all of them, for the shares; then until the tile with the
   // share's first unit (where there are no more than that, the first turn's values still serve).
   uint32_t mine = 0, end = 0, x = 0;
+  int r = 0;
   run = 0;
   bool sought = false;
 #pragma unroll 1
@@ -173,35 +248,34 @@ __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShar
       const int i = i0 + tid;
       mine = 0;
       if (i < w.tiles) {
-        const int r = attn_find(ends, a.R, i);
-        mine = (uint32_t)(attn_units<KT>(attn_tile(a, attn_req(a, r), i - (r ? ends[r - 1] : 0), TR)) + EXTRA);
+        r = attn_find(plan, a.R, i);
+        mine = (uint32_t)(attn_units<KT>(attn_tile(a, attn_req(plan, a, r), i - (r ? attn_end(plan, a.R, r - 1) : 0), TR)) + EXTRA);
       }
-      end = run + attn_scan(mine, waves, &all);
+      end = run + attn_scan(mine, plan->waves, &all);
       run += all;
     }
-    if (sought && x < end && x >= end - mine) found[0] = (uint32_t)(i0 + tid), found[1] = x - (end - mine);
+    if (sought && x < end && x >= end - mine)
+      plan->found[0] = (uint32_t)(i0 + tid), plan->found[1] = x - (end - mine), plan->found[2] = (uint32_t)r;
     i0 += ATTN_THREADS;
     if (!sought && i0 >= w.tiles) {
-      const uint32_t per_head = run, total = run * (uint32_t)a.Hkv;
-      w.groups = (int)(total < gridDim.x ? total : gridDim.x);
-      w.share = (int)(total / (uint32_t)w.groups);
-      w.longer = (int)(total - (uint32_t)w.share * (uint32_t)w.groups);
-      // consecutive shares, which read the same keys, on one XCD (workgroups go to the 8 in turn)
-      const int per = (w.groups + 7) >> 3, y = blockIdx.x >> 3;
-      w.g = (blockIdx.x & 7) * per + y;
-      if (y >= per || w.g >= w.groups) return w;
-      w.at = (uint32_t)w.g * (uint32_t)w.share + (uint32_t)(w.g < w.longer ? w.g : w.longer);
-      w.left = w.share + (w.g < w.longer);
-      w.head = (int)(w.at / per_head);
-      x = w.at - (uint32_t)w.head * per_head;
+      x = cut(run);
+      if (!w.left) return w;
       sought = true;
       i0 = 0, run = 0;
     }
   }
   __syncthreads();
-  w.tile = (int)found[0];
-  w.u = (int)found[1];
+  w.tile = (int)plan->found[0];
+  w.u = (int)plan->found[1];
+  w.r = (int)plan->found[2];
   return w;
+}
+// The request of the share's tile: that of the last one, the one after, or sought.
+__device__ __forceinline__ int attn_request(const AttnPlan *plan, int R, const AttnWork &w) {
+  if (w.tile == 0) return attn_find(plan, R, 0);
+  if (attn_end(plan, R, w.r) > w.tile) return w.r;
+  if (w.r + 1 < R && attn_end(plan, R, w.r + 1) > w.tile) return w.r + 1;
+  return attn_find(plan, R, w.tile);
 }
 // The workgroup whose share unit `at` of the line is in.
 __device__ __forceinline__ int attn_group_of(const AttnWork &w, uint32_t at) {

@@ -62,24 +62,22 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
   constexpr int DT = DP / 32;     // 32-column tiles of O^T
   constexpr int OPS = DP / 32;    // DMA operations of a wave's 16 rows
   constexpr int TILE = ch_tile(DP), PITCH = 2 * DP;
+  constexpr int PLAN = 4 * TILE + CH_TAB + 16 * ATTN_THREADS;
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   uint8_t *tab = lds + 4 * TILE;
   uint32_t *vm = (uint32_t *)(tab + 4 * 2 * 256);  // [2][4]
   int *seen_at = (int *)(tab + CH_TAB);  // [thread][2][2]: what its rows see
-  uint32_t *scratch = (uint32_t *)(seen_at + 4 * ATTN_THREADS);
-  int *ends = (int *)((uint8_t *)scratch + ATTN_SCAN_LDS + sizeof(AttnWork)), *poison = (int *)scratch + 15, *redo = (int *)scratch + 14;
+  AttnPlan *plan = (AttnPlan *)(seen_at + 4 * ATTN_THREADS);
+  int *poison = plan->poison, *redo = &plan->redo;
 
   const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
-  auto work = [&]() __attribute__((always_inline)) {  // this workgroup's share, out of the registers
-    return (AttnWork *)(scratch + attn_opaque(ATTN_SCAN_LDS / 4));
-  };
   auto here = [&]() __attribute__((always_inline)) { return wv * 64 + (int)attn_lane(); };  // the thread's number
   int left;
   {
+    const AttnWork w = attn_uniform(attn_share<CH_TR, CH_KT, CH_EXTRA>(args, share, plan));
     if (share.first) attn_zero_rest(args);
-    const AttnWork w = attn_uniform(attn_share<CH_TR, CH_KT, CH_EXTRA>(args, share, ends, scratch));
     attn_note_none(share, w);
-    if (tid == 0) *work() = w;
+    if (tid == 0) plan->work[0] = w;
     left = attn_uniform(w.left);
   }
   const uint32_t la = lds_addr(lds), ta = lds_addr(tab) + wv * 512;
@@ -87,25 +85,28 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
     for (int i = tid; i < 4 * TILE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
   }
 
+  int turn = 0;
   while (left > 0) {
     __syncthreads();
     const AttnArgs a = attn_again<AttnArgs>(0);
-    const AttnWork w = attn_uniform(*work());
-    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
-    const AttnReq rq = attn_uniform(attn_req(a, r));
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), CH_TR);
+    AttnPlan *plan = (AttnPlan *)((int *)lds + attn_uniform(attn_opaque(PLAN / 4)));
+    const AttnWork w = attn_uniform(plan->work[turn]);
+    const int r = attn_uniform(attn_request(plan, a.R, w));
+    const AttnReq rq = attn_uniform(attn_req(plan, a, r));
+    const AttnTile t = attn_uniform(attn_tile(a, rq, w.tile - (r ? attn_end(plan, a.R, r - 1) : 0), CH_TR));
     const int units = attn_units<CH_KT>(t);
     const AttnPiece pc = attn_piece<CH_EXTRA>(w, units);
     const int ks = (int)((uint32_t)t.b / CH_KT + pc.u0) * CH_KT, nt = pc.u1 - pc.u0;
     const bool whole = pc.whole;
     const int part = w.g * 2 + pc.start, head = w.head;
     if (pc.start && !pc.none && here() == 0) attn_note(attn_again<AttnShare>(sizeof(AttnArgs)), w, rq, t, units + CH_EXTRA, whole);
-    __syncthreads();
     {
       AttnWork on = w;
+      on.r = r;
       attn_move_on(on, pc.take, units + CH_EXTRA);
       left = on.left;
-      if (here() == 0) *work() = on;
+      turn ^= 1;
+      if (here() == 0) plan->work[turn] = on;
     }
     if (pc.none) continue;
     if (units == 0) {  // no keys
@@ -521,7 +522,7 @@ hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int grid, hipStream_
 }  // namespace
 
 size_t attn_chunk_lds(int DP, int R) {
-  return 4 * ch_tile(DP) + CH_TAB + 16 * ATTN_THREADS + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
+  return 4 * ch_tile(DP) + CH_TAB + 16 * ATTN_THREADS + attn_plan_lds(R);
 }
 
 hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st) {

@@ -56,18 +56,16 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   uint8_t *tab = lds + ar_fixed(DP);
   int *seen_at = (int *)(tab + AR_TAB);  // [thread][2][2]: what its rows see
-  uint32_t *scratch = (uint32_t *)(seen_at + 4 * ATTN_THREADS);
-  AttnWork *work = (AttnWork *)(scratch + ATTN_SCAN_LDS / 4);  // (this workgroup's share, out of the registers)
-  int *ends = (int *)((uint8_t *)work + sizeof(AttnWork)), *poison = (int *)scratch + 15;
+  AttnPlan *plan = (AttnPlan *)(seen_at + 4 * ATTN_THREADS);
 
   const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
   auto here = [&]() __attribute__((always_inline)) { return wv * 64 + (int)attn_lane(); };  // the thread's number
   int left;
   {
+    const AttnWork w = attn_uniform(attn_share<TR, KT, AR_EXTRA>(args, share, plan));
     if (share.first) attn_zero_rest(args);
-    const AttnWork w = attn_uniform(attn_share<TR, KT, AR_EXTRA>(args, share, ends, scratch));
     attn_note_none(share, w);
-    if (tid == 0) *work = w;
+    if (tid == 0) plan->work[0] = w, plan->poison[0] = 0;
     left = w.left;
   }
   uint8_t *kl = lds + wv * 2 * AR_TILE, *vl = kl + AR_TILE;
@@ -77,14 +75,16 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
   }
 
+  int turn = 0;
 #pragma unroll 1
   while (left > 0) {
     __syncthreads();  // (the last tile's merge is read; the zeros above are written)
     const AttnArgs a = attn_again<AttnArgs>(0);
-    const AttnWork w = attn_uniform(*work);
-    const int r = attn_uniform(attn_find(ends, a.R, w.tile));
-    const AttnReq rq = attn_uniform(attn_req(a, r));
-    const AttnTile t = attn_tile(a, rq, w.tile - (r ? attn_uniform(ends[r - 1]) : 0), TR);
+    const AttnWork w = attn_uniform(plan->work[turn]);
+    int *poison = &plan->poison[turn];
+    const int r = attn_uniform(attn_request(plan, a.R, w));
+    const AttnReq rq = attn_uniform(attn_req(plan, a, r));
+    const AttnTile t = attn_uniform(attn_tile(a, rq, w.tile - (r ? attn_end(plan, a.R, r - 1) : 0), TR));
     const int units = attn_units<KT>(t);
     const AttnPiece pc = attn_piece<AR_EXTRA>(w, units);
     const bool whole = pc.whole;
@@ -93,14 +93,14 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     ke = ke < t.e ? ke : t.e;
     if (pc.start && !pc.none && here() == 0)
       attn_note(attn_again<AttnShare>(sizeof(AttnArgs)), w, rq, t, units + AR_EXTRA, whole);
-    __syncthreads();
     {
       AttnWork on = w;
+      on.r = r;
       attn_move_on(on, pc.take, units + AR_EXTRA);
       left = on.left;
-      if (here() == 0) *work = on, *poison = 0;
+      turn ^= 1;
+      if (here() == 0) plan->work[turn] = on, plan->poison[turn] = 0;
     }
-    __syncthreads();
     if (pc.none) continue;
 
     // This wave's tiles are the keys k0 = ks + KW (wave + 4 i), this lane's key of them the (lane % KW)th: `page`
@@ -453,7 +453,7 @@ hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int tr, int grid, hi
 }  // namespace
 
 size_t attn_rows_lds(int DP, int R) {
-  return ar_fixed(DP) + AR_TAB + 16 * ATTN_THREADS + ATTN_SCAN_LDS + sizeof(AttnWork) + (size_t)R * 4;
+  return ar_fixed(DP) + AR_TAB + 16 * ATTN_THREADS + attn_plan_lds(R);
 }
 
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st) {
