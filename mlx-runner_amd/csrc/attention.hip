@@ -15,88 +15,145 @@ namespace {
 
 constexpr int AC_MOST = 1024;  // workgroups of a launch, so partials of a tile
 
-// One workgroup per tile and row: the waves take the partials in turn.
-template <int DP>
-__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs a, const AttnShare s, int tr) {
-  constexpr int LPR = DP / 4;                // lanes of a row, four values each
-  constexpr int SETS = ATTN_THREADS / LPR;   // partials in flight
-  __shared__ float wt[AC_MOST], red[8];
-  __shared__ __attribute__((aligned(16))) float part[SETS][DP];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if ((int64_t)blockIdx.x >= (s.by_tile ? (int64_t)s.count[0] * a.Hkv : (int64_t)s.count[1])) return;
-  const int *d = s.desc + (int64_t)blockIdx.x * 8;
-  const int g0 = d[0], row = blockIdx.y;
-  if (g0 < 0 || row >= d[4]) return;
-  const int np = d[1] - g0 + 1;
-  auto place = [&](int p) -> int64_t { return (int64_t)((g0 + p) * 2 + (p == 0)) * tr + row; };
-  float top = -__builtin_inff();
-  for (int p = tid; p < np; p += ATTN_THREADS) top = fmaxf(top, s.ml[place(p) * 2]);
-#pragma unroll
-  for (int off = 32; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 64));
-  if (lane == 0) red[wave] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-  float sum = 0.f;
-  for (int p = tid; p < np; p += ATTN_THREADS) {
-    const float2 ml = *(const float2 *)(s.ml + place(p) * 2);
-    const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
-    wt[p] = f;
-    sum += f * ml.y;
-  }
-  sum = wave_sum(sum);
-  if (lane == 0) red[4 + wave] = sum;
-  __syncthreads();
-  sum = red[4] + red[5] + red[6] + red[7];
-  const int set = tid / LPR, d0 = tid % LPR * 4;
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  if (d0 < a.D) {
-#pragma unroll 8
-    for (int p = set; p < np; p += SETS) {
-      const float f = wt[p];
-      if (f == 0.f) continue;  // (a part without keys has no sums)
-      const float4 x = *(const float4 *)(s.acc + place(p) * DP + d0);
-      o.x += f * x.x, o.y += f * x.y, o.z += f * x.z, o.w += f * x.w;
-    }
-  }
-  *(float4 *)&part[set][d0] = o;
-  __syncthreads();
-  if (tid * 8 < a.D) {
-    float v[8];
-    const float inv = sum != 0.f ? 1.f / sum : 0.f;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      v[e] = 0.f;
-#pragma unroll
-      for (int i = 0; i < SETS; ++i) v[e] += part[i][tid * 8 + e];
-      v[e] *= inv;
-    }
-    attn_store8(a, attn_row(a, d[2], d[3] + row, d[5]), tid * 8, v);
-  }
+// Over the wave's lanes, in all of them.
+__device__ __forceinline__ float wave_top(float x) {
+#define QMM_STEP(ctrl, rows)                                                                                    \
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(__float_as_int(x), __float_as_int(x), ctrl, rows, 0xF, false)))
+  QMM_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8; row_bcast:15, 31 (as attn_wave_scan)
+  QMM_STEP(0x112, 0xF);
+  QMM_STEP(0x114, 0xF);
+  QMM_STEP(0x118, 0xF);
+  QMM_STEP(0x142, 0xA);
+  QMM_STEP(0x143, 0xC);
+#undef QMM_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+__device__ __forceinline__ float wave_total(float x) {
+#define QMM_STEP(ctrl, rows) \
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), ctrl, rows, 0xF, false))
+  QMM_STEP(0x111, 0xF);
+  QMM_STEP(0x112, 0xF);
+  QMM_STEP(0x114, 0xF);
+  QMM_STEP(0x118, 0xF);
+  QMM_STEP(0x142, 0xA);
+  QMM_STEP(0x143, 0xC);
+#undef QMM_STEP
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
 }
 
-// Tiles of many rows, mostly cut in few parts: 16 rows per workgroup, their weights first.
+// The tile that a workgroup joins; none: first < 0.  (Its entry is read beside the count that says whether there is one.)
+struct Cut {
+  int first, last, q0, row0, rows, head;
+};
+__device__ __forceinline__ Cut cut_of(const AttnArgs &a, const AttnShare &s) {
+  const int4 x = *(const int4 *)(s.desc + (int64_t)blockIdx.x * 8);
+  const int2 y = *(const int2 *)(s.desc + (int64_t)blockIdx.x * 8 + 4);
+  const int2 n = *(const int2 *)s.count;
+  Cut c{x.x, x.y, x.z, x.w, y.x, y.y};
+  if ((int64_t)blockIdx.x >= (s.by_tile ? (int64_t)n.x * a.Hkv : (int64_t)n.y)) c.first = -1;
+  return c;
+}
+
+// One workgroup per tile, row and COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every
+// wave works out the partials' weights for itself.
+template <int DP, int COLS>
+__global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs a, const AttnShare s, int tr) {
+  constexpr int LPR = COLS / 4;              // lanes of a row, four values each
+  constexpr int SETS = ATTN_THREADS / LPR;   // partials side by side
+  constexpr int HELD = 4, AHEAD = 8;
+  __shared__ float wt[ATTN_THREADS / 64][AC_MOST];
+  __shared__ __attribute__((aligned(16))) float part[SETS][COLS];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const Cut c = cut_of(a, s);
+  const int row = blockIdx.y;
+  if (c.first < 0 || row >= c.rows) return;
+  const int np = c.last - c.first + 1;
+  auto place = [&](int p) -> int64_t { return (int64_t)((c.first + p) * 2 + (p == 0)) * tr + row; };
+  const int set = tid / LPR, d0 = blockIdx.z * COLS + tid % LPR * 4, col = blockIdx.z * COLS + tid;
+  const bool in = d0 < a.D, out = tid < COLS && col < a.D;
+  float2 ml[HELD];
+#pragma unroll
+  for (int k = 0; k < HELD; ++k) {
+    ml[k] = make_float2(-__builtin_inff(), 0.f);
+    if (k * 64 + lane < np) ml[k] = *(const float2 *)(s.ml + place(k * 64 + lane) * 2);
+  }
+  float4 x[AHEAD];
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (set + i * SETS < np && in) x[i] = *(const float4 *)(s.acc + place(set + i * SETS) * DP + d0);
+  const int64_t orow = attn_row(a, c.q0, c.row0 + row, c.head);
+  uint32_t gate = 0;
+  if (a.gate && out) gate = a.gate[orow * a.Dg + (a.Dg - a.D) + col];
+
+  float top = ml[0].x, sum = 0.f;
+#pragma unroll
+  for (int k = 1; k < HELD; ++k) top = fmaxf(top, ml[k].x);
+  for (int p = HELD * 64 + lane; p < np; p += 64) top = fmaxf(top, s.ml[place(p) * 2]);
+  top = wave_top(top);
+  auto weigh = [&](int p, float2 v) __attribute__((always_inline)) {
+    const float f = v.x == -__builtin_inff() ? 0.f : attn_exp2(v.x - top);
+    wt[wave][p] = f;
+    sum += f * v.y;
+  };
+#pragma unroll
+  for (int k = 0; k < HELD; ++k)
+    if (k * 64 + lane < np) weigh(k * 64 + lane, ml[k]);
+  for (int p = HELD * 64 + lane; p < np; p += 64) weigh(p, *(const float2 *)(s.ml + place(p) * 2));
+  sum = wave_total(sum);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  auto add = [&](float f, float4 v) __attribute__((always_inline)) {
+    if (f != 0.f) o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;  // (a part without keys has no sums)
+  };
+#pragma unroll
+  for (int i = 0; i < AHEAD; ++i)
+    if (set + i * SETS < np && in) add(wt[wave][set + i * SETS], x[i]);
+#pragma unroll 8
+  for (int p = set + AHEAD * SETS; p < np; p += SETS)
+    if (in) add(wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
+  *(float4 *)&part[set][tid % LPR * 4] = o;
+  __syncthreads();
+  if (!out) return;
+  float v = 0.f;
+#pragma unroll
+  for (int i = 0; i < SETS; ++i) v += part[i][tid];
+  v *= sum != 0.f ? 1.f / sum : 0.f;
+  if (a.gate) v *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-1.44269504088896341f * __uint_as_float(gate << 16)));
+  a.o[orow * a.D + col] = __builtin_bit_cast(uint16_t, (__bf16)v);
+}
+
+// Tiles of many rows, mostly cut in few parts: 16 rows per workgroup, their weights while the first parts are on their way.
 constexpr int AJ_ROWS = 16;
 template <int DP>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const AttnArgs a, const AttnShare s, int tr) {
-  constexpr int LPR = DP / 4, RP = ATTN_THREADS / LPR, TURNS = AJ_ROWS / RP;
+  constexpr int LPR = DP / 4, RP = ATTN_THREADS / LPR, TURNS = AJ_ROWS / RP, AHEAD = 2;
   __shared__ float wt[AJ_ROWS][AC_MOST / 2], total[AJ_ROWS];
   __shared__ __attribute__((aligned(16))) float part[AJ_ROWS][DP];
   const int tid = threadIdx.x;
-  if ((int64_t)blockIdx.x >= (s.by_tile ? (int64_t)s.count[0] * a.Hkv : (int64_t)s.count[1])) return;
-  const int *d = s.desc + (int64_t)blockIdx.x * 8;
-  const int g0 = d[0], row0 = blockIdx.y * AJ_ROWS, rows = d[4];
-  if (g0 < 0 || row0 >= rows) return;
-  const int np = d[1] - g0 + 1;
-  auto place = [&](int p, int row) -> int64_t { return (int64_t)((g0 + p) * 2 + (p == 0)) * tr + row0 + row; };
+  const Cut c = cut_of(a, s);
+  const int row0 = blockIdx.y * AJ_ROWS, rows = c.rows;
+  if (c.first < 0 || row0 >= rows) return;
+  const int np = c.last - c.first + 1;
+  auto place = [&](int p, int row) -> int64_t { return (int64_t)((c.first + p) * 2 + (p == 0)) * tr + row0 + row; };
+  const int r0 = tid / LPR, d0 = tid % LPR * 4;
+  const int row = tid >> 4, l = tid & 15;
+  const bool on = row0 + row < rows;
+  float2 ml = make_float2(-__builtin_inff(), 0.f);
+  if (l < np && on) ml = *(const float2 *)(s.ml + place(l, row) * 2);
+  float4 x[AHEAD][TURNS];
+#pragma unroll
+  for (int p = 0; p < AHEAD; ++p)
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t)
+      if (p < np && row0 + t * RP + r0 < rows && d0 < a.D) x[p][t] = *(const float4 *)(s.acc + place(p, t * RP + r0) * DP + d0);
   {
-    const int row = tid >> 4, l = tid & 15;
-    const bool on = row0 + row < rows;
-    float top = -__builtin_inff(), sum = 0.f;
-    for (int p = l; p < np && on; p += 16) top = fmaxf(top, s.ml[place(p, row) * 2]);
+    float top = ml.x, sum = 0.f;
+    for (int p = l + 16; p < np && on; p += 16) top = fmaxf(top, s.ml[place(p, row) * 2]);
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
     for (int p = l; p < np && on; p += 16) {
-      const float2 ml = *(const float2 *)(s.ml + place(p, row) * 2);
+      if (p >= 16) ml = *(const float2 *)(s.ml + place(p, row) * 2);
       const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
       wt[row][p] = f;
       sum += f * ml.y;
@@ -106,26 +163,26 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
     if (l == 0) total[row] = sum;
   }
   __syncthreads();
-  const int r0 = tid / LPR, d0 = tid % LPR * 4;
   float4 o[TURNS];
 #pragma unroll
   for (int t = 0; t < TURNS; ++t) o[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 2
-  for (int p = 0; p < np; ++p) {
-    float4 x[TURNS];
+  auto add = [&](int t, float f, float4 v) __attribute__((always_inline)) {
+    // (a part without keys has no sums)
+    if (f != 0.f) o[t].x += f * v.x, o[t].y += f * v.y, o[t].z += f * v.z, o[t].w += f * v.w;
+  };
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {
-      const int row = t * RP + r0;
-      x[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-      // (a part without keys has no sums)
-      if (row0 + row < rows && d0 < a.D && wt[row][p] != 0.f) x[t] = *(const float4 *)(s.acc + place(p, row) * DP + d0);
-    }
+  for (int p = 0; p < AHEAD; ++p)
 #pragma unroll
-    for (int t = 0; t < TURNS; ++t) {
-      const int row = t * RP + r0;
-      const float f = row0 + row < rows ? wt[row][p] : 0.f;
-      o[t].x += f * x[t].x, o[t].y += f * x[t].y, o[t].z += f * x[t].z, o[t].w += f * x[t].w;
-    }
+    for (int t = 0; t < TURNS; ++t)
+      if (p < np && row0 + t * RP + r0 < rows && d0 < a.D) add(t, wt[t * RP + r0][p], x[p][t]);
+#pragma unroll 1
+  for (int p = AHEAD; p < np; ++p) {
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t)
+      if (row0 + t * RP + r0 < rows && d0 < a.D) x[0][t] = *(const float4 *)(s.acc + place(p, t * RP + r0) * DP + d0);
+#pragma unroll
+    for (int t = 0; t < TURNS; ++t)
+      if (row0 + t * RP + r0 < rows && d0 < a.D) add(t, wt[t * RP + r0][p], x[0][t]);
   }
 #pragma unroll
   for (int t = 0; t < TURNS; ++t) *(float4 *)&part[t * RP + r0][d0] = o[t];
@@ -137,7 +194,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
     float v[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = part[row][c0 + e] * inv;
-    attn_store8(a, attn_row(a, d[2], d[3] + row0 + row, d[5]), c0, v);
+    attn_store8(a, attn_row(a, c.q0, c.row0 + row0 + row, c.head), c0, v);
   }
 }
 
@@ -222,8 +279,10 @@ void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) 
   const unsigned n = (unsigned)(p.by_tile ? p.tiles * a.Hkv : p.grid);
   if (p.tr > 32)
     hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(n, p.rows / AJ_ROWS), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+  else if (DP > 64 && n * (unsigned)p.rows <= 1024)
+    hipLaunchKernelGGL((attn_join_kernel<DP, 64>), dim3(n, p.rows, DP / 64), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
   else
-    hipLaunchKernelGGL((attn_join_kernel<DP>), dim3(n, p.rows), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+    hipLaunchKernelGGL((attn_join_kernel<DP, DP>), dim3(n, p.rows), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
 }
 
 }  // namespace
