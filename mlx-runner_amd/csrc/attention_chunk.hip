@@ -255,7 +255,9 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             const int lo = seen_b[u] - k0, hi = seen_e[u] - k0;
             uint32_t seen = hi < 0 ? 0u : hi > 30 ? ~0u : (2u << hi) - 1u;
             seen &= lo > 31 ? 0u : lo > 0 ? ~0u << lo : ~0u;
-            seen = (seen & valid) >> h4;
+            seen &= valid;
+            if (__all(seen == ~0u)) continue;  // (a wave's 64 rows differ on fewer keys than the tile's)
+            seen >>= h4;
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
               const int on = __builtin_amdgcn_sbfe((int)seen, 8 * (i / 4) + i % 4, 1);  // 0 or -1
@@ -380,7 +382,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         // values of tile i (the page ids and keys asked for after them may be on their way)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
         const int own = ks + i * CH_KT + wv * 16;  // (the values that this wave has moved; see attention_rows.hip)
-        if (edge && (own < t.full_b || own + 16 > t.full_e || ((valid >> wv * 16) & 0xFFFFu) != 0xFFFFu)) {
+        if (edge && (((valid >> wv * 16) & 0xFFFFu) != 0xFFFFu || (again && (own < t.full_b || own + 16 > t.full_e)))) {
           const uint32_t ln = attn_lane();
           bool odd = false;
 #pragma unroll
@@ -413,6 +415,22 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       }
       product((nt - 1) & 1, 1, false, -1);
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    if (!again && (ks < t.full_b || ks + nt * CH_KT > t.full_e)) {
+      // Keys that some rows do not see had weights of zero there, and 0 inf is NaN: sums that are not finite are
+      // formed again with such values held back.
+      float z = 0.f;
+#pragma unroll
+      for (int d = 0; d < DT; ++d)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          f32x16_t x = acc[d][u];
+          asm volatile("" : "+a"(x));
+#pragma unroll
+          for (int i = 0; i < 16; ++i) z = __builtin_fmaf(x[i], 0.f, z);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      passed |= z != 0.f;
+    }
     if (__any(passed)) *redo = attn_opaque(1);
     __syncthreads();
     again = !again && *redo;
