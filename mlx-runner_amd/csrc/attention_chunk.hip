@@ -199,19 +199,23 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       };
       // DMA operation n: rows RPI n .. of the wave's 16, chunk (lane % CPR) ^ swizzle of each
       constexpr int RPI = 64 / CPR;
-      auto move = [&](const uint16_t *cache, int n, int to, auto swz) __attribute__((always_inline)) {
+      struct From {
+        uint32_t row, c;  // of operation 0: whose row, and where in it
+      };
+      auto from_of = [&](auto swz) __attribute__((always_inline)) {
         const uint32_t ln = attn_lane();
-        const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(ln / CPR * 4) + RPI * n * 4, (int)mine);
-        const uint32_t c = (ln % CPR ^ (uint32_t)swz((int)(ln / CPR)) ^ (uint32_t)swz(RPI * n)) * 16;
+        return From{ln / CPR * 4, (ln % CPR ^ (uint32_t)swz((int)(ln / CPR))) * 16};
+      };
+      auto move = [&](const uint16_t *cache, const From &f, int n, int to, auto swz) __attribute__((always_inline)) {
+        const uint32_t row = __builtin_amdgcn_ds_bpermute((int)f.row + RPI * n * 4, (int)mine);
+        const uint32_t c = f.c ^ (uint32_t)swz(RPI * n) * 16;
         if (FULL || c < 2 * (uint32_t)D)
           gp_dma16((const char *)cache + ((uint64_t)row * (2 * (uint32_t)D) + c), la + to + wv * 16 * PITCH + n * 1024);
       };
-      auto move_k = [&](int set, int n) __attribute__((always_inline)) {
-        move(kc, n, set * TILE, [](int r) { return attn_swz<DP>(r); });
-      };
-      auto move_v = [&](int set, int n) __attribute__((always_inline)) {
-        move(vc, n, (2 + set) * TILE, [](int r) { return ch_swz_v<DP>(r); });
-      };
+      const auto swz_k = [](int r) { return attn_swz<DP>(r); };
+      const auto swz_v = [](int r) { return ch_swz_v<DP>(r); };
+      auto move_k = [&](const From &f, int set, int n) __attribute__((always_inline)) { move(kc, f, n, set * TILE, swz_k); };
+      auto move_v = [&](const From &f, int set, int n) __attribute__((always_inline)) { move(vc, f, n, (2 + set) * TILE, swz_v); };
 
       // S^T of 32 keys; beside it, the DMA of a tile's values
       auto scores = [&](int set, int half, bool values) __attribute__((always_inline)) {
@@ -224,6 +228,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         };
         constexpr int AHEAD = 2;
         bf16x8_t kf[KS];
+        From f{};
+        if (values) f = from_of(swz_v);
 #pragma unroll
         for (int k = 0; k < AHEAD; ++k) kf[k] = load(k);
 #pragma unroll
@@ -236,7 +242,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             else
               ch_mfma(sv[u], kf[k], q[u][k]);
           }
-          if (values && k % 2 == 0) move_v(set, k / 2);
+          if (values && k % 2 == 0) move_v(f, set, k / 2);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
@@ -287,7 +293,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         for (int j = n * (16 / N); j < (n + 1) * (16 / N); ++j) {
           const int c = j >> 3, u = j >> 2 & 1, e = (j & 3) * 2;
           const float s0 = sv[u][c * 8 + e], s1 = sv[u][c * 8 + e + 1];
-          top[u] = fmaxf(top[u], fmaxf(s0, s1));
+          asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top[u]) : "v"(s0), "v"(s1));  // (fmaxf would first quiet each)
           bf16x2_t x;
           x[0] = (__bf16)attn_exp2(__builtin_fmaf(s0, sc, -ref[u]));
           x[1] = (__bf16)attn_exp2(__builtin_fmaf(s1, sc, -ref[u]));
@@ -326,6 +332,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
         };
         bf16x8_t vf[N];
+        From f{};
+        if (keys >= 0) f = from_of(swz_k);
 #pragma unroll
         for (int n = 0; n < AHEAD; ++n) vf[n] = load(n);
 #pragma unroll
@@ -336,7 +344,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
             acc[n % DT][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], p[n / DT][u], acc[n % DT][u], 0, 0, 0);
           if (n == 0 && with) ch_mfma_done(sv[0], sv[1]);
           if (with) weights(n, N);
-          if (keys >= 0 && n % 2 == 0) move_k(keys, n / 2);
+          if (keys >= 0 && n % 2 == 0) move_k(f, keys, n / 2);
           __builtin_amdgcn_sched_barrier(0);
         }
       };
@@ -354,8 +362,11 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       ask(1);
       off = poff;
       onward(page, poff);
+      {
+        const From f = from_of(swz_k);
 #pragma unroll
-      for (int n = 0; n < OPS; ++n) move_k(0, n);
+        for (int n = 0; n < OPS; ++n) move_k(f, 0, n);
+      }
       // Tile i: scores of its first half | values of tile i; weights of those with the product of tile i - 1's
       // second half | keys of tile i + 1; the same for its second half.
       // (what is asked for past the last tile is not used; the waits count on it)
