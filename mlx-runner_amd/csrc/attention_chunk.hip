@@ -39,6 +39,10 @@ __device__ __forceinline__ int ch_swz_v(int row) {
 __device__ __forceinline__ void ch_dma4(const void *g, uint32_t l) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(l), "v"(g) : "memory", "m0");
 }
+// LDS DMA of 16 bytes per lane to l + `at` (see gp_dma16).
+__device__ __forceinline__ void ch_dma16(const void *g, uint32_t l, int at) {
+  asm volatile("s_add_i32 m0, %0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" ::"s"(l), "v"(g), "i"(at) : "memory", "m0", "scc");
+}
 #pragma clang diagnostic pop
 
 // S^T's products, written out so that S^T lies in vector registers: the sums of O^T (of 256
@@ -122,7 +126,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
 
     if (here() == 0) *poison = attn_opaque(0), *redo = attn_opaque(0);
     const int *tabrow = a.table + (int64_t)r * a.W;
-    const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
+    const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = a.D;
+    const uint32_t pitch = 2 * (uint32_t)D;  // (of a cache row; a multiply-add beats a shift and two adds)
     const uint16_t *kc = a.k, *vc = a.v;
     // the lane's rows
     float m[2], l[2];
@@ -210,7 +215,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         const uint32_t row = __builtin_amdgcn_ds_bpermute((int)f.row + RPI * n * 4, (int)mine);
         const uint32_t c = f.c ^ (uint32_t)swz(RPI * n) * 16;
         if (FULL || c < 2 * (uint32_t)D)
-          gp_dma16((const char *)cache + ((uint64_t)row * (2 * (uint32_t)D) + c), la + to + wv * 16 * PITCH + n * 1024);
+          ch_dma16((const char *)cache + c + (uint64_t)row * pitch, la + to + wv * 16 * PITCH, n * 1024);
       };
       const auto swz_k = [](int r) { return attn_swz<DP>(r); };
       const auto swz_v = [](int r) { return ch_swz_v<DP>(r); };
@@ -342,7 +347,8 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
 #pragma unroll
           for (int u = 0; u < 2; ++u)
             acc[n % DT][u] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], p[n / DT][u], acc[n % DT][u], 0, 0, 0);
-          if (n == 0 && with) ch_mfma_done(sv[0], sv[1]);
+          if (n == 0 && with)  // (since the last score's product: two products, six reads and their addresses)
+            asm volatile("s_nop 3" : "+v"(sv[0]), "+v"(sv[1]));
           if (with) weights(n, N);
           if (keys >= 0 && n % 2 == 0) move_k(f, keys, n / 2);
           __builtin_amdgcn_sched_barrier(0);
