@@ -205,22 +205,24 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       // DMA operation n: rows RPI n .. of the wave's 16, chunk (lane % CPR) ^ swizzle of each
       constexpr int RPI = 64 / CPR;
       struct From {
-        uint32_t row, c;  // of operation 0: whose row, and where in it
+        uint32_t lane, c;  // whose row operation 0 moves, and where in it
+        uint32_t row;      // of the next operation, asked for an operation before
       };
       auto from_of = [&](auto swz) __attribute__((always_inline)) {
         const uint32_t ln = attn_lane();
-        return From{ln / CPR * 4, (ln % CPR ^ (uint32_t)swz((int)(ln / CPR))) * 16};
+        const uint32_t lane = ln / CPR * 4;
+        return From{lane, (ln % CPR ^ (uint32_t)swz((int)(ln / CPR))) * 16, (uint32_t)__builtin_amdgcn_ds_bpermute((int)lane, (int)mine)};
       };
-      auto move = [&](const uint16_t *cache, const From &f, int n, int to, auto swz) __attribute__((always_inline)) {
-        const uint32_t row = __builtin_amdgcn_ds_bpermute((int)f.row + RPI * n * 4, (int)mine);
-        const uint32_t c = f.c ^ (uint32_t)swz(RPI * n) * 16;
+      auto move = [&](const uint16_t *cache, From &f, int n, int to, auto swz) __attribute__((always_inline)) {
+        const uint32_t row = f.row, c = f.c ^ (uint32_t)swz(RPI * n) * 16;
+        if (n + 1 < OPS) f.row = __builtin_amdgcn_ds_bpermute((int)f.lane + RPI * (n + 1) * 4, (int)mine);
         if (FULL || c < 2 * (uint32_t)D)
           ch_dma16((const char *)cache + c + (uint64_t)row * pitch, la + to + wv * 16 * PITCH, n * 1024);
       };
       const auto swz_k = [](int r) { return attn_swz<DP>(r); };
       const auto swz_v = [](int r) { return ch_swz_v<DP>(r); };
-      auto move_k = [&](const From &f, int set, int n) __attribute__((always_inline)) { move(kc, f, n, set * TILE, swz_k); };
-      auto move_v = [&](const From &f, int set, int n) __attribute__((always_inline)) { move(vc, f, n, (2 + set) * TILE, swz_v); };
+      auto move_k = [&](From &f, int set, int n) __attribute__((always_inline)) { move(kc, f, n, set * TILE, swz_k); };
+      auto move_v = [&](From &f, int set, int n) __attribute__((always_inline)) { move(vc, f, n, (2 + set) * TILE, swz_v); };
 
       // S^T of 32 keys; beside it, the DMA of a tile's values
       auto scores = [&](int set, int half, bool values) __attribute__((always_inline)) {
@@ -369,7 +371,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       off = poff;
       onward(page, poff);
       {
-        const From f = from_of(swz_k);
+        From f = from_of(swz_k);
 #pragma unroll
         for (int n = 0; n < OPS; ++n) move_k(f, 0, n);
       }
