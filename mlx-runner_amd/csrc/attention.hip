@@ -54,8 +54,9 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const AttnShare &s) {
   return c;
 }
 
-// One workgroup per tile, row and COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every
-// wave works out the partials' weights for itself.
+// One workgroup per tile, row (then every gridDim.y-th: the grid follows from shapes, a tile's rows from the lengths) and
+// COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every wave works out the partials' weights
+// for itself.
 template <int DP, int COLS>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs a, const AttnShare s, int tr) {
   constexpr int LPR = COLS / 4;              // lanes of a row, four values each
@@ -65,62 +66,69 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
   __shared__ __attribute__((aligned(16))) float part[SETS][COLS];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const Cut c = cut_of(a, s);
-  const int row = blockIdx.y;
+  int row = blockIdx.y;
   if (c.first < 0 || row >= c.rows) return;
   const int np = c.last - c.first + 1;
   auto place = [&](int p) -> int64_t { return (int64_t)((c.first + p) * 2 + (p == 0)) * tr + row; };
   const int set = tid / LPR, d0 = blockIdx.z * COLS + tid % LPR * 4, col = blockIdx.z * COLS + tid;
   const bool in = d0 < a.D, out = tid < COLS && col < a.D;
-  float2 ml[HELD];
+#pragma unroll 1
+  while (true) {
+    float2 ml[HELD];
 #pragma unroll
-  for (int k = 0; k < HELD; ++k) {
-    ml[k] = make_float2(-__builtin_inff(), 0.f);
-    if (k * 64 + lane < np) ml[k] = *(const float2 *)(s.ml + place(k * 64 + lane) * 2);
-  }
-  float4 x[AHEAD];
+    for (int k = 0; k < HELD; ++k) {
+      ml[k] = make_float2(-__builtin_inff(), 0.f);
+      if (k * 64 + lane < np) ml[k] = *(const float2 *)(s.ml + place(k * 64 + lane) * 2);
+    }
+    float4 x[AHEAD];
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (set + i * SETS < np && in) x[i] = *(const float4 *)(s.acc + place(set + i * SETS) * DP + d0);
-  const int64_t orow = attn_row(a, c.q0, c.row0 + row, c.head);
-  uint32_t gate = 0;
-  if (a.gate && out) gate = a.gate[orow * a.Dg + (a.Dg - a.D) + col];
+    for (int i = 0; i < AHEAD; ++i)
+      if (set + i * SETS < np && in) x[i] = *(const float4 *)(s.acc + place(set + i * SETS) * DP + d0);
+    const int64_t orow = attn_row(a, c.q0, c.row0 + row, c.head);
+    uint32_t gate = 0;
+    if (a.gate && out) gate = a.gate[orow * a.Dg + (a.Dg - a.D) + col];
 
-  float top = ml[0].x, sum = 0.f;
+    float top = ml[0].x, sum = 0.f;
 #pragma unroll
-  for (int k = 1; k < HELD; ++k) top = fmaxf(top, ml[k].x);
-  for (int p = HELD * 64 + lane; p < np; p += 64) top = fmaxf(top, s.ml[place(p) * 2]);
-  top = wave_top(top);
-  auto weigh = [&](int p, float2 v) __attribute__((always_inline)) {
-    const float f = v.x == -__builtin_inff() ? 0.f : attn_exp2(v.x - top);
-    wt[wave][p] = f;
-    sum += f * v.y;
-  };
+    for (int k = 1; k < HELD; ++k) top = fmaxf(top, ml[k].x);
+    for (int p = HELD * 64 + lane; p < np; p += 64) top = fmaxf(top, s.ml[place(p) * 2]);
+    top = wave_top(top);
+    auto weigh = [&](int p, float2 v) __attribute__((always_inline)) {
+      const float f = v.x == -__builtin_inff() ? 0.f : attn_exp2(v.x - top);
+      wt[wave][p] = f;
+      sum += f * v.y;
+    };
 #pragma unroll
-  for (int k = 0; k < HELD; ++k)
-    if (k * 64 + lane < np) weigh(k * 64 + lane, ml[k]);
-  for (int p = HELD * 64 + lane; p < np; p += 64) weigh(p, *(const float2 *)(s.ml + place(p) * 2));
-  sum = wave_total(sum);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](float f, float4 v) __attribute__((always_inline)) {
-    if (f != 0.f) o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;  // (a part without keys has no sums)
-  };
+    for (int k = 0; k < HELD; ++k)
+      if (k * 64 + lane < np) weigh(k * 64 + lane, ml[k]);
+    for (int p = HELD * 64 + lane; p < np; p += 64) weigh(p, *(const float2 *)(s.ml + place(p) * 2));
+    sum = wave_total(sum);
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    auto add = [&](float f, float4 v) __attribute__((always_inline)) {
+      if (f != 0.f) o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;  // (a part without keys has no sums)
+    };
 #pragma unroll
-  for (int i = 0; i < AHEAD; ++i)
-    if (set + i * SETS < np && in) add(wt[wave][set + i * SETS], x[i]);
+    for (int i = 0; i < AHEAD; ++i)
+      if (set + i * SETS < np && in) add(wt[wave][set + i * SETS], x[i]);
 #pragma unroll 8
-  for (int p = set + AHEAD * SETS; p < np; p += SETS)
-    if (in) add(wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
-  *(float4 *)&part[set][tid % LPR * 4] = o;
-  __syncthreads();
-  if (!out) return;
-  float v = 0.f;
+    for (int p = set + AHEAD * SETS; p < np; p += SETS)
+      if (in) add(wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
+    *(float4 *)&part[set][tid % LPR * 4] = o;
+    __syncthreads();
+    if (out) {
+      float v = 0.f;
 #pragma unroll
-  for (int i = 0; i < SETS; ++i) v += part[i][tid];
-  v *= sum != 0.f ? 1.f / sum : 0.f;
-  if (a.gate) v *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-1.44269504088896341f * __uint_as_float(gate << 16)));
-  a.o[orow * a.D + col] = __builtin_bit_cast(uint16_t, (__bf16)v);
+      for (int i = 0; i < SETS; ++i) v += part[i][tid];
+      v *= sum != 0.f ? 1.f / sum : 0.f;
+      if (a.gate) v *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-1.44269504088896341f * __uint_as_float(gate << 16)));
+      a.o[orow * a.D + col] = __builtin_bit_cast(uint16_t, (__bf16)v);
+    }
+    row += gridDim.y;
+    if (row >= c.rows) return;
+    __syncthreads();  // (part is read)
+  }
 }
 
 // Tiles of many rows, mostly cut in few parts: 16 rows per workgroup, their weights while the first parts are on their way.
@@ -200,13 +208,15 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
 
 // The kernels of a call: requests of up to 32 rows per key head (tokens x query heads that share
 // it) on the kernel that streams, the others on the one for many rows.  Lengths are known on the
-// GPU only, so both are launched where both kinds can be there (a launch without work: 5 us); where
-// no request can have over 256 rows the streaming kernel takes them all, 32 at a time.
+// GPU only, so both are launched where both kinds can be expected (a launch without work: 5 us); where
+// shapes say that no request has over 256 rows, if each has a token, the streaming kernel takes
+// them all, 16 or 32 at a time.  That is a guess for speed only (a request may have none of the tokens and
+// another all of them): every kernel takes requests of any lengths.
 constexpr int ROWS_MOST = 32;
 
 struct Part {
   int tr = 0, grid = 0, min_rows = 0, max_rows = 0;
-  int rows = 0;       // of a tile at most
+  int rows = 0;       // of a tile, for the joining launch's grid (a tile may have more, up to tr)
   int by_tile = 0;
   int64_t tiles = 0;  // at most, per head
   size_t at = 0, desc = 0, ml = 0, acc = 0;
@@ -243,7 +253,7 @@ Route route_of(const AttnArgs &a) {
   int cus = device_cu_count();
   cus = (cus > 0 ? cus : 256) / 8 * 8;
   cus = cus < 8 ? 8 : cus < AC_MOST / 2 ? cus : AC_MOST / 2;
-  // (most: the rows of the longest request there can be, if each has a token)
+  // (most: the rows of the longest request, if each has a token)
   const int64_t most = (int64_t)(a.T > a.R ? a.T - a.R + 1 : 1) * r.g;
   const bool few = most <= 8 * ROWS_MOST;
   const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
