@@ -305,7 +305,8 @@ int qmm_mlp_forward_q(qmm_array *res, qmm_weight_map m, qmm_array x, const char 
  * block table [R, W] int32; -1 (or any id that is no page) stands for a page it does not have.
  * Lengths, tables and slots stay on the GPU: no call waits for them, and all of them can be
  * captured into a graph.  Head dimensions D are multiples of 8 from 8 to 256; arrays of
- * vectors must be 16-byte aligned. */
+ * vectors must be 16-byte aligned.  A result may be an input's handle, or lie over an input, only
+ * where that is said below; other such calls are refused before anything is freed or written. */
 
 /* The tables of one step.  cached_lens [R] tokens are in the cache, new_lens [R] come in this
  * step (negative: none), together at most n_tokens, the rows of the step's x (what is over is
@@ -316,8 +317,8 @@ int qmm_mlp_forward_q(qmm_array *res, qmm_weight_map m, qmm_array x, const char 
  *  q_starts [R + 1]: the first row of each request's new tokens, then their number;
  *  kv_lens [R]: cached plus new; positions, slots [n_tokens]: each row's position in its
  *  request and its cache slot (0 and -1 for rows of no request; -1 without a page).
- * table_out, head_out and kv_lens may be the handles of table, head and cached_lens (the update
- * is then in place).  R is at most 4096. */
+ * table_out, head_out and kv_lens may be the handles of table, head and cached_lens (or new_lens;
+ * the update is then in place).  R is at most 4096. */
 int qmm_block_tables(qmm_array *table_out, qmm_array *head_out, qmm_array *q_starts, qmm_array *kv_lens,
                      qmm_array *positions, qmm_array *slots, qmm_array table, qmm_array head, qmm_array cached_lens,
                      qmm_array new_lens, qmm_array free_blocks, int block_size, int n_tokens, qmm_stream s);
@@ -347,7 +348,8 @@ int qmm_rope(qmm_array *res, qmm_array x, qmm_array positions, qmm_array freqs, 
  * (x * rsqrt(mean(x^2) + norm_eps) * w over each head; w [D], bfloat16 or float32, or the null
  * handle for none) and the rotation of qmm_rope, q into *q_out [T, Hq, D], k and v [T, Hkv, D] into
  * the rows slots[t] of k_cache and v_cache (slots that are none, as -1, are left out).  q, k and v
- * all bfloat16 or all float32; results bfloat16, rounded once.  Two rows of one slot race. */
+ * all bfloat16 or all float32; results bfloat16, rounded once.  *q_out may be q's own handle where q
+ * is bfloat16 [T, Hq, D].  Two rows of one slot race. */
 int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_array q, qmm_array k, qmm_array v,
                    qmm_array positions, qmm_array slots, qmm_array freqs, float amplitude, bool interleaved,
                    qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s);
@@ -359,9 +361,10 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
  *  res [T, Hq, D] = softmax(scale q . k) v, zero for a row that sees nothing and for the rows
  *  from q_starts[R] on; times sigmoid(gate), if given: gate [T, Hq, Dg >= D] bfloat16, the last
  *  D values of each head (so the q projection's own array, where the gate lies beside the query).
- * Stale contents of pages past kv_lens do not reach the result, whatever they are.  R is at most
- * 4096, T Hq / Hkv at most 2^27, and a cache (here and in qmm_rope_cache) has at most 2^32 - 1
- * keys, those of all its heads counted.  Partial sums of contexts that several workgroups share lie in the stream's workspace
+ * Stale contents of pages past kv_lens do not reach the result, whatever they are.  *res may be q's
+ * own handle, or the gate's where Dg = D.  R is at most 4096, T Hq / Hkv at most 2^27, and a cache
+ * (here and in qmm_rope_cache) has at most 2^32 - 1 keys, those of all its heads counted.  Partial
+ * sums of contexts that several workgroups share lie in the stream's workspace
  * (see qmm_gdn_recurrence). */
 int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array table,
                         qmm_array q_starts, qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s);

@@ -86,3 +86,22 @@ def test_a_captured_step_whose_tokens_move_between_requests():
         want, bound = ref.attend(q, c.keys, c.values, starts.tolist(), lens, 1 / 16)
         assert not torch.isnan(got).any(), new
         assert ((got.double() - want).abs() <= bound).all(), new
+
+
+@pytest.mark.parametrize("Hq,Hkv,D,lens", [
+    (24, 4, 256, [(3000, 1), (5, 2)]), (8, 2, 128, [(300, 200), (900, 1), (0, 0), (17, 40)]), (4, 4, 72, [(0, 300)]),
+])
+def test_the_result_in_place_of_q_or_of_the_gate(Hq, Hkv, D, lens):
+    """The same bits as in an array of its own, whole tiles and joined ones, both kernels."""
+    new, kv = [n for _, n in lens], [c + n for c, n in lens]
+    T, g = sum(new) + 2, torch.Generator().manual_seed(D)
+    c = ref.Cache(kv, Hkv, D, 16, seed=D)
+    q, gate = (torch.randn(T, Hq, D, generator=g).to(torch.bfloat16) for _ in range(2))
+    starts = [0] + np.cumsum(new).tolist()
+    apart = into_nan(c, q, starts, kv, scale=0.1, gate=dev(gate))
+    for which in (0, 1):
+        a = [t.cuda() for t in (q, gate)]
+        h = [Q.Array.from_torch(t) for t in a]
+        Q.paged_attention(h[0], dev(c.k), dev(c.v), ints(c.table), ints(starts), ints(kv), scale=0.1, gate=h[1], out=h[which])
+        torch.cuda.synchronize()
+        assert torch.equal(a[which].cpu(), apart) and torch.equal(a[1 - which].cpu(), (q, gate)[1 - which])
