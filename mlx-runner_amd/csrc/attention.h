@@ -79,11 +79,9 @@ __device__ __forceinline__ AttnTile attn_tile(const AttnArgs &a, const AttnReq &
   t.e = p1 < cap ? p1 + 1 : cap;
   t.full_e = p0 < cap ? p0 + 1 : cap;
   t.b = 0, t.full_b = 0;
-  if (a.window) {
-    t.b = p0 - a.window + 1;
-    t.full_b = p1 - a.window + 1;
-    t.b = t.b < 0 ? 0 : t.b;
-    t.full_b = t.full_b < 0 ? 0 : t.full_b;
+  if (a.window) {  // (p0 may be below 0 and the window 2^31 - 1: no difference of them before the comparison)
+    t.b = p0 >= a.window ? p0 - a.window + 1 : 0;
+    t.full_b = p1 >= a.window ? p1 - a.window + 1 : 0;
   }
   if (t.e < t.b) t.e = t.b;  // (also no key at all: e <= 0)
   return t;
@@ -395,7 +393,7 @@ __device__ __forceinline__ void attn_poison(const AttnArgs &a, const AttnReq &q,
                                                       int row, int ks, int ke, int d0, float (&o)[8]) {
   const int pos = q.base + (int)attn_div(row, a.by_g);
   const int hi = pos < ke - 1 ? pos : ke - 1;
-  int lo = a.window && pos - a.window + 1 > ks ? pos - a.window + 1 : ks;
+  int lo = a.window && pos >= a.window && pos - a.window + 1 > ks ? pos - a.window + 1 : ks;
 #pragma unroll 1
   for (int key = lo; key <= hi; ++key) {
     const uint32_t page = attn_div(key, a.by_block);
