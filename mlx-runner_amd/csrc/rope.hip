@@ -228,7 +228,26 @@ void launch_pairs(const RopeArgs &a, unsigned grid, int lph, int parts, hipStrea
 
 }  // namespace
 
+// Tokens of a launch at most: a grid's lanes are counted in 32 bits (past that the count wraps, with no error).
+constexpr int ROPE_TOKENS = 1 << 23;
+static_assert((int64_t)ROPE_TOKENS * ROPE_THREADS < (int64_t)1 << 32, "lanes of a grid");
+
 hipError_t launch_rope(const RopeArgs &a, hipStream_t st) {
+  if (a.T > ROPE_TOKENS) {
+    RopeArgs part = a;
+    for (int t0 = 0; t0 < a.T; t0 += part.T) {
+      part.T = a.T - t0 < ROPE_TOKENS ? a.T - t0 : ROPE_TOKENS;
+      part.positions = a.positions + t0, part.slots = a.slots ? a.slots + t0 : nullptr;
+      for (int i = 0; i < a.sets; ++i) {
+        const int64_t row = (int64_t)t0 * a.set[i].heads;
+        part.set[i].in = (const char *)a.set[i].in + row * a.set[i].in_stride * (a.in_f32 ? 4 : 2);
+        if (!a.set[i].cache) part.set[i].out = (char *)a.set[i].out + row * a.D * (a.out_f32 ? 4 : 2);
+      }
+      const hipError_t e = launch_rope(part, st);
+      if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+  }
   if (a.T <= 0 || a.D < 8 || a.D > 256 || a.D % 8 || a.half < 0 || 2 * a.half > a.D || a.sets < 1 ||
       a.sets > ROPE_MAX_SETS || (!a.in_f32 && a.out_f32) || a.block < 1)
     return hipErrorInvalidValue;
@@ -243,7 +262,6 @@ hipError_t launch_rope(const RopeArgs &a, hipStream_t st) {
   const int64_t turns = (items + ROPE_THREADS / 64 - 1) / (ROPE_THREADS / 64);
   int64_t parts = 1024 / a.T;
   parts = parts < 1 ? 1 : parts > turns ? turns : parts;
-  if (a.T * parts > INT32_MAX) return hipErrorInvalidValue;
   const unsigned grid = (unsigned)(a.T * parts);
   a.half % 8    ? launch_pairs<ACROSS>(a, grid, lph, (int)parts, st)
   : a.interleaved ? launch_pairs<NEXT>(a, grid, lph, (int)parts, st)

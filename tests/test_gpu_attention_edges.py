@@ -40,3 +40,30 @@ def test_the_largest_windows_of_rows_before_the_first_key(new, kv, window):
     want, bound = ref.attend(q, c.keys, c.values, starts, kv, 0.125)
     got = attention(c, q, starts, kv, scale=0.125, window=window)
     assert ((got.double() - want).abs() <= bound).all() and (want != 0).any()
+
+
+def test_rotation_of_very_many_tokens():
+    """More tokens than one launch takes (2^32 lanes): the same bits as the tokens' own calls, in the rows of the cache
+    as well."""
+    T, D = 2 ** 24 + 77, 8
+    g = torch.Generator(device="cuda").manual_seed(45)
+    x = torch.randn(T, 1, D, generator=g, device="cuda").to(torch.bfloat16)
+    p = torch.randint(0, 262144, (T,), generator=g, device="cuda", dtype=torch.int32)
+    f = dev(torch.tensor([1.0, 0.25, 0.125, 0.01]))
+
+    def turned(a, b, norm):
+        k, v = (torch.zeros(1, 1, b - a, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        q, y = torch.empty(b - a, 1, D, dtype=torch.bfloat16, device="cuda"), torch.empty(b - a, 1, D, dtype=torch.bfloat16, device="cuda")
+        A = Q.Array.from_torch
+        Q.rope(A(x[a:b]), A(p[a:b], Q.INT32), f, out=A(y))
+        slots = torch.arange(b - a, dtype=torch.int32, device="cuda")
+        Q.rope_cache(A(x[a:b]), A(x[a:b]), A(x[a:b]), A(k), A(v), A(p[a:b], Q.INT32), A(slots, Q.INT32), f, q_out=A(q),
+                     q_norm=norm)
+        torch.cuda.synchronize()
+        return y, q, k[0, 0], v[0, 0]
+
+    norm = dev(torch.linspace(0.5, 2, D))
+    whole = turned(0, T, norm)
+    for a, b in ((0, 100), (2 ** 23 - 50, 2 ** 23 + 50), (2 ** 24 - 64, 2 ** 24 + 64 - 51), (T - 100, T)):
+        for w, part in zip(whole, turned(a, b, norm)):
+            assert torch.equal(w[a:b], part)
