@@ -137,11 +137,12 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
       const uint32_t ln = attn_lane();
       const int in = wv * 64 + u * 32 + (int)(ln & 31), lh = (int)(ln >> 5);
       const bool on = in < t.rows;
-      const int row = t.row0 + (on ? in : 0);  // (a row past the end: the first one's queries, and no keys)
+      const int row = t.row0 + (on ? in : 0);  // (a row past the end: the first one's queries)
       const int tok = (int)attn_div(row, a.by_g), pos = rq.base + tok;
       seen_at[(wv * 64 + (int)ln) * 4 + 2 * u] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
       seen_at[(wv * 64 + (int)ln) * 4 + 2 * u + 1] = on ? pos : -1;
-      m[u] = on && pos >= 0 ? -__builtin_inff() : 0.f;  // (a row that sees nothing needs no reference)
+      // (a row that sees nothing needs no reference; one past the end has no weights and passes none)
+      m[u] = !on ? __builtin_inff() : pos >= 0 ? -__builtin_inff() : 0.f;
       const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D + lh * 8;
 #pragma unroll
       for (int k = 0; k < KS; ++k) {

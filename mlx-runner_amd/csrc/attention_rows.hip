@@ -121,11 +121,12 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const bool on = n * 16 + lr < t.rows;
-      const int row = t.row0 + (on ? n * 16 + lr : 0);  // (a row past the end: the first one's queries, and no keys)
+      const int row = t.row0 + (on ? n * 16 + lr : 0);  // (a row past the end: the first one's queries)
       const int pos = rq.base + (int)attn_div(row, a.by_g);
       seen_at[here() * 4 + 2 * n] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
       seen_at[here() * 4 + 2 * n + 1] = on ? pos : -1;
-      m[n] = on && pos >= 0 ? -__builtin_inff() : 0.f;  // (a row that sees nothing needs no reference)
+      // (a row that sees nothing needs no reference; one past the end has no weights and passes none)
+      m[n] = !on ? __builtin_inff() : pos >= 0 ? -__builtin_inff() : 0.f;
       const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D + lg * 8;
 #pragma unroll
       for (int st = 0; st < ST; ++st) {

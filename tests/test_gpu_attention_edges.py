@@ -42,6 +42,26 @@ def test_the_largest_windows_of_rows_before_the_first_key(new, kv, window):
     assert ((got.double() - want).abs() <= bound).all() and (want != 0).any()
 
 
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_rows_past_a_tiles_end_have_no_part_in_it(D):
+    """A tile's rows beyond its request are filled up with its first row's queries.  However far that row's scores reach
+    (its own reference covers them), the other rows' results stay the same bits: nothing is run a second time for rows
+    that are none."""
+    new, L = 40, 540
+    c = ref.Cache([L], 1, D, 16, seed=43)
+    c.k[..., 5] = 0
+    for j, x in ((3, 0.5), (40, 1.0)):  # (400 x / 8 in powers of 2: 36, that row's reference, and 72, less than 2^60 past it)
+        c.k[int(c.table[0, j // 16]), 0, j % 16, 5] = x
+    q = torch.randn(new, 1, D, generator=torch.Generator().manual_seed(44)).to(torch.bfloat16)
+    q[:, 0, 5] = 0
+    got = []
+    for far in (4.0, 400.0):
+        q[0] = 0
+        q[0, 0, 5] = far
+        got.append(attention(c, q, [0, new], [L], scale=0.125))
+    assert torch.isfinite(got[1]).all() and torch.equal(got[0][1:], got[1][1:])
+
+
 def test_rotation_of_very_many_tokens():
     """More tokens than one launch takes (2^32 lanes): the same bits as the tokens' own calls, in the rows of the cache
     as well."""
