@@ -54,10 +54,10 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const AttnShare &s) {
   return c;
 }
 
-// One workgroup per tile, row (then every gridDim.y-th: the grid follows from shapes, a tile's rows from the lengths) and
-// COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every wave works out the partials' weights
-// for itself.
-template <int DP, int COLS>
+// One workgroup per tile, row and COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every
+// wave works out the partials' weights for itself.  MORE: tiles may have more rows than the grid, so a workgroup goes on to
+// every gridDim.y-th (what the compiler forms ahead of such a loop costs 0.2 us where there is one row for each).
+template <int DP, int COLS, bool MORE>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs a, const AttnShare s, int tr) {
   constexpr int LPR = COLS / 4;              // lanes of a row, four values each
   constexpr int SETS = ATTN_THREADS / LPR;   // partials side by side
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
   const int set = tid / LPR, d0 = blockIdx.z * COLS + tid % LPR * 4, col = blockIdx.z * COLS + tid;
   const bool in = d0 < a.D, out = tid < COLS && col < a.D;
 #pragma unroll 1
-  while (true) {
+  do {
     float2 ml[HELD];
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
@@ -125,10 +125,9 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
       if (a.gate) v *= __builtin_amdgcn_rcpf(1.f + attn_exp2(-1.44269504088896341f * __uint_as_float(gate << 16)));
       a.o[orow * a.D + col] = __builtin_bit_cast(uint16_t, (__bf16)v);
     }
+    if (MORE) __syncthreads();  // (part is read)
     row += gridDim.y;
-    if (row >= c.rows) return;
-    __syncthreads();  // (part is read)
-  }
+  } while (MORE && row < c.rows);
 }
 
 // Tiles of many rows, mostly cut in few parts: 16 rows per workgroup, their weights while the first parts are on their way.
@@ -216,7 +215,8 @@ constexpr int ROWS_MOST = 32;
 
 struct Part {
   int tr = 0, grid = 0, min_rows = 0, max_rows = 0;
-  int rows = 0;       // of a tile, for the joining launch's grid (a tile may have more, up to tr)
+  int rows = 0;       // of a tile, for the joining launch's grid
+  bool more = false;  // a tile may have more, up to tr
   int by_tile = 0;
   int64_t tiles = 0;  // at most, per head
   size_t at = 0, desc = 0, ml = 0, acc = 0;
@@ -261,7 +261,11 @@ Route route_of(const AttnArgs &a) {
     r.rows.tr = most <= 16 ? 16 : 32;
     r.rows.grid = 2 * cus;
     r.rows.min_rows = 0, r.rows.max_rows = few ? INT32_MAX : ROWS_MOST;
-    r.rows.rows = (int)(a.R == 1 && a.T * r.g < r.rows.tr ? a.T * r.g : a.T <= a.R && r.g < r.rows.tr ? r.g : r.rows.tr);
+    // (one token each, as when decoding, is the common case of T <= R; 16 rows for 6 would be 10 empty workgroups a tile)
+    const bool each = a.R > 1 && a.T <= a.R;
+    const int64_t rows = each ? r.g : (int64_t)a.T * r.g;
+    r.rows.rows = (int)(rows < r.rows.tr ? rows : r.rows.tr);
+    r.rows.more = each && r.rows.rows < r.rows.tr;
   }
   if (one || !few) {
     r.chunk.tr = r.chunk.rows = 256;
@@ -284,15 +288,24 @@ AttnShare share_of(const Part &p, void *workspace) {
   return s;
 }
 
+template <int DP, int COLS>
+void join_few(const AttnArgs &a, const Part &p, const AttnShare &s, unsigned n, hipStream_t st) {
+  const dim3 grid(n, p.rows, DP / COLS), block(ATTN_THREADS);
+  if (p.more)
+    hipLaunchKernelGGL((attn_join_kernel<DP, COLS, true>), grid, block, 0, st, a, s, p.tr);
+  else
+    hipLaunchKernelGGL((attn_join_kernel<DP, COLS, false>), grid, block, 0, st, a, s, p.tr);
+}
+
 template <int DP>
 void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) {
   const unsigned n = (unsigned)(p.by_tile ? p.tiles * a.Hkv : p.grid);
   if (p.tr > 32)
     hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(n, p.rows / AJ_ROWS), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
   else if (DP > 64 && n * (unsigned)p.rows <= 1024)
-    hipLaunchKernelGGL((attn_join_kernel<DP, 64>), dim3(n, p.rows, DP / 64), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+    join_few<DP, 64>(a, p, s, n, st);
   else
-    hipLaunchKernelGGL((attn_join_kernel<DP, DP>), dim3(n, p.rows), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
+    join_few<DP, DP>(a, p, s, n, st);
 }
 
 }  // namespace

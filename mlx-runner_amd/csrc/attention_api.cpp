@@ -3,6 +3,7 @@
 // its projections).
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cmath>
 #include <initializer_list>
 #include <vector>
@@ -71,36 +72,44 @@ int check_norm(const char *op, const char *name, const Arr *a, int D) {
   return 0;
 }
 
-// Whether *res's array serves as it is for a result of this shape and dtype (see alloc_arr).
-bool reused(const qmm_array *res, const std::vector<int> &shape, qmm_dtype dtype) {
-  const Arr *a = arr(*res);
-  if (!a || !a->data || a->dtype != dtype || a->ndim != (int)shape.size()) return false;
-  for (int i = 0; i < a->ndim; ++i)
-    if (a->shape[i] != shape[i]) return false;
-  return true;
-}
+struct Shape {
+  int ndim, dims[QMM_MAX_DIM];
+};
 
-bool overlap(const Arr *a, const Arr *b) {
-  const uintptr_t x = (uintptr_t)a->data, y = (uintptr_t)b->data;
-  return x && y && x < y + b->nbytes() && y < x + a->nbytes();
-}
+// An array and the bytes that it takes.
+struct Span {
+  const Arr *a;
+  uintptr_t lo, hi;
+  Span(const Arr *x) : a(x), lo(x ? (uintptr_t)x->data : 0), hi(lo ? lo + x->nbytes() : 0) {}
+};
+bool overlap(const Span &x, const Span &y) { return x.lo < y.hi && y.lo < x.hi; }
+
+// A result's handle before the call: none, one whose array serves as it is (see alloc_arr), or one that is replaced.
+struct Result {
+  const char *name;
+  const qmm_array *res;
+  Span cur;
+  bool kept;
+  Result(const char *n, const qmm_array *r, const Shape &s, qmm_dtype dtype) : name(n), res(r), cur(arr(*r)) {
+    const Arr *a = cur.a;
+    kept = cur.lo && a->dtype == dtype && a->ndim == s.ndim && std::equal(s.dims, s.dims + s.ndim, a->shape);
+  }
+};
 
 // A result may not be the handle of an input that it would replace (the input would be freed before it is read), nor lie
 // over an input, except exactly over one of `same`, which the kernels read before they write.
-int check_result(const char *op, const char *name, const qmm_array *res, const std::vector<int> &shape, qmm_dtype dtype,
-                 std::initializer_list<const Arr *> inputs, std::initializer_list<const Arr *> same = {}) {
-  const Arr *cur = arr(*res);
-  if (!cur) return 0;
-  const bool kept = reused(res, shape, dtype);
-  for (const Arr *in : inputs) {
-    if (!in) continue;
-    if (!kept) {
-      if (cur == in) return fail("[%s] %s is the handle of an input of another shape or type", op, name);
+int check_result(const char *op, const Result &r, std::initializer_list<Span> inputs, std::initializer_list<const Arr *> same) {
+  if (!r.cur.a) return 0;
+  for (const Span &in : inputs) {
+    if (!in.a) continue;
+    if (!r.kept) {
+      if (r.cur.a == in.a) return fail("[%s] %s is the handle of an input of another shape or type", op, r.name);
       continue;
     }
-    bool ok = !overlap(cur, in);
-    for (const Arr *x : same) ok = ok || (in == x && in->data == cur->data && in->nbytes() == cur->nbytes());
-    if (!ok) return fail("[%s] %s lies over an input", op, name);
+    if (!overlap(r.cur, in)) continue;
+    bool ok = false;
+    for (const Arr *x : same) ok = ok || (in.a == x && in.lo == r.cur.lo && in.hi == r.cur.hi);
+    if (!ok) return fail("[%s] %s lies over an input", op, r.name);
   }
   return 0;
 }
@@ -166,24 +175,18 @@ int qmm_block_tables(qmm_array *table_out, qmm_array *head_out, qmm_array *q_sta
   if (block_size < 1) return finish(fail("[%s] block_size must be positive, got %d", op, block_size));
   if (n_tokens < 0) return finish(fail("[%s] n_tokens must not be negative", op));
   if (R > BLOCK_TABLES_MAX_R) return finish(fail("[%s] %d requests: at most %d", op, R, BLOCK_TABLES_MAX_R));
-  {
-    const struct {
-      const char *name;
-      qmm_array *res;
-      std::vector<int> shape;
-      const Arr *same[2];
-    } out[] = {{"table_out", table_out, {R, W}, {ta}}, {"head_out", head_out, {1}, {ha}}, {"q_starts", q_starts, {R + 1}, {}},
-               {"kv_lens", kv_lens, {R}, {ca, na}}, {"positions", positions, {n_tokens}, {}}, {"slots", slots, {n_tokens}, {}}};
-    for (const auto &o : out) {
-      if (check_result(op, o.name, o.res, o.shape, QMM_INT32, {ta, ha, ca, na, fa}, {o.same[0], o.same[1]})) return finish(1);
-      for (const auto &p : out) {
-        if (&p == &o) break;
-        if (p.res == o.res || (arr(*p.res) && arr(*p.res) == arr(*o.res)) ||
-            (reused(p.res, p.shape, QMM_INT32) && reused(o.res, o.shape, QMM_INT32) && overlap(arr(*p.res), arr(*o.res))))
-          return finish(fail("[%s] %s lies over %s", op, o.name, p.name));
-      }
-    }
-  }
+  const Result out[] = {{"table_out", table_out, {2, {R, W}}, QMM_INT32}, {"head_out", head_out, {1, {1}}, QMM_INT32},
+                        {"q_starts", q_starts, {1, {R + 1}}, QMM_INT32}, {"kv_lens", kv_lens, {1, {R}}, QMM_INT32},
+                        {"positions", positions, {1, {n_tokens}}, QMM_INT32}, {"slots", slots, {1, {n_tokens}}, QMM_INT32}};
+  const std::initializer_list<Span> inputs = {ta, ha, ca, na, fa};
+  if (check_result(op, out[0], inputs, {ta}) || check_result(op, out[1], inputs, {ha}) ||
+      check_result(op, out[2], inputs, {}) || check_result(op, out[3], inputs, {ca, na}) ||
+      check_result(op, out[4], inputs, {}) || check_result(op, out[5], inputs, {}))
+    return finish(1);
+  for (const Result &o : out)
+    for (const Result *p = out; p != &o; ++p)
+      if (p->res == o.res || (o.cur.a && o.cur.a == p->cur.a) || (o.kept && p->kept && overlap(o.cur, p->cur)))
+        return finish(fail("[%s] %s lies over %s", op, o.name, p->name));
   hipStream_t st = stream_of(s);
   Arr *to, *ho, *qo, *ko, *po, *so;
   if (alloc_arr(table_out, {R, W}, QMM_INT32, st, &to) || alloc_arr(head_out, {1}, QMM_INT32, st, &ho) ||
@@ -217,11 +220,12 @@ int qmm_rope(qmm_array *res, qmm_array x, qmm_array positions, qmm_array freqs, 
   for (int i = 0; i < xa->ndim - 2; ++i) T *= xa->shape[i];
   if (T > INT32_MAX) return finish(fail("[%s] too many tokens", op));
   if (check_int(op, "positions", pa, {(int)T})) return finish(1);
-  const std::vector<int> shape(xa->shape, xa->shape + xa->ndim);
-  if (check_result(op, "the result", res, shape, xa->dtype, {xa, pa, fa}, {xa})) return finish(1);
+  Shape shape{xa->ndim, {}};
+  std::copy(xa->shape, xa->shape + xa->ndim, shape.dims);
+  if (check_result(op, {"the result", res, shape, xa->dtype}, {xa, pa, fa}, {xa})) return finish(1);
   hipStream_t st = stream_of(s);
   Arr *ya;
-  if (alloc_arr(res, shape, xa->dtype, st, &ya)) return finish(1);
+  if (alloc_arr(res, std::vector<int>(xa->shape, xa->shape + xa->ndim), xa->dtype, st, &ya)) return finish(1);
   if (misaligned(ya)) return finish(fail("[%s] the result must be 16-byte aligned", op));
   if (T == 0 || H == 0) return finish(0);
   RopeArgs a{};
@@ -266,7 +270,7 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
   const Arr *qc = arr(*q_out);
   if (qc && (qc == qa || (qc->data && qc->data == qa->data)) && (qa->shape[2] != D || qa->dtype != QMM_BFLOAT16))
     return finish(fail("[%s] q_out can be q's own array only at q's layout", op));
-  if (check_result(op, "q_out", q_out, {T, Hq, D}, QMM_BFLOAT16, {qa, ka, va, kc, vc, pa, sa, fa, qn, kn}, {qa}))
+  if (check_result(op, {"q_out", q_out, {3, {T, Hq, D}}, QMM_BFLOAT16}, {qa, ka, va, kc, vc, pa, sa, fa, qn, kn}, {qa}))
     return finish(1);
   hipStream_t st = stream_of(s);
   Arr *qo;
@@ -324,7 +328,8 @@ int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_arra
   a.NB = NB, a.block = block, a.window = window, a.scale = scale;
   const char *too_much = attention_limits(a);
   if (too_much) return finish(fail("[%s] too many %s", op, too_much));
-  if (check_result(op, "the result", res, {T, Hq, D}, QMM_BFLOAT16, {qa, kc, vc, ta, sa, la, ga}, {qa, ga})) return finish(1);
+  if (check_result(op, {"the result", res, {3, {T, Hq, D}}, QMM_BFLOAT16}, {qa, kc, vc, ta, sa, la, ga}, {qa, ga}))
+    return finish(1);
   hipStream_t st = stream_of(s);
   Arr *oa;
   if (alloc_arr(res, {T, Hq, D}, QMM_BFLOAT16, st, &oa)) return finish(1);
