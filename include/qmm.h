@@ -363,9 +363,10 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
  *  D values of each head (so the q projection's own array, where the gate lies beside the query).
  * Stale contents of pages past kv_lens do not reach the result, whatever they are.  *res may be q's
  * own handle, or the gate's where Dg = D.  R is at most 4096, T Hq / Hkv at most 2^27, and a cache
- * (here and in qmm_rope_cache) has at most 2^32 - 1 keys, those of all its heads counted.  Partial
- * sums of contexts that several workgroups share lie in the stream's workspace
- * (see qmm_gdn_recurrence). */
+ * (here and in qmm_rope_cache) has at most 2^32 - 1 keys, those of all its heads counted.  Scores,
+ * softmax statistics and sums are float32; the softmax's weights go into their product with v as two
+ * bfloat16 parts (2^-17) for requests of few rows, rounded to bfloat16 for others.  Partial sums of
+ * contexts that several workgroups share lie in the stream's workspace (see qmm_gdn_recurrence). */
 int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array table,
                         qmm_array q_starts, qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s);
 

@@ -11,10 +11,12 @@
 //
 // The products of one half tile's weights with the values are issued together with the
 // exponentials of the next one's scores, so that the vector unit works while the matrix unit does.
-// Weights are rounded to bf16 for the product (see attention_rows.hip).  They are relative to the
-// row's first maximum, not to the running one: bf16 and f32 hold weights of 2^60 as exactly as
-// those below 1, and nothing is left to multiply the sums with in the loop.  A tile with a score
-// past 2^60 times its reference is run again from the maxima that the first time has found.
+// Weights are rounded to bf16 for the product, 2^-9 of each: a second part (as for few rows) would be
+// half as many products again, of a kernel that they bound.  The sum that they are divided by is that of the
+// rounded ones, so that a row of one heavy key is exact.  They are relative to the row's first
+// maximum, not to the running one: bf16 and f32 hold weights of 2^60 as exactly as those below 1, and
+// nothing is left to multiply the sums with in the loop.  A tile with a score past 2^60 times its
+// reference is run again from the maxima that the first time has found.
 #include "attention.h"
 #include "gemm_pipe.h"
 
@@ -401,7 +403,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         special(ks + i * CH_KT + 32, (uint32_t)(valid >> 32), edge);
         // values of tile i (the page ids and keys asked for after them may be on their way)
         asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OPS + 1) : "memory");
-        const int own = ks + i * CH_KT + wv * 16;  // (the values that this wave has moved; see attention_rows.hip)
+        const int own = ks + i * CH_KT + wv * 16;  // (the values that this wave has moved)
         if (edge && (((valid >> wv * 16) & 0xFFFFu) != 0xFFFFu || (again && (own < t.full_b || own + 16 > t.full_e)))) {
           const uint32_t ln = attn_lane();
           bool odd = false;

@@ -11,9 +11,8 @@
 // S^T = K Q^T and O^T = V^T P^T on the 16x16 MFMA.  In S^T a lane holds one row (lane % 16) and
 // keys 4 (lane / 16) .. + 3: the shape that P^T needs as the second operand when the keys of a
 // product are taken in that order, so the weights never leave their registers; V^T comes through
-// the transposing LDS read in the same order of keys.  The weights are rounded to bf16 for that
-// product (2^-9 of each, which averages out over keys; the sum they are divided by is that of the
-// rounded ones, so that a row of one heavy key is exact).
+// the transposing LDS read in the same order of keys.  A weight goes into that product as two bf16
+// parts, its rounding and what that has taken (2^-17 of it is lost): HBM leaves the matrix cores the time.
 #include "attention.h"
 #include "gemm_pipe.h"
 
@@ -281,7 +280,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
             for (int d = 0; d < DT; ++d) acc[n][d] *= f;
           }
         }
-        i16x4_t p[NQ][KB];
+        i16x4_t p[NQ][KB], pl[NQ][KB];  // weights rounded, and what the rounding has taken
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
           const float ref = m[n] == -__builtin_inff() ? 0.f : m[n];
@@ -289,11 +288,15 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              bf16x2_t x;
-              x[0] = (__bf16)attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
-              x[1] = (__bf16)attn_exp2(__builtin_fmaf(sv[n][b][i + 1], sc, -ref));
-              l[n] = dot2_bf16(x, 0x3F803F80u, l[n]);
+              const float e0 = attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
+              const float e1 = attn_exp2(__builtin_fmaf(sv[n][b][i + 1], sc, -ref));
+              l[n] += e0 + e1;
+              bf16x2_t x, y;
+              x[0] = (__bf16)e0, x[1] = (__bf16)e1;
+              const uint32_t w = __builtin_bit_cast(uint32_t, x);
+              y[0] = (__bf16)(e0 - __uint_as_float(w << 16)), y[1] = (__bf16)(e1 - __uint_as_float(w & 0xFFFF0000u));
               p[n][b][i] = __builtin_bit_cast(short, (__bf16)x[0]), p[n][b][i + 1] = __builtin_bit_cast(short, (__bf16)x[1]);
+              pl[n][b][i] = __builtin_bit_cast(short, (__bf16)y[0]), pl[n][b][i + 1] = __builtin_bit_cast(short, (__bf16)y[1]);
             }
         }
         // the values
@@ -346,13 +349,17 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
             const int d = j / CB, b = j % CB * 2;
 #pragma unroll
             for (int n = 0; n < NQ; ++n) {
-              if constexpr (KB == 1) {
-                const i16x4_t v0 = __builtin_shufflevector(vf[j], vf[j], 0, 1, 2, 3);
-                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(v0, p[n][0], acc[n][d], 0, 0, 0);
-              } else {
-                const i16x8_t pf = __builtin_shufflevector(p[n][b], p[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+              if constexpr (KB == 1) {  // (one product: 16 keys with the weights, the same 16 with their rests)
+                const i16x8_t pf = __builtin_shufflevector(p[n][0], pl[n][0], 0, 1, 2, 3, 4, 5, 6, 7);
                 acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[j]),
                                                                     __builtin_bit_cast(bf16x8_t, pf), acc[n][d], 0, 0, 0);
+              } else {
+                const i16x8_t pf = __builtin_shufflevector(p[n][b], p[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                const i16x8_t pr = __builtin_shufflevector(pl[n][b], pl[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[j]),
+                                                                    __builtin_bit_cast(bf16x8_t, pf), acc[n][d], 0, 0, 0);
+                acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, vf[j]),
+                                                                    __builtin_bit_cast(bf16x8_t, pr), acc[n][d], 0, 0, 0);
               }
             }
             if (j % 2) __builtin_amdgcn_sched_barrier(0);
@@ -412,7 +419,17 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
             o[0] += f[v] * x.x, o[1] += f[v] * x.y, o[2] += f[v] * x.z, o[3] += f[v] * x.w;
             o[4] += f[v] * y.x, o[5] += f[v] * y.y, o[6] += f[v] * y.z, o[7] += f[v] * y.w;
           }
-          if (*poison) attn_poison(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, o);
+          float z = 0.f;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) z = __builtin_fmaf(o[e], 0.f, z);
+          if (*poison || z != 0.f) {
+            // values that are not finite: those held back; and those that met both parts of a weight (inf - inf), whose
+            // own sum says what the result is
+            float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            attn_poison(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, x);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) o[e] = o[e] * 0.f == 0.f ? o[e] + x[e] : x[e] * 0.f == 0.f ? o[e] : x[e];
+          }
           if (whole) {
             const float inv = sum != 0.f ? 1.f / sum : 0.f;
 #pragma unroll
