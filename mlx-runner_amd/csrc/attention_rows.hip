@@ -15,7 +15,7 @@
 // parts, its rounding and what that has taken (2^-17 of it is lost): HBM leaves the matrix cores the time.
 //
 // One token over 262144 keys (24 query heads on 4 of 256; 1.07 GB, each byte fetched once): 189-191 us, 5.65
-// TB/s, the matrix cores 6% busy.  64 requests of 1 to 8192 keys (32 on 8 of 128; 370 MB): 77-78 us.
+// TB/s, the matrix cores 6% busy.  64 requests of 1 to 8192 keys (32 on 8 of 128; 370 MB): 77-79 us.
 #include "attention.h"
 #include "gemm_pipe.h"
 
@@ -425,9 +425,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           float z = 0.f;
 #pragma unroll
           for (int e = 0; e < 8; ++e) z = __builtin_fmaf(o[e], 0.f, z);
-          if (*poison || z != 0.f) {
+          if (*poison || (z != 0.f && sum == sum)) {
             // values that are not finite: those held back; and those that met both parts of a weight (inf - inf), whose
-            // own sum says what the result is
+            // own sum says what the result is (where weights are NaN, as of NaN queries, it is that anyway)
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
             attn_poison(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, x);
 #pragma unroll

@@ -86,3 +86,20 @@ def test_finite_sums_past_f32_stay_infinite():
     q = torch.ones(1, 2, D, dtype=torch.bfloat16)
     got = into_nan(c, q, [0, 1], [L], 1.0)
     assert (got[..., 0] == math.inf).all() and torch.isfinite(got[..., 1:]).all()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_a_query_that_is_not_a_number_is_its_own_rows_only(D):
+    """NaN queries (rows that nobody reads, in a step of a fixed size) give NaN, whatever the values, and the tile's other
+    rows what they are without them."""
+    L = 2000
+    c = ref.Cache([L], 1, D, 16, seed=54)
+    c.values[0][700, 0, 2] = math.inf
+    rewrite(c, 0)
+    q = torch.randn(3, 4, D, generator=torch.Generator().manual_seed(55)).to(torch.bfloat16)
+    plain = into_nan(c, q, [0, 3], [L], D ** -0.5).cpu()
+    q[1, 2] = math.nan
+    got = into_nan(c, q, [0, 3], [L], D ** -0.5).cpu()
+    assert torch.isnan(got[1, 2]).all()
+    got[1, 2] = plain[1, 2]
+    assert torch.equal(got, plain)
