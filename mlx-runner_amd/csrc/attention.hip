@@ -212,7 +212,9 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
 // GPU only, so both are launched where both kinds can be expected (a launch without work: 3-5 us); where
 // shapes say that no request has over 256 rows, if each has a token, the streaming kernel takes
 // them all, 16 or 32 at a time.  That is a guess for speed only (a request may have none of the tokens and
-// another all of them): every kernel takes requests of any lengths.
+// another all of them): every kernel takes requests of any lengths.  Without the guess every decode step of many
+// requests would launch the second kernel and its join (7 us beside 77); with it, 512 tokens in one of 512
+// slots take 58 us, 55 on the kernel for chunks (24 heads on 4 of 256).
 constexpr int ROWS_MOST = 32;
 
 struct Part {
