@@ -370,6 +370,37 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
 int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array table,
                         qmm_array q_starts, qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s);
 
+/* ---- the same over a cache held in 8 bits ----
+ * Codes are E4M3 [pages, Hkv, block, D] uint8 (D a multiple of 16 from 16 to 256, 16-byte aligned), with a scale for each
+ * page and head, [pages, Hkv] uint8: byte X stands for 2^(X - 127), 255 for NaN (E8M0, as mxfp8's).  Half the bytes of a
+ * bfloat16 cache, in the same block tables and slots.  Keys and values have codes and scales of their own. */
+
+/* qmm_rope_cache into such a cache: q as there; k and v, after their norm and rotation in float32, become codes.  The
+ * call's rows of one page must follow one another in slots, as qmm_block_tables gives them (rows without a slot may lie
+ * before and after them; two runs of one page, like two rows of one slot, race).  For each page and head that they reach, m the largest finite |value| of theirs and t the smallest exponent, at
+ * least -127, with 448 * 2^t >= m:
+ *  where the page's first row is among them the page starts anew: its scale becomes 2^t (what its other rows held is lost);
+ *  elsewhere the scale becomes the larger of 2^t and the one before; if it grew, the codes that the page holds are divided
+ *  by what it grew by (exact but where they become subnormal; rounded to nearest even).
+ * A value x becomes the code nearest to x / scale, ties to even; infinities and NaN become NaN.  k_cache, v_cache,
+ * k_scales and v_scales must not overlap one another or an input. */
+int qmm_rope_cache_fp8(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales, qmm_array v_scales,
+                       qmm_array q, qmm_array k, qmm_array v, qmm_array positions, qmm_array slots, qmm_array freqs,
+                       float amplitude, bool interleaved, qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s);
+
+/* Rows of such a cache read back: k_out[t] = code * 2^(scale - 127) of row slots[t] (int32 [T]; zeros for a slot that is
+ * none, as -1), [T, Hkv, D] of `dtype` (bfloat16 or float32, exact but where bfloat16 underflows); v_out likewise.
+ * k_out or v_out may be NULL: that one is not read, and its cache and scales may be null handles. */
+int qmm_cache_read_fp8(qmm_array *k_out, qmm_array *v_out, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
+                       qmm_array v_scales, qmm_array slots, qmm_dtype dtype, qmm_stream s);
+
+/* qmm_paged_attention over such a cache, with the same arguments, limits and rules (stale codes and scales of what a row
+ * does not see do not reach it).  Keys and values are what qmm_cache_read_fp8 gives in float32.  A query that is not finite
+ * gives NaN. */
+int qmm_paged_attention_fp8(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
+                            qmm_array v_scales, qmm_array table, qmm_array q_starts, qmm_array kv_lens, qmm_array gate,
+                            float scale, int window, qmm_stream s);
+
 /* Library / device info. */
 const char *qmm_version(void);
 int qmm_device_info(char *buf, size_t len);

@@ -387,8 +387,18 @@ __device__ __forceinline__ uint4 attn_finite(uint4 x) {
   return make_uint4(attn_finite(x.x), attn_finite(x.y), attn_finite(x.z), attn_finite(x.w));
 }
 
+// E4M3 codes in fours, NaN replaced by zero.
+__device__ __forceinline__ uint32_t attn_finite_codes(uint32_t x) {
+  const uint32_t nan = ((x & 0x7F7F7F7Fu) + 0x01010101u) & 0x80808080u;
+  return x & ~((nan >> 7) * 0xFFu);
+}
+__device__ __forceinline__ uint4 attn_finite_codes(uint4 x) {
+  return make_uint4(attn_finite_codes(x.x), attn_finite_codes(x.y), attn_finite_codes(x.z), attn_finite_codes(x.w));
+}
+
 // Adds to 8 sums of a row the values that are not finite of the keys in [ks, ke) that it sees: what was
 // left out where the rows of a tile see different keys.  Slow, and only where there are any.
+template <bool E8 = false>
 __device__ __forceinline__ void attn_poison(const AttnArgs &a, const AttnReq &q, const int *tabrow, int head,
                                                       int row, int ks, int ke, int d0, float (&o)[8]) {
   const int pos = q.base + (int)attn_div(row, a.by_g);
@@ -400,6 +410,14 @@ __device__ __forceinline__ void attn_poison(const AttnArgs &a, const AttnReq &q,
     const int blk = tabrow[page];
     if ((uint32_t)blk >= (uint32_t)a.NB) continue;
     const uint64_t r = ((uint64_t)blk * a.Hkv + head) * a.block + ((uint32_t)key - page * (uint32_t)a.block);
+    if constexpr (E8) {  // (codes that are NaN, scales that are)
+      const uint2 v = *(const uint2 *)((const uint8_t *)a.v + r * a.D + d0);
+      const bool all = a.v_scales[(uint64_t)blk * a.Hkv + head] == 255;
+#pragma unroll
+      for (int e = 0; e < 8; ++e)
+        if (all || ((e < 4 ? v.x : v.y) >> 8 * (e & 3) & 127u) == 127u) o[e] = __uint_as_float(0x7FC00000u);
+      continue;
+    }
     const uint4 v = *(const uint4 *)(a.v + r * a.D + d0);
     const uint32_t x[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
@@ -417,6 +435,12 @@ __device__ __forceinline__ int attn_swz(int row) {
   return DP >= 128 ? row & 15 : (row >> 1) & 7;
 }
 
+
+// The same for E4M3 codes: rows of DP bytes.
+template <int DP>
+__device__ __forceinline__ int attn_swz8(int row) {
+  return DP >= 256 ? row & 15 : DP >= 128 ? (row >> 1) & 7 : (row >> 2) & 3;
+}
 
 // A value that the compiler takes as new here: what follows from it (swizzled addresses) is formed
 // again where it is used, a few xors, instead of being kept in registers through the loop.
@@ -440,6 +464,53 @@ __device__ __forceinline__ uint4 attn_zeros() {
 // x of lane ^ `other`.
 __device__ __forceinline__ float attn_across(float x, int other) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(((int)attn_lane() ^ other) * 4, __float_as_int(x)));
+}
+
+// 128 bf16 values of a row, 32 to a lane (of those 16 and 32 apart), as two E4M3 parts, each with a scale 2^t of its own:
+// x = hi 2^th + lo 2^tl.  Two 4-bit significands hold bf16's 8 bits, so what is lost is 2^-22 of the 128 values' largest, if
+// anything.  (The matrix unit takes a scale for every 32 values, but those are 16 of two lanes.)  The scales as bytes of its
+// operand; 255 (NaN) where a value is not finite.
+__device__ __forceinline__ void attn_split(const u32x4_t (&x)[4], i32x8_t &hi, i32x8_t &lo, int &scale_hi, int &scale_lo) {
+  float v[32], top = 0.f, rest = 0.f;
+  bool odd = false;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const uint32_t w = x[i / 4][i % 4];
+    v[2 * i] = __uint_as_float(w << 16), v[2 * i + 1] = __uint_as_float(w & 0xFFFF0000u);
+    odd |= (w & 0x7F80u) == 0x7F80u || (w & 0x7F800000u) == 0x7F800000u;
+  }
+#pragma unroll
+  for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
+  top = odd ? __builtin_inff() : top;
+  top = fmaxf(top, attn_across(top, 16));
+  top = fmaxf(top, attn_across(top, 32));
+  odd = top == __builtin_inff();
+  const int th = odd ? 0 : top > 0.f ? ceil_scale_exp(top) : -127;
+  const float sh = e8m0_scale_operand(th);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    i16x2_t c = {0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[4 * i], v[4 * i + 1], sh, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[4 * i + 2], v[4 * i + 3], sh, true);
+    hi[i] = __builtin_bit_cast(int, c);
+    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi[i], sh, false);
+    const f32x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi[i], sh, true);
+    v[4 * i] -= a.x, v[4 * i + 1] -= a.y, v[4 * i + 2] -= b.x, v[4 * i + 3] -= b.y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) rest = fmaxf(rest, fabsf(v[4 * i + j]));
+  }
+  rest = fmaxf(rest, attn_across(rest, 16));
+  rest = fmaxf(rest, attn_across(rest, 32));
+  const int tl = odd ? 0 : rest > 0.f ? ceil_scale_exp(rest) : -127;
+  const float sl = e8m0_scale_operand(tl);
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    i16x2_t c = {0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[4 * i], v[4 * i + 1], sl, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, v[4 * i + 2], v[4 * i + 3], sl, true);
+    lo[i] = __builtin_bit_cast(int, c);
+  }
+  scale_hi = odd ? 255 : th + 127, scale_lo = odd ? 255 : tl + 127;
 }
 
 // A kernel's arguments (at `offset` of its argument block) read again where they are needed, instead of
@@ -466,8 +537,16 @@ __device__ __forceinline__ i16x4_t attn_read_tr(uint32_t at) {
   return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) i16x4_t *)(uintptr_t)at);
 }
 
+// 16 lanes give the addresses of eight rows of 16 bytes, lane i that of bytes 8 (i % 2) of row i / 2; lane i gets column i
+// of the eight rows.
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ i32x2_t attn_read_tr8(uint32_t at) {
+  return __builtin_amdgcn_ds_read_tr8_b64_v2i32((__attribute__((address_space(3))) i32x2_t *)(uintptr_t)at);
+}
+
 // Launches of the kernels (the workspace's parts in s).
-size_t attn_rows_lds(int DP, int R);
+size_t attn_rows_lds(int DP, int R, bool fp8);
 size_t attn_chunk_lds(int DP, int R);
 hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st);
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st);

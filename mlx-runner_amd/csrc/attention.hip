@@ -259,8 +259,8 @@ Route route_of(const AttnArgs &a) {
   cus = cus < 8 ? 8 : cus < AC_MOST / 2 ? cus : AC_MOST / 2;
   // (most: the rows of the longest request, if each has a token)
   const int64_t most = (int64_t)(a.T > a.R ? a.T - a.R + 1 : 1) * r.g;
-  const bool few = most <= 8 * ROWS_MOST;
-  const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
+  const bool few = a.k_scales || most <= 8 * ROWS_MOST;
+  const bool one = !a.k_scales && a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
   if (!one) {
     r.rows.tr = most <= 16 ? 16 : 32;
     r.rows.grid = 2 * cus;

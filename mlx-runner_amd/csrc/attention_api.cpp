@@ -37,11 +37,11 @@ bool misaligned(const Arr *a) { return ((uintptr_t)a->data & 15) != 0; }
 
 bool floating(const Arr *a) { return a->dtype == QMM_BFLOAT16 || a->dtype == QMM_FLOAT32; }
 
-// [pages, heads, block, D] bfloat16, 16-byte aligned.
-int check_cache(const char *op, const char *name, const Arr *a) {
+// [pages, heads, block, D] bfloat16 (or E4M3 codes), 16-byte aligned.
+int check_cache(const char *op, const char *name, const Arr *a, bool fp8 = false) {
   if (!a) return fail("[%s] missing %s", op, name);
-  if (a->dtype != QMM_BFLOAT16 || a->ndim != 4)
-    return fail("[%s] %s must be a bfloat16 array [pages, heads, block, D]", op, name);
+  if (a->dtype != (fp8 ? QMM_UINT8 : QMM_BFLOAT16) || a->ndim != 4)
+    return fail("[%s] %s must be a %s array [pages, heads, block, D]", op, name, fp8 ? "uint8" : "bfloat16");
   if (a->shape[1] < 1 || a->shape[2] < 1) return fail("[%s] %s needs heads and a block size", op, name);
   if ((double)a->shape[0] * a->shape[1] * a->shape[2] > UINT32_MAX)  // (they are counted in 32 bits)
     return fail("[%s] %s has over 2^32 - 1 keys", op, name);
@@ -49,10 +49,37 @@ int check_cache(const char *op, const char *name, const Arr *a) {
   return 0;
 }
 
-int check_head_dim(const char *op, int D) {
-  if (D < 8 || D > 256 || D % 8)
-    return fail("[%s] the head dimension must be a multiple of 8 from 8 to 256, got %d", op, D);
+int check_head_dim(const char *op, int D, bool fp8 = false) {
+  const int step = fp8 ? 16 : 8;
+  if (D < step || D > 256 || D % step)
+    return fail("[%s] the head dimension must be a multiple of %d from %d to 256, got %d", op, step, step, D);
   return 0;
+}
+
+// Scale bytes [pages, heads] of a cache of codes.
+int check_scales(const char *op, const char *name, const Arr *a, const Arr *cache) {
+  if (!a) return fail("[%s] missing %s", op, name);
+  if (a->dtype != QMM_UINT8 || a->ndim != 2 || a->shape[0] != cache->shape[0] || a->shape[1] != cache->shape[1])
+    return fail("[%s] %s must be a uint8 array [%d, %d]", op, name, cache->shape[0], cache->shape[1]);
+  return 0;
+}
+
+// A layer's cache: its arrays (scales of a cache of codes only) and their shape.
+struct Cache {
+  const Arr *k, *v, *ks = nullptr, *vs = nullptr;
+  int NB, Hkv, block, D;
+  bool fp8;
+};
+int check_caches(const char *op, Cache &c, qmm_array k, qmm_array v, const qmm_array *k_scales, const qmm_array *v_scales) {
+  c.k = arr(k), c.v = arr(v), c.fp8 = k_scales != nullptr;
+  if (check_cache(op, "k_cache", c.k, c.fp8) || check_cache(op, "v_cache", c.v, c.fp8)) return 1;
+  for (int i = 0; i < 4; ++i)
+    if (c.k->shape[i] != c.v->shape[i]) return fail("[%s] k_cache and v_cache shapes differ", op);
+  c.NB = c.k->shape[0], c.Hkv = c.k->shape[1], c.block = c.k->shape[2], c.D = c.k->shape[3];
+  if (check_head_dim(op, c.D, c.fp8)) return 1;
+  if (!c.fp8) return 0;
+  c.ks = arr(*k_scales), c.vs = arr(*v_scales);
+  return check_scales(op, "k_scales", c.ks, c.k) || check_scales(op, "v_scales", c.vs, c.v);
 }
 
 int check_freqs(const char *op, const Arr *f, int D) {
@@ -111,6 +138,119 @@ int check_result(const char *op, const Result &r, std::initializer_list<Span> in
     for (const Arr *x : same) ok = ok || (in.a == x && in.lo == r.cur.lo && in.hi == r.cur.hi);
     if (!ok) return fail("[%s] %s lies over an input", op, r.name);
   }
+  return 0;
+}
+
+// qmm_rope_cache and, with scales, qmm_rope_cache_fp8.
+int rope_cache(const char *op, qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, const qmm_array *k_scales,
+               const qmm_array *v_scales, qmm_array q, qmm_array k, qmm_array v, qmm_array positions, qmm_array slots,
+               qmm_array freqs, float amplitude, bool interleaved, qmm_array q_norm, qmm_array k_norm, float norm_eps,
+               qmm_stream s) {
+  if (!q_out) return fail("[%s] null result pointer", op);
+  Cache c;
+  if (check_caches(op, c, k_cache, v_cache, k_scales, v_scales)) return 1;
+  const int NB = c.NB, Hkv = c.Hkv, block = c.block, D = c.D;
+  Arr *qa = arr(q), *ka = arr(k), *va = arr(v), *pa = arr(positions), *sa = arr(slots), *fa = arr(freqs),
+      *qn = arr(q_norm), *kn = arr(k_norm);
+  if (check_freqs(op, fa, D)) return 1;
+  if (!qa || !ka || !va) return fail("[%s] missing input", op);
+  if (!floating(qa) || ka->dtype != qa->dtype || va->dtype != qa->dtype)
+    return fail("[%s] q, k, v must all be bfloat16 or all float32", op);
+  if (qa->ndim != 3 || qa->shape[2] < D || qa->shape[2] % 8)
+    return fail("[%s] q must be [T, Hq, %d or more, a multiple of 8]", op, D);
+  const int T = qa->shape[0], Hq = qa->shape[1];
+  for (const Arr *x : {ka, va})
+    if (x->ndim != 3 || x->shape[0] != T || x->shape[1] != Hkv || x->shape[2] != D)
+      return fail("[%s] k and v must be [%d, %d, %d]", op, T, Hkv, D);
+  if (check_int(op, "positions", pa, {T}) || check_int(op, "slots", sa, {T})) return 1;
+  if (check_norm(op, "q_norm", qn, D) || check_norm(op, "k_norm", kn, D)) return 1;
+  if (misaligned(qa) || misaligned(ka) || misaligned(va)) return fail("[%s] q, k and v must be 16-byte aligned", op);
+  const Arr *qc = arr(*q_out);
+  if (qc && (qc == qa || (qc->data && qc->data == qa->data)) && (qa->shape[2] != D || qa->dtype != QMM_BFLOAT16))
+    return fail("[%s] q_out can be q's own array only at q's layout", op);
+  const std::initializer_list<Span> inputs = {qa, ka, va, c.k, c.v, pa, sa, fa, qn, kn, c.ks, c.vs};
+  if (check_result(op, {"q_out", q_out, {3, {T, Hq, D}}, QMM_BFLOAT16}, inputs, {qa})) return 1;
+  if (c.fp8) {  // (what it writes is read again: pages whose scale grows)
+    const Arr *const written[] = {c.k, c.v, c.ks, c.vs};
+    for (const Arr *const *x = written; x != written + 4; ++x) {
+      for (const Arr *const *y = written; y != x; ++y)
+        if (overlap(*x, *y)) return fail("[%s] the caches and their scales lie over one another", op);
+      for (const Arr *y : {qa, ka, va, pa, sa, fa, qn, kn})
+        if (y && overlap(*x, y)) return fail("[%s] the caches and their scales lie over an input", op);
+    }
+  }
+  hipStream_t st = stream_of(s);
+  Arr *qo;
+  if (alloc_arr(q_out, {T, Hq, D}, QMM_BFLOAT16, st, &qo)) return 1;
+  if (misaligned(qo)) return fail("[%s] the result must be 16-byte aligned", op);
+  if (T == 0) return 0;
+  RopeArgs a{};
+  a.set[0] = RopeHeads{qa->data, qo->data, qn ? qn->data : nullptr, Hq, qa->shape[2], qn && qn->dtype == QMM_FLOAT32, 1, 0};
+  a.set[1] = RopeHeads{ka->data, c.k->data, kn ? kn->data : nullptr, Hkv, D, kn && kn->dtype == QMM_FLOAT32, 1, 1};
+  a.set[2] = RopeHeads{va->data, c.v->data, nullptr, Hkv, D, 0, 0, 1};
+  a.sets = 3, a.T = T, a.D = D, a.half = fa->shape[0];
+  a.in_f32 = qa->dtype == QMM_FLOAT32, a.out_f32 = 0;
+  a.interleaved = interleaved;
+  a.amplitude = amplitude, a.sign = 1.f, a.eps = norm_eps;
+  a.positions = (const int *)pa->data, a.slots = (const int *)sa->data, a.freqs = (const float *)fa->data;
+  a.NB = NB, a.block = block;
+  hipError_t e;
+  if (c.fp8) {
+    uint8_t *const scales[ROPE_MAX_SETS] = {nullptr, (uint8_t *)c.ks->data, (uint8_t *)c.vs->data};
+    e = launch_rope_fp8(a, scales, st);
+  } else {
+    e = launch_rope(a, st);
+  }
+  return e != hipSuccess ? fail_hip(e, op) : 0;
+}
+
+// qmm_paged_attention and, with scales, qmm_paged_attention_fp8.
+int paged_attention(const char *op, qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache,
+                    const qmm_array *k_scales, const qmm_array *v_scales, qmm_array table, qmm_array q_starts,
+                    qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s) {
+  if (!res) return fail("[%s] null result pointer", op);
+  Cache c;
+  if (check_caches(op, c, k_cache, v_cache, k_scales, v_scales)) return 1;
+  const int NB = c.NB, Hkv = c.Hkv, block = c.block, D = c.D;
+  Arr *qa = arr(q), *ta = arr(table), *sa = arr(q_starts), *la = arr(kv_lens), *ga = arr(gate);
+  if (!qa) return fail("[%s] missing q", op);
+  if (qa->dtype != QMM_BFLOAT16 || qa->ndim != 3 || qa->shape[2] != D)
+    return fail("[%s] q must be a bfloat16 array [T, Hq, %d]", op, D);
+  const int T = qa->shape[0], Hq = qa->shape[1];
+  if (Hq < 1 || Hq % Hkv) return fail("[%s] %d query heads do not share %d key heads evenly", op, Hq, Hkv);
+  if (check_int(op, "table", ta, {-1, -1})) return 1;
+  const int R = ta->shape[0], W = ta->shape[1];
+  if (check_int(op, "q_starts", sa, {R + 1}) || check_int(op, "kv_lens", la, {R})) return 1;
+  if (R > ATTN_MAX_R) return fail("[%s] %d requests: at most %d", op, R, ATTN_MAX_R);
+  if (ga && (ga->dtype != QMM_BFLOAT16 || ga->ndim != 3 || ga->shape[0] != T || ga->shape[1] != Hq ||
+             ga->shape[2] < D || ga->shape[2] % 8 || misaligned(ga)))
+    return fail("[%s] gate must be a 16-byte aligned bfloat16 array [%d, %d, %d or more, a multiple of 8]", op, T,
+                       Hq, D);
+  if (window < 0) return fail("[%s] window must not be negative, got %d", op, window);
+  if (!std::isfinite(scale)) return fail("[%s] scale must be finite", op);
+  if (misaligned(qa)) return fail("[%s] q must be 16-byte aligned", op);
+  AttnArgs a;
+  a.q = (const uint16_t *)qa->data, a.k = (const uint16_t *)c.k->data, a.v = (const uint16_t *)c.v->data;
+  a.k_scales = c.ks ? (const uint8_t *)c.ks->data : nullptr, a.v_scales = c.vs ? (const uint8_t *)c.vs->data : nullptr;
+  a.gate = ga ? (const uint16_t *)ga->data : nullptr;
+  a.table = (const int *)ta->data, a.q_starts = (const int *)sa->data, a.kv_lens = (const int *)la->data;
+  a.T = T, a.R = R, a.W = W, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.Dg = ga ? ga->shape[2] : 0;
+  a.NB = NB, a.block = block, a.window = window, a.scale = scale;
+  const char *too_much = attention_limits(a);
+  if (too_much) return fail("[%s] too many %s", op, too_much);
+  if (check_result(op, {"the result", res, {3, {T, Hq, D}}, QMM_BFLOAT16}, {qa, c.k, c.v, c.ks, c.vs, ta, sa, la, ga}, {qa, ga}))
+    return 1;
+  hipStream_t st = stream_of(s);
+  Arr *oa;
+  if (alloc_arr(res, {T, Hq, D}, QMM_BFLOAT16, st, &oa)) return 1;
+  if (misaligned(oa)) return fail("[%s] the result must be 16-byte aligned", op);
+  if (T == 0) return 0;
+  a.o = (uint16_t *)oa->data;
+  Scratch scratch;
+  const size_t need = attention_workspace(a);
+  if (need && scratch.take(st, need)) return 1;
+  hipError_t e = launch_attention(a, scratch.get(), st);
+  if (e != hipSuccess) return fail_hip(e, op);
   return 0;
 }
 
@@ -245,49 +385,66 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
                    qmm_array positions, qmm_array slots, qmm_array freqs, float amplitude, bool interleaved,
                    qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s) {
   begin_op();
-  const char *op = "rope_cache";
-  if (!q_out) return finish(fail("[%s] null result pointer", op));
-  Arr *kc = arr(k_cache), *vc = arr(v_cache), *qa = arr(q), *ka = arr(k), *va = arr(v), *pa = arr(positions),
-      *sa = arr(slots), *fa = arr(freqs), *qn = arr(q_norm), *kn = arr(k_norm);
-  if (check_cache(op, "k_cache", kc) || check_cache(op, "v_cache", vc)) return finish(1);
-  const int NB = kc->shape[0], Hkv = kc->shape[1], block = kc->shape[2], D = kc->shape[3];
+  return finish(rope_cache("rope_cache", q_out, k_cache, v_cache, nullptr, nullptr, q, k, v, positions, slots, freqs,
+                           amplitude, interleaved, q_norm, k_norm, norm_eps, s));
+}
+
+int qmm_rope_cache_fp8(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales, qmm_array v_scales,
+                       qmm_array q, qmm_array k, qmm_array v, qmm_array positions, qmm_array slots, qmm_array freqs,
+                       float amplitude, bool interleaved, qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s) {
+  begin_op();
+  return finish(rope_cache("rope_cache_fp8", q_out, k_cache, v_cache, &k_scales, &v_scales, q, k, v, positions, slots, freqs,
+                           amplitude, interleaved, q_norm, k_norm, norm_eps, s));
+}
+
+int qmm_cache_read_fp8(qmm_array *k_out, qmm_array *v_out, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
+                       qmm_array v_scales, qmm_array slots, qmm_dtype dtype, qmm_stream s) {
+  begin_op();
+  const char *op = "cache_read_fp8";
+  if (!k_out && !v_out) return finish(fail("[%s] null result pointers", op));
+  if (dtype != QMM_BFLOAT16 && dtype != QMM_FLOAT32) return finish(fail("[%s] dtype must be bfloat16 or float32", op));
+  struct Side {
+    const char *name, *cache_name, *scales_name;
+    qmm_array *res;
+    const Arr *cache, *scales;
+    Arr *out;
+  } sides[2];
+  int n = 0;
+  if (k_out) sides[n++] = Side{"k_out", "k_cache", "k_scales", k_out, arr(k_cache), arr(k_scales), nullptr};
+  if (v_out) sides[n++] = Side{"v_out", "v_cache", "v_scales", v_out, arr(v_cache), arr(v_scales), nullptr};
+  for (Side *x = sides; x != sides + n; ++x)
+    if (check_cache(op, x->cache_name, x->cache, true) || check_head_dim(op, x->cache->shape[3], true) ||
+        check_scales(op, x->scales_name, x->scales, x->cache))
+      return finish(1);
+  const Arr *c = sides[0].cache;
   for (int i = 0; i < 4; ++i)
-    if (kc->shape[i] != vc->shape[i]) return finish(fail("[%s] k_cache and v_cache shapes differ", op));
-  if (check_head_dim(op, D) || check_freqs(op, fa, D)) return finish(1);
-  if (!qa || !ka || !va) return finish(fail("[%s] missing input", op));
-  if (!floating(qa) || ka->dtype != qa->dtype || va->dtype != qa->dtype)
-    return finish(fail("[%s] q, k, v must all be bfloat16 or all float32", op));
-  if (qa->ndim != 3 || qa->shape[2] < D || qa->shape[2] % 8)
-    return finish(fail("[%s] q must be [T, Hq, %d or more, a multiple of 8]", op, D));
-  const int T = qa->shape[0], Hq = qa->shape[1];
-  for (const Arr *x : {ka, va})
-    if (x->ndim != 3 || x->shape[0] != T || x->shape[1] != Hkv || x->shape[2] != D)
-      return finish(fail("[%s] k and v must be [%d, %d, %d]", op, T, Hkv, D));
-  if (check_int(op, "positions", pa, {T}) || check_int(op, "slots", sa, {T})) return finish(1);
-  if (check_norm(op, "q_norm", qn, D) || check_norm(op, "k_norm", kn, D)) return finish(1);
-  if (misaligned(qa) || misaligned(ka) || misaligned(va))
-    return finish(fail("[%s] q, k and v must be 16-byte aligned", op));
-  const Arr *qc = arr(*q_out);
-  if (qc && (qc == qa || (qc->data && qc->data == qa->data)) && (qa->shape[2] != D || qa->dtype != QMM_BFLOAT16))
-    return finish(fail("[%s] q_out can be q's own array only at q's layout", op));
-  if (check_result(op, {"q_out", q_out, {3, {T, Hq, D}}, QMM_BFLOAT16}, {qa, ka, va, kc, vc, pa, sa, fa, qn, kn}, {qa}))
-    return finish(1);
+    if (c->shape[i] != sides[n - 1].cache->shape[i]) return finish(fail("[%s] k_cache and v_cache shapes differ", op));
+  Arr *sa = arr(slots);
+  if (check_int(op, "slots", sa, {-1})) return finish(1);
+  const int T = sa->shape[0], H = c->shape[1], D = c->shape[3];
+  const Arr *const last = sides[n - 1].cache, *const last_scales = sides[n - 1].scales;
+  for (Side *x = sides; x != sides + n; ++x)
+    if (check_result(op, {x->name, x->res, {3, {T, H, D}}, dtype}, {c, sides[0].scales, last, last_scales, sa}, {}))
+      return finish(1);
+  if (n == 2) {
+    const Result k{"k_out", k_out, {3, {T, H, D}}, dtype}, v{"v_out", v_out, {3, {T, H, D}}, dtype};
+    if (k_out == v_out || (k.cur.a && k.cur.a == v.cur.a) || (k.kept && v.kept && overlap(k.cur, v.cur)))
+      return finish(fail("[%s] v_out lies over k_out", op));
+  }
   hipStream_t st = stream_of(s);
-  Arr *qo;
-  if (alloc_arr(q_out, {T, Hq, D}, QMM_BFLOAT16, st, &qo)) return finish(1);
-  if (misaligned(qo)) return finish(fail("[%s] the result must be 16-byte aligned", op));
+  for (Side *x = sides; x != sides + n; ++x) {
+    if (alloc_arr(x->res, {T, H, D}, dtype, st, &x->out)) return finish(1);
+    if (misaligned(x->out)) return finish(fail("[%s] the results must be 16-byte aligned", op));
+  }
   if (T == 0) return finish(0);
-  RopeArgs a{};
-  a.set[0] = RopeHeads{qa->data, qo->data, qn ? qn->data : nullptr, Hq, qa->shape[2], qn && qn->dtype == QMM_FLOAT32, 1, 0};
-  a.set[1] = RopeHeads{ka->data, kc->data, kn ? kn->data : nullptr, Hkv, D, kn && kn->dtype == QMM_FLOAT32, 1, 1};
-  a.set[2] = RopeHeads{va->data, vc->data, nullptr, Hkv, D, 0, 0, 1};
-  a.sets = 3, a.T = T, a.D = D, a.half = fa->shape[0];
-  a.in_f32 = qa->dtype == QMM_FLOAT32, a.out_f32 = 0;
-  a.interleaved = interleaved;
-  a.amplitude = amplitude, a.sign = 1.f, a.eps = norm_eps;
-  a.positions = (const int *)pa->data, a.slots = (const int *)sa->data, a.freqs = (const float *)fa->data;
-  a.NB = NB, a.block = block;
-  hipError_t e = launch_rope(a, st);
+  CacheReadArgs a{};
+  for (int i = 0; i < n; ++i) {
+    a.codes[i] = (const uint8_t *)sides[i].cache->data, a.scales[i] = (const uint8_t *)sides[i].scales->data;
+    a.out[i] = sides[i].out->data;
+  }
+  a.sets = n, a.T = T, a.NB = c->shape[0], a.H = H, a.block = c->shape[2], a.D = D, a.out_f32 = dtype == QMM_FLOAT32;
+  a.slots = (const int *)sa->data;
+  hipError_t e = launch_cache_read(a, st);
   if (e != hipSuccess) return finish(fail_hip(e, op));
   return finish(0);
 }
@@ -295,53 +452,16 @@ int qmm_rope_cache(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, qmm_a
 int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array table,
                         qmm_array q_starts, qmm_array kv_lens, qmm_array gate, float scale, int window, qmm_stream s) {
   begin_op();
-  const char *op = "paged_attention";
-  if (!res) return finish(fail("[%s] null result pointer", op));
-  Arr *qa = arr(q), *kc = arr(k_cache), *vc = arr(v_cache), *ta = arr(table), *sa = arr(q_starts), *la = arr(kv_lens),
-      *ga = arr(gate);
-  if (check_cache(op, "k_cache", kc) || check_cache(op, "v_cache", vc)) return finish(1);
-  for (int i = 0; i < 4; ++i)
-    if (kc->shape[i] != vc->shape[i]) return finish(fail("[%s] k_cache and v_cache shapes differ", op));
-  const int NB = kc->shape[0], Hkv = kc->shape[1], block = kc->shape[2], D = kc->shape[3];
-  if (check_head_dim(op, D)) return finish(1);
-  if (!qa) return finish(fail("[%s] missing q", op));
-  if (qa->dtype != QMM_BFLOAT16 || qa->ndim != 3 || qa->shape[2] != D)
-    return finish(fail("[%s] q must be a bfloat16 array [T, Hq, %d]", op, D));
-  const int T = qa->shape[0], Hq = qa->shape[1];
-  if (Hq < 1 || Hq % Hkv) return finish(fail("[%s] %d query heads do not share %d key heads evenly", op, Hq, Hkv));
-  if (check_int(op, "table", ta, {-1, -1})) return finish(1);
-  const int R = ta->shape[0], W = ta->shape[1];
-  if (check_int(op, "q_starts", sa, {R + 1}) || check_int(op, "kv_lens", la, {R})) return finish(1);
-  if (R > ATTN_MAX_R) return finish(fail("[%s] %d requests: at most %d", op, R, ATTN_MAX_R));
-  if (ga && (ga->dtype != QMM_BFLOAT16 || ga->ndim != 3 || ga->shape[0] != T || ga->shape[1] != Hq ||
-             ga->shape[2] < D || ga->shape[2] % 8 || misaligned(ga)))
-    return finish(fail("[%s] gate must be a 16-byte aligned bfloat16 array [%d, %d, %d or more, a multiple of 8]", op, T,
-                       Hq, D));
-  if (window < 0) return finish(fail("[%s] window must not be negative, got %d", op, window));
-  if (!std::isfinite(scale)) return finish(fail("[%s] scale must be finite", op));
-  if (misaligned(qa)) return finish(fail("[%s] q must be 16-byte aligned", op));
-  AttnArgs a;
-  a.q = (const uint16_t *)qa->data, a.k = (const uint16_t *)kc->data, a.v = (const uint16_t *)vc->data;
-  a.gate = ga ? (const uint16_t *)ga->data : nullptr;
-  a.table = (const int *)ta->data, a.q_starts = (const int *)sa->data, a.kv_lens = (const int *)la->data;
-  a.T = T, a.R = R, a.W = W, a.Hq = Hq, a.Hkv = Hkv, a.D = D, a.Dg = ga ? ga->shape[2] : 0;
-  a.NB = NB, a.block = block, a.window = window, a.scale = scale;
-  const char *too_much = attention_limits(a);
-  if (too_much) return finish(fail("[%s] too many %s", op, too_much));
-  if (check_result(op, {"the result", res, {3, {T, Hq, D}}, QMM_BFLOAT16}, {qa, kc, vc, ta, sa, la, ga}, {qa, ga}))
-    return finish(1);
-  hipStream_t st = stream_of(s);
-  Arr *oa;
-  if (alloc_arr(res, {T, Hq, D}, QMM_BFLOAT16, st, &oa)) return finish(1);
-  if (misaligned(oa)) return finish(fail("[%s] the result must be 16-byte aligned", op));
-  if (T == 0) return finish(0);
-  a.o = (uint16_t *)oa->data;
-  Scratch scratch;
-  const size_t need = attention_workspace(a);
-  if (need && scratch.take(st, need)) return finish(1);
-  hipError_t e = launch_attention(a, scratch.get(), st);
-  if (e != hipSuccess) return finish(fail_hip(e, op));
-  return finish(0);
+  return finish(paged_attention("paged_attention", res, q, k_cache, v_cache, nullptr, nullptr, table, q_starts, kv_lens,
+                                gate, scale, window, s));
+}
+
+int qmm_paged_attention_fp8(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
+                            qmm_array v_scales, qmm_array table, qmm_array q_starts, qmm_array kv_lens, qmm_array gate,
+                            float scale, int window, qmm_stream s) {
+  begin_op();
+  return finish(paged_attention("paged_attention_fp8", res, q, k_cache, v_cache, &k_scales, &v_scales, table, q_starts,
+                                kv_lens, gate, scale, window, s));
 }
 
 }  // extern "C"

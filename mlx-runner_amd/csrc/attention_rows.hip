@@ -16,6 +16,8 @@
 //
 // One token over 262144 keys (24 query heads on 4 of 256; 1.07 GB, each byte fetched once): 189-191 us, 5.65
 // TB/s, the matrix cores 6% busy.  64 requests of 1 to 8192 keys (32 on 8 of 128; 370 MB): 77-79 us.
+#include <type_traits>
+
 #include "attention.h"
 #include "gemm_pipe.h"
 
@@ -28,6 +30,7 @@ constexpr int AR_EXTRA = 1;  // a tile's own overhead, in units of its keys
 constexpr int AR_TILE = 8192;  // bytes of a wave's tile of keys (and of values)
 constexpr int AR_STAGE = AR_WAVES * 2 * AR_TILE;
 constexpr int AR_TAB = AR_WAVES * 2 * 256;  // the next tile's page ids, two sets per wave
+constexpr int AR_SCALES = AR_WAVES * 4 * 256;  // E4M3: its keys' and values' scale bytes, a dword each, two sets per wave
 
 constexpr int ar_merge(int DP) { return AR_WAVES * 16 * (DP + 4) * 4 + AR_WAVES * 16 * 8; }
 constexpr int ar_fixed(int DP) { return AR_STAGE > ar_merge(DP) ? AR_STAGE : ar_merge(DP); }
@@ -38,26 +41,45 @@ constexpr int ar_fixed(int DP) { return AR_STAGE > ar_merge(DP) ? AR_STAGE : ar_
 __device__ __forceinline__ void ar_dma4(const void *g, uint32_t l) {
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(l), "v"(g) : "memory", "m0");
 }
+// The same of a byte per lane, a dword each in LDS.
+__device__ __forceinline__ void ar_dma1(const void *g, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+}
 #pragma clang diagnostic pop
 template <int N>
 __device__ __forceinline__ void ar_wait() {
   asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
 }
 
-// FULL: D = DP (else the lanes of chunks past D stay out of the DMA).
-template <int DP, int NQ, bool FULL>
-__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnArgs args, const AttnShare share) {
+// f(0) and, where N is 2, f(1), their argument a constant.
+template <int N, class F>
+__device__ __forceinline__ void for_parts(F f) {
+  f(std::integral_constant<int, 0>{});
+  if constexpr (N > 1) f(std::integral_constant<int, 1>{});
+}
+
+// FULL: D = DP (else the lanes of chunks past D stay out of the DMA).  E8: pages of E4M3 codes with scales.
+// (args and share are the kernel's whole argument block, in this order: see attn_again.)
+template <int DP, int NQ, bool FULL, bool E8>
+__device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare &share) {
   constexpr int TR = 16 * NQ;
-  constexpr int KW = AR_TILE / (2 * DP);  // keys of a wave's tile: 16, 32, 64
+  constexpr int EB = E8 ? 1 : 2;          // bytes of a value
+  constexpr int TILE = E8 && DP == 64 ? AR_TILE / 2 : AR_TILE;
+  constexpr int KW = TILE / (EB * DP);    // keys of a wave's tile: 16, 32, 64; E4M3: 32, 64, 64
   constexpr int KT = AR_WAVES * KW;
-  constexpr int CPR = DP / 8;             // 16-byte chunks of a row
+  constexpr int CPR = EB * DP / 16;       // 16-byte chunks of a row
   constexpr int RPI = 64 / CPR;           // rows of a DMA operation
   constexpr int KB = KW / 16;             // 16-key blocks of a tile
-  constexpr int ST = DP / 32, DT = DP / 16, PITCH = 2 * DP;
-  constexpr int OPS = AR_TILE / 1024;     // DMA operations of a tile
+  constexpr int ST = DP / 32, DT = DP / 16, PITCH = EB * DP;
+  constexpr int S8 = DP > 128 ? 2 : 1;    // E4M3: k steps of 128 values
+  constexpr int P8 = DP > 64 ? 2 : 1;     // the queries' parts are products of their own (DP 64: the two halves of one)
+  constexpr int OPS = TILE / 1024;        // DMA operations of a tile
+  constexpr int ASKED = E8 ? 3 : 1;       // those of page ids and scales before them
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
   uint8_t *tab = lds + ar_fixed(DP);
-  int *seen_at = (int *)(tab + AR_TAB);  // [thread][2][2]: what its rows see
+  uint8_t *scl = tab + AR_TAB;
+  int *seen_at = (int *)(scl + (E8 ? AR_SCALES : 0));  // [thread][2][2]: what its rows see
+  const auto swz = [](int row) { return E8 ? attn_swz8<DP>(row) : attn_swz<DP>(row); };
   AttnPlan *plan = (AttnPlan *)(seen_at + 4 * ATTN_THREADS);
 
   const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -71,7 +93,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     left = w.left;
   }
   uint8_t *kl = lds + wv * 2 * AR_TILE, *vl = kl + AR_TILE;
-  const uint32_t ka = lds_addr(kl), va = lds_addr(vl), ta = lds_addr(tab) + wv * 512;
+  const uint32_t ka = lds_addr(kl), va = lds_addr(vl), ta = lds_addr(tab) + wv * 512, sa = lds_addr(scl) + wv * 1024;
   // head values past D: never written by the DMA, zero for good
   if constexpr (!FULL) {
     for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
@@ -109,6 +131,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     // and `off` of the tile whose page ids are asked for next (held to the last page), `at` its place in its page.
     const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
     const uint16_t *kc = a.k, *vc = a.v;
+    const uint8_t *ksc = a.k_scales, *vsc = a.v_scales;
     const int *tabrow = a.table + (int64_t)r * a.W;
     int k0 = ks + KW * wv;
     const uint32_t last_page = t.e > 0 ? attn_div(t.e - 1, a.by_block) : 0u;
@@ -119,7 +142,9 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
     // the rows of this lane: what they see, their queries
     float m[NQ], l[NQ];
     const int ln0 = (int)attn_lane(), lr = ln0 & 15, lg = ln0 >> 4;
-    bf16x8_t q[NQ][ST];
+    bf16x8_t q[NQ][E8 ? 1 : ST];
+    i32x8_t q8[NQ][E8 ? S8 : 1][P8];  // E4M3: the queries in two parts, and their scales, a byte for each
+    int qs[NQ];
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const bool on = n * 16 + lr < t.rows;
@@ -129,20 +154,48 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
       seen_at[here() * 4 + 2 * n + 1] = on ? pos : -1;
       // (a row that sees nothing needs no reference; one past the end has no weights and passes none)
       m[n] = !on ? __builtin_inff() : pos >= 0 ? -__builtin_inff() : 0.f;
-      const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D + lg * 8;
+      const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D;
+      // values 32 lg .. + 31 of each 128 (DP 64: 32 (lg % 2); the upper half of the lanes has the second part); which of the
+      // matrix unit's k they are does not matter, where keys and queries agree
+      if constexpr (E8) {
 #pragma unroll
-      for (int st = 0; st < ST; ++st) {
-        if (FULL || st * 32 + lg * 8 < a.D)
-          q[n][st] = *(const bf16x8_t *)(qp + st * 32);
-        else
-          q[n][st] = __builtin_bit_cast(bf16x8_t, u32x4_t{0u, 0u, 0u, 0u});
+        for (int st = 0; st < S8; ++st) {
+          if (st == 0) qs[n] = 0;
+          const int at = st * 128 + (DP == 64 ? lg & 1 : lg) * 32;
+          u32x4_t x[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            x[i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (at + i * 8 < D) x[i] = *(const u32x4_t *)(qp + at + i * 8);
+            x[i] = a.scale > 0.f ? x[i] : a.scale < 0.f ? x[i] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};  // (as below)
+          }
+          if constexpr (P8 == 2) {
+            int sh, sl;
+            attn_split(x, q8[n][st][0], q8[n][st][1], sh, sl);
+            qs[n] |= (sl << 8 | sh) << 16 * st;
+          } else {
+            i32x8_t lo;
+            int sh, sl;
+            attn_split(x, q8[n][st][0], lo, sh, sl);
+            q8[n][st][0] = lg < 2 ? q8[n][st][0] : lo;
+            qs[n] = lg & 1 ? sl : sh;  // (the lanes' scales are those of the 32-value blocks 0 .. 3, hi and lo by turns)
+          }
+        }
+      } else {
+#pragma unroll
+        for (int st = 0; st < ST; ++st) {
+          if (FULL || st * 32 + lg * 8 < a.D)
+            q[n][st] = *(const bf16x8_t *)(qp + lg * 8 + st * 32);
+          else
+            q[n][st] = __builtin_bit_cast(bf16x8_t, u32x4_t{0u, 0u, 0u, 0u});
+        }
       }
     }
-    if (!(a.scale > 0.f)) {  // a negative scale: -q, so that maxima stay maxima; none: no scores
+    if (!E8 && !(a.scale > 0.f)) {  // a negative scale: -q, so that maxima stay maxima; none: no scores
 #pragma unroll
       for (int n = 0; n < NQ; ++n)
 #pragma unroll
-        for (int st = 0; st < ST; ++st) {
+        for (int st = 0; st < (E8 ? 0 : ST); ++st) {
           u32x4_t x = __builtin_bit_cast(u32x4_t, q[n][st]);
           x = a.scale < 0.f ? x ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
           q[n][st] = __builtin_bit_cast(bf16x8_t, x);
@@ -171,35 +224,41 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
       auto ask = [&](int buf) __attribute__((always_inline)) {
         ar_dma4(tabrow + (page < last_page ? page : last_page), ta + buf * 256);
       };
-      // the row (of the whole cache) of this lane's key, 0 where there is none; a bit for each key that there is
+      // the row (of the whole cache) of this lane's key, 0 where there is none; a bit for each key that there is;
+      // E4M3: its keys' and values' scales into set `set`
       uint32_t mine;
       uint64_t valid;
-      auto rows_of = [&](int k, int blk) __attribute__((always_inline)) {
+      auto rows_of = [&](int k, int blk, int set) __attribute__((always_inline)) {
         const bool ok = k + ((int)attn_lane() & (KW - 1)) < t.e && (uint32_t)blk < (uint32_t)NB;
-        mine = (((uint32_t)blk * Hkv + head) * block + at) & (ok ? ~0u : 0u);
+        const uint32_t on = ok ? ~0u : 0u, of = (uint32_t)blk * Hkv + head;
+        mine = (of * block + at) & on;
         valid = __ballot(ok);
+        if constexpr (E8) {
+          ar_dma1(ksc + (of & on), sa + set * 512);
+          ar_dma1(vsc + (of & on), sa + set * 512 + 256);
+        }
       };
       // DMA operations: RPI rows each, chunk (lane % CPR) ^ swizzle
       auto move = [&](const uint16_t *cache, uint32_t to) __attribute__((always_inline)) {
-        const uint32_t ln = attn_lane(), c0 = ln % CPR ^ (uint32_t)attn_swz<DP>((int)(ln / CPR));
+        const uint32_t ln = attn_lane(), c0 = ln % CPR ^ (uint32_t)swz((int)(ln / CPR));
 #pragma unroll
         for (int i = 0; i < OPS; ++i) {
           const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(ln / CPR * 4) + RPI * i * 4, (int)mine);
-          const uint32_t c = (c0 ^ (uint32_t)attn_swz<DP>(RPI * i)) * 16;
-          if (FULL || c < 2 * (uint32_t)D)
-            gp_dma16((const char *)cache + ((uint64_t)row * (2 * (uint32_t)D) + c), to + i * 1024);
+          const uint32_t c = (c0 ^ (uint32_t)swz(RPI * i)) * 16;
+          if (FULL || c < EB * (uint32_t)D)
+            gp_dma16((const char *)cache + ((uint64_t)row * (EB * (uint32_t)D) + c), to + i * 1024);
           if (i % 2) __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
         }
       };
 
-      rows_of(k0, page0);
+      rows_of(k0, page0, 0);
       onward();
       at = off;
       ask(1);
       onward();
       move(kc, ka);
       move(vc, va);
-      int buf = 1;
+      int buf = 1;  // (the scales' set of a tile is 1 - buf)
 #pragma unroll 1
       while (true) {
         const bool more = k0 + KT < ke;
@@ -208,7 +267,41 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
         const bool edge = k0 < t.full_b || k0 + KW > t.full_e || now != ~0ull;
         // S^T
         f32x4_t sv[NQ][KB];
-        {
+        const int set = 1 - buf;
+        int kx[KB];  // E4M3: the keys' scales
+        if constexpr (E8) {
+          const uint32_t ln = attn_lane();
+          const int row = ln & 15, lg = (int)(ln >> 4), c = DP == 64 ? (lg & 1) * 2 : lg * 2;
+          const int from = row * PITCH + (c ^ swz(row)) * 16;
+          const int *ks = (const int *)(scl + wv * 1024 + set * 512) + row;
+          auto load = [&](int j) __attribute__((always_inline)) {  // k step j % S8 of block j / S8
+            const int x = from ^ (j % S8) * 128, b = j / S8 * 16 * PITCH;
+            const u32x4_t lo = *(const u32x4_t *)(kl + x + b), hi = *(const u32x4_t *)(kl + (x ^ 16) + b);
+            return __builtin_bit_cast(i32x8_t, __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7));
+          };
+          i32x8_t kf[KB * S8];
+#pragma unroll
+          for (int b = 0; b < KB; ++b) kx[b] = ks[b * 16];
+          constexpr int AHEAD = NQ == 1 ? 2 : 1;
+#pragma unroll
+          for (int j = 0; j < AHEAD && j < KB * S8; ++j) kf[j] = load(j);
+#pragma unroll
+          for (int j = 0; j < KB * S8; ++j) {
+            if (j + AHEAD < KB * S8) kf[j + AHEAD] = load(j + AHEAD);
+            const int b = j / S8, st = j % S8;
+#pragma unroll
+            for (int n = 0; n < NQ; ++n)
+              for_parts<P8>([&](auto part) __attribute__((always_inline)) {
+                constexpr int PART = decltype(part)::value;
+                const f32x4_t c = st + PART ? sv[n][b] : f32x4_t{0.f, 0.f, 0.f, 0.f};
+                sv[n][b] = st == 0 ? __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[j], q8[n][0][PART], c, 0, 0, 0, kx[b],
+                                                                                      PART, qs[n])
+                                   : __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kf[j], q8[n][S8 - 1][PART], c, 0, 0, 0, kx[b],
+                                                                                      2 + PART, qs[n]);
+              });
+            __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
           const uint32_t ln = attn_lane();
           const int row = ln & 15, from = row * PITCH + ((int)(ln >> 4) ^ attn_swz<DP>(row)) * 16;
           auto load = [&](int j) __attribute__((always_inline)) {  // k step j % ST of block j / ST
@@ -231,7 +324,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
         if (more) {  // the next keys into the buffer just read
           asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
           const int blk = *(const int *)(tab + wv * 512 + buf * 256 + (int)attn_lane() * 4);
-          rows_of(k0 + KT, blk);
+          rows_of(k0 + KT, blk, buf);
           at = off;
           buf ^= 1;
           ask(buf);  // (past the end: not read; the waits count on it)
@@ -270,6 +363,12 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           top[n] *= sc;
           far |= top[n] > m[n] + 60.f;
         }
+        // (the matrix unit reads its scale operands after the instruction has issued, and the compiler does not know: they
+        // stay in their registers until the products are read)
+        if constexpr (E8) {
+#pragma unroll
+          for (int b = 0; b < KB; ++b) asm volatile("" ::"v"(kx[b]), "v"(top[0]), "v"(top[NQ - 1]));
+        }
         if (__any(far)) {
 #pragma unroll
           for (int n = 0; n < NQ; ++n) {
@@ -283,6 +382,15 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
             for (int d = 0; d < DT; ++d) acc[n][d] *= f;
           }
         }
+        // E4M3: the values' scales go into the weights, whose two parts have f32's exponents
+        i32x4_t vx[E8 ? KB : 1];
+        if constexpr (E8) {
+          const int *vs = (const int *)(scl + wv * 1024 + set * 512 + 256);
+          const uint32_t ln = attn_lane();
+#pragma unroll
+          for (int b = 0; b < KB; ++b) vx[b] = *(const i32x4_t *)(vs + b * 16 + (ln >> 4) * 4);
+          if (__any(vs[ln & (KW - 1)] == 255 && (now >> (ln & (KW - 1)) & 1))) *poison = 1;  // (NaN for the rows that see it)
+        }
         i16x4_t p[NQ][KB], pl[NQ][KB];  // weights rounded, and what the rounding has taken
 #pragma unroll
         for (int n = 0; n < NQ; ++n) {
@@ -291,9 +399,10 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           for (int b = 0; b < KB; ++b)
 #pragma unroll
             for (int i = 0; i < 4; i += 2) {
-              const float e0 = attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
-              const float e1 = attn_exp2(__builtin_fmaf(sv[n][b][i + 1], sc, -ref));
+              float e0 = attn_exp2(__builtin_fmaf(sv[n][b][i], sc, -ref));
+              float e1 = attn_exp2(__builtin_fmaf(sv[n][b][i + 1], sc, -ref));
               l[n] += e0 + e1;
+              if constexpr (E8) e0 = ldexpf(e0, vx[b][i] - 127), e1 = ldexpf(e1, vx[b][i + 1] - 127);
               bf16x2_t x, y;
               x[0] = (__bf16)e0, x[1] = (__bf16)e1;
               const uint32_t w = __builtin_bit_cast(uint32_t, x);
@@ -304,7 +413,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
         }
         // the values
         if (more)
-          ar_wait<OPS + 1>();
+          ar_wait<OPS + ASKED>();
         else
           ar_wait<0>();
         if (edge) {
@@ -315,7 +424,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           for (int i = 0; i < OPS; ++i) {
             const uint32_t lane = attn_lane();
             uint4 *x4 = (uint4 *)(vl + i * 1024 + lane * 16);
-            const uint4 x = *x4, y = attn_finite(x);
+            const uint4 x = *x4, y = E8 ? attn_finite_codes(x) : attn_finite(x);
             const bool in = now >> ((uint32_t)(i * 64 + lane) / CPR) & 1;
             odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
             const uint32_t keep = in ? ~0u : 0u;
@@ -323,7 +432,36 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
           }
           if (__any(odd)) *poison = 1;
         }
-        {
+        if constexpr (E8) {
+          const uint32_t ln = attn_lane();
+          // eight keys: this lane group's four of one 16-key block and of the next, as the weights lie
+          const int row = (int)((ln >> 3 & 1) * 16 + (ln >> 4) * 4 + (ln >> 1 & 3));
+          const uint32_t from = va + row * PITCH + swz(row & 15) * 16 + (ln & 1) * 8;
+          constexpr int CB = KB / 2, N = DT * CB, AHEAD = NQ == 1 ? 4 : 2;
+          auto load = [&](int j) __attribute__((always_inline)) {  // key blocks 2 (j % CB) and the next, columns j / CB
+            return attn_read_tr8((from ^ j / CB * 16) + j % CB * 32 * PITCH);
+          };
+          i32x2_t vf[N];
+#pragma unroll
+          for (int j = 0; j < AHEAD; ++j) vf[j] = load(j);
+#pragma unroll
+          for (int j = 0; j < N; ++j) {
+            if (j + AHEAD < N) vf[j + AHEAD] = load(j + AHEAD);
+            const int d = j / CB, b = j % CB * 2;
+            const bf16x2_t v0 = fp8x2_to_bf16x2<false>(vf[j].x), v1 = fp8x2_to_bf16x2<true>(vf[j].x);
+            const bf16x2_t v2 = fp8x2_to_bf16x2<false>(vf[j].y), v3 = fp8x2_to_bf16x2<true>(vf[j].y);
+            const bf16x8_t v = __builtin_shufflevector(__builtin_shufflevector(v0, v1, 0, 1, 2, 3),
+                                                       __builtin_shufflevector(v2, v3, 0, 1, 2, 3), 0, 1, 2, 3, 4, 5, 6, 7);
+#pragma unroll
+            for (int n = 0; n < NQ; ++n) {
+              const i16x8_t pf = __builtin_shufflevector(p[n][b], p[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+              const i16x8_t pr = __builtin_shufflevector(pl[n][b], pl[n][b + 1], 0, 1, 2, 3, 4, 5, 6, 7);
+              acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, pf), acc[n][d], 0, 0, 0);
+              acc[n][d] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(v, __builtin_bit_cast(bf16x8_t, pr), acc[n][d], 0, 0, 0);
+            }
+            if (j % 2) __builtin_amdgcn_sched_barrier(0);
+          }
+        } else {
           const uint32_t ln = attn_lane();
           const int row = (int)((ln >> 4) * 4 + (ln >> 2 & 3));
           // this lane's place in the 16 x 16 block (b, d) of the values
@@ -393,8 +531,8 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
         for (int d = 0; d < DT; ++d) *(f32x4_t *)(macc + (wv * 16 + lr) * (DP + 4) + d * 16 + lg * 4) = acc[n][d];
         __syncthreads();
 #pragma unroll 1
-        for (uint32_t i = here(); i < 16 * CPR; i += ATTN_THREADS) {
-          const int row = (int)(i / CPR), d0 = (int)(i % CPR * 8);
+        for (uint32_t i = here(); i < 16 * (DP / 8); i += ATTN_THREADS) {
+          const int row = (int)(i / (DP / 8)), d0 = (int)(i % (DP / 8) * 8);
           if (n * 16 + row >= t.rows || d0 >= D) continue;
           const int64_t orow = attn_row(a, rq.q0, t.row0 + n * 16 + row, head);
           uint4 gate = attn_zeros();
@@ -429,7 +567,7 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
             // values that are not finite: those held back; and those that met both parts of a weight (inf - inf), whose
             // own sum says what the result is (where weights are NaN, as of NaN queries, it is that anyway)
             float x[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            attn_poison(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, x);
+            attn_poison<E8>(a, rq, tabrow, head, t.row0 + n * 16 + row, ks, ke, d0, x);
 #pragma unroll
             for (int e = 0; e < 8; ++e) o[e] = o[e] * 0.f == 0.f ? o[e] + x[e] : x[e] * 0.f == 0.f ? o[e] : x[e];
           }
@@ -456,30 +594,44 @@ __global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnAr
 }
 
 template <int DP, int NQ, bool FULL>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows_kernel(const AttnArgs args, const AttnShare share) {
+  attn_rows<DP, NQ, FULL, false>(args, share);
+}
+template <int DP, int NQ, bool FULL>
+__global__ __launch_bounds__(ATTN_THREADS, 2) void attn_rows8_kernel(const AttnArgs args, const AttnShare share) {
+  attn_rows<DP, NQ, FULL, true>(args, share);
+}
+
+template <int DP, int NQ, bool FULL, bool E8>
 hipError_t launch_t(const AttnArgs &a, const AttnShare &s, int grid, hipStream_t st) {
   static std::atomic<uint64_t> done{0};
-  const void *k = (const void *)attn_rows_kernel<DP, NQ, FULL>;
-  const hipError_t e = ensure_dynamic_lds(done, k, (int)attn_rows_lds(DP, ATTN_MAX_R));
+  void (*const k)(AttnArgs, AttnShare) = E8 ? attn_rows8_kernel<DP, NQ, FULL> : attn_rows_kernel<DP, NQ, FULL>;
+  const hipError_t e = ensure_dynamic_lds(done, (const void *)k, (int)attn_rows_lds(DP, ATTN_MAX_R, E8));
   if (e != hipSuccess) return e;
-  hipLaunchKernelGGL((attn_rows_kernel<DP, NQ, FULL>), dim3(grid), dim3(ATTN_THREADS), attn_rows_lds(DP, a.R), st, a, s);
+  hipLaunchKernelGGL(k, dim3(grid), dim3(ATTN_THREADS), attn_rows_lds(DP, a.R, E8), st, a, s);
   return hipGetLastError();
 }
 
-template <int DP>
+template <int DP, bool E8>
 hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int tr, int grid, hipStream_t st) {
-  if (a.D == DP) return tr == 16 ? launch_t<DP, 1, true>(a, s, grid, st) : launch_t<DP, 2, true>(a, s, grid, st);
-  return tr == 16 ? launch_t<DP, 1, false>(a, s, grid, st) : launch_t<DP, 2, false>(a, s, grid, st);
+  if (a.D == DP) return tr == 16 ? launch_t<DP, 1, true, E8>(a, s, grid, st) : launch_t<DP, 2, true, E8>(a, s, grid, st);
+  return tr == 16 ? launch_t<DP, 1, false, E8>(a, s, grid, st) : launch_t<DP, 2, false, E8>(a, s, grid, st);
+}
+
+template <bool E8>
+hipError_t launch(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st) {
+  return DP == 64 ? launch_dp<64, E8>(a, s, tr, grid, st)
+                  : DP == 128 ? launch_dp<128, E8>(a, s, tr, grid, st) : launch_dp<256, E8>(a, s, tr, grid, st);
 }
 
 }  // namespace
 
-size_t attn_rows_lds(int DP, int R) {
-  return ar_fixed(DP) + AR_TAB + 16 * ATTN_THREADS + attn_plan_lds(R);
+size_t attn_rows_lds(int DP, int R, bool fp8) {
+  return ar_fixed(DP) + AR_TAB + (fp8 ? AR_SCALES : 0) + 16 * ATTN_THREADS + attn_plan_lds(R);
 }
 
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st) {
-  return DP == 64 ? launch_dp<64>(a, s, tr, grid, st)
-                  : DP == 128 ? launch_dp<128>(a, s, tr, grid, st) : launch_dp<256>(a, s, tr, grid, st);
+  return a.k_scales ? launch<true>(a, s, DP, tr, grid, st) : launch<false>(a, s, DP, tr, grid, st);
 }
 
 }  // namespace qmm

@@ -1,0 +1,318 @@
+// A paged cache held in 8 bits: E4M3 codes [pages, heads, block, D], a scale 2^(X - 127) for each page and head.
+//
+// cache_write_kernel: y = the head's values after norm and rotation (rope.h), in f32.  The call's rows of one page (a run:
+// they follow one another) and one head share
+//
+//   t = min { t >= -127 : 448 * 2^t >= max |y| }  (finite y),   t' = t if the run holds the page's first row, else max(t, old t)
+//   code = rne_e4m3(y * 2^-t');   a page whose scale grows: its codes c -> rne_e4m3(c * 2^(old t - t'))
+//
+// An E4M3 value keeps 4 significant bits at any scale that leaves it normal (2^-6 .. 448), so one power of two for a whole
+// page loses next to nothing, and when it grows only codes that become subnormal are rounded again.
+//
+// A workgroup takes one head of k or v and the runs that start in a window of as many tokens as its lanes hold rows
+// (16 values a lane), so a run is seen whole by one workgroup and no atomics leave it.  Rows past the window (of its last
+// run) take further turns.
+#include "rope.h"
+
+namespace qmm {
+
+namespace {
+
+constexpr int CW_RUNS = 64;  // of a window at most
+
+__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+
+// Codes of eight values over 2^t; what is not finite: NaN.
+__device__ __forceinline__ uint2 codes8(const float (&x)[8], int t) {
+  const float scale = e8m0_scale_operand(t < 127 ? t : 127);
+  uint32_t w[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    float y[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) y[j] = finite(x[4 * k + j]) ? x[4 * k + j] : __uint_as_float(0x7FC00000u);
+    i16x2_t c = {0, 0};
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, y[0], y[1], scale, false);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, y[2], y[3], scale, true);
+    w[k] = __builtin_bit_cast(uint32_t, c);
+  }
+  return make_uint2(w[0], w[1]);
+}
+// Four codes times 2^-by.
+__device__ __forceinline__ uint32_t shrink4(uint32_t w, int by) {
+  const f32x2_t a = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+  int c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(a.x, -by), ldexpf(a.y, -by), 0, false);
+  c = __builtin_amdgcn_cvt_pk_fp8_f32(ldexpf(b.x, -by), ldexpf(b.y, -by), c, true);
+  return (uint32_t)c;
+}
+
+struct CacheWrite {
+  uint8_t *scales[2];  // of k, of v
+  int windows;
+};
+
+template <int PAIRS, bool IN_F32>
+__global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
+  constexpr int HELD = 2;  // turns whose values stay in registers
+  __shared__ __attribute__((aligned(16))) float norm[256], cs[ROPE_THREADS * 8], sn[ROPE_THREADS * 8];
+  __shared__ __attribute__((aligned(16))) float swap[PAIRS == ACROSS ? ROPE_THREADS * 16 : 4];
+  __shared__ uint32_t top[CW_RUNS];
+  __shared__ int begun[CW_RUNS], page_of[CW_RUNS], exponent[CW_RUNS], grown[CW_RUNS];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int rows = ROPE_THREADS >> lph;  // of a turn, and a window's
+  const int l = tid & ((1 << lph) - 1), g = tid >> lph;
+  const bool turned = PAIRS != ACROSS && l < a.half / 8;
+  const int d0 = (PAIRS == HALVES && turned ? l : 2 * l) * 8, d1 = PAIRS == HALVES && turned ? d0 + a.half : d0 + 8;
+  const bool in0 = d0 < a.D, in1 = d1 < a.D;
+  const int heads = a.set[1].heads;
+
+  auto page_at = [&](int t) -> int {  // -1: none
+    const int slot = a.slots[t];
+    const int page = slot / a.block;
+    return slot >= 0 && page < a.NB ? page : -1;
+  };
+#pragma unroll 1
+  for (int64_t item = blockIdx.x; item < (int64_t)w.windows * 2 * heads; item += gridDim.x) {
+    const int side = (int)(item % (2 * heads)) / heads, head = (int)(item % heads), w0 = (int)(item / (2 * heads)) * rows;
+    const RopeHeads &s = a.set[1 + side];
+    // the runs that start in the window, by every wave for itself: a bit for the first row of each
+    const int w1 = a.T - w0 < rows ? a.T : w0 + rows;
+    const int t = w0 + lane, mine = t < w1 ? page_at(t) : -1, before = t < w1 && t > 0 ? page_at(t - 1) : -1;
+    const uint64_t starts = __ballot(mine >= 0 && mine != before);
+    if (starts == 0) continue;
+    const int first = w0 + __builtin_ctzll(starts), last_page = __builtin_amdgcn_readlane(mine, w1 - w0 - 1);
+    int end = w1;
+    while (last_page >= 0 && end < a.T) {  // its last run's end
+      const uint64_t other = __ballot(end + lane >= a.T || page_at(end + lane) != last_page);
+      if (other) {
+        end += __builtin_ctzll(other);
+        break;
+      }
+      end += 64;
+    }
+    const int runs = __popcll(starts);
+    __syncthreads();  // (the last item's are read)
+    if (tid < CW_RUNS) top[tid] = 0, begun[tid] = 0;
+    if (mine >= 0 && mine != before && tid < 64) page_of[__popcll(starts & ((1ull << lane) - 1))] = mine;
+    if (s.norm)
+      norm[tid] = tid >= a.D ? 0.f
+                  : s.norm_f32 ? ((const float *)s.norm)[tid]
+                               : __uint_as_float((uint32_t)((const uint16_t *)s.norm)[tid] << 16);
+    __syncthreads();
+
+    auto run_of = [&](int row) -> int {
+      const int i = row - w0;
+      return __popcll(starts & (i < 63 ? (2ull << i) - 1 : ~0ull)) - 1;
+    };
+    // the values of row `row0 + g` (all threads: there are barriers)
+    auto values = [&](int row0, float (&x)[2][8]) __attribute__((always_inline)) {
+      const int row = row0 + g;
+      const bool on = row < end;
+      Eight<IN_F32> raw[2] = {};
+      const int64_t at = ((int64_t)(on ? row : first) * heads + head) * s.in_stride;
+      if (in0) raw[0] = load8<IN_F32>(s.in, at + d0);
+      if (in1) raw[1] = load8<IN_F32>(s.in, at + d1);
+      if (s.rotate) {
+        __syncthreads();
+        const int half = a.half;
+        for (int i = tid; i < rows * half; i += ROPE_THREADS) {
+          const int r = i / half, j = i - r * half;
+          if (row0 + r >= end) break;
+          float sv, c;
+          rope_angle(a.positions[row0 + r], a.freqs[j], sv, c);
+          cs[i] = c * a.amplitude, sn[i] = sv * a.amplitude * a.sign;
+        }
+        __syncthreads();
+      }
+#pragma unroll
+      for (int k = 0; k < 2; ++k) widen<IN_F32>(raw[k], x[k]);
+      if (s.norm) rope_norm(x, &norm[d0 & 255], &norm[d1 & 255], in0, in1, lph, a.D, a.eps);
+      if (!s.rotate) return;
+      if constexpr (PAIRS == ACROSS) {
+        rope_turn_across(x, swap + (tid >> lph << lph) * 16, l, a.half, a.interleaved, cs + g * a.half, sn + g * a.half);
+      } else if (turned) {
+        float c[8], sv[8];
+#pragma unroll
+        for (int j = 0; j < 8; j += 4)
+          *(float4 *)&c[j] = *(const float4 *)&cs[g * a.half + l * 8 + j],
+          *(float4 *)&sv[j] = *(const float4 *)&sn[g * a.half + l * 8 + j];
+        rope_turn<PAIRS>(x, c, sv);
+      }
+    };
+    float held[HELD][2][8];
+    auto measure = [&](int row0, const float (&x)[2][8]) __attribute__((always_inline)) {
+      const int row = row0 + g;
+      float m = 0.f;
+#pragma unroll
+      for (int j = 0; j < 8; ++j) {
+        if (in0 && finite(x[0][j])) m = fmaxf(m, fabsf(x[0][j]));
+        if (in1 && finite(x[1][j])) m = fmaxf(m, fabsf(x[1][j]));
+      }
+      for (int off = 1 << lph >> 1; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+      if (l == 0 && row < end && page_at(row) >= 0) {
+        const int run = run_of(row);
+        atomicMax(&top[run], __float_as_uint(m));
+        if (a.slots[row] % a.block == 0) begun[run] = 1;
+      }
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (first + h * rows < end) {
+        values(first + h * rows, held[h]);
+        measure(first + h * rows, held[h]);
+      }
+#pragma unroll 1
+    for (int row0 = first + HELD * rows; row0 < end; row0 += rows) {
+      float x[2][8];
+      values(row0, x);
+      measure(row0, x);
+    }
+    __syncthreads();
+    if (tid < runs) {
+      const float m = __uint_as_float(top[tid]);
+      int e = m > 0.f ? ceil_scale_exp(m) : -127;
+      uint8_t *scale = w.scales[side] + (int64_t)page_of[tid] * heads + head;
+      const int old = (int)*scale - 127;
+      int by = 0;
+      if (!begun[tid]) {
+        by = e > old ? e - old : 0;
+        e = e > old ? e : old;
+      }
+      *scale = (uint8_t)(e + 127);
+      exponent[tid] = e, grown[tid] = by;
+    }
+    __syncthreads();
+    for (int r = 0; r < runs; ++r) {
+      const int by = grown[r];
+      if (by == 0) continue;
+      uint4 *codes = (uint4 *)((uint8_t *)s.out + ((int64_t)page_of[r] * heads + head) * a.block * a.D);
+      for (int64_t i = tid; i < (int64_t)a.block * a.D / 16; i += ROPE_THREADS) {
+        uint4 c = codes[i];
+        c = make_uint4(shrink4(c.x, by), shrink4(c.y, by), shrink4(c.z, by), shrink4(c.w, by));
+        codes[i] = c;
+      }
+    }
+    __syncthreads();  // (their rows of this call come after)
+    auto store = [&](int row0, const float (&x)[2][8]) __attribute__((always_inline)) {
+      const int row = row0 + g;
+      if (row >= end) return;
+      const int page = page_at(row);
+      if (page < 0) return;
+      const int e = exponent[run_of(row)];
+      uint8_t *to = (uint8_t *)s.out + (((int64_t)page * heads + head) * a.block + (a.slots[row] - page * a.block)) * a.D;
+      if (in0) *(uint2 *)(to + d0) = codes8(x[0], e);
+      if (in1) *(uint2 *)(to + d1) = codes8(x[1], e);
+    };
+#pragma unroll
+    for (int h = 0; h < HELD; ++h)
+      if (first + h * rows < end) store(first + h * rows, held[h]);
+#pragma unroll 1
+    for (int row0 = first + HELD * rows; row0 < end; row0 += rows) {
+      float x[2][8];
+      values(row0, x);
+      store(row0, x);
+    }
+  }
+}
+
+// Codes to values, E to a lane: 16 bytes out where they are bfloat16.
+template <bool F32>
+__global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadArgs a, int chunks) {
+  constexpr int E = F32 ? 4 : 8, U = 4;
+  const int set = blockIdx.y;
+  const uint8_t *codes = a.codes[set], *scales = a.scales[set];
+  const int cpr = a.D / E;
+  const int64_t t0 = (int64_t)blockIdx.x * (256 * U) / chunks;
+  const int i0 = (int)((int64_t)blockIdx.x * (256 * U) - t0 * chunks) + (int)threadIdx.x;
+  uint32_t w[U][E / 4];
+  int e[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int i = i0 + u * 256, t = i / chunks, j = i - t * chunks, h = j / cpr, c = j - h * cpr;
+    e[u] = -1;
+    if (t0 + t >= a.T) continue;
+    const int slot = a.slots[t0 + t], page = slot / a.block;
+    if (slot < 0 || page >= a.NB) continue;
+    const int64_t at = (int64_t)page * a.H + h;
+    e[u] = scales[at];
+    const uint32_t *p = (const uint32_t *)(codes + (at * a.block + (slot - page * a.block)) * a.D + c * E);
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k) w[u][k] = p[k];
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int64_t at = (t0 * chunks + i0 + u * 256) * E;
+    if (at >= (int64_t)a.T * chunks * E) continue;
+    float v[E];
+    const float f = e[u] < 0 ? 0.f : e8m0_to_f32((uint32_t)e[u]);
+#pragma unroll
+    for (int k = 0; k < E / 4; ++k) {
+      const f32x2_t x = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[u][k], false), y = __builtin_amdgcn_cvt_pk_f32_fp8((int)w[u][k], true);
+      v[4 * k] = x.x * f, v[4 * k + 1] = x.y * f, v[4 * k + 2] = y.x * f, v[4 * k + 3] = y.y * f;
+    }
+#pragma unroll
+    for (int k = 0; k < E; ++k) v[k] = e[u] < 0 ? 0.f : v[k];
+    if constexpr (F32) {
+      *(float4 *)((float *)a.out[set] + at) = make_float4(v[0], v[1], v[2], v[3]);
+    } else {
+      store8<false>(a.out[set], at, v);
+    }
+  }
+}
+
+template <int PAIRS>
+void launch_pairs(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph, hipStream_t st) {
+  if (a.in_f32)
+    hipLaunchKernelGGL((cache_write_kernel<PAIRS, true>), dim3(grid), dim3(ROPE_THREADS), 0, st, a, w, lph);
+  else
+    hipLaunchKernelGGL((cache_write_kernel<PAIRS, false>), dim3(grid), dim3(ROPE_THREADS), 0, st, a, w, lph);
+}
+
+}  // namespace
+
+hipError_t launch_rope_fp8(const RopeArgs &args, uint8_t *const (&scales)[ROPE_MAX_SETS], hipStream_t st) {
+  RopeArgs q = args;
+  q.sets = 1;
+  if (q.set[0].heads > 0) {
+    const hipError_t e = launch_rope(q, st);
+    if (e != hipSuccess) return e;
+  }
+  const RopeArgs &a = args;
+  if (a.T <= 0 || a.D < 16 || a.D > 256 || a.D % 16 || a.half < 0 || 2 * a.half > a.D || a.sets != 3 || a.block < 1 ||
+      a.set[1].heads < 1 || a.set[1].heads != a.set[2].heads)
+    return hipErrorInvalidValue;
+  const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4, rows = ROPE_THREADS >> lph;
+  CacheWrite w{{scales[1], scales[2]}, (int)(((int64_t)a.T + rows - 1) / rows)};
+  const int64_t items = (int64_t)w.windows * 2 * a.set[1].heads;
+  const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
+  a.half % 8      ? launch_pairs<ACROSS>(a, w, grid, lph, st)
+  : a.interleaved ? launch_pairs<NEXT>(a, w, grid, lph, st)
+                  : launch_pairs<HALVES>(a, w, grid, lph, st);
+  return hipGetLastError();
+}
+
+hipError_t launch_cache_read(const CacheReadArgs &a, hipStream_t st) {
+  if (a.T <= 0 || a.sets < 1 || a.sets > 2 || a.H < 1 || a.D < 16 || a.D > 256 || a.D % 16 || a.block < 1)
+    return hipErrorInvalidValue;
+  const int E = a.out_f32 ? 4 : 8;
+  const int64_t chunks = (int64_t)a.H * (a.D / E);
+  if (chunks > INT32_MAX / 2) return hipErrorInvalidValue;
+  // (a grid's lanes are counted in 32 bits: what is over in further launches)
+  CacheReadArgs part = a;
+  const int64_t most = ((int64_t)1 << 33) / chunks / 8 * 8 > 0 ? ((int64_t)1 << 33) / chunks / 8 * 8 : 1;
+  for (int64_t t0 = 0; t0 < a.T; t0 += part.T) {
+    part.T = (int)(a.T - t0 < most ? a.T - t0 : most);
+    part.slots = a.slots + t0;
+    for (int i = 0; i < a.sets; ++i) part.out[i] = (char *)a.out[i] + t0 * a.H * a.D * (a.out_f32 ? 4 : 2);
+    const dim3 grid((unsigned)((part.T * chunks + 1023) / 1024), a.sets);
+    if (a.out_f32)
+      hipLaunchKernelGGL((cache_read_kernel<true>), grid, dim3(256), 0, st, part, (int)chunks);
+    else
+      hipLaunchKernelGGL((cache_read_kernel<false>), grid, dim3(256), 0, st, part, (int)chunks);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
+}
+
+}  // namespace qmm

@@ -210,6 +210,18 @@ struct RopeArgs {
   int NB, block;
 };
 hipError_t launch_rope(const RopeArgs &a, hipStream_t st);
+// The same for set 0, with sets 1 and 2 quantised into cache pages of E4M3 codes (formulas at cache_write_kernel):
+// their `out` holds codes, scales[i] the set's scale bytes [NB, heads].
+hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_SETS], hipStream_t st);
+
+// Rows of caches of E4M3 codes as bfloat16 or float32.
+struct CacheReadArgs {
+  const uint8_t *codes[2], *scales[2];  // [NB, H, block, D], [NB, H]
+  void *out[2];                         // [T, H, D]
+  int sets, T, NB, H, block, D, out_f32;
+  const int *slots;
+};
+hipError_t launch_cache_read(const CacheReadArgs &a, hipStream_t st);
 
 // Attention of the requests' new tokens over their pages.
 constexpr int ATTN_MAX_R = 4096;
@@ -219,6 +231,7 @@ struct FastDiv {
 };
 struct AttnArgs {
   const uint16_t *q, *k, *v, *gate;  // q [T, Hq, D]; pages [NB, Hkv, block, D]; gate [T, Hq, Dg] (its last D) or null
+  const uint8_t *k_scales, *v_scales;  // [NB, Hkv] where the pages hold E4M3 codes (k and v then point to bytes), else null
   uint16_t *o;
   const int *table, *q_starts, *kv_lens;
   int T, R, W, Hq, Hkv, D, Dg, NB, block, window;

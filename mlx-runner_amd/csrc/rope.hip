@@ -13,67 +13,11 @@
 // NEXT: neighbours) and nothing leaves it; else (ACROSS) the sides meet through LDS, within a wave.
 // Bound by the copy rate: 4096 tokens of 24 heads of 256 (101 MB) 22.7-23.0 us, 4.4 TB/s; where a
 // pair's halves met through LDS 28.2 us, bound by the vector unit.
-#include "qmm_device.h"
-#include "qmm_launch.h"
+#include "rope.h"
 
 namespace qmm {
 
 namespace {
-
-constexpr int ROPE_THREADS = 256;
-
-// Eight values as they lie in memory.
-template <bool F32>
-struct Eight {
-  uint4 w[F32 ? 2 : 1];
-};
-template <bool F32>
-__device__ __forceinline__ Eight<F32> load8(const void *p, int64_t i) {
-  Eight<F32> x;
-  if constexpr (F32) {
-    x.w[0] = ((const uint4 *)((const float *)p + i))[0];
-    x.w[1] = ((const uint4 *)((const float *)p + i))[1];
-  } else {
-    x.w[0] = *(const uint4 *)((const uint16_t *)p + i);
-  }
-  return x;
-}
-template <bool F32>
-__device__ __forceinline__ void widen(const Eight<F32> &x, float (&o)[8]) {
-  if constexpr (F32) {
-    const uint32_t w[8] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w, x.w[1].x, x.w[1].y, x.w[1].z, x.w[1].w};
-#pragma unroll
-    for (int j = 0; j < 8; ++j) o[j] = __uint_as_float(w[j]);
-  } else {
-    const uint32_t w[4] = {x.w[0].x, x.w[0].y, x.w[0].z, x.w[0].w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      o[2 * j] = __uint_as_float(w[j] << 16);
-      o[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
-    }
-  }
-}
-
-template <bool F32>
-__device__ __forceinline__ void store8(void *p, int64_t i, const float (&v)[8]) {
-  if constexpr (F32) {
-    float4 *o = (float4 *)((float *)p + i);
-    o[0] = make_float4(v[0], v[1], v[2], v[3]);
-    o[1] = make_float4(v[4], v[5], v[6], v[7]);
-  } else {
-    uint32_t w[4];
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      bf16x2_t x;
-      x[0] = (__bf16)v[2 * j], x[1] = (__bf16)v[2 * j + 1];
-      w[j] = __builtin_bit_cast(uint32_t, x);
-    }
-    *(uint4 *)((uint16_t *)p + i) = make_uint4(w[0], w[1], w[2], w[3]);
-  }
-}
-
-// Where the pairs of a head lie: both sides (HALVES) or all (NEXT) in a lane's 16 values, or anywhere.
-enum { HALVES, NEXT, ACROSS };
 
 // lph: log2 of a head's lanes (16 values each); a wave takes heads of one set only.
 template <int PAIRS, bool IN_F32, bool OUT_F32>
@@ -127,11 +71,8 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(const RopeArgs a, in
   fetch(i0);
 
   if (tid < a.half) {
-    // in turns and in 64 bits: at position 2^18 an f32 product is off by up to 2^-7 rad
-    double turns = (double)pos * (double)freq * 0.15915494309189533577;
-    turns -= __builtin_rint(turns);
     float s, c;
-    sincospif(2.f * (float)turns, &s, &c);
+    rope_angle(pos, freq, s, c);
     cs[tid] = c * a.amplitude;
     sn[tid] = s * a.amplitude * a.sign;
   }
@@ -160,54 +101,9 @@ __global__ __launch_bounds__(ROPE_THREADS) void rope_kernel(const RopeArgs a, in
       float x[2][8];
 #pragma unroll
       for (int k = 0; k < 2; ++k) widen<IN_F32>(raw[u][k], x[k]);
-      if (s.norm) {
-        float sq[2] = {0.f, 0.f};
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) sq[k] = __builtin_fmaf(x[k][j], x[k][j], sq[k]);
-        float sum = (in0 ? sq[0] : 0.f) + (in1 ? sq[1] : 0.f);
-        for (int off = 1 << lph >> 1; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
-        const float r = 1.f / sqrtf(sum / (float)a.D + a.eps);
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) {
-            const float4 w = *(const float4 *)&norm[set][((k ? d1 : d0) & 255) + j];
-            x[k][j] *= r * w.x, x[k][j + 1] *= r * w.y, x[k][j + 2] *= r * w.z, x[k][j + 3] *= r * w.w;
-          }
-      }
-      if (PAIRS != ACROSS && s.rotate && turned) {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) {
-          float &p = PAIRS == NEXT ? x[j >> 2][(j & 3) * 2] : x[0][j], &q = PAIRS == NEXT ? x[j >> 2][(j & 3) * 2 + 1] : x[1][j];
-          const float v = p;
-          p = v * c[j] - q * sv[j], q = v * sv[j] + q * c[j];
-        }
-      }
-      if (PAIRS == ACROSS && s.rotate) {  // (a head's lanes are lanes of one wave: no barrier)
-        float *mine = swap + (tid >> lph << lph) * 16;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; j += 4) *(float4 *)&mine[(2 * l + k) * 8 + j] = *(float4 *)&x[k][j];
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        const bool next = a.interleaved;
-#pragma unroll
-        for (int k = 0; k < 2; ++k)
-#pragma unroll
-          for (int j = 0; j < 8; ++j) {
-            const int d = (2 * l + k) * 8 + j;
-            if (d >= 2 * a.half) continue;
-            const bool first = next ? j % 2 == 0 : d < a.half;
-            const int i = next ? d / 2 : first ? d : d - a.half;
-            const float other = mine[next ? d ^ 1 : first ? d + a.half : i];
-            x[k][j] = first ? x[k][j] * cs[i] - other * sn[i] : other * sn[i] + x[k][j] * cs[i];
-          }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-      }
+      if (s.norm) rope_norm(x, &norm[set][d0 & 255], &norm[set][d1 & 255], in0, in1, lph, a.D, a.eps);
+      if (PAIRS != ACROSS && s.rotate && turned) rope_turn<PAIRS>(x, c, sv);
+      if (PAIRS == ACROSS && s.rotate) rope_turn_across(x, swap + (tid >> lph << lph) * 16, l, a.half, a.interleaved, cs, sn);
       if (!on || (s.cache && !kept)) continue;
       const int64_t at = s.cache ? (((int64_t)page * s.heads + h + g) * a.block + (slot - page * a.block)) * a.D
                                  : ((int64_t)t * s.heads + h + g) * a.D;

@@ -146,6 +146,10 @@ _SIGS = {
     "qmm_rope_cache": (c_int, [POINTER(qmm_array)] + [qmm_array] * 8 + [c_float, c_bool, qmm_array, qmm_array, c_float,
                                                                         qmm_stream]),
     "qmm_paged_attention": (c_int, [POINTER(qmm_array)] + [qmm_array] * 7 + [c_float, c_int, qmm_stream]),
+    "qmm_rope_cache_fp8": (c_int, [POINTER(qmm_array)] + [qmm_array] * 10 + [c_float, c_bool, qmm_array, qmm_array,
+                                                                             c_float, qmm_stream]),
+    "qmm_cache_read_fp8": (c_int, [POINTER(qmm_array)] * 2 + [qmm_array] * 5 + [c_int, qmm_stream]),
+    "qmm_paged_attention_fp8": (c_int, [POINTER(qmm_array)] + [qmm_array] * 9 + [c_float, c_int, qmm_stream]),
     "qmm_named_linear_q_group": (c_int, [POINTER(qmm_array), c_size_t, qmm_weight_map, qmm_array,
                                          POINTER(c_char_p), qmm_stream]),
 }
@@ -451,6 +455,41 @@ def paged_attention(q: Array, k_cache: Array, v_cache: Array, table: Array, q_st
     s = _stream(stream)
     check(lib.qmm_paged_attention(byref(res.h), q.h, k_cache.h, v_cache.h, table.h, q_starts.h, kv_lens.h,
                                   gate.h if gate else _NULL, scale, window, s.h), "paged_attention")
+    return res
+
+
+def rope_cache_fp8(q: Array, k: Array, v: Array, k_cache: Array, v_cache: Array, k_scales: Array, v_scales: Array,
+                   positions: Array, slots: Array, freqs: Array, *, amplitude: float = 1.0, interleaved: bool = False,
+                   q_norm: Array | None = None, k_norm: Array | None = None, norm_eps: float = 1e-6,
+                   q_out: Array | None = None, stream: Stream | None = None) -> Array:
+    """`rope_cache` into a cache of E4M3 codes (uint8 [pages, Hkv, block, D]) with a scale byte for each page and head."""
+    res = q_out if q_out is not None else Array()
+    s = _stream(stream)
+    check(lib.qmm_rope_cache_fp8(byref(res.h), k_cache.h, v_cache.h, k_scales.h, v_scales.h, q.h, k.h, v.h, positions.h,
+                                 slots.h, freqs.h, amplitude, interleaved, q_norm.h if q_norm else _NULL,
+                                 k_norm.h if k_norm else _NULL, norm_eps, s.h), "rope_cache_fp8")
+    return res
+
+
+def cache_read_fp8(k_cache: Array, v_cache: Array, k_scales: Array, v_scales: Array, slots: Array, *,
+                   dtype: int = BFLOAT16, k_out: Array | None = None, v_out: Array | None = None,
+                   stream: Stream | None = None) -> tuple[Array, Array]:
+    """The rows `slots` of such a cache as (k, v) [T, Hkv, D] in dtype; zeros where a slot is none."""
+    ks, vs = (a if a is not None else Array() for a in (k_out, v_out))
+    s = _stream(stream)
+    check(lib.qmm_cache_read_fp8(byref(ks.h), byref(vs.h), k_cache.h, v_cache.h, k_scales.h, v_scales.h, slots.h, dtype,
+                                 s.h), "cache_read_fp8")
+    return ks, vs
+
+
+def paged_attention_fp8(q: Array, k_cache: Array, v_cache: Array, k_scales: Array, v_scales: Array, table: Array,
+                        q_starts: Array, kv_lens: Array, *, gate: Array | None = None, scale: float, window: int = 0,
+                        out: Array | None = None, stream: Stream | None = None) -> Array:
+    """`paged_attention` over such a cache."""
+    res = out if out is not None else Array()
+    s = _stream(stream)
+    check(lib.qmm_paged_attention_fp8(byref(res.h), q.h, k_cache.h, v_cache.h, k_scales.h, v_scales.h, table.h, q_starts.h,
+                                      kv_lens.h, gate.h if gate else _NULL, scale, window, s.h), "paged_attention_fp8")
     return res
 
 
