@@ -103,6 +103,7 @@ __device__ __forceinline__ uint32_t attn_wave_scan(uint32_t v) {
   return v;
 }
 // Over the workgroup; the total too.
+template <int THREADS = ATTN_THREADS>
 __device__ __forceinline__ uint32_t attn_scan(uint32_t v, uint32_t *waves, uint32_t *total) {
   const int wave = threadIdx.x >> 6;
   v = attn_wave_scan(v);
@@ -111,7 +112,7 @@ __device__ __forceinline__ uint32_t attn_scan(uint32_t v, uint32_t *waves, uint3
   __syncthreads();
   uint32_t before = 0, all = 0;
 #pragma unroll
-  for (int w = 0; w < ATTN_THREADS / 64; ++w) {
+  for (int w = 0; w < THREADS / 64; ++w) {
     if (w == wave) before = all;
     all += waves[w];
   }
@@ -133,7 +134,7 @@ struct AttnWork {
 constexpr int ATTN_KEPT = 256;
 struct __attribute__((aligned(16))) AttnPlan {
   AttnWork work[2];     // this segment's, the next one's: out of the registers
-  uint32_t waves[4], found[3];
+  uint32_t waves[8], found[3];
   uint16_t owner[64];   // a tile's request, and its number there
   int poison[2], redo;
 };
@@ -167,7 +168,7 @@ __device__ __forceinline__ int attn_find(const AttnPlan *plan, int R, int i) {
 }
 
 // EXTRA units a tile costs beside its keys'.
-template <int TR, int KT, int EXTRA>
+template <int TR, int KT, int EXTRA, int THREADS = ATTN_THREADS>
 __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShare &s, AttnPlan *plan) {
   const int tid = threadIdx.x, lane = tid & 63;
   const uint32_t most = (uint32_t)s.tiles;
@@ -223,18 +224,18 @@ __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShar
     }
   } else {
 #pragma unroll 1
-    for (int r0 = 0; r0 < a.R; r0 += ATTN_THREADS) {
+    for (int r0 = 0; r0 < a.R; r0 += THREADS) {
       const int r = r0 + tid;
       AttnReq q{0, 0, 0, 0};
       if (r < a.R) q = attn_req(a, r);
-      const uint32_t end = run + attn_scan(tiles_of(q), plan->waves, &all);
+      const uint32_t end = run + attn_scan<THREADS>(tiles_of(q), plan->waves, &all);
       if (r < a.R) attn_keep(plan, a.R, r, end < most ? end : most, q);
       run = run + all < most ? run + all : most;
     }
     w.tiles = (int)run;
   }
   __syncthreads();
-  // Units of the tiles, ATTN_THREADS at a time: first all of them, for the shares; then until the tile with the
+  // Units of the tiles, THREADS at a time: first all of them, for the shares; then until the tile with the
   // share's first unit (where there are no more than that, the first turn's values still serve).
   uint32_t mine = 0, end = 0, x = 0;
   int r = 0;
@@ -242,19 +243,19 @@ __device__ __forceinline__ AttnWork attn_share(const AttnArgs &a, const AttnShar
   bool sought = false;
 #pragma unroll 1
   for (int i0 = 0; i0 < w.tiles;) {
-    if (!sought || w.tiles > ATTN_THREADS) {
+    if (!sought || w.tiles > THREADS) {
       const int i = i0 + tid;
       mine = 0;
       if (i < w.tiles) {
         r = attn_find(plan, a.R, i);
         mine = (uint32_t)(attn_units<KT>(attn_tile(a, attn_req(plan, a, r), i - (r ? attn_end(plan, a.R, r - 1) : 0), TR)) + EXTRA);
       }
-      end = run + attn_scan(mine, plan->waves, &all);
+      end = run + attn_scan<THREADS>(mine, plan->waves, &all);
       run += all;
     }
     if (sought && x < end && x >= end - mine)
       plan->found[0] = (uint32_t)(i0 + tid), plan->found[1] = x - (end - mine), plan->found[2] = (uint32_t)r;
-    i0 += ATTN_THREADS;
+    i0 += THREADS;
     if (!sought && i0 >= w.tiles) {
       x = cut(run);
       if (!w.left) return w;
@@ -330,13 +331,14 @@ __device__ __forceinline__ void attn_note_none(const AttnShare &s, const AttnWor
 }
 
 // Zeros for the rows of no request, by all workgroups of a launch.
+template <int THREADS = ATTN_THREADS>
 __device__ __forceinline__ void attn_zero_rest(const AttnArgs &a) {
   const int lo = a.R ? a.q_starts[0] : a.T, hi = a.R ? a.q_starts[a.R] : a.T;
   const int cpr = a.D / 8;
   const int64_t per_row = (int64_t)a.Hq * cpr;
   auto fill = [&](int t0, int t1) {
-    for (int64_t i = t0 * per_row + (int64_t)blockIdx.x * ATTN_THREADS + threadIdx.x; i < t1 * per_row;
-         i += (int64_t)gridDim.x * ATTN_THREADS)
+    for (int64_t i = t0 * per_row + (int64_t)blockIdx.x * THREADS + threadIdx.x; i < t1 * per_row;
+         i += (int64_t)gridDim.x * THREADS)
       ((uint4 *)a.o)[i] = make_uint4(0, 0, 0, 0);
   };
   fill(0, a.R ? (lo < 0 ? 0 : lo < a.T ? lo : a.T) : a.T);
@@ -466,10 +468,11 @@ __device__ __forceinline__ float attn_across(float x, int other) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(((int)attn_lane() ^ other) * 4, __float_as_int(x)));
 }
 
-// 128 bf16 values of a row, 32 to a lane (of those 16 and 32 apart), as two E4M3 parts, each with a scale 2^t of its own:
-// x = hi 2^th + lo 2^tl.  Two 4-bit significands hold bf16's 8 bits, so what is lost is 2^-22 of the 128 values' largest, if
+// 128 bf16 values of a row, 32 to a lane (of those 16 and 32 apart; PAIR: 64 values, lanes 32 apart), as two E4M3 parts, each with a scale 2^t of its own:
+// x = hi 2^th + lo 2^tl.  Two 4-bit significands hold bf16's 8 bits, so what is lost is 2^-22 of those values' largest, if
 // anything.  (The matrix unit takes a scale for every 32 values, but those are 16 of two lanes.)  The scales as bytes of its
 // operand; 255 (NaN) where a value is not finite.
+template <bool PAIR = false>
 __device__ __forceinline__ void attn_split(const u32x4_t (&x)[4], i32x8_t &hi, i32x8_t &lo, int &scale_hi, int &scale_lo) {
   float v[32], top = 0.f, rest = 0.f;
   bool odd = false;
@@ -482,7 +485,7 @@ __device__ __forceinline__ void attn_split(const u32x4_t (&x)[4], i32x8_t &hi, i
 #pragma unroll
   for (int i = 0; i < 32; ++i) top = fmaxf(top, fabsf(v[i]));
   top = odd ? __builtin_inff() : top;
-  top = fmaxf(top, attn_across(top, 16));
+  if (!PAIR) top = fmaxf(top, attn_across(top, 16));
   top = fmaxf(top, attn_across(top, 32));
   odd = top == __builtin_inff();
   const int th = odd ? 0 : top > 0.f ? ceil_scale_exp(top) : -127;
@@ -499,7 +502,7 @@ __device__ __forceinline__ void attn_split(const u32x4_t (&x)[4], i32x8_t &hi, i
 #pragma unroll
     for (int j = 0; j < 4; ++j) rest = fmaxf(rest, fabsf(v[4 * i + j]));
   }
-  rest = fmaxf(rest, attn_across(rest, 16));
+  if (!PAIR) rest = fmaxf(rest, attn_across(rest, 16));
   rest = fmaxf(rest, attn_across(rest, 32));
   const int tl = odd ? 0 : rest > 0.f ? ceil_scale_exp(rest) : -127;
   const float sl = e8m0_scale_operand(tl);
@@ -548,6 +551,8 @@ __device__ __forceinline__ i32x2_t attn_read_tr8(uint32_t at) {
 // Launches of the kernels (the workspace's parts in s).
 size_t attn_rows_lds(int DP, int R, bool fp8);
 size_t attn_chunk_lds(int DP, int R);
+size_t attn_chunk8_lds(int DP, int R);
+hipError_t launch_attn_chunk8(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st);
 hipError_t launch_attn_chunk(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st);
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st);
 

@@ -259,8 +259,8 @@ Route route_of(const AttnArgs &a) {
   cus = cus < 8 ? 8 : cus < AC_MOST / 2 ? cus : AC_MOST / 2;
   // (most: the rows of the longest request, if each has a token)
   const int64_t most = (int64_t)(a.T > a.R ? a.T - a.R + 1 : 1) * r.g;
-  const bool few = a.k_scales || most <= 8 * ROWS_MOST;
-  const bool one = !a.k_scales && a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
+  const bool few = most <= 8 * ROWS_MOST;
+  const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
   if (!one) {
     r.rows.tr = most <= 16 ? 16 : 32;
     r.rows.grid = 2 * cus;
@@ -273,7 +273,7 @@ Route route_of(const AttnArgs &a) {
   }
   if (one || !few) {
     r.chunk.tr = r.chunk.rows = 256;
-    r.chunk.grid = r.DP == 64 ? 2 * cus : cus;
+    r.chunk.grid = r.DP == 64 && !a.k_scales ? 2 * cus : cus;
     r.chunk.min_rows = one ? 0 : ROWS_MOST, r.chunk.max_rows = INT32_MAX;
   }
   r.bytes = 0;
@@ -339,7 +339,8 @@ hipError_t launch_attention(const AttnArgs &args, void *workspace, hipStream_t s
     AttnShare s = share_of(*p, workspace);
     s.first = first;
     first = false;
-    const hipError_t e = p == &r.rows ? launch_attn_rows(a, s, r.DP, p->tr, p->grid, st)
+    const hipError_t e = p == &r.rows   ? launch_attn_rows(a, s, r.DP, p->tr, p->grid, st)
+                         : a.k_scales ? launch_attn_chunk8(a, s, r.DP, p->grid, st)
                                       : launch_attn_chunk(a, s, r.DP, p->grid, st);
     if (e != hipSuccess) return e;
     r.DP == 64 ? join<64>(a, *p, s, st) : r.DP == 128 ? join<128>(a, *p, s, st) : join<256>(a, *p, s, st);

@@ -1,0 +1,506 @@
+// Paged attention of many rows per key head over a cache of E4M3 codes: all products on the scaled 32x32x64 MFMA, which
+// takes the codes as they are and a key's scale with them.
+//
+// bf16 queries go in as two E4M3 parts (attn_split: exact but for 2^-22 of a row's largest), so S^T = K Q^T costs what it
+// costs in bf16, two products at twice the rate.  The weights of O^T = V^T P^T go in as two parts as well (2^-8 of a weight
+// lost, as with bf16), scaled for each row and 32 keys by a power of two of those keys' own maximum, which the matrix unit
+// takes off again: what E4M3's 18 binades cannot hold is 2^-22 of the largest weight of 32 keys.  A page's scale of values is
+// the other operand's where the tile's keys share it; else it goes into the weights, relative to the tile's largest.
+//
+// A tile is 256 rows, 32 for each of eight waves, two a SIMD: one's softmax beside the other's products, with nothing
+// interleaved by hand.  (Codes are half of bf16's bytes: eight waves' operands from LDS take the bandwidth that four waves' of
+// 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, one barrier a tile.
+#include <type_traits>
+
+#include "attention.h"
+#include "gemm_pipe.h"
+
+namespace qmm {
+
+namespace {
+
+constexpr int C8_THREADS = 512, C8_WAVES = C8_THREADS / 64;
+constexpr int C8_TR = 256, C8_KT = 64;
+constexpr int C8_EXTRA = 3;   // what a tile's own overhead costs, in units of 64 keys
+constexpr int C8_SCALES = 2 * 2 * 256;                  // scale bytes of the keys, of the values; a dword each, two sets
+constexpr int C8_TAB = C8_WAVES * 2 * 32;               // page ids of the tiles to come
+constexpr int C8_SMALL = C8_SCALES + C8_TAB + 2 * C8_WAVES * 4 + 8 * C8_THREADS;
+
+constexpr int c8_tile(int DP) { return C8_KT * DP; }
+constexpr int c8_queries(int DP) { return DP == 256 ? C8_TR * DP : 0; }  // the queries' second parts
+constexpr int c8_fixed(int DP) {
+  const int out = C8_WAVES * 32 * 64 * 4, tiles = 4 * c8_tile(DP);  // (rows out: 64 columns of a wave's rows at a time)
+  return (tiles > out ? tiles : out) + c8_queries(DP);
+}
+
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"
+__device__ __forceinline__ void c8_dma4(const void *g, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dword %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+}
+__device__ __forceinline__ void c8_dma1(const void *g, uint32_t l) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_ubyte %1, off" ::"s"(l), "v"(g) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+
+// The larger of x here and 32 lanes away.
+__device__ __forceinline__ float c8_pair_max(float x) {
+  const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+// The wave's largest.
+__device__ __forceinline__ int c8_top(int x) {
+#define QMM_STEP(ctrl, rows)                                                          \
+  {                                                                                   \
+    const int y = __builtin_amdgcn_update_dpp(x, x, ctrl, rows, 0xF, false);          \
+    x = y > x ? y : x;                                                                \
+  }
+  QMM_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8; row_bcast:15, 31
+  QMM_STEP(0x112, 0xF);
+  QMM_STEP(0x114, 0xF);
+  QMM_STEP(0x118, 0xF);
+  QMM_STEP(0x142, 0xA);
+  QMM_STEP(0x143, 0xC);
+#undef QMM_STEP
+  return __builtin_amdgcn_readlane(x, 63);
+}
+
+template <int DP, bool FULL>
+__global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnArgs args, const AttnShare share) {
+  constexpr int CPR = DP / 16;     // 16-byte chunks of a row
+  constexpr int KS = DP / 64;      // k steps of S^T
+  constexpr int DT = DP / 32;      // 32-column tiles of O^T
+  constexpr int RPI = 64 / CPR;    // rows of a DMA operation
+  constexpr int OPS = 8 > RPI ? 8 / RPI : 1;  // operations of a wave's 8 rows
+  constexpr int TILE = c8_tile(DP), PITCH = DP;
+  constexpr bool LO_LDS = DP == 256;
+  extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
+  uint8_t *qlo = lds + c8_fixed(DP) - c8_queries(DP);
+  uint8_t *scl = lds + c8_fixed(DP);                 // [2][keys, values][64]
+  uint8_t *tab = scl + C8_SCALES;                    // [wave][2][8]
+  uint8_t *vm = tab + C8_TAB;                        // [2][8 waves], a byte each: keys that there are
+  int *seen_at = (int *)(vm + 2 * C8_WAVES * 4);     // [thread][2]: what its row sees
+  AttnPlan *plan = (AttnPlan *)(seen_at + 2 * C8_THREADS);
+
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  auto here = [&]() __attribute__((always_inline)) { return wv * 64 + (int)attn_lane(); };  // the thread's number
+  int left;
+  {
+    const AttnWork w = attn_uniform(attn_share<C8_TR, C8_KT, C8_EXTRA, C8_THREADS>(args, share, plan));
+    if (share.first) attn_zero_rest<C8_THREADS>(args);
+    attn_note_none(share, w);
+    if (tid == 0) plan->work[0] = w, plan->poison[0] = 0;
+    left = w.left;
+  }
+  const uint32_t la = lds_addr(lds), ta = lds_addr(tab) + wv * 64, sa = lds_addr(scl);
+  if constexpr (!FULL) {  // head values past D: never written by the DMA, zero for good
+    for (int i = tid; i < 4 * TILE / 16; i += C8_THREADS) ((uint4 *)lds)[i] = attn_zeros();
+  }
+
+  int turn = 0;
+#pragma unroll 1
+  while (left > 0) {
+    __syncthreads();
+    const AttnArgs a = attn_again<AttnArgs>(0);
+    const AttnWork w = attn_uniform(plan->work[turn]);
+    int *poison = &plan->poison[turn];
+    const int r = attn_uniform(attn_request(plan, a.R, w));
+    const AttnReq rq = attn_uniform(attn_req(plan, a, r));
+    const AttnTile t = attn_uniform(attn_tile(a, rq, w.tile - (r ? attn_end(plan, a.R, r - 1) : 0), C8_TR));
+    const int units = attn_units<C8_KT>(t);
+    const AttnPiece pc = attn_piece<C8_EXTRA>(w, units);
+    const int ks = (int)((uint32_t)t.b / C8_KT + pc.u0) * C8_KT, nt = pc.u1 - pc.u0;
+    const bool whole = pc.whole;
+    const int part = w.g * 2 + pc.start, head = w.head;
+    if (pc.start && !pc.none && here() == 0)
+      attn_note(attn_again<AttnShare>(sizeof(AttnArgs)), w, rq, t, units + C8_EXTRA, whole);
+    {
+      AttnWork on = w;
+      on.r = r;
+      attn_move_on(on, pc.take, units + C8_EXTRA);
+      left = on.left;
+      turn ^= 1;
+      if (here() == 0) plan->work[turn] = on, plan->poison[turn] = 0;
+    }
+    if (pc.none) continue;
+
+    const int *tabrow = a.table + (int64_t)r * a.W;
+    const int block = a.block, NB = a.NB, Hkv = a.Hkv, D = FULL ? DP : a.D;
+    const uint8_t *kc = (const uint8_t *)a.k, *vc = (const uint8_t *)a.v, *ksc = a.k_scales, *vsc = a.v_scales;
+    const float sc = a.scale == 0.f ? 1.f : fabsf(a.scale) * 1.44269504088896341f;
+
+    // the lane's row: what it sees, its queries
+    float m, l = 0.f;
+    i32x8_t qh[KS], ql[LO_LDS ? 1 : KS];
+    int qs[2] = {0, 0};  // their scales, a byte for each step
+    {
+      const int ln = (int)attn_lane(), in = wv * 32 + (ln & 31), lh = ln >> 5;
+      const bool on = in < t.rows;
+      const int row = t.row0 + (on ? in : 0);  // (a row past the end: the first one's queries)
+      const int pos = rq.base + (int)attn_div(row, a.by_g);
+      seen_at[here() * 2] = a.window && pos >= a.window ? pos - a.window + 1 : 0;
+      seen_at[here() * 2 + 1] = on ? pos : -1;
+      // (a row that sees nothing needs no reference; one past the end has no weights and passes none)
+      m = !on ? __builtin_inff() : pos >= 0 ? -__builtin_inff() : 0.f;
+      const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D;
+#pragma unroll
+      for (int s = 0; s < KS; ++s) {
+        const int at = s * 64 + lh * 32;
+        u32x4_t x[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          x[i] = u32x4_t{0u, 0u, 0u, 0u};
+          if (at + i * 8 < D) x[i] = *(const u32x4_t *)(qp + at + i * 8);
+          // a negative scale: -q, so that maxima stay maxima; none: no scores
+          x[i] = a.scale > 0.f ? x[i] : a.scale < 0.f ? x[i] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
+        }
+        i32x8_t lo;
+        int sh, sl;
+        attn_split<true>(x, qh[s], lo, sh, sl);
+        qs[0] |= sh << 8 * s, qs[1] |= sl << 8 * s;
+        if constexpr (LO_LDS) {
+          i32x4_t *to = (i32x4_t *)(qlo + wv * 32 * DP) + s * 128 + ln;
+          to[0] = __builtin_shufflevector(lo, lo, 0, 1, 2, 3), to[64] = __builtin_shufflevector(lo, lo, 4, 5, 6, 7);
+        } else {
+          ql[s] = lo;
+        }
+      }
+    }
+    f32x16_t acc[DT];
+#pragma unroll
+    for (int d = 0; d < DT; ++d)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
+
+    if (nt > 0) {
+      // Keys on their way: this lane looks up key wv * 8 + lane % 8 of each tile.  `off` is its place in its page, for the
+      // tile whose rows come next; `page` and `poff` are a tile on.
+      const uint32_t per = attn_div(C8_KT, a.by_block), rest = C8_KT - per * (uint32_t)block;
+      const uint32_t first = ks + wv * 8 + ((int)attn_lane() & 7);
+      uint32_t page = attn_div(first, a.by_block), poff = first - page * block, off = poff;
+      const uint32_t last_page = attn_div(t.e - 1, a.by_block);
+      auto onward = [&]() __attribute__((always_inline)) {
+        page += per, poff += rest;
+        if (poff >= (uint32_t)block) poff -= block, ++page;
+      };
+      auto ask = [&](int set) __attribute__((always_inline)) {  // page ids of tile `page`
+        if (attn_lane() < 8) c8_dma4(tabrow + (page < last_page ? page : last_page), ta + set * 32);
+      };
+      // a tile's keys and values, and their scales, into set `set`
+      auto move = [&](int k0, int blk, int set) __attribute__((always_inline)) {
+        const uint32_t ln = attn_lane();
+        const bool ok = k0 + wv * 8 + (int)(ln & 7) < t.e && (uint32_t)blk < (uint32_t)NB;
+        const uint32_t on = ok ? ~0u : 0u, of = ((uint32_t)blk * Hkv + head) & on;
+        const uint32_t mine = (of * block + off) & on;  // the row (of the whole cache) of this lane's key, 0 where there is none
+        vm[set * 32 + wv] = (uint8_t)__ballot(ok);
+        if (ln < 8) {
+          c8_dma1(ksc + of, sa + set * 512 + wv * 32);
+          c8_dma1(vsc + of, sa + set * 512 + 256 + wv * 32);
+        }
+        const uint32_t c0 = ln % CPR;
+#pragma unroll
+        for (int n = 0; n < OPS; ++n) {
+          const uint32_t in = n * RPI + ln / CPR;  // of the wave's 8 rows
+          const uint32_t row = __builtin_amdgcn_ds_bpermute((int)in * 4, (int)mine);
+          const uint32_t c = (c0 ^ (uint32_t)attn_swz8<DP>((int)(wv * 8 + in))) * 16;
+          const uint64_t at = (uint64_t)row * (uint32_t)D + c;
+          if ((RPI <= 8 || ln < 8 * CPR) && (FULL || c < (uint32_t)D)) {
+            const uint32_t to = la + set * TILE + wv * 8 * PITCH + n * 1024;
+            gp_dma16(kc + at, to);
+            gp_dma16(vc + at, to + 2 * TILE);
+          }
+        }
+      };
+      move(ks, tabrow[page < last_page ? page : last_page], 0);
+      onward();
+      ask(1);
+      int sb_was = 0, tv_was = 0;  // the last product's scales
+
+#pragma unroll 1
+      for (int i = 0; i < nt; ++i) {
+        const int set = i & 1, k0 = ks + i * C8_KT;
+        gp_wait_barrier<0>();  // tile i, its valid bits, page ids of tile i + 1; everyone has done with tile i - 1
+        if (i + 1 < nt) {
+          const int blk = *(const int *)(tab + wv * 64 + (set ^ 1) * 32 + (attn_lane() & 7) * 4);
+          off = poff;
+          move(k0 + C8_KT, blk, set ^ 1);
+          onward();
+          ask(set);
+        }
+        const uint2 bits = *(const uint2 *)(vm + set * 32);
+        const uint64_t valid = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)bits.y) << 32 |
+                               (uint32_t)__builtin_amdgcn_readfirstlane((int)bits.x);
+        const bool edge = k0 < t.full_b || k0 + C8_KT > t.full_e || valid != ~0ull;
+
+        // S^T of 2 x 32 keys
+        f32x16_t sv[2];
+        int kx[2];
+        {
+          const uint32_t ln = attn_lane();
+          const int row = ln & 31, lh = (int)(ln >> 5);
+          const int from = set * TILE + row * PITCH + ((lh * 2) ^ attn_swz8<DP>(row)) * 16;
+          const int *kxl = (const int *)(scl + set * 512) + row;
+          kx[0] = kxl[0], kx[1] = kxl[32];
+          auto load = [&](int s, int half) __attribute__((always_inline)) {
+            const int x = (from ^ s * 64) + half * 32 * PITCH, y = (from ^ (s * 64 + 16)) + half * 32 * PITCH;
+            const i32x4_t lo = *(const i32x4_t *)(lds + x), hi = *(const i32x4_t *)(lds + y);
+            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
+          };
+          auto step = [&](auto s_c) __attribute__((always_inline)) {
+            constexpr int s = decltype(s_c)::value;
+            const i32x8_t k0f = load(s, 0), k1f = load(s, 1);
+            i32x8_t lo;
+            if constexpr (LO_LDS) {
+              const i32x4_t *q = (const i32x4_t *)(qlo + wv * 32 * DP) + s * 128 + ln;
+              lo = __builtin_shufflevector(q[0], q[64], 0, 1, 2, 3, 4, 5, 6, 7);
+            } else {
+              lo = ql[s];
+            }
+            const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0f, qh[s], s ? sv[0] : z, 0, 0, 0, kx[0], s, qs[0]);
+            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1f, qh[s], s ? sv[1] : z, 0, 0, 0, kx[1], s, qs[0]);
+            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0f, lo, sv[0], 0, 0, 0, kx[0], s, qs[1]);
+            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1f, lo, sv[1], 0, 0, 0, kx[1], s, qs[1]);
+          };
+          step(std::integral_constant<int, 0>{});
+          if constexpr (KS > 1) step(std::integral_constant<int, 1>{});
+          if constexpr (KS > 2) step(std::integral_constant<int, 2>{}), step(std::integral_constant<int, 3>{});
+        }
+        if (edge) {
+          const int h4 = (int)attn_lane() >> 5 << 2;
+          const int2 sees = *(const int2 *)(seen_at + here() * 2);
+          const int lo = sees.x - k0, hi = sees.y - k0;
+          // bit o: key k0 + o is seen
+          uint64_t seen = hi < 0 ? 0ull : hi > 62 ? ~0ull : (2ull << hi) - 1ull;
+          seen &= lo > 63 ? 0ull : lo > 0 ? ~0ull << lo : ~0ull;
+          seen &= valid;
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t s32 = (uint32_t)(seen >> 32 * half) >> h4;
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const int on = __builtin_amdgcn_sbfe((int)s32, 8 * (j / 4) + j % 4, 1);  // 0 or -1
+              sv[half][j] = __uint_as_float((__float_as_uint(sv[half][j]) & (uint32_t)on) | (0xFF800000u & ~(uint32_t)on));
+            }
+          }
+        }
+
+        // The values' scales: one for all of the tile's keys, or the largest, with the weights of the others' keys less.
+        // (Pages whose scale is NaN add that to the rows that see them at the end.)
+        const int *vsl = (const int *)(scl + set * 512 + 256);
+        int tv;
+        bool mixed;
+        {
+          const uint32_t ln = attn_lane();
+          const int vs = vsl[ln];
+          const bool there = valid >> ln & 1;
+          const uint64_t fine = __ballot(there && vs != 255);
+          if (__any(there && vs == 255)) *poison = 1;
+          tv = fine ? __builtin_amdgcn_readlane(vs, __builtin_ctzll(fine)) : 127;
+          mixed = __any(there && vs != 255 && vs != tv);
+          if (mixed) tv = c8_top(there && vs != 255 ? vs : 0);
+        }
+        // Maxima of the scores (in powers of two, rounded up), and of what the weights with their scales come to
+        float top[2], most[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          top[half] = -__builtin_inff();
+#pragma unroll
+          for (int j = 0; j < 16; j += 2)
+            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top[half]) : "v"(sv[half][j]), "v"(sv[half][j + 1]));  // (fmaxf would first quiet each)
+          top[half] = __builtin_ceilf(c8_pair_max(top[half]) * sc);
+          most[half] = top[half];
+        }
+        // (the matrix unit reads its scale operands after the instruction has issued, and the compiler does not know: they
+        // stay in their registers until the products are read)
+        asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(sb_was), "v"(tv_was), "v"(top[0]), "v"(top[1]));
+        {
+          // The reference is the row's first maximum; it follows, and the sums with it, when a score passes it by 2^60.
+          const float all = fmaxf(top[0], top[1]);
+          m = m == -__builtin_inff() ? all : m;
+          if (__any(all > m + 60.f)) {
+            const bool up = all > m + 60.f;
+            const float f = up ? attn_exp2(m - all) : 1.f;
+            m = up ? all : m;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+          }
+        }
+        const float ref = m == -__builtin_inff() ? 0.f : m;
+        i32x8_t ph, pl;
+        int sb;
+        auto weights = [&](auto mixed_c) __attribute__((always_inline)) {
+          constexpr bool MIXED = decltype(mixed_c)::value;
+          int by[2];
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            i32x4_t vs[4];
+            if constexpr (MIXED) {
+              float y = -__builtin_inff();
+#pragma unroll
+              for (int v = 0; v < 4; ++v) {
+                vs[v] = *(const i32x4_t *)(vsl + half * 32 + v * 8 + ((int)attn_lane() >> 5) * 4) - tv;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) y = fmaxf(y, __builtin_fmaf(sv[half][v * 4 + j], sc, (float)vs[v][j]));
+              }
+              most[half] = __builtin_ceilf(c8_pair_max(y));
+            }
+            // weights up to 2^8 relative to 2^e, which the product takes back
+            const float e = fmaxf(most[half] - 8.f, ref - 120.f);
+            const float from = MIXED ? fmaxf(top[half], ref - 120.f) : e;
+            float sum = 0.f;
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              float x[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) {
+                x[j] = attn_exp2(__builtin_fmaf(sv[half][v * 4 + j], sc, -from));
+                sum += x[j];
+                if constexpr (MIXED) x[j] = ldexpf(x[j], vs[v][j] + (int)(from - e));
+              }
+              int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
+              hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
+              ph[half * 4 + v] = hi;
+              const f32x2_t b0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+              const float less = __uint_as_float((127u - 5u) << 23);  // the rest is at most 2^3: times 2^5
+              i16x2_t lo = {0, 0};
+              lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0] - b0.x, x[1] - b0.y, less, false);
+              lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2] - b1.x, x[3] - b1.y, less, true);
+              pl[half * 4 + v] = __builtin_bit_cast(int, lo);
+            }
+            l += ldexpf(sum, (int)(from - ref));
+            by[half] = (int)(e - ref) + 127;
+          }
+          sb = (int)attn_lane() >> 5 ? by[1] : by[0];  // (the lanes' scales are those of the two halves' keys)
+          sb = sb < 254 ? sb : 254;
+          sb = sb * 257 - (5 << 8);
+        };
+        if (mixed)
+          weights(std::true_type{});
+        else
+          weights(std::false_type{});
+
+        if (edge) {
+          // keys that are none, and codes that are NaN (which must not reach the rows that do not see their keys): zeros
+          // for now, in the rows that this wave has moved
+          bool odd = false;
+          const uint32_t ln = attn_lane();
+#pragma unroll
+          for (int n = 0; n < OPS; ++n) {
+            if (RPI <= 8 || ln < 8 * CPR) {
+              uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 8 * PITCH + n * 1024 + ln * 16);
+              const uint4 x = *at, y = attn_finite_codes(x);
+              const bool in = valid >> (wv * 8 + n * RPI + ln / CPR) & 1;
+              odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
+              *at = in ? y : attn_zeros();
+            }
+          }
+          if (__any(odd)) *poison = 1;
+          gp_lds_barrier();
+        }
+        // O^T += V^T P^T
+        int tvv = tv;
+        {
+          asm volatile("" : "+v"(tvv));  // (in a register of its own)
+          const uint32_t ln = attn_lane();
+          const int row = (int)((ln >> 3 & 1) * 8 + (ln >> 5) * 4 + (ln >> 1 & 3));
+          const uint32_t from = la + (2 + set) * TILE + row * PITCH + ((int)(ln >> 4 & 1) ^ attn_swz8<DP>(row)) * 16 + (ln & 1) * 8;
+#pragma unroll
+          for (int d = 0; d < DT; ++d) {
+            i32x8_t v;
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+              const i32x2_t x = attn_read_tr8((from ^ d * 32) + n * 16 * PITCH);
+              v[2 * n] = x.x, v[2 * n + 1] = x.y;
+            }
+            acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v, ph, acc[d], 0, 0, 0, tvv, 0, sb);
+            acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v, pl, acc[d], 0, 0, 0, tvv, 1, sb);
+          }
+        }
+        sb_was = sb, tv_was = tvv;
+      }
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      asm volatile("" ::"v"(sb_was), "v"(tv_was));
+    }
+
+    // Rows out, 64 columns of a wave's 32 rows at a time, through its part of the LDS (16-byte chunks, swizzled by row)
+    {
+      const AttnArgs a = attn_again<AttnArgs>(0);
+      const AttnShare s = attn_again<AttnShare>(sizeof(AttnArgs));
+      __syncthreads();
+      const int in0 = wv * 32;
+      if (in0 < t.rows) {
+        const float lu = l + attn_across(l, 32);
+        const float scale = !whole ? 1.f : lu != 0.f ? 1.f / lu : 0.f;
+        const int ln = (int)attn_lane();
+        if (!whole && ln < 32 && in0 + ln < t.rows) {
+          const int64_t pr = (int64_t)part * C8_TR + in0 + ln;
+          s.ml[pr * 2] = m, s.ml[pr * 2 + 1] = lu;
+        }
+        float *out = (float *)(lds + wv * 32 * 64 * 4);
+        const int end = ks + nt * C8_KT < t.e ? ks + nt * C8_KT : t.e;
+#pragma unroll
+        for (int c = 0; c < DP / 64; ++c) {
+#pragma unroll
+          for (int d = 0; d < 2; ++d)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const f32x16_t &x = acc[c * 2 + d];
+              *(float4 *)(out + (ln & 31) * 64 + ((d * 8 + v * 2 + (ln >> 5)) ^ (ln & 15)) * 4) =
+                  make_float4(x[4 * v] * scale, x[4 * v + 1] * scale, x[4 * v + 2] * scale, x[4 * v + 3] * scale);
+            }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+          for (int it = 0; it < 4; ++it) {
+            const int rr = it * 8 + (ln >> 3), k = ln & 7, in = in0 + rr, d0 = c * 64 + k * 8;
+            if (in >= t.rows || (!FULL && d0 >= a.D)) continue;
+            const float *x = out + rr * 64;
+            float o[8];
+            *(float4 *)&o[0] = *(const float4 *)(x + ((2 * k) ^ (rr & 15)) * 4);
+            *(float4 *)&o[4] = *(const float4 *)(x + ((2 * k + 1) ^ (rr & 15)) * 4);
+            if (*poison) attn_poison<true>(a, rq, tabrow, head, t.row0 + in, ks, end, d0, o);
+            if (whole) {
+              attn_store8(a, attn_row(a, rq.q0, t.row0 + in, head), d0, o);
+            } else {
+              float4 *to = (float4 *)(s.acc + ((int64_t)part * C8_TR + in) * DP + d0);
+              to[0] = make_float4(o[0], o[1], o[2], o[3]), to[1] = make_float4(o[4], o[5], o[6], o[7]);
+            }
+          }
+          __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+          __builtin_amdgcn_wave_barrier();
+        }
+      }
+    }
+    if constexpr (!FULL) {
+      __syncthreads();
+      for (int j = here(); j < 4 * TILE / 16; j += C8_THREADS) ((uint4 *)lds)[j] = attn_zeros();
+    }
+  }
+}
+
+template <int DP, bool FULL>
+hipError_t launch_t(const AttnArgs &a, const AttnShare &s, int grid, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const void *k = (const void *)attn_chunk8_kernel<DP, FULL>;
+  const hipError_t e = ensure_dynamic_lds(done, k, (int)attn_chunk8_lds(DP, ATTN_MAX_R));
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((attn_chunk8_kernel<DP, FULL>), dim3(grid), dim3(C8_THREADS), attn_chunk8_lds(DP, a.R), st, a, s);
+  return hipGetLastError();
+}
+
+template <int DP>
+hipError_t launch_dp(const AttnArgs &a, const AttnShare &s, int grid, hipStream_t st) {
+  return a.D == DP ? launch_t<DP, true>(a, s, grid, st) : launch_t<DP, false>(a, s, grid, st);
+}
+
+}  // namespace
+
+size_t attn_chunk8_lds(int DP, int R) { return c8_fixed(DP) + C8_SMALL + attn_plan_lds(R); }
+
+hipError_t launch_attn_chunk8(const AttnArgs &a, const AttnShare &s, int DP, int grid, hipStream_t st) {
+  return DP == 64 ? launch_dp<64>(a, s, grid, st) : DP == 128 ? launch_dp<128>(a, s, grid, st) : launch_dp<256>(a, s, grid, st);
+}
+
+}  // namespace qmm

@@ -110,15 +110,25 @@ class Cache:
     def values(self):
         return self._wide(self.v, self.vs)
 
+    @property
+    def scales(self):
+        """The scale of each value row: [L, Hkv] per request (1 where it is NaN)."""
+        return [self._wide(torch.full_like(self.v, 0x38), torch.where(self.vs == 255, 127, self.vs))[r][..., 0]
+                for r in range(len(self.lens))]
 
-def attend(q, keys, values, starts, kv_lens, scale, window=0, gate=None, few=False):
+
+def attend(q, keys, values, starts, kv_lens, scale, window=0, gate=None, few=False, scales=None):
     """(o, bound) of paged attention in float64, a key head's rows at a time, on q's device; q [T, Hq, D].
 
-    bound: the result's rounding to bf16 (2^-8); of sum p |v|: the weights' rounding (two E4M3 parts: 2^-4 of 2^-4, so 2^-8,
-    and 2^-22 of the largest of 32; few: two bf16 parts, 2^-16) and as much for the sum that divides, f32 dot products and
-    exponents (D + 8 roundings of 2^-24 of scale sum |q k|), the queries' two parts (2^-22 of the largest of 128 values, times
+    bound: the result's rounding to bf16 (2^-8); of sum p |v|: the weights' rounding (two E4M3 parts: 2^-4 of 2^-4, so 2^-8;
+    few: two bf16 parts, 2^-16) and as much for the sum that divides, f32 dot products and exponents (D + 8 roundings of 2^-24 of scale sum |q k|), the queries' two parts (2^-22 of the largest of 128 values, times
     the sum of |k| there), both twice: in the weight and in the sum; exp2 (2^-22 twice); f32 sums over L keys, at worst 16
-    at a time in a line (L / 16 + 64 roundings of 2^-24, in the sum as well)."""
+    at a time in a line (L / 16 + 64 roundings of 2^-24, in the sum as well).
+
+    Not few: E4M3's steps end at 2^-9.  The weights of 32 keys (each times its value's scale) go in relative to their largest,
+    which lies above 2^7; what the first part leaves is at most 2^3 and goes in times 2^5, so its own steps end at 2^-14 and
+    leave 2^-15: 2^-22 of the largest weight, on the codes of all 32 keys.  scales: those of the values, [L, Hkv] per request
+    (none: 1 for all)."""
     T, Hq, D = q.shape
     o = torch.zeros(T, Hq, D, dtype=torch.float64, device=q.device)
     bound = torch.full_like(o, 1e-30)
@@ -146,9 +156,15 @@ def attend(q, keys, values, starts, kv_lens, scale, window=0, gate=None, few=Fal
                 p = torch.where(seen.any(-1, keepdim=True), p, 0.0)
                 pv = torch.where(seen.any(-1, keepdim=True).expand(b - a, g, 1).reshape(-1, 1), masked(p.view(-1, L), v, seen, g), 0.0)
                 o[a:b, h * g:(h + 1) * g] = pv.view(b - a, g, D)
-                parts = 2 ** -16 if few else 2 ** -8 + 32 * 2 ** -22
+                parts = 2 ** -16 if few else 2 ** -8
                 weight = 2 * parts + size + 2 ** -21 + 2 * (L / 16 + 64) * 2 ** -24
-                bound[a:b, h * g:(h + 1) * g] += weight * (p.view(-1, L) @ v.abs().nan_to_num(0.0)).view(b - a, g, D)
+                size_v = v.abs().nan_to_num(0.0)
+                bound[a:b, h * g:(h + 1) * g] += weight * (p.view(-1, L) @ size_v).view(b - a, g, D)
+                if not few:
+                    f = scales[r][:, h].to(q.device) if scales else torch.ones(L, dtype=torch.float64, device=q.device)
+                    big = torch.nn.functional.pad((p.view(-1, L) * f).nan_to_num(0.0), (0, -L % 32)).view(p.view(-1, L).shape[0], -1, 32)
+                    codes = torch.nn.functional.pad(size_v / f[:, None], (0, 0, 0, -L % 32)).view(-1, 32, D)
+                    bound[a:b, h * g:(h + 1) * g] += 2 ** -22 * (big.amax(-1) @ codes.sum(1)).view(b - a, g, D)
     bound += 2 ** -8 * o.abs().nan_to_num(0.0)
     if gate is not None:
         f = 1 / (1 + torch.exp(-gate.double()))

@@ -67,7 +67,7 @@ def test_attention(Hq, Hkv, D, block, lens, window, gated):
     q = (2 * torch.randn(T, Hq, D, generator=g)).to(torch.bfloat16)
     gate = torch.randn(T, Hq, 2 * D, generator=g).to(torch.bfloat16) if gated else None
     want, bound = ref.attend(q.cuda(), c.keys, c.values, starts_of(new), kv, D ** -0.5, window,
-                             gate[..., D:].cuda() if gated else None)
+                             gate[..., D:].cuda() if gated else None, scales=c.scales)
     got = attention(c, q, starts_of(new), kv, window=window, gate=gate)
     assert torch.isfinite(got).all()
     assert close(got, want, bound)
@@ -79,7 +79,7 @@ def test_rows_that_see_nothing():
     D, new, kv = 64, [5, 3, 70, 2], [2, 0, 40, 9]
     c = ref.Cache(kv, 2, D, 16, seed=1)
     q = torch.randn(sum(new) + 9, 8, D, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, starts_of(new), kv, 0.125)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, starts_of(new), kv, 0.125, scales=c.scales)
     got = attention(c, q, starts_of(new), kv)
     assert close(got, want, bound)
     for rows in (slice(0, 3), slice(5, 8), slice(8, 38), slice(80, 89)):
@@ -127,7 +127,7 @@ def test_past_the_tables_width():
     c = ref.Cache([64], 2, D, 16, seed=3)
     q = torch.randn(10, 4, D, generator=torch.Generator().manual_seed(4)).to(torch.bfloat16)
     for kv in (70, 2 ** 31 - 1):
-        want, bound = ref.attend(q, c.keys, c.values, [0, 10], [kv], 0.125)
+        want, bound = ref.attend(q, c.keys, c.values, [0, 10], [kv], 0.125, scales=c.scales)
         assert close(attention(c, q, [0, 10], [kv]), want, bound)
 
 
@@ -149,7 +149,7 @@ def test_extreme_scores(new, L, kind):
         x += dict(equal=0 * j, rising=j / 10, falling=-j / 10, low=0 * j - 50)[kind]
         slots = [int(c.table[0, i // 16]) * 16 + i % 16 for i in range(L)]
         c.k, c.ks, _ = ref.store(c.k, c.ks, slots, x.double())
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], scale)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], scale, scales=c.scales)
     got = attention(c, q, [0, new], [L], scale=scale)
     assert torch.isfinite(got).all() and close(got, want, bound)
 
@@ -159,7 +159,7 @@ def test_extreme_scores(new, L, kind):
 def test_other_scales(new, scale):
     c = ref.Cache([200], 1, 64, 16, seed=8)
     q = torch.rand(new, 2, 64, generator=torch.Generator().manual_seed(9)).to(torch.bfloat16) + 0.5
-    want, bound = ref.attend(q, c.keys, c.values, [0, new], [200], scale)
+    want, bound = ref.attend(q, c.keys, c.values, [0, new], [200], scale, scales=c.scales)
     assert close(attention(c, q, [0, new], [200], scale=scale), want, bound)
 
 
@@ -176,7 +176,7 @@ def test_values_that_are_nan(new, window, D):
     for page in (None, 23, 20):
         if page:
             c.vs[int(c.table[0, page]), 1] = 255
-        want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, window)
+        want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, window, scales=c.scales)
         got = attention(c, q, [0, new], [L], window=window).double()
         want, bound = want.cpu(), bound.cpu()
         assert torch.equal(torch.isnan(got), torch.isnan(want))
@@ -191,7 +191,7 @@ def test_keys_that_are_nan_and_not_seen(D, new):
     L = 300
     c = ref.Cache([L], 1, D, 16, seed=22)
     q = torch.randn(new, 2, D, generator=torch.Generator().manual_seed(23)).to(torch.bfloat16)
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
     c.k[int(c.table[0, (L - 30) // 16]), :, (L - 30) % 16] = 127
     got = attention(c, q, [0, new], [L])
     sees = max(0, new - 30)
@@ -200,7 +200,7 @@ def test_keys_that_are_nan_and_not_seen(D, new):
     c.ks[int(c.table[0, 18])] = 255  # positions 288 and on
     got = attention(c, q, [0, new], [L])
     sees = max(0, new - 12)
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
     assert torch.isnan(got[sees:]).all() and close(got[:sees], want[:sees], bound[:sees])
 
 
@@ -231,7 +231,7 @@ def test_queries_and_scales_of_all_sizes(new, D):
     c.ks[pages] = torch.randint(112, 122, (len(pages), 2), generator=g, dtype=torch.uint8)
     q = torch.randn(new, 4, D, generator=g) * 2.0 ** -torch.randint(0, 21, (D,), generator=g)
     q = q.to(torch.bfloat16)
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
     assert close(attention(c, q, [0, new], [L]), want, bound)
 
 
@@ -263,7 +263,7 @@ def test_past_32_bit_offsets(new):
         for big, small in ((k, c.k), (v, c.v), (ks, c.ks), (vs, c.vs)):
             big[p] = small[int(c.table[0, i])].cuda()
     q = torch.randn(new, 8, D, generator=torch.Generator().manual_seed(11)).to(torch.bfloat16)
-    want, bound = ref.attend(q, c.keys, c.values, [0, new], [300], 1 / 16)
+    want, bound = ref.attend(q, c.keys, c.values, [0, new], [300], 1 / 16, scales=c.scales)
     got = host(Q.paged_attention_fp8(dev(q), *[Q.Array.from_torch(t) for t in (k, v, ks, vs)], ints([pages]), ints([0, new]),
                                      ints([300]), scale=1 / 16))
     assert close(got, want, bound)
@@ -278,7 +278,7 @@ def test_many_requests():
         new = [min(k, 1 + (r % 50 == 7) * 40) for r, k in enumerate(kv)]
         c = ref.Cache(kv, Hkv, D, 16, seed=31)
         q = torch.randn(sum(new), Hq, D, generator=g).to(torch.bfloat16)
-        want, bound = ref.attend(q.cuda(), c.keys, c.values, starts_of(new), kv, D ** -0.5)
+        want, bound = ref.attend(q.cuda(), c.keys, c.values, starts_of(new), kv, D ** -0.5, scales=c.scales)
         assert close(attention(c, q, starts_of(new), kv), want, bound), R
 
 
@@ -288,7 +288,7 @@ def test_two_streams_at_once_and_in_place():
     c = ref.Cache([9000, 3000], 2, D, 16, seed=12)
     g = torch.Generator().manual_seed(13)
     q, gate = (torch.randn(2, 8, D, generator=g).to(torch.bfloat16) for _ in range(2))
-    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, 1, 2], [9000, 3000], D ** -0.5, gate=gate.cuda())
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, 1, 2], [9000, 3000], D ** -0.5, gate=gate.cuda(), scales=c.scales)
     cache = [dev(t) for t in (c.k, c.v, c.ks, c.vs)]
     rest = [ints(c.table), ints([0, 1, 2]), ints([9000, 3000])]
     a, w = dev(q), dev(gate)
