@@ -273,7 +273,7 @@ Route route_of(const AttnArgs &a) {
   }
   if (one || !few) {
     r.chunk.tr = r.chunk.rows = 256;
-    r.chunk.grid = r.DP == 64 && !a.k_scales ? 2 * cus : cus;
+    r.chunk.grid = r.DP == 64 ? 2 * cus : cus;
     r.chunk.min_rows = one ? 0 : ROWS_MOST, r.chunk.max_rows = INT32_MAX;
   }
   r.bytes = 0;

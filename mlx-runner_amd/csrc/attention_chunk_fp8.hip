@@ -9,7 +9,8 @@
 //
 // A tile is 256 rows, 32 for each of eight waves, two a SIMD: one's softmax beside the other's products, with nothing
 // interleaved by hand.  (Codes are half of bf16's bytes: eight waves' operands from LDS take the bandwidth that four waves' of
-// 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, one barrier a tile.
+// 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, eight keys by each wave; one
+// barrier a tile.
 #include <type_traits>
 
 #include "attention.h"
@@ -24,7 +25,9 @@ constexpr int C8_TR = 256, C8_KT = 64;
 constexpr int C8_EXTRA = 3;   // what a tile's own overhead costs, in units of 64 keys
 constexpr int C8_SCALES = 2 * 2 * 256;                  // scale bytes of the keys, of the values; a dword each, two sets
 constexpr int C8_TAB = C8_WAVES * 2 * 32;               // page ids of the tiles to come
-constexpr int C8_SMALL = C8_SCALES + C8_TAB + 2 * C8_WAVES * 4 + 8 * C8_THREADS;
+constexpr int C8_VALID = 2 * C8_WAVES;                  // bits of the keys that there are, two sets
+constexpr int C8_SMALL = C8_SCALES + C8_TAB + C8_VALID + 8 * C8_THREADS;
+constexpr int C8_NEAR = 8;  // scales of 32 keys' values that differ by up to 2^8 go in relative to the largest
 
 constexpr int c8_tile(int DP) { return C8_KT * DP; }
 constexpr int c8_queries(int DP) { return DP == 256 ? C8_TR * DP : 0; }  // the queries' second parts
@@ -43,30 +46,24 @@ __device__ __forceinline__ void c8_dma1(const void *g, uint32_t l) {
 }
 #pragma clang diagnostic pop
 
+// A register as it is: for conversions that write half of one.
+__device__ __forceinline__ int c8_any() {
+  int x;
+  asm volatile("" : "=v"(x));
+  return x;
+}
+// (fmaxf would first quiet each)
+__device__ __forceinline__ float c8_max3(float x, float y, float z) {
+  asm("v_max3_f32 %0, %0, %1, %2" : "+v"(x) : "v"(y), "v"(z));
+  return x;
+}
 // The larger of x here and 32 lanes away.
 __device__ __forceinline__ float c8_pair_max(float x) {
   const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
   return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-// The wave's largest.
-__device__ __forceinline__ int c8_top(int x) {
-#define QMM_STEP(ctrl, rows)                                                          \
-  {                                                                                   \
-    const int y = __builtin_amdgcn_update_dpp(x, x, ctrl, rows, 0xF, false);          \
-    x = y > x ? y : x;                                                                \
-  }
-  QMM_STEP(0x111, 0xF);  // row_shr:1, 2, 4, 8; row_bcast:15, 31
-  QMM_STEP(0x112, 0xF);
-  QMM_STEP(0x114, 0xF);
-  QMM_STEP(0x118, 0xF);
-  QMM_STEP(0x142, 0xA);
-  QMM_STEP(0x143, 0xC);
-#undef QMM_STEP
-  return __builtin_amdgcn_readlane(x, 63);
-}
-
 template <int DP, bool FULL>
-__global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnArgs args, const AttnShare share) {
+__global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kernel(const AttnArgs args, const AttnShare share) {
   constexpr int CPR = DP / 16;     // 16-byte chunks of a row
   constexpr int KS = DP / 64;      // k steps of S^T
   constexpr int DT = DP / 32;      // 32-column tiles of O^T
@@ -78,8 +75,8 @@ __global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnAr
   uint8_t *qlo = lds + c8_fixed(DP) - c8_queries(DP);
   uint8_t *scl = lds + c8_fixed(DP);                 // [2][keys, values][64]
   uint8_t *tab = scl + C8_SCALES;                    // [wave][2][8]
-  uint8_t *vm = tab + C8_TAB;                        // [2][8 waves], a byte each: keys that there are
-  int *seen_at = (int *)(vm + 2 * C8_WAVES * 4);     // [thread][2]: what its row sees
+  uint8_t *vm = tab + C8_TAB;                        // [2][8 waves], a byte each
+  int *seen_at = (int *)(vm + C8_VALID);             // [thread][2]: what its row sees
   AttnPlan *plan = (AttnPlan *)(seen_at + 2 * C8_THREADS);
 
   const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -173,68 +170,67 @@ __global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnAr
       for (int i = 0; i < 16; ++i) acc[d][i] = 0.f;
 
     if (nt > 0) {
-      // Keys on their way: this lane looks up key wv * 8 + lane % 8 of each tile.  `off` is its place in its page, for the
-      // tile whose rows come next; `page` and `poff` are a tile on.
+      // Keys on their way: this lane looks up key wv * 8 + lane % 8 of each tile; `page` and `off` (its place in its page)
+      // are those of the tile whose page ids are asked for next.
       const uint32_t per = attn_div(C8_KT, a.by_block), rest = C8_KT - per * (uint32_t)block;
       const uint32_t first = ks + wv * 8 + ((int)attn_lane() & 7);
-      uint32_t page = attn_div(first, a.by_block), poff = first - page * block, off = poff;
+      uint32_t page = attn_div(first, a.by_block), off = first - page * block;
       const uint32_t last_page = attn_div(t.e - 1, a.by_block);
       auto onward = [&]() __attribute__((always_inline)) {
-        page += per, poff += rest;
-        if (poff >= (uint32_t)block) poff -= block, ++page;
+        page += per, off += rest;
+        if (off >= (uint32_t)block) off -= block, ++page;
       };
-      auto ask = [&](int set) __attribute__((always_inline)) {  // page ids of tile `page`
-        if (attn_lane() < 8) c8_dma4(tabrow + (page < last_page ? page : last_page), ta + set * 32);
+      auto ask = [&](int set) __attribute__((always_inline)) {
+        if (attn_lane() < 8) c8_dma4(tabrow + (page < last_page ? page : last_page), attn_uniform(ta + set * 32));
       };
-      // a tile's keys and values, and their scales, into set `set`
-      auto move = [&](int k0, int blk, int set) __attribute__((always_inline)) {
+      // tile j's rows of the whole cache, for this lane's key (0 where there is none), and their pages' scales' places
+      uint32_t mine = 0, of = 0, there = 0;
+      auto look_up = [&](int j, int blk, uint32_t at) __attribute__((always_inline)) {
+        const bool page_there = (uint32_t)blk < (uint32_t)NB;
+        const bool ok = page_there && ks + j * C8_KT + wv * 8 + ((int)attn_lane() & 7) < t.e;
+        of = ((uint32_t)blk * Hkv + head) & (page_there ? ~0u : 0u);
+        mine = (of * block + at) & (ok ? ~0u : 0u);
+        there = (uint32_t)__ballot(ok) & 0xFFu;
+        vm[(j & 1) * C8_WAVES + wv] = (uint8_t)there;
+      };
+      auto move = [&](const uint8_t *cache, int to) __attribute__((always_inline)) {
         const uint32_t ln = attn_lane();
-        const bool ok = k0 + wv * 8 + (int)(ln & 7) < t.e && (uint32_t)blk < (uint32_t)NB;
-        const uint32_t on = ok ? ~0u : 0u, of = ((uint32_t)blk * Hkv + head) & on;
-        const uint32_t mine = (of * block + off) & on;  // the row (of the whole cache) of this lane's key, 0 where there is none
-        vm[set * 32 + wv] = (uint8_t)__ballot(ok);
-        if (ln < 8) {
-          c8_dma1(ksc + of, sa + set * 512 + wv * 32);
-          c8_dma1(vsc + of, sa + set * 512 + 256 + wv * 32);
-        }
         const uint32_t c0 = ln % CPR;
 #pragma unroll
         for (int n = 0; n < OPS; ++n) {
           const uint32_t in = n * RPI + ln / CPR;  // of the wave's 8 rows
           const uint32_t row = __builtin_amdgcn_ds_bpermute((int)in * 4, (int)mine);
           const uint32_t c = (c0 ^ (uint32_t)attn_swz8<DP>((int)(wv * 8 + in))) * 16;
-          const uint64_t at = (uint64_t)row * (uint32_t)D + c;
-          if ((RPI <= 8 || ln < 8 * CPR) && (FULL || c < (uint32_t)D)) {
-            const uint32_t to = la + set * TILE + wv * 8 * PITCH + n * 1024;
-            gp_dma16(kc + at, to);
-            gp_dma16(vc + at, to + 2 * TILE);
-          }
+          if ((RPI <= 8 || ln < 8 * CPR) && (FULL || c < (uint32_t)D))
+            gp_dma16(cache + ((uint64_t)row * (uint32_t)D + c), attn_uniform(la + to + wv * 8 * PITCH + n * 1024));
         }
       };
-      move(ks, tabrow[page < last_page ? page : last_page], 0);
-      onward();
-      ask(1);
-      int sb_was = 0, tv_was = 0;  // the last product's scales
-
-#pragma unroll 1
-      for (int i = 0; i < nt; ++i) {
-        const int set = i & 1, k0 = ks + i * C8_KT;
-        gp_wait_barrier<0>();  // tile i, its valid bits, page ids of tile i + 1; everyone has done with tile i - 1
-        if (i + 1 < nt) {
-          const int blk = *(const int *)(tab + wv * 64 + (set ^ 1) * 32 + (attn_lane() & 7) * 4);
-          off = poff;
-          move(k0 + C8_KT, blk, set ^ 1);
-          onward();
-          ask(set);
+      auto move_all = [&](int j) __attribute__((always_inline)) {
+        const int set = j & 1;
+        if (attn_lane() < 8) {
+          c8_dma1(ksc + of, attn_uniform(sa + set * 512 + wv * 32));
+          c8_dma1(vsc + of, attn_uniform(sa + set * 512 + 256 + wv * 32));
         }
-        const uint2 bits = *(const uint2 *)(vm + set * 32);
-        const uint64_t valid = (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)bits.y) << 32 |
-                               (uint32_t)__builtin_amdgcn_readfirstlane((int)bits.x);
-        const bool edge = k0 < t.full_b || k0 + C8_KT > t.full_e || valid != ~0ull;
+        move(kc, set * TILE);
+        move(vc, (2 + set) * TILE);
+      };
+      auto valid_of = [&](int j) __attribute__((always_inline)) -> uint64_t {
+        const uint2 bits = *(const uint2 *)(vm + (j & 1) * C8_WAVES);
+        return (uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)bits.y) << 32 |
+               (uint32_t)__builtin_amdgcn_readfirstlane((int)bits.x);
+      };
+      // whether rows of the tile see different keys of tile j
+      auto differ = [&](int j) __attribute__((always_inline)) -> bool {
+        const int k0 = ks + j * C8_KT;
+        return k0 < t.full_b || k0 + C8_KT > t.full_e;
+      };
 
-        // S^T of 2 x 32 keys
-        f32x16_t sv[2];
-        int kx[2];
+      f32x16_t sv[2];
+      int kx[2] = {0, 0}, sb = 0, tvv = 0;  // the products' scales
+      i32x8_t ph{}, pl{};
+      // S^T of tile j: 2 x 32 keys
+      auto scores = [&](int j) __attribute__((always_inline)) {
+        const int set = j & 1;
         {
           const uint32_t ln = attn_lane();
           const int row = ln & 31, lh = (int)(ln >> 5);
@@ -246,26 +242,85 @@ __global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnAr
             const i32x4_t lo = *(const i32x4_t *)(lds + x), hi = *(const i32x4_t *)(lds + y);
             return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
           };
-          auto step = [&](auto s_c) __attribute__((always_inline)) {
-            constexpr int s = decltype(s_c)::value;
-            const i32x8_t k0f = load(s, 0), k1f = load(s, 1);
-            i32x8_t lo;
+          auto second = [&](int s) __attribute__((always_inline)) {
             if constexpr (LO_LDS) {
               const i32x4_t *q = (const i32x4_t *)(qlo + wv * 32 * DP) + s * 128 + ln;
-              lo = __builtin_shufflevector(q[0], q[64], 0, 1, 2, 3, 4, 5, 6, 7);
+              return __builtin_shufflevector(q[0], q[64], 0, 1, 2, 3, 4, 5, 6, 7);
             } else {
-              lo = ql[s];
+              return ql[s];
             }
+          };
+          i32x8_t k0 = load(0, 0), k1;
+          auto step = [&](auto s_c) __attribute__((always_inline)) {
+            constexpr int s = decltype(s_c)::value;
             const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0f, qh[s], s ? sv[0] : z, 0, 0, 0, kx[0], s, qs[0]);
-            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1f, qh[s], s ? sv[1] : z, 0, 0, 0, kx[1], s, qs[0]);
-            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0f, lo, sv[0], 0, 0, 0, kx[0], s, qs[1]);
-            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1f, lo, sv[1], 0, 0, 0, kx[1], s, qs[1]);
+            i32x8_t k0n;
+            const i32x8_t lo = second(s);
+            k1 = load(s, 1);
+            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0, qh[s], s ? sv[0] : z, 0, 0, 0, kx[0], s, qs[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0, lo, sv[0], 0, 0, 0, kx[0], s, qs[1]);
+            if constexpr (s + 1 < KS) k0n = load(s + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1, qh[s], s ? sv[1] : z, 0, 0, 0, kx[1], s, qs[0]);
+            __builtin_amdgcn_sched_barrier(0);
+            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1, lo, sv[1], 0, 0, 0, kx[1], s, qs[1]);
+            __builtin_amdgcn_sched_barrier(0);
+            if constexpr (s + 1 < KS) k0 = k0n;
           };
           step(std::integral_constant<int, 0>{});
           if constexpr (KS > 1) step(std::integral_constant<int, 1>{});
           if constexpr (KS > 2) step(std::integral_constant<int, 2>{}), step(std::integral_constant<int, 3>{});
+          asm volatile("" : "+v"(sv[0]), "+v"(sv[1]));  // (as after a product)
         }
+      };
+      // What the scales of tile j's values do to its weights: of eight keys each (they have one, where pages are multiples of
+      // eight), how far it is below the largest of their half, 4 bits each; `far`: the halves where that does not do.
+      // (Pages whose scale is NaN add that to the rows that see them at the end.)
+      int tv[2], less = 0, far = 0;
+      auto prepare = [&](int j) __attribute__((always_inline)) {
+        const uint32_t ln = attn_lane();
+        const int vs = *((const int *)(scl + (j & 1) * 512 + 256) + ln);
+        const uint64_t valid = valid_of(j);
+        const uint64_t nan = __ballot(vs == 255) & valid, fine = valid & ~nan;
+        if (nan) *poison = 1;
+        // (a lane beside the one before it, but for the first of eight; one that is not there has its page's, or the first page's)
+        const uint64_t other = __ballot(vs != __builtin_amdgcn_update_dpp(vs, vs, 0x111, 0xF, 0xF, false)) & 0xFEFEFEFEFEFEFEFEull;
+        far = ((uint32_t)other != 0) | ((uint32_t)(other >> 32) != 0) << 1;
+        less = 0;
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          int x[4], most = 0;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            x[v] = __builtin_amdgcn_readlane(vs, half * 32 + v * 8);
+            x[v] = fine >> (half * 32 + v * 8) & 1 ? x[v] : -1;
+            most = x[v] > most ? x[v] : most;
+          }
+          tv[half] = most;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int d = x[v] < 0 ? 0 : most - x[v];
+            far |= (d > C8_NEAR) << half;
+            less |= (d & 15) << (half * 16 + v * 4);
+          }
+          if (far >> half & 1) {  // the largest of all
+            uint64_t keys = 0xFFFFFFFFull << 32 * half & fine;
+            while (keys) {  // (once for each scale there is)
+              const int y = __builtin_amdgcn_readlane(vs, __builtin_ctzll(keys));
+              tv[half] = y > tv[half] ? y : tv[half];
+              keys &= ~__ballot(vs == y);
+            }
+          }
+        }
+      };
+      // the weights of tile j's scores
+      auto soften = [&](int j) __attribute__((always_inline)) {
+        const int k0 = ks + j * C8_KT;
+        const uint64_t valid = valid_of(j);
+        const bool edge = differ(j) || valid != ~0ull;
+        // (inline assembly reads S^T below: a 16-pass product's results can be read after 19 wait states)
+        asm volatile("s_nop 15\n\ts_nop 3" : "+v"(sv[0]), "+v"(sv[1]));
         if (edge) {
           const int h4 = (int)attn_lane() >> 5 << 2;
           const int2 sees = *(const int2 *)(seen_at + here() * 2);
@@ -285,35 +340,18 @@ __global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnAr
           }
         }
 
-        // The values' scales: one for all of the tile's keys, or the largest, with the weights of the others' keys less.
-        // (Pages whose scale is NaN add that to the rows that see them at the end.)
-        const int *vsl = (const int *)(scl + set * 512 + 256);
-        int tv;
-        bool mixed;
-        {
-          const uint32_t ln = attn_lane();
-          const int vs = vsl[ln];
-          const bool there = valid >> ln & 1;
-          const uint64_t fine = __ballot(there && vs != 255);
-          if (__any(there && vs == 255)) *poison = 1;
-          tv = fine ? __builtin_amdgcn_readlane(vs, __builtin_ctzll(fine)) : 127;
-          mixed = __any(there && vs != 255 && vs != tv);
-          if (mixed) tv = c8_top(there && vs != 255 ? vs : 0);
-        }
-        // Maxima of the scores (in powers of two, rounded up), and of what the weights with their scales come to
-        float top[2], most[2];
+        // Maxima of the scores, in powers of two, rounded up
+        float top[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           top[half] = -__builtin_inff();
 #pragma unroll
-          for (int j = 0; j < 16; j += 2)
-            asm("v_max3_f32 %0, %0, %1, %2" : "+v"(top[half]) : "v"(sv[half][j]), "v"(sv[half][j + 1]));  // (fmaxf would first quiet each)
+          for (int j = 0; j < 16; j += 2) top[half] = c8_max3(top[half], sv[half][j], sv[half][j + 1]);
           top[half] = __builtin_ceilf(c8_pair_max(top[half]) * sc);
-          most[half] = top[half];
         }
         // (the matrix unit reads its scale operands after the instruction has issued, and the compiler does not know: they
         // stay in their registers until the products are read)
-        asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(sb_was), "v"(tv_was), "v"(top[0]), "v"(top[1]));
+        asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(sb), "v"(tvv), "v"(top[0]), "v"(top[1]));
         {
           // The reference is the row's first maximum; it follows, and the sums with it, when a score passes it by 2^60.
           const float all = fmaxf(top[0], top[1]);
@@ -328,100 +366,151 @@ __global__ __launch_bounds__(C8_THREADS, 2) void attn_chunk8_kernel(const AttnAr
           }
         }
         const float ref = m == -__builtin_inff() ? 0.f : m;
-        i32x8_t ph, pl;
-        int sb;
-        auto weights = [&](auto mixed_c) __attribute__((always_inline)) {
-          constexpr bool MIXED = decltype(mixed_c)::value;
-          int by[2];
-#pragma unroll
-          for (int half = 0; half < 2; ++half) {
-            i32x4_t vs[4];
-            if constexpr (MIXED) {
-              float y = -__builtin_inff();
-#pragma unroll
-              for (int v = 0; v < 4; ++v) {
-                vs[v] = *(const i32x4_t *)(vsl + half * 32 + v * 8 + ((int)attn_lane() >> 5) * 4) - tv;
-#pragma unroll
-                for (int j = 0; j < 4; ++j) y = fmaxf(y, __builtin_fmaf(sv[half][v * 4 + j], sc, (float)vs[v][j]));
-              }
-              most[half] = __builtin_ceilf(c8_pair_max(y));
-            }
-            // weights up to 2^8 relative to 2^e, which the product takes back
-            const float e = fmaxf(most[half] - 8.f, ref - 120.f);
-            const float from = MIXED ? fmaxf(top[half], ref - 120.f) : e;
-            float sum = 0.f;
+        int by[2];
+        const int *vsl = (const int *)(scl + (j & 1) * 512 + 256);
+        // x = 2^(scale s - d - e), d how far eight keys' scale is below the largest.  FAR: relative to the largest of what the
+        // weights with their scales come to, which e does not follow otherwise.
+        auto weights = [&](auto half_c, auto far_c) __attribute__((always_inline)) {
+          constexpr int half = decltype(half_c)::value;
+          constexpr bool FAR = decltype(far_c)::value;
+          float most = top[half];
+          if constexpr (FAR) {
+            most = -__builtin_inff();
 #pragma unroll
             for (int v = 0; v < 4; ++v) {
-              float x[4];
+              const i32x4_t vs = *(const i32x4_t *)(vsl + half * 32 + v * 8 + ((int)attn_lane() >> 5) * 4);
+              float y[4];
 #pragma unroll
-              for (int j = 0; j < 4; ++j) {
-                x[j] = attn_exp2(__builtin_fmaf(sv[half][v * 4 + j], sc, -from));
-                sum += x[j];
-                if constexpr (MIXED) x[j] = ldexpf(x[j], vs[v][j] + (int)(from - e));
-              }
-              int hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], 0, false);
-              hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
-              ph[half * 4 + v] = hi;
-              const f32x2_t b0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
-              const float less = __uint_as_float((127u - 5u) << 23);  // the rest is at most 2^3: times 2^5
-              i16x2_t lo = {0, 0};
-              lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0] - b0.x, x[1] - b0.y, less, false);
-              lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2] - b1.x, x[3] - b1.y, less, true);
-              pl[half * 4 + v] = __builtin_bit_cast(int, lo);
+              for (int j = 0; j < 4; ++j) y[j] = __builtin_fmaf(sv[half][v * 4 + j], sc, (float)(uint8_t)vs[j]);
+              most = c8_max3(c8_max3(most, y[0], y[1]), y[2], y[3]);
+              __builtin_amdgcn_sched_barrier(0);
             }
-            l += ldexpf(sum, (int)(from - ref));
-            by[half] = (int)(e - ref) + 127;
+            most = __builtin_ceilf(c8_pair_max(most) - (float)tv[half]);
           }
-          sb = (int)attn_lane() >> 5 ? by[1] : by[0];  // (the lanes' scales are those of the two halves' keys)
-          sb = sb < 254 ? sb : 254;
-          sb = sb * 257 - (5 << 8);
+          // weights up to 2^8 relative to 2^e, which the product takes back
+          const float e = fmaxf(most - 8.f, ref - 120.f);
+          const float from = FAR ? fmaxf(top[half], ref - 120.f) : e;
+          const int rest = FAR ? (int)(from - e) - tv[half] : 0;
+          float sum = 0.f;
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            float x[4];
+            i32x4_t vs;
+            if constexpr (FAR) vs = *(const i32x4_t *)(vsl + half * 32 + v * 8 + ((int)attn_lane() >> 5) * 4);
+            const int d = FAR ? 0 : less >> (half * 16 + v * 4) & 15;
+            const float down = -from - (float)d;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) x[j] = attn_exp2(__builtin_fmaf(sv[half][v * 4 + j], sc, down));
+            sum = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), (float)(1 << d), sum);
+            if constexpr (FAR) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_ldexpf(x[j], vs[j] + rest);
+            }
+            int hi = c8_any();
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[0], x[1], hi, false);
+            hi = __builtin_amdgcn_cvt_pk_fp8_f32(x[2], x[3], hi, true);
+            ph[half * 4 + v] = hi;
+            const f32x2_t b0 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, false), b1 = __builtin_amdgcn_cvt_pk_f32_fp8(hi, true);
+            const float under = __uint_as_float((127u - 5u) << 23);  // the rest is at most 2^3: times 2^5
+            i16x2_t lo = __builtin_bit_cast(i16x2_t, c8_any());
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[0] - b0.x, x[1] - b0.y, under, false);
+            lo = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(lo, x[2] - b1.x, x[3] - b1.y, under, true);
+            pl[half * 4 + v] = __builtin_bit_cast(int, lo);
+            if constexpr (FAR) __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
+          }
+          l += __builtin_amdgcn_ldexpf(sum, (int)(from - ref));
+          by[half] = (int)(e - ref) + 127;
         };
-        if (mixed)
-          weights(std::true_type{});
-        else
-          weights(std::false_type{});
+        auto weights_of = [&](auto half_c) __attribute__((always_inline)) {
+          constexpr int half = decltype(half_c)::value;
+          if (far >> half & 1)
+            weights(half_c, std::true_type{});
+          else
+            weights(half_c, std::false_type{});
+        };
+        weights_of(std::integral_constant<int, 0>{});
+        weights_of(std::integral_constant<int, 1>{});
+        // (the lanes' scales are those of the two halves' keys)
+        const bool upper = (int)attn_lane() >> 5;
+        sb = upper ? by[1] : by[0];
+        sb = sb < 254 ? sb : 254;
+        sb = sb * 257 - (5 << 8);
 
-        if (edge) {
-          // keys that are none, and codes that are NaN (which must not reach the rows that do not see their keys): zeros
-          // for now, in the rows that this wave has moved
-          bool odd = false;
-          const uint32_t ln = attn_lane();
+        tvv = upper ? tv[1] : tv[0];
+        asm volatile("" : "+v"(tvv));  // (in a register of its own)
+      };
+      // Keys that are none, and codes that are NaN (which must not reach the rows that do not see their keys): zeros for now,
+      // in the rows of the values that this wave has moved
+      auto clean = [&](int j) __attribute__((always_inline)) {
+        if (!differ(j) && there == 0xFFu) return;
+        bool odd = false;
+        const uint32_t ln = attn_lane();
 #pragma unroll
-          for (int n = 0; n < OPS; ++n) {
-            if (RPI <= 8 || ln < 8 * CPR) {
-              uint4 *at = (uint4 *)(lds + (2 + set) * TILE + wv * 8 * PITCH + n * 1024 + ln * 16);
-              const uint4 x = *at, y = attn_finite_codes(x);
-              const bool in = valid >> (wv * 8 + n * RPI + ln / CPR) & 1;
-              odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
-              *at = in ? y : attn_zeros();
-            }
-          }
-          if (__any(odd)) *poison = 1;
-          gp_lds_barrier();
-        }
-        // O^T += V^T P^T
-        int tvv = tv;
-        {
-          asm volatile("" : "+v"(tvv));  // (in a register of its own)
-          const uint32_t ln = attn_lane();
-          const int row = (int)((ln >> 3 & 1) * 8 + (ln >> 5) * 4 + (ln >> 1 & 3));
-          const uint32_t from = la + (2 + set) * TILE + row * PITCH + ((int)(ln >> 4 & 1) ^ attn_swz8<DP>(row)) * 16 + (ln & 1) * 8;
-#pragma unroll
-          for (int d = 0; d < DT; ++d) {
-            i32x8_t v;
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-              const i32x2_t x = attn_read_tr8((from ^ d * 32) + n * 16 * PITCH);
-              v[2 * n] = x.x, v[2 * n + 1] = x.y;
-            }
-            acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v, ph, acc[d], 0, 0, 0, tvv, 0, sb);
-            acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(v, pl, acc[d], 0, 0, 0, tvv, 1, sb);
+        for (int n = 0; n < OPS; ++n) {
+          if (RPI <= 8 || ln < 8 * CPR) {
+            uint4 *to = (uint4 *)(lds + (2 + (j & 1)) * TILE + wv * 8 * PITCH + n * 1024 + ln * 16);
+            const uint4 x = *to, y = attn_finite_codes(x);
+            const bool in = there >> (n * RPI + ln / CPR) & 1;
+            odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
+            *to = in ? y : attn_zeros();
           }
         }
-        sb_was = sb, tv_was = tvv;
+        if (__any(odd)) *poison = 1;
+      };
+      // O^T += V^T P^T
+      auto product = [&](int j) __attribute__((always_inline)) {
+        const int set = j & 1;
+        const uint32_t ln = attn_lane();
+        const int row = (int)((ln >> 3 & 1) * 8 + (ln >> 5) * 4 + (ln >> 1 & 3));
+        const uint32_t from = la + (2 + set) * TILE + row * PITCH + ((int)(ln >> 4 & 1) ^ attn_swz8<DP>(row)) * 16 + (ln & 1) * 8;
+        auto load = [&](int d) __attribute__((always_inline)) {
+          i32x8_t v;
+#pragma unroll
+          for (int n = 0; n < 4; ++n) {
+            const i32x2_t x = attn_read_tr8((from ^ d * 32) + n * 16 * PITCH);
+            v[2 * n] = x.x, v[2 * n + 1] = x.y;
+          }
+          return v;
+        };
+        i32x8_t vf[DT];
+        constexpr int AHEAD = 3;
+#pragma unroll
+        for (int d = 0; d < AHEAD && d < DT; ++d) vf[d] = load(d);
+#pragma unroll
+        for (int d = 0; d < DT; ++d) {
+          if (d + AHEAD < DT) vf[d + AHEAD] = load(d + AHEAD);
+          acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vf[d], ph, acc[d], 0, 0, 0, tvv, 0, sb);
+          acc[d] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(vf[d], pl, acc[d], 0, 0, 0, tvv, 1, sb);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        // (the compiler would put products off behind the branches that follow, and keep their operands till then)
+#pragma unroll
+        for (int d = 0; d < DT; ++d) asm volatile("" : "+v"(acc[d]));
+      };
+
+      look_up(0, tabrow[page < last_page ? page : last_page], off);
+      move_all(0);
+      onward();
+      ask(1);
+#pragma unroll 1
+      for (int i = 0; i < nt; ++i) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        clean(i);
+        gp_lds_barrier();  // tile i, its valid bits, page ids of tile i + 1; everyone has done with tile i - 1
+        if (i + 1 < nt) {
+          const int blk = *(const int *)(tab + wv * 64 + ((i + 1) & 1) * 32 + (attn_lane() & 7) * 4);
+          look_up(i + 1, blk, off);
+          move_all(i + 1);
+          onward();
+          ask(i & 1);
+        }
+        scores(i);
+        prepare(i);
+        soften(i);
+        product(i);
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      asm volatile("" ::"v"(sb_was), "v"(tv_was));
+      asm volatile("" ::"v"(sb), "v"(tvv), "v"(kx[0]), "v"(kx[1]));
     }
 
     // Rows out, 64 columns of a wave's 32 rows at a time, through its part of the LDS (16-byte chunks, swizzled by row)

@@ -125,10 +125,11 @@ def attend(q, keys, values, starts, kv_lens, scale, window=0, gate=None, few=Fal
     the sum of |k| there), both twice: in the weight and in the sum; exp2 (2^-22 twice); f32 sums over L keys, at worst 16
     at a time in a line (L / 16 + 64 roundings of 2^-24, in the sum as well).
 
-    Not few: E4M3's steps end at 2^-9.  The weights of 32 keys (each times its value's scale) go in relative to their largest,
-    which lies above 2^7; what the first part leaves is at most 2^3 and goes in times 2^5, so its own steps end at 2^-14 and
-    leave 2^-15: 2^-22 of the largest weight, on the codes of all 32 keys.  scales: those of the values, [L, Hkv] per request
-    (none: 1 for all)."""
+    Not few: E4M3's steps end at 2^-9.  The weights of 32 keys go in relative to their largest, which lies above 2^7, each
+    times its value's scale over the largest scale of the 32 (scales that differ by more than 2^8: relative to the largest
+    product of weight and scale); what the first part leaves is at most 2^3 and goes in times 2^5, so its own steps end at
+    2^-14 and leave 2^-15: 2^-22 of the largest weight, on the codes of all 32 keys at the largest scale.  scales: those of
+    the values, [L, Hkv] per request (none: 1 for all)."""
     T, Hq, D = q.shape
     o = torch.zeros(T, Hq, D, dtype=torch.float64, device=q.device)
     bound = torch.full_like(o, 1e-30)
@@ -162,9 +163,13 @@ def attend(q, keys, values, starts, kv_lens, scale, window=0, gate=None, few=Fal
                 bound[a:b, h * g:(h + 1) * g] += weight * (p.view(-1, L) @ size_v).view(b - a, g, D)
                 if not few:
                     f = scales[r][:, h].to(q.device) if scales else torch.ones(L, dtype=torch.float64, device=q.device)
-                    big = torch.nn.functional.pad((p.view(-1, L) * f).nan_to_num(0.0), (0, -L % 32)).view(p.view(-1, L).shape[0], -1, 32)
-                    codes = torch.nn.functional.pad(size_v / f[:, None], (0, 0, 0, -L % 32)).view(-1, 32, D)
-                    bound[a:b, h * g:(h + 1) * g] += 2 ** -22 * (big.amax(-1) @ codes.sum(1)).view(b - a, g, D)
+                    grouped = lambda x, dim: torch.nn.functional.pad(x, (0, 0) * (x.dim() - 1 - dim) + (0, -L % 32)).unflatten(dim, (-1, 32))  # noqa: E731
+                    pf, most = grouped((p.view(-1, L) * f).nan_to_num(0.0), 1).amax(-1), grouped(p.view(-1, L).nan_to_num(0.0), 1).amax(-1)
+                    fs = grouped(f, 0)
+                    top = fs.amax(-1)
+                    near = top <= 2.0 ** 8 * torch.where(fs > 0, fs, math.inf).amin(-1)
+                    codes = grouped(size_v / f[:, None], 0).sum(1)
+                    bound[a:b, h * g:(h + 1) * g] += 2 ** -22 * (torch.where(near, most * top, pf) @ codes).view(b - a, g, D)
     bound += 2 ** -8 * o.abs().nan_to_num(0.0)
     if gate is not None:
         f = 1 / (1 + torch.exp(-gate.double()))
