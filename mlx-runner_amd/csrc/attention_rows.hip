@@ -145,6 +145,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
     bf16x8_t q[NQ][E8 ? 1 : ST];
     i32x8_t q8[NQ][E8 ? S8 : 1][P8];  // E4M3: the queries in two parts, and their scales, a byte for each
     int qs[NQ];
+    u32x4_t raw[NQ][E8 ? S8 : 1][4];  // as they lie in memory: split when the first keys are on their way
 #pragma unroll
     for (int n = 0; n < NQ; ++n) {
       const bool on = n * 16 + lr < t.rows;
@@ -159,28 +160,13 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
       // matrix unit's k they are does not matter, where keys and queries agree
       if constexpr (E8) {
 #pragma unroll
-        for (int st = 0; st < S8; ++st) {
-          if (st == 0) qs[n] = 0;
-          const int at = st * 128 + (DP == 64 ? lg & 1 : lg) * 32;
-          u32x4_t x[4];
+        for (int st = 0; st < S8; ++st)
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            x[i] = u32x4_t{0u, 0u, 0u, 0u};
-            if (at + i * 8 < D) x[i] = *(const u32x4_t *)(qp + at + i * 8);
-            x[i] = a.scale > 0.f ? x[i] : a.scale < 0.f ? x[i] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};  // (as below)
+            const int at = st * 128 + (DP == 64 ? lg & 1 : lg) * 32 + i * 8;
+            raw[n][st][i] = u32x4_t{0u, 0u, 0u, 0u};
+            if (at < D) raw[n][st][i] = *(const u32x4_t *)(qp + at);
           }
-          if constexpr (P8 == 2) {
-            int sh, sl;
-            attn_split(x, q8[n][st][0], q8[n][st][1], sh, sl);
-            qs[n] |= (sl << 8 | sh) << 16 * st;
-          } else {
-            i32x8_t lo;
-            int sh, sl;
-            attn_split(x, q8[n][st][0], lo, sh, sl);
-            q8[n][st][0] = lg < 2 ? q8[n][st][0] : lo;
-            qs[n] = lg & 1 ? sl : sh;  // (the lanes' scales are those of the 32-value blocks 0 .. 3, hi and lo by turns)
-          }
-        }
       } else {
 #pragma unroll
         for (int st = 0; st < ST; ++st) {
@@ -258,6 +244,31 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
       onward();
       move(kc, ka);
       move(vc, va);
+      if constexpr (E8) {
+        const float scale = a.scale;
+        const int lg = (int)attn_lane() >> 4;
+#pragma unroll
+        for (int n = 0; n < NQ; ++n) {
+          qs[n] = 0;
+#pragma unroll
+          for (int st = 0; st < S8; ++st) {
+            if (!(scale > 0.f)) {  // (as above)
+#pragma unroll
+              for (int i = 0; i < 4; ++i) raw[n][st][i] = scale < 0.f ? raw[n][st][i] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
+            }
+            i32x8_t lo;
+            int sh, sl;
+            attn_split(raw[n][st], q8[n][st][0], lo, sh, sl);
+            if constexpr (P8 == 2) {
+              q8[n][st][P8 - 1] = lo;
+              qs[n] |= (sl << 8 | sh) << 16 * st;
+            } else {
+              q8[n][st][0] = lg < 2 ? q8[n][st][0] : lo;
+              qs[n] = lg & 1 ? sl : sh;  // (the lanes' scales are those of the 32-value blocks 0 .. 3, hi and lo by turns)
+            }
+          }
+        }
+      }
       int buf = 1;  // (the scales' set of a tile is 1 - buf)
 #pragma unroll 1
       while (true) {
