@@ -232,12 +232,6 @@ struct Route {
 };
 
 // ceil(2^(31 + l) / d), l = ceil(log2 d): exact quotients for n < 2^31
-FastDiv fast_div(uint32_t d) {
-  uint32_t l = 0;
-  while (((uint64_t)1 << l) < d) ++l;
-  return FastDiv{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), l};
-}
-
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t lay_out(Part &p, const AttnArgs &a, int DP, int g, size_t at) {

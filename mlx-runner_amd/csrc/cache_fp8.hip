@@ -49,15 +49,27 @@ __device__ __forceinline__ uint32_t shrink4(uint32_t w, int by) {
 struct CacheWrite {
   uint8_t *scales[2];  // of k, of v
   int windows;
+  FastDiv by_block, by_half;
+  // The grid: `writers` workgroups for k and v, one behind every `period` - 1 of those that turn q's heads, `parts` to a token.
+  int writers, period, parts;
 };
+
+__device__ __forceinline__ int fast_quot(int n, FastDiv d) { return (int)(__umulhi((uint32_t)n << 1, d.mul) >> d.shift); }
 
 template <int PAIRS, bool IN_F32>
 __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
-  constexpr int HELD = 2;  // turns whose values stay in registers
-  __shared__ __attribute__((aligned(16))) float norm[256], cs[ROPE_THREADS * 8], sn[ROPE_THREADS * 8];
+  __shared__ __attribute__((aligned(16))) float cs[ROPE_THREADS * 8], sn[ROPE_THREADS * 8], norm[ROPE_MAX_SETS][256];
   __shared__ __attribute__((aligned(16))) float swap[PAIRS == ACROSS ? ROPE_THREADS * 16 : 4];
+  __shared__ float freq[128];
+  __shared__ int pos[CW_RUNS];
   __shared__ uint32_t top[CW_RUNS];
-  __shared__ int begun[CW_RUNS], page_of[CW_RUNS], exponent[CW_RUNS], grown[CW_RUNS];
+  __shared__ int begun[CW_RUNS], exponent[CW_RUNS], grown[CW_RUNS], grown_page[CW_RUNS], n_grown;
+  const int writer = (int)blockIdx.x / w.period;
+  if (writer >= w.writers || (int)blockIdx.x != writer * w.period) {
+    const int before = writer < w.writers ? writer + 1 : w.writers;
+    rope_heads<PAIRS, IN_F32, false>(a, 1, lph, w.parts, blockIdx.x - before, cs, sn, norm, swap);
+    return;
+  }
   const int tid = threadIdx.x, lane = tid & 63;
   const int rows = ROPE_THREADS >> lph;  // of a turn, and a window's
   const int l = tid & ((1 << lph) - 1), g = tid >> lph;
@@ -66,71 +78,93 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
   const bool in0 = d0 < a.D, in1 = d1 < a.D;
   const int heads = a.set[1].heads;
 
-  auto page_at = [&](int t) -> int {  // -1: none
-    const int slot = a.slots[t];
-    const int page = slot / a.block;
+  auto page_of = [&](int slot) -> int {  // -1: none
+    const int page = fast_quot(slot, w.by_block);
     return slot >= 0 && page < a.NB ? page : -1;
   };
 #pragma unroll 1
-  for (int64_t item = blockIdx.x; item < (int64_t)w.windows * 2 * heads; item += gridDim.x) {
+  for (int64_t item = writer; item < (int64_t)w.windows * 2 * heads; item += w.writers) {
     const int side = (int)(item % (2 * heads)) / heads, head = (int)(item % heads), w0 = (int)(item / (2 * heads)) * rows;
     const RopeHeads &s = a.set[1 + side];
-    // the runs that start in the window, by every wave for itself: a bit for the first row of each
+    // What the first steps need, on its way at once: slots from the window's first row on (64 at least), weights and
+    // frequencies; where the call is one window, also the rows and what their pages hold.
     const int w1 = a.T - w0 < rows ? a.T : w0 + rows;
-    const int t = w0 + lane, mine = t < w1 ? page_at(t) : -1, before = t < w1 && t > 0 ? page_at(t - 1) : -1;
-    const uint64_t starts = __ballot(mine >= 0 && mine != before);
+    const int t = w0 + lane;
+    const int slot_t = t < a.T ? a.slots[t] : -1, slot_b = w0 > 0 ? a.slots[w0 - 1] : -1;
+    const float freq_l = s.rotate && tid < a.half ? a.freqs[tid] : 0.f;
+    const bool one = a.T <= rows;
+    const int pos_l = one && s.rotate && tid < a.T ? a.positions[tid] : 0;
+    auto load = [&](int row, Eight<IN_F32> (&raw)[2]) __attribute__((always_inline)) {
+      const int64_t at = ((int64_t)row * heads + head) * s.in_stride;
+      if (in0) raw[0] = load8<IN_F32>(s.in, at + d0);
+      if (in1) raw[1] = load8<IN_F32>(s.in, at + d1);
+    };
+    Eight<IN_F32> early[2] = {};
+    if (one && g < a.T) load(g, early);
+    float norm_l = 0.f;
+    if (s.norm && tid < a.D)
+      norm_l = s.norm_f32 ? ((const float *)s.norm)[tid] : __uint_as_float((uint32_t)((const uint16_t *)s.norm)[tid] << 16);
+
+    // the runs that start in the window, by every wave for itself: a bit for the first row of each
+    const int mine = page_of(slot_t);
+    const int up = __shfl_up(mine, 1, 64), before = lane ? up : page_of(slot_b);
+    const uint64_t starts = __ballot(t < w1 && mine >= 0 && mine != before);
     if (starts == 0) continue;
-    const int first = w0 + __builtin_ctzll(starts), last_page = __builtin_amdgcn_readlane(mine, w1 - w0 - 1);
+    const int lead = __builtin_ctzll(starts), first = w0 + lead;
+    const int last_page = __builtin_amdgcn_readlane(mine, w1 - w0 - 1);
     int end = w1;
-    while (last_page >= 0 && end < a.T) {  // its last run's end
-      const uint64_t other = __ballot(end + lane >= a.T || page_at(end + lane) != last_page);
-      if (other) {
-        end += __builtin_ctzll(other);
-        break;
+    if (last_page >= 0 && end < a.T) {  // its last run's end
+      uint64_t other = __ballot(t >= a.T || mine != last_page);
+      other &= rows < 64 ? ~0ull << rows : 0;
+      end = w0 + 64;
+      while (!other) {
+        other = __ballot(end + lane >= a.T || page_of(a.slots[end + lane]) != last_page);
+        end += 64;
       }
-      end += 64;
+      end += __builtin_ctzll(other) - 64;
     }
-    const int runs = __popcll(starts);
+    const bool starter = tid < 64 && (starts >> lane & 1);  // has a run of its own
+    uint8_t *const scale = w.scales[side] + (int64_t)mine * heads + head;
+    const int old = starter ? (int)*scale - 127 : 0;
     __syncthreads();  // (the last item's are read)
     if (tid < CW_RUNS) top[tid] = 0, begun[tid] = 0;
-    if (mine >= 0 && mine != before && tid < 64) page_of[__popcll(starts & ((1ull << lane) - 1))] = mine;
-    if (s.norm)
-      norm[tid] = tid >= a.D ? 0.f
-                  : s.norm_f32 ? ((const float *)s.norm)[tid]
-                               : __uint_as_float((uint32_t)((const uint16_t *)s.norm)[tid] << 16);
-    __syncthreads();
+    if (tid < 128) freq[tid] = freq_l;
+    norm[0][tid] = norm_l;
 
     auto run_of = [&](int row) -> int {
       const int i = row - w0;
       return __popcll(starts & (i < 63 ? (2ull << i) - 1 : ~0ull)) - 1;
     };
-    // the values of row `row0 + g` (all threads: there are barriers)
-    auto values = [&](int row0, float (&x)[2][8]) __attribute__((always_inline)) {
-      const int row = row0 + g;
-      const bool on = row < end;
-      Eight<IN_F32> raw[2] = {};
-      const int64_t at = ((int64_t)(on ? row : first) * heads + head) * s.in_stride;
-      if (in0) raw[0] = load8<IN_F32>(s.in, at + d0);
-      if (in1) raw[1] = load8<IN_F32>(s.in, at + d1);
+    // The turns, last to first, for the maxima: then the first one's values are still there, and only the others' are formed
+    // again for their codes (16 rows of 256, 32 of 128 or 64 of 64 values are one turn).
+    const int turns = (end - first + rows - 1) / rows;
+#pragma unroll 1
+    for (int step = 0; step < 2 * turns - 1; ++step) {
+      const int row0 = first + (step < turns ? turns - 1 - step : step - turns + 1) * rows, row = row0 + g;
+      if (step) __syncthreads();  // (the angles of the turn before are read)
+      Eight<IN_F32> raw[2] = {early[0], early[1]};
+      if (!(one && lead == 0)) load(row < end ? row : first, raw);
+      const int slot = row < end ? a.slots[row] : -1;
       if (s.rotate) {
+        if (tid < rows) pos[tid] = one && lead == 0 ? pos_l : row0 + tid < end ? a.positions[row0 + tid] : 0;
         __syncthreads();
-        const int half = a.half;
-        for (int i = tid; i < rows * half; i += ROPE_THREADS) {
-          const int r = i / half, j = i - r * half;
-          if (row0 + r >= end) break;
+        const int half = a.half, n = (end - row0 < rows ? end - row0 : rows) * half;
+        for (int i = tid; i < n; i += ROPE_THREADS) {
+          const int r = fast_quot(i, w.by_half), j = i - r * half;
           float sv, c;
-          rope_angle(a.positions[row0 + r], a.freqs[j], sv, c);
+          rope_angle(pos[r], freq[j], sv, c);
           cs[i] = c * a.amplitude, sn[i] = sv * a.amplitude * a.sign;
         }
-        __syncthreads();
       }
+      __syncthreads();
+      float x[2][8];
 #pragma unroll
       for (int k = 0; k < 2; ++k) widen<IN_F32>(raw[k], x[k]);
-      if (s.norm) rope_norm(x, &norm[d0 & 255], &norm[d1 & 255], in0, in1, lph, a.D, a.eps);
-      if (!s.rotate) return;
+      if (s.norm) rope_norm(x, &norm[0][d0 & 255], &norm[0][d1 & 255], in0, in1, lph, a.D, a.eps);
       if constexpr (PAIRS == ACROSS) {
-        rope_turn_across(x, swap + (tid >> lph << lph) * 16, l, a.half, a.interleaved, cs + g * a.half, sn + g * a.half);
-      } else if (turned) {
+        if (s.rotate)
+          rope_turn_across(x, swap + (tid >> lph << lph) * 16, l, a.half, a.interleaved, cs + g * a.half, sn + g * a.half);
+      } else if (s.rotate && turned) {
         float c[8], sv[8];
 #pragma unroll
         for (int j = 0; j < 8; j += 4)
@@ -138,79 +172,65 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
           *(float4 *)&sv[j] = *(const float4 *)&sn[g * a.half + l * 8 + j];
         rope_turn<PAIRS>(x, c, sv);
       }
-    };
-    float held[HELD][2][8];
-    auto measure = [&](int row0, const float (&x)[2][8]) __attribute__((always_inline)) {
-      const int row = row0 + g;
-      float m = 0.f;
+      const int page = page_of(slot);
+      if (step < turns) {
+        float m = 0.f;
 #pragma unroll
-      for (int j = 0; j < 8; ++j) {
-        if (in0 && finite(x[0][j])) m = fmaxf(m, fabsf(x[0][j]));
-        if (in1 && finite(x[1][j])) m = fmaxf(m, fabsf(x[1][j]));
+        for (int j = 0; j < 8; ++j) {
+          if (in0 && finite(x[0][j])) m = fmaxf(m, fabsf(x[0][j]));
+          if (in1 && finite(x[1][j])) m = fmaxf(m, fabsf(x[1][j]));
+        }
+        for (int off = 1 << lph >> 1; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        if (l == 0 && page >= 0) {
+          const int run = run_of(row);
+          atomicMax(&top[run], __float_as_uint(m));
+          if (slot == page * a.block) begun[run] = 1;
+        }
       }
-      for (int off = 1 << lph >> 1; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
-      if (l == 0 && row < end && page_at(row) >= 0) {
-        const int run = run_of(row);
-        atomicMax(&top[run], __float_as_uint(m));
-        if (a.slots[row] % a.block == 0) begun[run] = 1;
-      }
-    };
-#pragma unroll
-    for (int h = 0; h < HELD; ++h)
-      if (first + h * rows < end) {
-        values(first + h * rows, held[h]);
-        measure(first + h * rows, held[h]);
-      }
+      if (step == turns - 1) {  // the scales, and older codes where they grow
+        __syncthreads();
+        if (tid < 64) {
+          const int run = __popcll(starts & ((1ull << lane) - 1));
+          int by = 0;
+          if (starter) {
+            const float m = __uint_as_float(top[run]);
+            int e = m > 0.f ? ceil_scale_exp(m) : -127;
+            if (!begun[run]) {
+              by = e > old ? e - old : 0;
+              e = e > old ? e : old;
+            }
+            *scale = (uint8_t)(e + 127);
+            exponent[run] = e;
+          }
+          const uint64_t all = __ballot(by > 0);
+          const int i = __popcll(all & ((1ull << lane) - 1));
+          if (by > 0) grown[i] = by, grown_page[i] = mine;
+          if (lane == 0) n_grown = __popcll(all);
+        }
+        __syncthreads();
+        if (n_grown) {
+          const int64_t per = (int64_t)a.block * a.D / 16;  // of a page, 16 codes each
+          int64_t i = tid;
+          int r = 0;
 #pragma unroll 1
-    for (int row0 = first + HELD * rows; row0 < end; row0 += rows) {
-      float x[2][8];
-      values(row0, x);
-      measure(row0, x);
-    }
-    __syncthreads();
-    if (tid < runs) {
-      const float m = __uint_as_float(top[tid]);
-      int e = m > 0.f ? ceil_scale_exp(m) : -127;
-      uint8_t *scale = w.scales[side] + (int64_t)page_of[tid] * heads + head;
-      const int old = (int)*scale - 127;
-      int by = 0;
-      if (!begun[tid]) {
-        by = e > old ? e - old : 0;
-        e = e > old ? e : old;
+          while (true) {
+            while (r < n_grown && i >= per) i -= per, ++r;
+            if (r >= n_grown) break;
+            uint4 *codes = (uint4 *)((uint8_t *)s.out + ((int64_t)grown_page[r] * heads + head) * a.block * a.D) + i;
+            const int by = grown[r];
+            const uint4 c = *codes;
+            *codes = make_uint4(shrink4(c.x, by), shrink4(c.y, by), shrink4(c.z, by), shrink4(c.w, by));
+            i += ROPE_THREADS;
+          }
+          __syncthreads();  // (their rows of this call come after)
+        }
       }
-      *scale = (uint8_t)(e + 127);
-      exponent[tid] = e, grown[tid] = by;
-    }
-    __syncthreads();
-    for (int r = 0; r < runs; ++r) {
-      const int by = grown[r];
-      if (by == 0) continue;
-      uint4 *codes = (uint4 *)((uint8_t *)s.out + ((int64_t)page_of[r] * heads + head) * a.block * a.D);
-      for (int64_t i = tid; i < (int64_t)a.block * a.D / 16; i += ROPE_THREADS) {
-        uint4 c = codes[i];
-        c = make_uint4(shrink4(c.x, by), shrink4(c.y, by), shrink4(c.z, by), shrink4(c.w, by));
-        codes[i] = c;
+      if (step >= turns - 1 && page >= 0) {
+        const int e = exponent[run_of(row)];
+        uint8_t *to = (uint8_t *)s.out + (((int64_t)page * heads + head) * a.block + (slot - page * a.block)) * a.D;
+        if (in0) *(uint2 *)(to + d0) = codes8(x[0], e);
+        if (in1) *(uint2 *)(to + d1) = codes8(x[1], e);
       }
-    }
-    __syncthreads();  // (their rows of this call come after)
-    auto store = [&](int row0, const float (&x)[2][8]) __attribute__((always_inline)) {
-      const int row = row0 + g;
-      if (row >= end) return;
-      const int page = page_at(row);
-      if (page < 0) return;
-      const int e = exponent[run_of(row)];
-      uint8_t *to = (uint8_t *)s.out + (((int64_t)page * heads + head) * a.block + (a.slots[row] - page * a.block)) * a.D;
-      if (in0) *(uint2 *)(to + d0) = codes8(x[0], e);
-      if (in1) *(uint2 *)(to + d1) = codes8(x[1], e);
-    };
-#pragma unroll
-    for (int h = 0; h < HELD; ++h)
-      if (first + h * rows < end) store(first + h * rows, held[h]);
-#pragma unroll 1
-    for (int row0 = first + HELD * rows; row0 < end; row0 += rows) {
-      float x[2][8];
-      values(row0, x);
-      store(row0, x);
     }
   }
 }
@@ -270,24 +290,30 @@ void launch_pairs(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph
 
 }  // namespace
 
-hipError_t launch_rope_fp8(const RopeArgs &args, uint8_t *const (&scales)[ROPE_MAX_SETS], hipStream_t st) {
-  RopeArgs q = args;
-  q.sets = 1;
-  if (q.set[0].heads > 0) {
-    const hipError_t e = launch_rope(q, st);
-    if (e != hipSuccess) return e;
-  }
-  const RopeArgs &a = args;
+hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_SETS], hipStream_t st) {
   if (a.T <= 0 || a.D < 16 || a.D > 256 || a.D % 16 || a.half < 0 || 2 * a.half > a.D || a.sets != 3 || a.block < 1 ||
-      a.set[1].heads < 1 || a.set[1].heads != a.set[2].heads)
+      a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
   const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4, rows = ROPE_THREADS >> lph;
-  CacheWrite w{{scales[1], scales[2]}, (int)(((int64_t)a.T + rows - 1) / rows)};
+  CacheWrite w{{scales[1], scales[2]}, (int)(((int64_t)a.T + rows - 1) / rows), fast_div(a.block), fast_div(a.half ? a.half : 1),
+               0, 1, 0};
   const int64_t items = (int64_t)w.windows * 2 * a.set[1].heads;
-  const unsigned grid = (unsigned)(items < 1 << 20 ? items : 1 << 20);
-  a.half % 8      ? launch_pairs<ACROSS>(a, w, grid, lph, st)
-  : a.interleaved ? launch_pairs<NEXT>(a, w, grid, lph, st)
-                  : launch_pairs<HALVES>(a, w, grid, lph, st);
+  w.writers = (int)(items < 1 << 20 ? items : 1 << 20);
+  int64_t grid = w.writers;
+  if (a.T > ROPE_TOKENS) {  // (a grid's lanes are counted in 32 bits: q in launches of its own)
+    RopeArgs q = a;
+    q.sets = 1;
+    const hipError_t e = launch_rope(q, st);
+    if (e != hipSuccess) return e;
+  } else {
+    w.parts = (int)rope_parts(a, 1, lph);
+    const int64_t turners = (int64_t)a.T * w.parts;
+    grid += turners;
+    w.period = 1 + (int)(turners / w.writers);
+  }
+  a.half % 8      ? launch_pairs<ACROSS>(a, w, (unsigned)grid, lph, st)
+  : a.interleaved ? launch_pairs<NEXT>(a, w, (unsigned)grid, lph, st)
+                  : launch_pairs<HALVES>(a, w, (unsigned)grid, lph, st);
   return hipGetLastError();
 }
 

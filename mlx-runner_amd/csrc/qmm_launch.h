@@ -191,6 +191,16 @@ struct BlockTableArgs {
 };
 hipError_t launch_block_tables(const BlockTableArgs &a, hipStream_t st);
 
+// n / d for n < 2^31 as the high half of 2 n * mul, shifted.
+struct FastDiv {
+  uint32_t mul, shift;
+};
+inline FastDiv fast_div(uint32_t d) {
+  uint32_t l = 0;
+  while (((uint64_t)1 << l) < d) ++l;
+  return FastDiv{(uint32_t)((((uint64_t)1 << (31 + l)) + d - 1) / d), l};
+}
+
 // Head norm, rotation and cache write of up to three sets of heads of T tokens.
 struct RopeHeads {
   const void *in;      // [T, heads, in_stride]: the first D values of each
@@ -225,10 +235,6 @@ hipError_t launch_cache_read(const CacheReadArgs &a, hipStream_t st);
 
 // Attention of the requests' new tokens over their pages.
 constexpr int ATTN_MAX_R = 4096;
-// n / d for n < 2^31 as the high half of 2 n * mul, shifted.
-struct FastDiv {
-  uint32_t mul, shift;
-};
 struct AttnArgs {
   const uint16_t *q, *k, *v, *gate;  // q [T, Hq, D]; pages [NB, Hkv, block, D]; gate [T, Hq, Dg] (its last D) or null
   const uint8_t *k_scales, *v_scales;  // [NB, Hkv] where the pages hold E4M3 codes (k and v then point to bytes), else null

@@ -125,4 +125,113 @@ __device__ __forceinline__ void rope_turn_across(float (&x)[2][8], float *mine, 
   __builtin_amdgcn_wave_barrier();
 }
 
+// Part `block % parts` of the heads (of the first `sets` sets) of token `block / parts`.  lph: log2 of a head's lanes; a wave takes heads of one set
+// only.  LDS, 16-byte aligned: cs and sn 128 values each, norm ROPE_MAX_SETS rows, swap (ACROSS) 16 a thread.
+template <int PAIRS, bool IN_F32, bool OUT_F32>
+__device__ __forceinline__ void rope_heads(const RopeArgs &a, int sets, int lph, int parts, unsigned block, float *cs,
+                                           float *sn, float (*norm)[256], float *swap) {
+  constexpr int WAVES = ROPE_THREADS / 64;
+  constexpr int TURNS = IN_F32 || PAIRS == ACROSS ? 1 : 2;  // loads of so many heads in flight per lane
+  const int tid = threadIdx.x, wv = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int l = tid & ((1 << lph) - 1), g = (tid & 63) >> lph, hpw = 64 >> lph;
+  const int t = (int)(block / parts), part = (int)block - t * parts;
+  // the lane's two chunks of eight values: both sides of eight pairs, or neighbours
+  const bool turned = PAIRS != ACROSS && l < a.half / 8;
+  const int d0 = (PAIRS == HALVES && turned ? l : 2 * l) * 8, d1 = PAIRS == HALVES && turned ? d0 + a.half : d0 + 8;
+  const bool in0 = d0 < a.D, in1 = d1 < a.D;
+
+  // wave item i -> its set, its first head there
+  auto which = [&](int &i) __attribute__((always_inline)) -> int {
+    int set = 0, n;
+    while (set < sets && i >= (n = (a.set[set].heads + hpw - 1) >> (6 - lph))) i -= n, ++set;
+    i *= hpw;
+    return set;
+  };
+  Eight<IN_F32> raw[TURNS][2];
+  auto fetch = [&](int i0) __attribute__((always_inline)) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+      int h = i0 + u * parts * WAVES;
+      const int set = which(h);
+      if (set == sets) break;
+      const RopeHeads &s = a.set[set];
+      if (h + g >= s.heads) continue;
+      const int64_t at = ((int64_t)t * s.heads + h + g) * s.in_stride;
+      if (in0) raw[u][0] = load8<IN_F32>(s.in, at + d0);
+      if (in1) raw[u][1] = load8<IN_F32>(s.in, at + d1);
+    }
+  };
+  // everything that is read on its way before the first is waited for
+  int i0 = part * WAVES + wv;
+  const int pos = a.positions[t];
+  const int slot = a.slots ? a.slots[t] : -1;
+  const float freq = tid < a.half ? a.freqs[tid] : 0.f;
+  float nw[ROPE_MAX_SETS];
+#pragma unroll
+  for (int i = 0; i < ROPE_MAX_SETS; ++i) {
+    nw[i] = 0.f;
+    if (i < sets && a.set[i].norm && tid < a.D)
+      nw[i] = a.set[i].norm_f32 ? ((const float *)a.set[i].norm)[tid]
+                                : __uint_as_float((uint32_t)((const uint16_t *)a.set[i].norm)[tid] << 16);
+  }
+  fetch(i0);
+
+  if (tid < a.half) {
+    float s, c;
+    rope_angle(pos, freq, s, c);
+    cs[tid] = c * a.amplitude;
+    sn[tid] = s * a.amplitude * a.sign;
+  }
+#pragma unroll
+  for (int i = 0; i < ROPE_MAX_SETS; ++i) norm[i][tid] = nw[i];
+  __syncthreads();
+  float c[8], sv[8];  // of the lane's pairs
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c[j] = sv[j] = 0.f;
+  if (turned) {
+#pragma unroll
+    for (int j = 0; j < 8; j += 4)
+      *(float4 *)&c[j] = *(const float4 *)&cs[l * 8 + j], *(float4 *)&sv[j] = *(const float4 *)&sn[l * 8 + j];
+  }
+
+  const int page = slot / a.block;
+  const bool kept = slot >= 0 && page < a.NB;
+  while (true) {
+#pragma unroll
+    for (int u = 0; u < TURNS; ++u) {
+      int h = i0 + u * parts * WAVES;
+      const int set = which(h);
+      if (set == sets) return;
+      const RopeHeads &s = a.set[set];
+      const bool on = h + g < s.heads;
+      float x[2][8];
+#pragma unroll
+      for (int k = 0; k < 2; ++k) widen<IN_F32>(raw[u][k], x[k]);
+      if (s.norm) rope_norm(x, &norm[set][d0 & 255], &norm[set][d1 & 255], in0, in1, lph, a.D, a.eps);
+      if (PAIRS != ACROSS && s.rotate && turned) rope_turn<PAIRS>(x, c, sv);
+      if (PAIRS == ACROSS && s.rotate) rope_turn_across(x, swap + (tid >> lph << lph) * 16, l, a.half, a.interleaved, cs, sn);
+      if (!on || (s.cache && !kept)) continue;
+      const int64_t at = s.cache ? (((int64_t)page * s.heads + h + g) * a.block + (slot - page * a.block)) * a.D
+                                 : ((int64_t)t * s.heads + h + g) * a.D;
+      if (in0) store8<OUT_F32>(s.out, at + d0, x[0]);
+      if (in1) store8<OUT_F32>(s.out, at + d1, x[1]);
+    }
+    i0 += TURNS * parts * WAVES;
+    fetch(i0);
+  }
+}
+
+// Workgroups of a token: several where there are few tokens.  0: no heads.
+inline int64_t rope_parts(const RopeArgs &a, int sets, int lph) {
+  int64_t items = 0;  // of a wave
+  for (int i = 0; i < sets; ++i) items += (a.set[i].heads + (64 >> lph) - 1) >> (6 - lph);
+  const int64_t turns = (items + ROPE_THREADS / 64 - 1) / (ROPE_THREADS / 64);
+  int64_t parts = 1024 / a.T;
+  return parts < 1 && turns ? 1 : parts > turns ? turns : parts;
+}
+
+// Tokens of a launch at most: a grid's lanes are counted in 32 bits (past that the count wraps, with no error).
+constexpr int ROPE_TOKENS = 1 << 23;
+static_assert((int64_t)ROPE_TOKENS * ROPE_THREADS < (int64_t)1 << 32, "lanes of a grid");
+
 }  // namespace qmm
