@@ -10,7 +10,7 @@
 // page loses next to nothing, and when it grows only codes that become subnormal are rounded again.
 //
 // A workgroup takes one head of k or v and the runs that start in a window of as many tokens as its lanes hold rows
-// (16 values a lane), so a run is seen whole by one workgroup and no atomics leave it.  Rows past the window (of its last
+// (16 values a lane), or of fewer where there are few, so a run is seen whole by one workgroup and no atomics leave it.  Rows past the window (of its last
 // run) take further turns.
 #include "rope.h"
 
@@ -48,30 +48,32 @@ __device__ __forceinline__ uint32_t shrink4(uint32_t w, int by) {
 
 struct CacheWrite {
   uint8_t *scales[2];  // of k, of v
-  int windows;
-  FastDiv by_block, by_half;
-  // The grid: `writers` workgroups for k and v, one behind every `period` - 1 of those that turn q's heads, `parts` to a token.
-  int writers, period, parts;
+  int windows, span;  // tokens of a window
+  bool early;         // few workgroups: loads ahead of what says whether they are needed
+  // The grid: `writers` workgroups for k and v, `pairs` (a head of k or v each) times `columns` (a window each), one before every `period` - 1 of
+  // those that turn q's heads, `parts` to a token.
+  int writers, pairs, columns, period, parts;
+  FastDiv by_block, by_half, by_pairs, by_period;
 };
 
 __device__ __forceinline__ int fast_quot(int n, FastDiv d) { return (int)(__umulhi((uint32_t)n << 1, d.mul) >> d.shift); }
 
 template <int PAIRS, bool IN_F32>
-__global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
+__global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5) void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
   __shared__ __attribute__((aligned(16))) float cs[ROPE_THREADS * 8], sn[ROPE_THREADS * 8], norm[ROPE_MAX_SETS][256];
   __shared__ __attribute__((aligned(16))) float swap[PAIRS == ACROSS ? ROPE_THREADS * 16 : 4];
   __shared__ float freq[128];
   __shared__ int pos[CW_RUNS];
   __shared__ uint32_t top[CW_RUNS];
   __shared__ int begun[CW_RUNS], exponent[CW_RUNS], grown[CW_RUNS], grown_page[CW_RUNS], n_grown;
-  const int writer = (int)blockIdx.x / w.period;
+  const int writer = fast_quot(blockIdx.x, w.by_period);
   if (writer >= w.writers || (int)blockIdx.x != writer * w.period) {
     const int before = writer < w.writers ? writer + 1 : w.writers;
     rope_heads<PAIRS, IN_F32, false>(a, 1, lph, w.parts, blockIdx.x - before, cs, sn, norm, swap);
     return;
   }
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rows = ROPE_THREADS >> lph;  // of a turn, and a window's
+  const int rows = ROPE_THREADS >> lph;  // of a turn
   const int l = tid & ((1 << lph) - 1), g = tid >> lph;
   const bool turned = PAIRS != ACROSS && l < a.half / 8;
   const int d0 = (PAIRS == HALVES && turned ? l : 2 * l) * 8, d1 = PAIRS == HALVES && turned ? d0 + a.half : d0 + 8;
@@ -82,25 +84,30 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
     const int page = fast_quot(slot, w.by_block);
     return slot >= 0 && page < a.NB ? page : -1;
   };
+  const int window0 = fast_quot(writer, w.by_pairs), pair0 = writer - window0 * w.pairs;
 #pragma unroll 1
-  for (int64_t item = writer; item < (int64_t)w.windows * 2 * heads; item += w.writers) {
-    const int side = (int)(item % (2 * heads)) / heads, head = (int)(item % heads), w0 = (int)(item / (2 * heads)) * rows;
+  for (int window = window0, pair = pair0; window < w.windows; pair += w.pairs) {
+    if (pair >= 2 * heads) {
+      pair = pair0 - w.pairs, window += w.columns;
+      continue;
+    }
+    const int side = pair >= heads, head = side ? pair - heads : pair, w0 = window * w.span;
     const RopeHeads &s = a.set[1 + side];
     // What the first steps need, on its way at once: slots from the window's first row on (64 at least), weights and
-    // frequencies; where the call is one window, also the rows and what their pages hold.
-    const int w1 = a.T - w0 < rows ? a.T : w0 + rows;
+    // frequencies, and the rows and positions of a turn from there on (of use where the first run starts there and it is the
+    // only turn).
+    const int w1 = a.T - w0 < w.span ? a.T : w0 + w.span;
     const int t = w0 + lane;
     const int slot_t = t < a.T ? a.slots[t] : -1, slot_b = w0 > 0 ? a.slots[w0 - 1] : -1;
     const float freq_l = s.rotate && tid < a.half ? a.freqs[tid] : 0.f;
-    const bool one = a.T <= rows;
-    const int pos_l = one && s.rotate && tid < a.T ? a.positions[tid] : 0;
+    const int pos_l = w.early && s.rotate && tid < rows && w0 + tid < a.T ? a.positions[w0 + tid] : 0;
     auto load = [&](int row, Eight<IN_F32> (&raw)[2]) __attribute__((always_inline)) {
       const int64_t at = ((int64_t)row * heads + head) * s.in_stride;
       if (in0) raw[0] = load8<IN_F32>(s.in, at + d0);
       if (in1) raw[1] = load8<IN_F32>(s.in, at + d1);
     };
     Eight<IN_F32> early[2] = {};
-    if (one && g < a.T) load(g, early);
+    if (w.early && w0 + g < a.T) load(w0 + g, early);
     float norm_l = 0.f;
     if (s.norm && tid < a.D)
       norm_l = s.norm_f32 ? ((const float *)s.norm)[tid] : __uint_as_float((uint32_t)((const uint16_t *)s.norm)[tid] << 16);
@@ -115,7 +122,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
     int end = w1;
     if (last_page >= 0 && end < a.T) {  // its last run's end
       uint64_t other = __ballot(t >= a.T || mine != last_page);
-      other &= rows < 64 ? ~0ull << rows : 0;
+      other &= w.span < 64 ? ~0ull << w.span : 0;
       end = w0 + 64;
       while (!other) {
         other = __ballot(end + lane >= a.T || page_of(a.slots[end + lane]) != last_page);
@@ -137,16 +144,17 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
     };
     // The turns, last to first, for the maxima: then the first one's values are still there, and only the others' are formed
     // again for their codes (16 rows of 256, 32 of 128 or 64 of 64 values are one turn).
-    const int turns = (end - first + rows - 1) / rows;
+    const int turns = (end - first + rows - 1) >> (8 - lph);
+    const bool there = w.early && lead == 0 && turns == 1;
 #pragma unroll 1
     for (int step = 0; step < 2 * turns - 1; ++step) {
       const int row0 = first + (step < turns ? turns - 1 - step : step - turns + 1) * rows, row = row0 + g;
       if (step) __syncthreads();  // (the angles of the turn before are read)
       Eight<IN_F32> raw[2] = {early[0], early[1]};
-      if (!(one && lead == 0)) load(row < end ? row : first, raw);
+      if (!there) load(row < end ? row : first, raw);
       const int slot = row < end ? a.slots[row] : -1;
       if (s.rotate) {
-        if (tid < rows) pos[tid] = one && lead == 0 ? pos_l : row0 + tid < end ? a.positions[row0 + tid] : 0;
+        if (tid < rows) pos[tid] = there ? pos_l : row0 + tid < end ? a.positions[row0 + tid] : 0;
         __syncthreads();
         const int half = a.half, n = (end - row0 < rows ? end - row0 : rows) * half;
         for (int i = tid; i < n; i += ROPE_THREADS) {
@@ -180,7 +188,7 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
           if (in0 && finite(x[0][j])) m = fmaxf(m, fabsf(x[0][j]));
           if (in1 && finite(x[1][j])) m = fmaxf(m, fabsf(x[1][j]));
         }
-        for (int off = 1 << lph >> 1; off >= 1; off >>= 1) m = fmaxf(m, __shfl_xor(m, off, 64));
+        m = over_head(m, lph, [](float a, float b) { return fmaxf(a, b); });
         if (l == 0 && page >= 0) {
           const int run = run_of(row);
           atomicMax(&top[run], __float_as_uint(m));
@@ -209,12 +217,12 @@ __global__ __launch_bounds__(ROPE_THREADS) void cache_write_kernel(const RopeArg
         }
         __syncthreads();
         if (n_grown) {
-          const int64_t per = (int64_t)a.block * a.D / 16;  // of a page, 16 codes each
+          const int64_t words = (int64_t)a.block * a.D / 16;  // of a page, 16 codes each
           int64_t i = tid;
           int r = 0;
 #pragma unroll 1
           while (true) {
-            while (r < n_grown && i >= per) i -= per, ++r;
+            while (r < n_grown && i >= words) i -= words, ++r;
             if (r >= n_grown) break;
             uint4 *codes = (uint4 *)((uint8_t *)s.out + ((int64_t)grown_page[r] * heads + head) * a.block * a.D) + i;
             const int by = grown[r];
@@ -292,14 +300,23 @@ void launch_pairs(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph
 
 hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_SETS], hipStream_t st) {
   if (a.T <= 0 || a.D < 16 || a.D > 256 || a.D % 16 || a.half < 0 || 2 * a.half > a.D || a.sets != 3 || a.block < 1 ||
-      a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads != a.set[2].heads)
+      a.T > 1 << 30 || a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads > 1 << 29 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
   const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4, rows = ROPE_THREADS >> lph;
-  CacheWrite w{{scales[1], scales[2]}, (int)(((int64_t)a.T + rows - 1) / rows), fast_div(a.block), fast_div(a.half ? a.half : 1),
-               0, 1, 0};
-  const int64_t items = (int64_t)w.windows * 2 * a.set[1].heads;
-  w.writers = (int)(items < 1 << 20 ? items : 1 << 20);
+  CacheWrite w{};
+  w.scales[0] = scales[1], w.scales[1] = scales[2];
+  w.pairs = a.set[1].heads < 1 << 15 ? 2 * a.set[1].heads : 1 << 16;
+  // few tokens: windows of fewer, down to one each, until there is a workgroup a CU (64 sequences' steps of 128 tokens in all,
+  // 4 heads of 96: 10.2 us with windows of 32, 6.2 us with those of 4, where fewer angles are formed one after the other)
+  w.span = rows;
+  while (w.span > 1 && ((int64_t)a.T + w.span - 1) / w.span * w.pairs < 256) w.span /= 2;
+  w.windows = (int)(((int64_t)a.T + w.span - 1) / w.span);
+  w.early = (int64_t)w.windows * w.pairs <= 512;
+  w.columns = w.windows < (1 << 20) / w.pairs ? w.windows : (1 << 20) / w.pairs;
+  w.writers = w.pairs * w.columns;
+  w.by_block = fast_div(a.block), w.by_half = fast_div(a.half ? a.half : 1), w.by_pairs = fast_div(w.pairs);
   int64_t grid = w.writers;
+  w.period = 1;
   if (a.T > ROPE_TOKENS) {  // (a grid's lanes are counted in 32 bits: q in launches of its own)
     RopeArgs q = a;
     q.sets = 1;
@@ -311,6 +328,7 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
     grid += turners;
     w.period = 1 + (int)(turners / w.writers);
   }
+  w.by_period = fast_div(w.period);
   a.half % 8      ? launch_pairs<ACROSS>(a, w, (unsigned)grid, lph, st)
   : a.interleaved ? launch_pairs<NEXT>(a, w, (unsigned)grid, lph, st)
                   : launch_pairs<HALVES>(a, w, (unsigned)grid, lph, st);

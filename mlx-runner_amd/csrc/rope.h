@@ -69,6 +69,25 @@ __device__ __forceinline__ void rope_angle(int pos, float freq, float &s, float 
   sincospif(2.f * (float)turns, &s, &c);
 }
 
+// The value of lane ^ OFF, within the vector unit; lane ^ 8 only where a row of 16 lanes is one head's.
+template <int OFF>
+__device__ __forceinline__ float lane_xor(float v) {
+  const int x = __float_as_int(v);
+  if constexpr (OFF == 1) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0xB1, 0xF, 0xF, true));   // quad_perm 1,0,3,2
+  if constexpr (OFF == 2) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x4E, 0xF, 0xF, true));   // quad_perm 2,3,0,1
+  if constexpr (OFF == 8) return __int_as_float(__builtin_amdgcn_mov_dpp(x, 0x128, 0xF, 0xF, true));  // row_ror:8
+  const int up = __builtin_amdgcn_update_dpp(x, x, 0x104, 0xF, 0x5, true);  // row_shl:4 into quads 0, 2
+  return __int_as_float(__builtin_amdgcn_update_dpp(up, x, 0x114, 0xF, 0xA, true));  // row_shr:4 into quads 1, 3
+}
+// f over a head's lanes (4, 8 or 16), halves first.
+template <class F>
+__device__ __forceinline__ float over_head(float v, int lph, F f) {
+  if (lph > 3) v = f(v, lane_xor<8>(v));
+  if (lph > 2) v = f(v, lane_xor<4>(v));
+  v = f(v, lane_xor<2>(v));
+  return f(v, lane_xor<1>(v));
+}
+
 // x * rsqrt(mean(x^2) + eps) * w over the head's D values; in0, in1: whether the lane's chunks are of them.
 __device__ __forceinline__ void rope_norm(float (&x)[2][8], const float *w0, const float *w1, bool in0, bool in1, int lph,
                                           int D, float eps) {
@@ -78,7 +97,7 @@ __device__ __forceinline__ void rope_norm(float (&x)[2][8], const float *w0, con
 #pragma unroll
     for (int j = 0; j < 8; ++j) sq[k] = __builtin_fmaf(x[k][j], x[k][j], sq[k]);
   float sum = (in0 ? sq[0] : 0.f) + (in1 ? sq[1] : 0.f);
-  for (int off = 1 << lph >> 1; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 64);
+  sum = over_head(sum, lph, [](float a, float b) { return a + b; });
   const float r = 1.f / sqrtf(sum / (float)D + eps);
 #pragma unroll
   for (int k = 0; k < 2; ++k)
@@ -108,6 +127,7 @@ __device__ __forceinline__ void rope_turn_across(float (&x)[2][8], float *mine, 
   for (int k = 0; k < 2; ++k)
 #pragma unroll
     for (int j = 0; j < 8; j += 4) *(float4 *)&mine[(2 * l + k) * 8 + j] = *(float4 *)&x[k][j];
+  asm volatile("" : "+s"(half));  // (else the sixteen conditions below are held as masks through the caller's loop)
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 #pragma unroll
