@@ -300,7 +300,10 @@ void join(const AttnArgs &a, const Part &p, const AttnShare &s, hipStream_t st) 
   const unsigned n = (unsigned)(p.by_tile ? p.tiles * a.Hkv : p.grid);
   if (p.tr > 32)
     hipLaunchKernelGGL((attn_join_rows_kernel<DP>), dim3(n, p.rows / AJ_ROWS), dim3(ATTN_THREADS), 0, st, a, s, p.tr);
-  else if (DP > 64 && n * (unsigned)p.rows <= 1024)
+  // A row's columns over several workgroups where that leaves few.  (Over E4M3 pages a tile is cut in more parts for its time,
+  // and of 256 columns only four are side by side: 8 requests of 18 rows, up to 32768 keys, 9.0 us on one workgroup a row,
+  // 6.9 on four; 64 of 4 rows of 128 columns 4.2 on one, 5.6 on two.)
+  else if (DP > 64 && n * (unsigned)p.rows <= (a.k_scales && DP == 256 ? 2048u : 1024u))
     join_few<DP, 64>(a, p, s, n, st);
   else
     join_few<DP, DP>(a, p, s, n, st);
