@@ -6,13 +6,18 @@ a batch of requests instead of one):
     paged_attention          every request's new tokens over its pages, times the gate's sigmoid
     quantized_matmul         the output projection
 
+With cache="e4m3" the pages hold 8 bits a value and the two calls between are `rope_cache_fp8` and `paged_attention_fp8`;
+`cache_read_fp8` gives rows of them back.
+
 A step's tables come from `block_tables`, once for all layers of a model.  `python attention_layer.py` prefills
 requests of different lengths and decodes a few tokens of each, the decode step as a captured graph: lengths and page
-ids live on the GPU and nothing is planned on the host, so every replay follows them.
+ids live on the GPU and nothing is planned on the host, so every replay follows them.  `python attention_layer.py e4m3`
+does the same over a cache held in 8 bits.
 """
 from __future__ import annotations
 
 import math
+import sys
 
 import torch
 
@@ -47,7 +52,9 @@ class AttentionLayer:
     """Hq query heads (each with a gate) over Hkv key heads of D values; `rot` of them turn with the position."""
 
     def __init__(self, K: int, Hq: int, Hkv: int, D: int, rot: int, pages: int, block: int, *, mode: str = "nvfp4",
-                 base: float = 1e7, seed: int = 0):
+                 base: float = 1e7, seed: int = 0, cache: str = "bfloat16"):
+        if cache not in ("bfloat16", "e4m3"):
+            raise ValueError(f"cache must be 'bfloat16' or 'e4m3', not {cache!r}")
         g = torch.Generator(device="cuda").manual_seed(seed)
 
         def normal(*shape):
@@ -67,8 +74,13 @@ class AttentionLayer:
         self.norms = Q.Array.from_torch(self.q_norm), Q.Array.from_torch(self.k_norm)
         freqs, self.amplitude = Q.rope_frequencies(rot, base)
         self.freqs = torch.from_numpy(freqs).cuda()
-        self.k_cache, self.v_cache = (torch.zeros(pages, Hkv, block, D, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        self.eight = cache == "e4m3"
+        dtype = torch.uint8 if self.eight else torch.bfloat16
+        self.k_cache, self.v_cache = (torch.zeros(pages, Hkv, block, D, dtype=dtype, device="cuda") for _ in range(2))
         self.caches = Q.Array.from_torch(self.k_cache), Q.Array.from_torch(self.v_cache)
+        if self.eight:  # a scale for each page and head
+            self.k_scales, self.v_scales = (torch.zeros(pages, Hkv, dtype=torch.uint8, device="cuda") for _ in range(2))
+            self.caches += Q.Array.from_torch(self.k_scales), Q.Array.from_torch(self.v_scales)
 
     def _quantize(self, w):
         wq, s = Q.quantize(Q.Array.from_torch(w), self.mode, stream=Q.Stream.torch_current())
@@ -86,19 +98,27 @@ class AttentionLayer:
         turned, o, y = empty(T, self.Hq, D), empty(T, self.Hq, D), empty(T, x.shape[1])
         A = Q.Array.from_torch
         Q.quantized_matmul_group(A(x), self.ws, self.ss, self.mode, outs=[A(t.view(T, -1)) for t in (q, k, v)], stream=stream)
-        Q.rope_cache(A(q), A(k), A(v), *self.caches, step["positions"], step["slots"], A(self.freqs),
-                     amplitude=self.amplitude, q_norm=self.norms[0], k_norm=self.norms[1], q_out=A(turned), stream=stream)
-        Q.paged_attention(A(turned), *self.caches, step["table"], step["starts"], step["lens"], gate=A(q),
-                          scale=D ** -0.5, out=A(o), stream=stream)
+        write, attend = (Q.rope_cache_fp8, Q.paged_attention_fp8) if self.eight else (Q.rope_cache, Q.paged_attention)
+        write(A(q), A(k), A(v), *self.caches, step["positions"], step["slots"], A(self.freqs),
+              amplitude=self.amplitude, q_norm=self.norms[0], k_norm=self.norms[1], q_out=A(turned), stream=stream)
+        attend(A(turned), *self.caches, step["table"], step["starts"], step["lens"], gate=A(q), scale=D ** -0.5,
+               out=A(o), stream=stream)
         Q.quantized_matmul(A(o.view(T, -1)), *self.o_proj, self.mode, out=A(y), stream=stream)
         return y
 
+    def read(self, slots: torch.Tensor, stream, dtype: torch.dtype = torch.float32):
+        """The keys and values in the rows `slots` (int32) of a cache held in 8 bits: two [T, Hkv, D], exact in float32."""
+        k, v = (torch.empty(slots.numel(), self.Hkv, self.D, dtype=dtype, device="cuda") for _ in range(2))
+        A = Q.Array.from_torch
+        Q.cache_read_fp8(*self.caches, A(slots, Q.INT32), dtype=A(k).dtype, k_out=A(k), v_out=A(v), stream=stream)
+        return k, v
 
-def main(prompts=(700, 96, 1, 2048), tokens: int = 16, K: int = 5120):
+
+def main(prompts=(700, 96, 1, 2048), tokens: int = 16, K: int = 5120, cache: str = "bfloat16"):
     R, block = len(prompts), 16
     width = -(-(max(prompts) + tokens) // block)
     pages = Pages(R, R * width, block, width)
-    layer = AttentionLayer(K, 24, 4, 256, 64, R * width, block)
+    layer = AttentionLayer(K, 24, 4, 256, 64, R * width, block, cache=cache)
     stream = torch.cuda.Stream()
     with torch.cuda.stream(stream):
         s = Q.Stream.torch_current()
@@ -123,4 +143,4 @@ def main(prompts=(700, 96, 1, 2048), tokens: int = 16, K: int = 5120):
 
 
 if __name__ == "__main__":
-    main()
+    main(cache=sys.argv[1] if len(sys.argv) > 1 else "bfloat16")
