@@ -281,9 +281,16 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadArgs a, 
 #pragma unroll
     for (int k = 0; k < E; ++k) v[k] = e[u] < 0 ? 0.f : v[k];
     if constexpr (F32) {
-      *(float4 *)((float *)a.out[set] + at) = make_float4(v[0], v[1], v[2], v[3]);
+      __builtin_nontemporal_store(f32x4_t{v[0], v[1], v[2], v[3]}, (f32x4_t *)((float *)a.out[set] + at));
     } else {
-      store8<false>(a.out[set], at, v);
+      u32x4_t y;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        bf16x2_t x;
+        x[0] = (__bf16)v[2 * k], x[1] = (__bf16)v[2 * k + 1];
+        y[k] = __builtin_bit_cast(uint32_t, x);
+      }
+      __builtin_nontemporal_store(y, (u32x4_t *)((uint16_t *)a.out[set] + at));
     }
   }
 }
