@@ -437,6 +437,11 @@ __device__ __forceinline__ int attn_swz(int row) {
   return DP >= 128 ? row & 15 : (row >> 1) & 7;
 }
 
+// The same for values that transposing reads take: 4 rows of 64 bytes (a transposing read of 32 lanes) in distinct banks.
+template <int DP>
+__device__ __forceinline__ int attn_swz_v(int row) {
+  return DP >= 128 ? (row & 3) << 2 : (row & 2) << 1;
+}
 
 // The same for E4M3 codes: rows of DP bytes.
 template <int DP>

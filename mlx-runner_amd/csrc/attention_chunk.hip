@@ -33,12 +33,6 @@ constexpr int CH_TAB = 4 * 2 * 256 + 2 * 4 * 4;  // page ids of the tiles to com
 
 constexpr int ch_tile(int DP) { return CH_KT * DP * 2; }  // bytes of a tile of keys (or of values)
 
-// Chunk c of row r of the values: 4 rows of 64 bytes (a transposing read of 32 lanes) in distinct banks.
-template <int DP>
-__device__ __forceinline__ int ch_swz_v(int row) {
-  return DP >= 128 ? (row & 3) << 2 : (row & 2) << 1;
-}
-
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
 __device__ __forceinline__ void ch_dma4(const void *g, uint32_t l) {
@@ -226,7 +220,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
           ch_dma16((const char *)cache + c + (uint64_t)row * pitch, la + to + wv * 16 * PITCH, n * 1024);
       };
       const auto swz_k = [](int r) { return attn_swz<DP>(r); };
-      const auto swz_v = [](int r) { return ch_swz_v<DP>(r); };
+      const auto swz_v = [](int r) { return attn_swz_v<DP>(r); };
       auto move_k = [&](From &f, int set, int n) __attribute__((always_inline)) { move(kc, f, n, set * TILE, swz_k); };
       auto move_v = [&](From &f, int set, int n) __attribute__((always_inline)) { move(vc, f, n, (2 + set) * TILE, swz_v); };
 
@@ -336,7 +330,7 @@ __global__ __launch_bounds__(ATTN_THREADS, DP == 64 ? 2 : 1) void attn_chunk_ker
         const uint32_t ln = attn_lane();
         const int row = 4 * (ln >> 5) + (ln >> 2 & 3);
         const int from = la + (2 + set) * TILE + (half * 32 + row) * PITCH +
-                         ((int)((ln >> 4 & 1) * 2 + (ln >> 1 & 1)) ^ ch_swz_v<DP>(row)) * 16 + (ln & 1) * 8;
+                         ((int)((ln >> 4 & 1) * 2 + (ln >> 1 & 1)) ^ attn_swz_v<DP>(row)) * 16 + (ln & 1) * 8;
         constexpr int N = 2 * DT, AHEAD = 2;
         auto load = [&](int n) __attribute__((always_inline)) {
           const int d = n % DT, c = n / DT;  // (the first 16 keys' weights are done with half way)

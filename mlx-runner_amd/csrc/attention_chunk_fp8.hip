@@ -1,16 +1,26 @@
-// Paged attention of many rows per key head over a cache of E4M3 codes: all products on the scaled 32x32x64 MFMA, which
-// takes the codes as they are and a key's scale with them.
+// Paged attention of many rows per key head over a cache of E4M3 codes.
 //
-// bf16 queries go in as two E4M3 parts (attn_split: exact but for 2^-22 of a row's largest), so S^T = K Q^T costs what it
-// costs in bf16, two products at twice the rate.  The weights of O^T = V^T P^T go in as two parts as well (2^-8 of a weight
-// lost, as with bf16), scaled for each row and 32 keys by a power of two of those keys' own maximum, which the matrix unit
-// takes off again: what E4M3's 18 binades cannot hold is 2^-22 of the largest weight of 32 keys.  A page's scale of values is
-// the other operand's where the tile's keys share it; else it goes into the weights, relative to the tile's largest.
+// S^T = K Q^T on the scaled 32x32x64 MFMA, which takes the codes as they are and a key's scale with them: bf16 queries go in
+// as two E4M3 parts (attn_split: exact but for 2^-22 of a row's largest), two products at twice the rate, so it costs what it
+// costs in bf16.
 //
-// A tile is 256 rows, 32 for each of eight waves, two a SIMD: one's softmax beside the other's products, with nothing
-// interleaved by hand.  (Codes are half of bf16's bytes: eight waves' operands from LDS take the bandwidth that four waves' of
-// 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, eight keys by each wave; one
-// barrier a tile.
+// O^T = V^T P^T, where a head has at most 128 values (WIDE): codes are exact in bf16, so every wave widens the rows that it
+// has moved, into LDS, and the weights, rounded to bf16 once, take the values' scales as exponents of two.  With 256 values
+// LDS has no room for that (second parts of the queries 64 KB, tiles 64 KB): the codes go in as they are, and the weights in
+// two E4M3 parts (2^-8 of a weight lost), scaled for each row and 32 keys by a power of two of those keys' own maximum, which
+// the matrix unit takes off again; what E4M3's 18 binades cannot hold is 2^-22 of the largest weight of 32 keys.  A page's
+// scale of values is the other operand's where the tile's keys share it; else it goes into the weights, relative to the
+// tile's largest.  The products cost the same; two parts cost 2.5 instructions a weight, one rounding half of one: 4000
+// tokens of 32 heads on 8 of 128 228 us with two parts, 201 with bf16; chunks of 7 prompts, 16 heads of 64, window 1000, 124
+// and 107.
+//
+// A tile is 256 rows, 32 for each of eight waves, two a SIMD (D 64: four): one's softmax beside the other's products, with
+// nothing interleaved by hand.  (Codes are half of bf16's bytes: eight waves' operands from LDS take the bandwidth that four
+// waves' of 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, eight keys by each wave;
+// one barrier a tile.
+//
+// Bound by the two units in turn: 2048 tokens over 32768 keys, 24 heads on 4 of 256, 1.49-1.56 ms, 1.05 PFLOP/s (bf16 pages
+// 1.43-1.48), the matrix unit busy for 45% of it, the vector unit for most of the rest.
 #include <type_traits>
 
 #include "attention.h"
@@ -27,13 +37,18 @@ constexpr int C8_SCALES = 2 * 2 * 256;                  // scale bytes of the ke
 constexpr int C8_TAB = C8_WAVES * 2 * 32;               // page ids of the tiles to come
 constexpr int C8_VALID = 2 * C8_WAVES;                  // bits of the keys that there are, two sets
 constexpr int C8_SMALL = C8_SCALES + C8_TAB + C8_VALID + 8 * C8_THREADS;
+constexpr int C8_RANGE = 40;  // weights up to 2^60 times scales up to 2^40 times codes stay far below f32's end
 constexpr int C8_NEAR = 8;  // scales of 32 keys' values that differ by up to 2^8 go in relative to the largest
 
+// Whether the values and their weights go in as bf16
+constexpr bool c8_wide(int DP) { return DP < 256; }
 constexpr int c8_tile(int DP) { return C8_KT * DP; }
-constexpr int c8_queries(int DP) { return DP == 256 ? C8_TR * DP : 0; }  // the queries' second parts
+constexpr int c8_tiles(int DP) { return (c8_wide(DP) ? 8 : 4) * c8_tile(DP); }
+// The queries' second parts, where registers do not hold them
+constexpr int c8_queries(int DP) { return DP == 128 ? 0 : C8_TR * DP; }
 constexpr int c8_fixed(int DP) {
-  const int out = C8_WAVES * 32 * 64 * 4, tiles = 4 * c8_tile(DP);  // (rows out: 64 columns of a wave's rows at a time)
-  return (tiles > out ? tiles : out) + c8_queries(DP);
+  const int out = C8_WAVES * 32 * 64 * 4, in = c8_tiles(DP) + c8_queries(DP);  // (rows out: 64 columns of a wave's rows at a time)
+  return in > out ? in : out;
 }
 
 #pragma clang diagnostic push
@@ -70,9 +85,9 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
   constexpr int RPI = 64 / CPR;    // rows of a DMA operation
   constexpr int OPS = 8 > RPI ? 8 / RPI : 1;  // operations of a wave's 8 rows
   constexpr int TILE = c8_tile(DP), PITCH = DP;
-  constexpr bool LO_LDS = DP == 256;
+  constexpr bool LO_LDS = c8_queries(DP) > 0, WIDE = c8_wide(DP);
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  uint8_t *qlo = lds + c8_fixed(DP) - c8_queries(DP);
+  uint8_t *qlo = lds + c8_tiles(DP);
   uint8_t *scl = lds + c8_fixed(DP);                 // [2][keys, values][64]
   uint8_t *tab = scl + C8_SCALES;                    // [wave][2][8]
   uint8_t *vm = tab + C8_TAB;                        // [2][8 waves], a byte each
@@ -228,6 +243,7 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
       f32x16_t sv[2];
       int kx[2] = {0, 0}, sb = 0, tvv = 0;  // the products' scales
       i32x8_t ph{}, pl{};
+      bf16x8_t pb[4]{};  // (WIDE: the weights of 16 keys each)
       // S^T of tile j: 2 x 32 keys
       auto scores = [&](int j) __attribute__((always_inline)) {
         const int set = j & 1;
@@ -277,13 +293,26 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
       // What the scales of tile j's values do to its weights: of eight keys each (they have one, where pages are multiples of
       // eight), how far it is below the largest of their half, 4 bits each; `far`: the halves where that does not do.
       // (Pages whose scale is NaN add that to the rows that see them at the end.)
+      // WIDE: 2^up of each eight keys' scale and 2^-up, `far` where eight differ or pass 2^(+-C8_RANGE).
       int tv[2], less = 0, far = 0;
+      float up[8], down[8];
       auto prepare = [&](int j) __attribute__((always_inline)) {
         const uint32_t ln = attn_lane();
         const int vs = *((const int *)(scl + (j & 1) * 512 + 256) + ln);
         const uint64_t valid = valid_of(j);
         const uint64_t nan = __ballot(vs == 255) & valid, fine = valid & ~nan;
         if (nan) *poison = 1;
+        if constexpr (WIDE) {
+          const uint64_t other = __ballot(vs != __builtin_amdgcn_update_dpp(vs, vs, 0x111, 0xF, 0xF, false)) & 0xFEFEFEFEFEFEFEFEull;
+          far = (other | (__ballot(vs - (127 - C8_RANGE) > 2u * C8_RANGE) & valid)) != 0;
+          const int x = __float_as_int((float)(vs - 127)), y = (254 - vs) << 23;
+#pragma unroll
+          for (int v = 0; v < 8; ++v) {
+            up[v] = __int_as_float(__builtin_amdgcn_readlane(x, v * 8));
+            down[v] = __int_as_float(__builtin_amdgcn_readlane(y, v * 8));
+          }
+          return;
+        }
         // (a lane beside the one before it, but for the first of eight; one that is not there has its page's, or the first page's)
         const uint64_t other = __ballot(vs != __builtin_amdgcn_update_dpp(vs, vs, 0x111, 0xF, 0xF, false)) & 0xFEFEFEFEFEFEFEFEull;
         far = ((uint32_t)other != 0) | ((uint32_t)(other >> 32) != 0) << 1;
@@ -340,6 +369,56 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
           }
         }
 
+        const int *vsl = (const int *)(scl + (j & 1) * 512 + 256);
+        if constexpr (WIDE) {
+          float top = -__builtin_inff();
+#pragma unroll
+          for (int j = 0; j < 32; j += 2) top = c8_max3(top, sv[j >> 4][j & 15], sv[j >> 4][(j & 15) + 1]);
+          asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(top));  // (as below)
+          // The reference is the row's first maximum; it follows, and the sums with it, when a score passes it by 2^60.
+          if (__any(m == -__builtin_inff() || top * sc > m + 60.f)) {
+            const float all = __builtin_ceilf(c8_pair_max(top) * sc);
+            m = m == -__builtin_inff() ? all : m;
+            const bool rise = all > m + 60.f;
+            const float f = rise ? attn_exp2(m - all) : 1.f;
+            m = rise ? all : m;
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < DT; ++d) acc[d] *= f;
+          }
+          const float ref = m == -__builtin_inff() ? 0.f : m;
+          auto pack = [&](int v, const float (&x)[4]) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) pb[v >> 1][(v & 1) * 4 + j] = (__bf16)x[j];
+          };
+          // the weights with their values' scales, f32's exponents over
+          if (far) {
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              const i32x4_t vs = *(const i32x4_t *)(vsl + v * 8 + ((int)attn_lane() >> 5) * 4);
+              float x[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j] = attn_exp2(__builtin_fmaf(sv[v >> 2][(v & 3) * 4 + j], sc, -ref));
+              l += (x[0] + x[1]) + (x[2] + x[3]);
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j] = __builtin_amdgcn_ldexpf(x[j], vs[j] - 127);
+              pack(v, x);
+              __builtin_amdgcn_sched_barrier(0);  // (few registers at a time)
+            }
+          } else {
+#pragma unroll
+            for (int v = 0; v < 8; ++v) {
+              const float from = up[v] - ref;
+              float x[4];
+#pragma unroll
+              for (int j = 0; j < 4; ++j) x[j] = attn_exp2(__builtin_fmaf(sv[v >> 2][(v & 3) * 4 + j], sc, from));
+              l = __builtin_fmaf((x[0] + x[1]) + (x[2] + x[3]), down[v], l);
+              pack(v, x);
+            }
+          }
+          return;
+        }
+
         // Maxima of the scores, in powers of two, rounded up
         float top[2];
 #pragma unroll
@@ -367,7 +446,6 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         }
         const float ref = m == -__builtin_inff() ? 0.f : m;
         int by[2];
-        const int *vsl = (const int *)(scl + (j & 1) * 512 + 256);
         // x = 2^(scale s - d - e), d how far eight keys' scale is below the largest.  FAR: relative to the largest of what the
         // weights with their scales come to, which e does not follow otherwise.
         auto weights = [&](auto half_c, auto far_c) __attribute__((always_inline)) {
@@ -457,6 +535,60 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         }
         if (__any(odd)) *poison = 1;
       };
+      // WIDE: the rows of the values that this wave has moved, as bf16, scales aside (codes are exact there); cleaned as above
+      auto widen = [&](int j) __attribute__((always_inline)) {
+        const bool strict = differ(j) || there != 0xFFu;
+        bool odd = false;
+        const uint32_t ln = attn_lane();
+#pragma unroll
+        for (int n = 0; n < OPS; ++n) {
+          if (RPI <= 8 || ln < 8 * CPR) {
+            uint4 x = *(const uint4 *)(lds + (2 + (j & 1)) * TILE + wv * 8 * PITCH + n * 1024 + ln * 16);
+            const int own = n * RPI + ln / CPR, row = wv * 8 + own;  // (of the wave's 8, of the tile's)
+            if (strict) {
+              const uint4 y = attn_finite_codes(x);
+              const bool in = there >> own & 1;
+              odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
+              x = in ? y : attn_zeros();
+            }
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            u32x4_t o[2];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+              const bf16x2_t y = k & 1 ? fp8x2_to_bf16x2<true>(w[k >> 1]) : fp8x2_to_bf16x2<false>(w[k >> 1]);
+              o[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, y);
+            }
+            const int c = 2 * ((int)(ln % CPR) ^ attn_swz8<DP>(row)) ^ attn_swz_v<DP>(row);  // (its two chunks stay side by side)
+            u32x4_t *to = (u32x4_t *)(lds + (4 + 2 * (j & 1)) * TILE + row * 2 * PITCH + c * 16);
+            to[0] = o[0], to[1] = o[1];
+          }
+        }
+        if (strict && __any(odd)) *poison = 1;
+      };
+      auto product_wide = [&](int j) __attribute__((always_inline)) {
+        const uint32_t ln = attn_lane();
+        const int row = 4 * (ln >> 5) + (ln >> 2 & 3);
+        const uint32_t from = la + (4 + 2 * (j & 1)) * TILE + row * 2 * PITCH +
+                              ((int)((ln >> 4 & 1) * 2 + (ln >> 1 & 1)) ^ attn_swz_v<DP>(row)) * 16 + (ln & 1) * 8;
+        constexpr int N = 4 * DT, AHEAD = 3;
+        auto load = [&](int n) __attribute__((always_inline)) {
+          const int d = n % DT, c = n / DT;
+          const uint32_t at = (from ^ d * 64) + c * 16 * 2 * PITCH;
+          const i16x4_t v0 = attn_read_tr(at), v1 = attn_read_tr(at + 8 * 2 * PITCH);
+          return __builtin_bit_cast(bf16x8_t, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        };
+        bf16x8_t vf[N];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) vf[n] = load(n);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n + AHEAD < N) vf[n + AHEAD] = load(n + AHEAD);
+          acc[n % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(vf[n], pb[n / DT], acc[n % DT], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
+        }
+#pragma unroll
+        for (int d = 0; d < DT; ++d) asm volatile("" : "+v"(acc[d]));  // (as below)
+      };
       // O^T += V^T P^T
       auto product = [&](int j) __attribute__((always_inline)) {
         const int set = j & 1;
@@ -495,7 +627,10 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
 #pragma unroll 1
       for (int i = 0; i < nt; ++i) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        clean(i);
+        if constexpr (WIDE)
+          widen(i);
+        else
+          clean(i);
         gp_lds_barrier();  // tile i, its valid bits, page ids of tile i + 1; everyone has done with tile i - 1
         if (i + 1 < nt) {
           const int blk = *(const int *)(tab + wv * 64 + ((i + 1) & 1) * 32 + (attn_lane() & 7) * 4);
@@ -507,7 +642,10 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         scores(i);
         prepare(i);
         soften(i);
-        product(i);
+        if constexpr (WIDE)
+          product_wide(i);
+        else
+          product(i);
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
       asm volatile("" ::"v"(sb), "v"(tvv), "v"(kx[0]), "v"(kx[1]));

@@ -235,6 +235,27 @@ def test_queries_and_scales_of_all_sizes(new, D):
     assert close(attention(c, q, [0, new], [L]), want, bound)
 
 
+@pytest.mark.parametrize("new", [1, 90])
+@pytest.mark.parametrize("D,block", [(64, 16), (128, 8), (256, 16), (64, 5), (128, 7), (256, 12)])
+def test_value_scales_far_apart(new, D, block):
+    """Pages of values from 2^-67 to 2^62, some of all zeros at the smallest scale there is: what they take of a row's weight
+    is what the scores say.  (No sum passes 2^62 * 448 * 60 keys of a tile, far from f32's end.)"""
+    L = 300
+    c = ref.Cache([L], 2, D, block, seed=28, spread=0.2)
+    g = torch.Generator().manual_seed(29)
+    pages = torch.from_numpy(c.table[0]).long()
+    c.vs[pages] = torch.randint(60, 190, (len(pages), 2), generator=g, dtype=torch.uint8)
+    c.v[pages[::3]], c.vs[pages[::3]] = 0, 0
+    q = torch.randn(new, 4, D, generator=g).to(torch.bfloat16)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
+    assert close(attention(c, q, [0, new], [L]), want, bound)
+    # nothing but zeros and one page: its share
+    c.v[pages], c.vs[pages] = 0, 0
+    c.v[pages[4]], c.vs[pages[4]] = 0x38, 127  # 1
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
+    assert close(attention(c, q, [0, new], [L]), want, bound)
+
+
 @pytest.mark.parametrize("Hq,D,new", [(4, 256, 1), (10, 256, 3), (8, 128, 1), (8, 128, 4), (6, 64, 1), (7, 64, 4), (3, 80, 2)])
 @pytest.mark.parametrize("L", [40, 700, 5000])
 def test_weights_of_few_rows(Hq, D, new, L):
