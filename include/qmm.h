@@ -377,8 +377,9 @@ int qmm_paged_attention(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_arra
 
 /* qmm_rope_cache into such a cache: q as there; k and v, after their norm and rotation in float32, become codes.  The
  * call's rows of one page must follow one another in slots, as qmm_block_tables gives them (rows without a slot may lie
- * before and after them; two runs of one page, like two rows of one slot, race).  For each page and head that they reach, m the largest finite |value| of theirs and t the smallest exponent, at
- * least -127, with 448 * 2^t >= m:
+ * before and after them; two runs of one page, like two rows of one slot, race); at most 2^30 of them.  For each page and
+ * head that they reach, m the largest finite |value| of theirs and t the smallest exponent, at least -127, with
+ * 448 * 2^t >= m:
  *  where the page's first row is among them the page starts anew: its scale becomes 2^t (what its other rows held is lost);
  *  elsewhere the scale becomes the larger of 2^t and the one before; if it grew, the codes that the page holds are divided
  *  by what it grew by (exact but where they become subnormal; rounded to nearest even).
@@ -396,7 +397,9 @@ int qmm_cache_read_fp8(qmm_array *k_out, qmm_array *v_out, qmm_array k_cache, qm
 
 /* qmm_paged_attention over such a cache, with the same arguments, limits and rules (stale codes and scales of what a row
  * does not see do not reach it).  Keys and values are what qmm_cache_read_fp8 gives in float32.  A query that is not finite
- * gives NaN. */
+ * gives NaN.  Queries go into their products as two E4M3 parts, which leave 2^-22 of the largest of 128 values; weights, for
+ * requests of few rows, as two bfloat16 parts (2^-16), for others rounded to bfloat16 where D is at most 128 (2^-9) and as two
+ * E4M3 parts above (2^-8, and 2^-22 of the largest of 32 keys'). */
 int qmm_paged_attention_fp8(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
                             qmm_array v_scales, qmm_array table, qmm_array q_starts, qmm_array kv_lens, qmm_array gate,
                             float scale, int window, qmm_stream s);

@@ -159,6 +159,7 @@ int rope_cache(const char *op, qmm_array *q_out, qmm_array k_cache, qmm_array v_
   if (qa->ndim != 3 || qa->shape[2] < D || qa->shape[2] % 8)
     return fail("[%s] q must be [T, Hq, %d or more, a multiple of 8]", op, D);
   const int T = qa->shape[0], Hq = qa->shape[1];
+  if (c.fp8 && (T > 1 << 30 || Hkv > 1 << 29)) return fail("[%s] more than 2^30 rows or 2^29 heads", op);
   for (const Arr *x : {ka, va})
     if (x->ndim != 3 || x->shape[0] != T || x->shape[1] != Hkv || x->shape[2] != D)
       return fail("[%s] k and v must be [%d, %d, %d]", op, T, Hkv, D);

@@ -57,6 +57,7 @@ OF_CACHES = [
 @pytest.mark.parametrize("change,needle", OF_CACHES + [
     (dict(q=apart(4, (T, Hq, D), Q.FLOAT32)), "all be bfloat16 or all float32"),
     (dict(q=apart(4, (T, Hq, D - 8))), "q must be [T, Hq, 64 or more"),
+    (dict(q=apart(4, ((1 << 30) + 1, Hq, D))), "more than 2^30 rows"),
     (dict(k=apart(5, (T, Hkv + 1, D))), "k and v must be [4, 2, 64]"),
     (dict(v=Q.Array()), "missing input"),
     (dict(slots=ints(T - 1)), "slots must be an array of shape [4]"),
