@@ -257,7 +257,10 @@ Route route_of(const AttnArgs &a) {
   const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
   if (!one) {
     r.rows.tr = most <= 16 ? 16 : 32;
-    r.rows.grid = 2 * cus;
+    // (E4M3 pages of up to 128 values: a CU holds three workgroups, with tiles of 4 KB a wave.  Two with 8 KB, and three: 16
+    // heads of 64, 64 requests of 300 keys 23.4 and 20.1 us, 3000 keys 48.9 and 51.2; 32 heads on 8 of 128, one request of 300
+    // keys 12.8 and 11.5, 128 of them 32.7 and 26.5, 64 of 3000 53.3 and 53.8; 12 heads of 96 16 of 3000 28.2 and 24.7)
+    r.rows.grid = a.k_scales && r.DP <= 128 ? 3 * cus < AC_MOST ? 3 * cus : AC_MOST : 2 * cus;
     r.rows.min_rows = 0, r.rows.max_rows = few ? INT32_MAX : ROWS_MOST;
     // (one token each, as when decoding, is the common case of T <= R; 16 rows for 6 would be 10 empty workgroups a tile)
     const bool each = a.R > 1 && a.T <= a.R;

@@ -28,12 +28,14 @@ namespace {
 constexpr int AR_WAVES = 4;
 constexpr int AR_EXTRA = 1;  // a tile's own overhead, in units of its keys
 constexpr int AR_TILE = 8192;  // bytes of a wave's tile of keys (and of values)
-constexpr int AR_STAGE = AR_WAVES * 2 * AR_TILE;
+// (E4M3 codes of up to 128 values: half, so that a CU holds three workgroups)
+constexpr int ar_tile(int DP, bool fp8) { return fp8 && DP <= 128 ? AR_TILE / 2 : AR_TILE; }
+constexpr int ar_stage(int DP, bool fp8) { return AR_WAVES * 2 * ar_tile(DP, fp8); }
 constexpr int AR_TAB = AR_WAVES * 2 * 256;  // the next tile's page ids, two sets per wave
 constexpr int AR_SCALES = AR_WAVES * 4 * 256;  // E4M3: its keys' and values' scale bytes, a dword each, two sets per wave
 
 constexpr int ar_merge(int DP) { return AR_WAVES * 16 * (DP + 4) * 4 + AR_WAVES * 16 * 8; }
-constexpr int ar_fixed(int DP) { return AR_STAGE > ar_merge(DP) ? AR_STAGE : ar_merge(DP); }
+constexpr int ar_fixed(int DP, bool fp8) { return ar_stage(DP, fp8) > ar_merge(DP) ? ar_stage(DP, fp8) : ar_merge(DP); }
 
 #pragma clang diagnostic push
 #pragma clang diagnostic ignored "-Winline-asm"
@@ -64,8 +66,8 @@ template <int DP, int NQ, bool FULL, bool E8>
 __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare &share) {
   constexpr int TR = 16 * NQ;
   constexpr int EB = E8 ? 1 : 2;          // bytes of a value
-  constexpr int TILE = E8 && DP == 64 ? AR_TILE / 2 : AR_TILE;
-  constexpr int KW = TILE / (EB * DP);    // keys of a wave's tile: 16, 32, 64; E4M3: 32, 64, 64
+  constexpr int TILE = ar_tile(DP, E8);
+  constexpr int KW = TILE / (EB * DP);    // keys of a wave's tile: 16, 32, 64; E4M3: 32, 32, 64
   constexpr int KT = AR_WAVES * KW;
   constexpr int CPR = EB * DP / 16;       // 16-byte chunks of a row
   constexpr int RPI = 64 / CPR;           // rows of a DMA operation
@@ -76,7 +78,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
   constexpr int OPS = TILE / 1024;        // DMA operations of a tile
   constexpr int ASKED = E8 ? 3 : 1;       // those of page ids and scales before them
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  uint8_t *tab = lds + ar_fixed(DP);
+  uint8_t *tab = lds + ar_fixed(DP, E8);
   uint8_t *scl = tab + AR_TAB;
   int *seen_at = (int *)(scl + (E8 ? AR_SCALES : 0));  // [thread][2][2]: what its rows see
   const auto swz = [](int row) { return E8 ? attn_swz8<DP>(row) : attn_swz<DP>(row); };
@@ -92,11 +94,11 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
     if (tid == 0) plan->work[0] = w, plan->poison[0] = 0;
     left = w.left;
   }
-  uint8_t *kl = lds + wv * 2 * AR_TILE, *vl = kl + AR_TILE;
+  uint8_t *kl = lds + wv * 2 * TILE, *vl = kl + TILE;
   const uint32_t ka = lds_addr(kl), va = lds_addr(vl), ta = lds_addr(tab) + wv * 512, sa = lds_addr(scl) + wv * 1024;
   // head values past D: never written by the DMA, zero for good
   if constexpr (!FULL) {
-    for (int i = tid; i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
+    for (int i = tid; i < ar_stage(DP, E8) / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
   }
 
   int turn = 0;
@@ -599,7 +601,7 @@ __device__ __forceinline__ void attn_rows(const AttnArgs &args, const AttnShare 
     }
     if constexpr (!FULL) {  // the merge has overwritten the zeros past D
       __syncthreads();
-      for (int i = here(); i < AR_STAGE / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
+      for (int i = here(); i < ar_stage(DP, E8) / 16; i += ATTN_THREADS) ((uint4 *)lds)[i] = attn_zeros();
     }
   }
 }
@@ -638,7 +640,7 @@ hipError_t launch(const AttnArgs &a, const AttnShare &s, int DP, int tr, int gri
 }  // namespace
 
 size_t attn_rows_lds(int DP, int R, bool fp8) {
-  return ar_fixed(DP) + AR_TAB + (fp8 ? AR_SCALES : 0) + 16 * ATTN_THREADS + attn_plan_lds(R);
+  return ar_fixed(DP, fp8) + AR_TAB + (fp8 ? AR_SCALES : 0) + 16 * ATTN_THREADS + attn_plan_lds(R);
 }
 
 hipError_t launch_attn_rows(const AttnArgs &a, const AttnShare &s, int DP, int tr, int grid, hipStream_t st) {
