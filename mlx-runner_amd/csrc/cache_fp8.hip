@@ -10,8 +10,13 @@
 // page loses next to nothing, and when it grows only codes that become subnormal are rounded again.
 //
 // A workgroup takes one head of k or v and the runs that start in a window of as many tokens as its lanes hold rows
-// (16 values a lane), or of fewer where there are few, so a run is seen whole by one workgroup and no atomics leave it.  Rows past the window (of its last
-// run) take further turns.
+// (16 values a lane), or of fewer where there are few, so a run is seen whole by one workgroup and no atomics leave it.  Rows
+// past the window (of its last run) take further turns.  The workgroups that turn q's heads lie between them.
+//
+// One token 5.4 us (latency: slots, the page's old scale, the head's sums, the maximum through LDS), 2048 tokens of 24 heads on
+// 4 of 256 (63 MB) 17.1-17.6 us, 3.6 TB/s, bound by the copy rate and the ramp as rope_kernel.
+#include <atomic>
+
 #include "rope.h"
 
 namespace qmm {
@@ -19,6 +24,7 @@ namespace qmm {
 namespace {
 
 constexpr int CW_RUNS = 64;  // of a window at most
+constexpr int CW_WIDE = 1024, CW_MANY = 256;
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
@@ -53,27 +59,42 @@ struct CacheWrite {
   // The grid: `writers` workgroups for k and v, `pairs` (a head of k or v each) times `columns` (a window each), one before every `period` - 1 of
   // those that turn q's heads, `parts` to a token.
   int writers, pairs, columns, period, parts;
+  int angles;  // (cw_angles)
   FastDiv by_block, by_half, by_pairs, by_period;
 };
 
 __device__ __forceinline__ int fast_quot(int n, FastDiv d) { return (int)(__umulhi((uint32_t)n << 1, d.mul) >> d.shift); }
 
-template <int PAIRS, bool IN_F32>
-__global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5) void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
-  __shared__ __attribute__((aligned(16))) float cs[ROPE_THREADS * 8], sn[ROPE_THREADS * 8], norm[ROPE_MAX_SETS][256];
-  __shared__ __attribute__((aligned(16))) float swap[PAIRS == ACROSS ? ROPE_THREADS * 16 : 4];
+// Dynamic LDS: cos and sin of a turn's angles (as of one token's, by the workgroups of q), and 16 values a thread (ACROSS).
+constexpr int cw_angles(int threads, int lph, int half) {
+  const int n = (threads >> lph) * half;
+  return n < 128 ? 128 : (n + 3) & ~3;
+}
+constexpr size_t cw_lds(int pairs, int threads, int lph, int half) {
+  return (size_t)cw_angles(threads, lph, half) * 8 + (pairs == ACROSS ? threads * 64 : 0);
+}
+
+// THREADS: ROPE_THREADS, workgroups of q among them, or CW_WIDE, without.
+template <int PAIRS, bool IN_F32, int THREADS>
+__global__ __launch_bounds__(THREADS, THREADS > ROPE_THREADS ? 4 : PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
+void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
+  extern __shared__ __attribute__((aligned(16))) float cw_dynamic[];
+  __shared__ __attribute__((aligned(16))) float norm[ROPE_MAX_SETS][256];
   __shared__ float freq[128];
-  __shared__ int pos[CW_RUNS];
+  __shared__ int pos[THREADS / 4];
   __shared__ uint32_t top[CW_RUNS];
   __shared__ int begun[CW_RUNS], exponent[CW_RUNS], grown[CW_RUNS], grown_page[CW_RUNS], n_grown;
+  float *cs = cw_dynamic, *sn = cs + w.angles, *swap = sn + w.angles;
   const int writer = fast_quot(blockIdx.x, w.by_period);
-  if (writer >= w.writers || (int)blockIdx.x != writer * w.period) {
-    const int before = writer < w.writers ? writer + 1 : w.writers;
-    rope_heads<PAIRS, IN_F32, false>(a, 1, lph, w.parts, blockIdx.x - before, cs, sn, norm, swap);
-    return;
+  if constexpr (THREADS == ROPE_THREADS) {
+    if (writer >= w.writers || (int)blockIdx.x != writer * w.period) {
+      const int before = writer < w.writers ? writer + 1 : w.writers;
+      rope_heads<PAIRS, IN_F32, false>(a, 1, lph, w.parts, blockIdx.x - before, cs, sn, norm, swap);
+      return;
+    }
   }
   const int tid = threadIdx.x, lane = tid & 63;
-  const int rows = ROPE_THREADS >> lph;  // of a turn
+  const int rows = THREADS >> lph;  // of a turn
   const int l = tid & ((1 << lph) - 1), g = tid >> lph;
   const bool turned = PAIRS != ACROSS && l < a.half / 8;
   const int d0 = (PAIRS == HALVES && turned ? l : 2 * l) * 8, d1 = PAIRS == HALVES && turned ? d0 + a.half : d0 + 8;
@@ -136,7 +157,7 @@ __global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
     __syncthreads();  // (the last item's are read)
     if (tid < CW_RUNS) top[tid] = 0, begun[tid] = 0;
     if (tid < 128) freq[tid] = freq_l;
-    norm[0][tid] = norm_l;
+    if (THREADS == 256 || tid < 256) norm[0][tid & 255] = norm_l;
 
     auto run_of = [&](int row) -> int {
       const int i = row - w0;
@@ -144,7 +165,7 @@ __global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
     };
     // The turns, last to first, for the maxima: then the first one's values are still there, and only the others' are formed
     // again for their codes (16 rows of 256, 32 of 128 or 64 of 64 values are one turn).
-    const int turns = (end - first + rows - 1) >> (8 - lph);
+    const int turns = (end - first + rows - 1) >> ((THREADS == ROPE_THREADS ? 8 : 10) - lph);
     const bool there = w.early && lead == 0 && turns == 1;
 #pragma unroll 1
     for (int step = 0; step < 2 * turns - 1; ++step) {
@@ -157,7 +178,7 @@ __global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
         if (tid < rows) pos[tid] = there ? pos_l : row0 + tid < end ? a.positions[row0 + tid] : 0;
         __syncthreads();
         const int half = a.half, n = (end - row0 < rows ? end - row0 : rows) * half;
-        for (int i = tid; i < n; i += ROPE_THREADS) {
+        for (int i = tid; i < n; i += THREADS) {
           const int r = fast_quot(i, w.by_half), j = i - r * half;
           float sv, c;
           rope_angle(pos[r], freq[j], sv, c);
@@ -228,7 +249,7 @@ __global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
             const int by = grown[r];
             const uint4 c = *codes;
             *codes = make_uint4(shrink4(c.x, by), shrink4(c.y, by), shrink4(c.z, by), shrink4(c.w, by));
-            i += ROPE_THREADS;
+            i += THREADS;
           }
           __syncthreads();  // (their rows of this call come after)
         }
@@ -243,7 +264,9 @@ __global__ __launch_bounds__(ROPE_THREADS, PAIRS == ACROSS ? 3 : IN_F32 ? 4 : 5)
   }
 }
 
-// Codes to values, E to a lane: 16 bytes out where they are bfloat16.
+// Codes to values, E to a lane: 16 bytes out of each at a time.  Bound by the copy rate; results are stored past the caches,
+// which they would only fill: 9 prefixes of 100 to 32768 rows as bfloat16 (658 MB) 133 us through them, 123 past them, 32000
+// rows of 4 heads of 256 as float32 (328 MB) 84 and 50, 6.6 TB/s.
 template <bool F32>
 __global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadArgs a, int chunks) {
   constexpr int E = F32 ? 4 : 8, U = 4;
@@ -295,12 +318,23 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadArgs a, 
   }
 }
 
+template <int PAIRS, bool IN_F32, int THREADS>
+hipError_t launch_write(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph, hipStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const hipError_t e =
+      ensure_dynamic_lds(done, (const void *)cache_write_kernel<PAIRS, IN_F32, THREADS>, (int)cw_lds(PAIRS, THREADS, 2, 32));
+  if (e != hipSuccess) return e;
+  hipLaunchKernelGGL((cache_write_kernel<PAIRS, IN_F32, THREADS>), dim3(grid), dim3(THREADS), cw_lds(PAIRS, THREADS, lph, a.half), st,
+                     a, w, lph);
+  return hipGetLastError();
+}
 template <int PAIRS>
-void launch_pairs(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph, hipStream_t st) {
-  if (a.in_f32)
-    hipLaunchKernelGGL((cache_write_kernel<PAIRS, true>), dim3(grid), dim3(ROPE_THREADS), 0, st, a, w, lph);
-  else
-    hipLaunchKernelGGL((cache_write_kernel<PAIRS, false>), dim3(grid), dim3(ROPE_THREADS), 0, st, a, w, lph);
+hipError_t launch_pairs(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph, int threads, hipStream_t st) {
+  if (PAIRS != ACROSS && threads == CW_WIDE)
+    return a.in_f32 ? launch_write<PAIRS == ACROSS ? HALVES : PAIRS, true, CW_WIDE>(a, w, grid, lph, st)
+                    : launch_write<PAIRS == ACROSS ? HALVES : PAIRS, false, CW_WIDE>(a, w, grid, lph, st);
+  return a.in_f32 ? launch_write<PAIRS, true, ROPE_THREADS>(a, w, grid, lph, st)
+                  : launch_write<PAIRS, false, ROPE_THREADS>(a, w, grid, lph, st);
 }
 
 }  // namespace
@@ -309,13 +343,17 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
   if (a.T <= 0 || a.D < 16 || a.D > 256 || a.D % 16 || a.half < 0 || 2 * a.half > a.D || a.sets != 3 || a.block < 1 ||
       a.T > 1 << 30 || a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads > 1 << 29 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
-  const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4, rows = ROPE_THREADS >> lph;
+  // Pages of more rows than two turns have, and tokens enough that requests may have that many: 1024 threads, q in a launch of
+  // its own.  (2048 tokens, 24 heads on 4 of 256, pages of 32, 64, 128 and 256 rows: with 256 threads 27, 44, 64 and 111 us, with
+  // 1024 27, 29, 36 and 50; 300 tokens 12, 23, 38 and 70, and 17, 13, 20 and 34.)
+  const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
+  const int threads = a.block > 2 * ROPE_THREADS >> lph && a.T > CW_MANY && a.half % 8 == 0 ? CW_WIDE : ROPE_THREADS, rows = threads >> lph;
   CacheWrite w{};
   w.scales[0] = scales[1], w.scales[1] = scales[2];
   w.pairs = a.set[1].heads < 1 << 15 ? 2 * a.set[1].heads : 1 << 16;
   // few tokens: windows of fewer, down to one each, until there is a workgroup a CU (64 sequences' steps of 128 tokens in all,
   // 4 heads of 96: 10.2 us with windows of 32, 6.2 us with those of 4, where fewer angles are formed one after the other)
-  w.span = rows;
+  w.span = rows < CW_RUNS ? rows : CW_RUNS;
   while (w.span > 1 && ((int64_t)a.T + w.span - 1) / w.span * w.pairs < 256) w.span /= 2;
   w.windows = (int)(((int64_t)a.T + w.span - 1) / w.span);
   w.early = (int64_t)w.windows * w.pairs <= 512;
@@ -324,11 +362,14 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
   w.by_block = fast_div(a.block), w.by_half = fast_div(a.half ? a.half : 1), w.by_pairs = fast_div(w.pairs);
   int64_t grid = w.writers;
   w.period = 1;
-  if (a.T > ROPE_TOKENS) {  // (a grid's lanes are counted in 32 bits: q in launches of its own)
+  w.angles = cw_angles(threads, lph, a.half);
+  if (threads != ROPE_THREADS || a.T > ROPE_TOKENS) {  // (a grid's lanes are counted in 32 bits: q in launches of its own)
     RopeArgs q = a;
     q.sets = 1;
-    const hipError_t e = launch_rope(q, st);
-    if (e != hipSuccess) return e;
+    if (q.set[0].heads > 0) {
+      const hipError_t e = launch_rope(q, st);
+      if (e != hipSuccess) return e;
+    }
   } else {
     w.parts = (int)rope_parts(a, 1, lph);
     const int64_t turners = (int64_t)a.T * w.parts;
@@ -336,10 +377,9 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
     w.period = 1 + (int)(turners / w.writers);
   }
   w.by_period = fast_div(w.period);
-  a.half % 8      ? launch_pairs<ACROSS>(a, w, (unsigned)grid, lph, st)
-  : a.interleaved ? launch_pairs<NEXT>(a, w, (unsigned)grid, lph, st)
-                  : launch_pairs<HALVES>(a, w, (unsigned)grid, lph, st);
-  return hipGetLastError();
+  return a.half % 8      ? launch_pairs<ACROSS>(a, w, (unsigned)grid, lph, threads, st)
+         : a.interleaved ? launch_pairs<NEXT>(a, w, (unsigned)grid, lph, threads, st)
+                         : launch_pairs<HALVES>(a, w, (unsigned)grid, lph, threads, st);
 }
 
 hipError_t launch_cache_read(const CacheReadArgs &a, hipStream_t st) {

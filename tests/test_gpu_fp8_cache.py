@@ -134,6 +134,22 @@ def test_write(lens, Hq, Hkv, D, Dq, rot, block, interleaved, dtype, norm):
     assert torch.equal(out.q, host(as_before))
 
 
+@pytest.mark.parametrize("lens,Hq,Hkv,D,Dq,rot,block", [
+    # tokens enough, and pages long enough, for the wide workgroups
+    ([(30, 300), (0, 70), (100, 64)], 4, 2, 256, 512, 64, 40),
+    ([(5, 500)], 2, 2, 128, 128, 128, 66),
+    ([(90, 400), (0, 1)], 3, 3, 64, 64, 64, 160),
+    ([(c, 1 + c % 3) for c in range(0, 270, 2)], 2, 2, 256, 256, 256, 36),
+    ([(17, 270)], 1, 1, 32, 40, 16, 130),
+    ([(0, 1100)], 1, 3, 208, 208, 0, 1000),
+])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("norm", [None, torch.float32])
+def test_write_to_long_pages(lens, Hq, Hkv, D, Dq, rot, block, interleaved, dtype, norm):
+    test_write(lens, Hq, Hkv, D, Dq, rot, block, interleaved, dtype, norm)
+
+
 @pytest.mark.parametrize("interleaved", [False, True])
 @pytest.mark.parametrize("rot", [64, 20])
 def test_keys_are_the_codes_of_the_rotation(rot, interleaved):
