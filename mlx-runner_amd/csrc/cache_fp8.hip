@@ -24,7 +24,7 @@ namespace qmm {
 namespace {
 
 constexpr int CW_RUNS = 64;  // of a window at most
-constexpr int CW_WIDE = 1024, CW_MANY = 256;
+constexpr int CW_WIDE = 1024, CW_MANY = 512;
 
 __device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
 
@@ -343,8 +343,8 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
   if (a.T <= 0 || a.D < 16 || a.D > 256 || a.D % 16 || a.half < 0 || 2 * a.half > a.D || a.sets != 3 || a.block < 1 ||
       a.T > 1 << 30 || a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads > 1 << 29 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
-  // Pages of more rows than two turns have, and tokens enough that requests may have that many: 1024 threads, q in a launch of
-  // its own.  (2048 tokens, 24 heads on 4 of 256, pages of 32, 64, 128 and 256 rows: with 256 threads 27, 44, 64 and 111 us, with
+  // Pages of more rows than two turns have, and more tokens than decoding requests mostly have together: 1024 threads, q in a
+  // launch of its own.  (64 requests of 3 tokens, pages of 64: 8.6 us with 256 threads, 15.7 with 1024.  2048 tokens, 24 heads on 4 of 256, pages of 32, 64, 128 and 256 rows: with 256 threads 27, 44, 64 and 111 us, with
   // 1024 27, 29, 36 and 50; 300 tokens 12, 23, 38 and 70, and 17, 13, 20 and 34.)
   const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
   const int threads = a.block > 2 * ROPE_THREADS >> lph && a.T > CW_MANY && a.half % 8 == 0 ? CW_WIDE : ROPE_THREADS, rows = threads >> lph;

@@ -136,11 +136,11 @@ def test_write(lens, Hq, Hkv, D, Dq, rot, block, interleaved, dtype, norm):
 
 @pytest.mark.parametrize("lens,Hq,Hkv,D,Dq,rot,block", [
     # tokens enough, and pages long enough, for the wide workgroups
-    ([(30, 300), (0, 70), (100, 64)], 4, 2, 256, 512, 64, 40),
-    ([(5, 500)], 2, 2, 128, 128, 128, 66),
-    ([(90, 400), (0, 1)], 3, 3, 64, 64, 64, 160),
-    ([(c, 1 + c % 3) for c in range(0, 270, 2)], 2, 2, 256, 256, 256, 36),
-    ([(17, 270)], 1, 1, 32, 40, 16, 130),
+    ([(30, 500), (0, 70), (100, 64)], 4, 2, 256, 512, 64, 40),
+    ([(5, 600)], 2, 2, 128, 128, 128, 66),
+    ([(90, 520), (0, 1)], 3, 3, 64, 64, 64, 160),
+    ([(c, 1 + c % 3) for c in range(0, 620, 2)], 2, 2, 256, 256, 256, 36),
+    ([(17, 540)], 1, 1, 32, 40, 16, 130),
     ([(0, 1100)], 1, 3, 208, 208, 0, 1000),
 ])
 @pytest.mark.parametrize("interleaved", [False, True])
