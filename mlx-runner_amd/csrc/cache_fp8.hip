@@ -163,12 +163,14 @@ void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
       const int i = row - w0;
       return __popcll(starts & (i < 63 ? (2ull << i) - 1 : ~0ull)) - 1;
     };
-    // The turns, last to first, for the maxima: then the first one's values are still there, and only the others' are formed
+    // The turns, last to first, for the maxima: then the first two's values are still there, and only the others' are formed
     // again for their codes (16 rows of 256, 32 of 128 or 64 of 64 values are one turn).
     const int turns = (end - first + rows - 1) >> ((THREADS == ROPE_THREADS ? 8 : 10) - lph);
     const bool there = w.early && lead == 0 && turns == 1;
+    float before_x[2][8] = {};
+    int slot_before = -1;
 #pragma unroll 1
-    for (int step = 0; step < 2 * turns - 1; ++step) {
+    for (int step = 0; step < 2 * turns - 1; step += step == turns - 1 ? 2 : 1) {
       const int row0 = first + (step < turns ? turns - 1 - step : step - turns + 1) * rows, row = row0 + g;
       if (step) __syncthreads();  // (the angles of the turn before are read)
       Eight<IN_F32> raw[2] = {early[0], early[1]};
@@ -254,11 +256,23 @@ void cache_write_kernel(const RopeArgs a, const CacheWrite w, int lph) {
           __syncthreads();  // (their rows of this call come after)
         }
       }
-      if (step >= turns - 1 && page >= 0) {
+      auto store = [&](int row, int slot, const float (&x)[2][8]) __attribute__((always_inline)) {
+        const int page = page_of(slot);
+        if (page < 0) return;
         const int e = exponent[run_of(row)];
         uint8_t *to = (uint8_t *)s.out + (((int64_t)page * heads + head) * a.block + (slot - page * a.block)) * a.D;
         if (in0) *(uint2 *)(to + d0) = codes8(x[0], e);
         if (in1) *(uint2 *)(to + d1) = codes8(x[1], e);
+      };
+      if (step >= turns - 1) store(row, slot, x);
+      if (step == turns - 1) {
+        if (turns > 1) store(row + rows, slot_before, before_x);
+      } else {
+        slot_before = slot;
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+          for (int j = 0; j < 8; ++j) before_x[k][j] = x[k][j];
       }
     }
   }
@@ -344,8 +358,8 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
       a.T > 1 << 30 || a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads > 1 << 29 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
   // Pages of more rows than two turns have, and more tokens than decoding requests mostly have together: 1024 threads, q in a
-  // launch of its own.  (64 requests of 3 tokens, pages of 64: 8.6 us with 256 threads, 15.7 with 1024.  2048 tokens, 24 heads on 4 of 256, pages of 32, 64, 128 and 256 rows: with 256 threads 27, 44, 64 and 111 us, with
-  // 1024 27, 29, 36 and 50; 300 tokens 12, 23, 38 and 70, and 17, 13, 20 and 34.)
+  // launch of its own.  (2048 tokens, 24 heads on 4 of 256, pages of 64, 128 and 256 rows: with 256 threads 40, 59 and 107 us,
+  // with 1024 27, 34 and 48.  64 requests of 3 tokens, pages of 64: 8.6 and 15.7.)
   const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
   const int threads = a.block > 2 * ROPE_THREADS >> lph && a.T > CW_MANY && a.half % 8 == 0 ? CW_WIDE : ROPE_THREADS, rows = threads >> lph;
   CacheWrite w{};
