@@ -334,10 +334,12 @@ __global__ __launch_bounds__(256) void cache_read_kernel(const CacheReadArgs a, 
 
 template <int PAIRS, bool IN_F32, int THREADS>
 hipError_t launch_write(const RopeArgs &a, const CacheWrite &w, unsigned grid, int lph, hipStream_t st) {
-  static std::atomic<uint64_t> done{0};
-  const hipError_t e =
-      ensure_dynamic_lds(done, (const void *)cache_write_kernel<PAIRS, IN_F32, THREADS>, (int)cw_lds(PAIRS, THREADS, 2, 32));
-  if (e != hipSuccess) return e;
+  if (cw_lds(PAIRS, THREADS, lph, a.half) > 32 << 10) {
+    static std::atomic<uint64_t> done{0};
+    const void *k = (const void *)cache_write_kernel<PAIRS, IN_F32, THREADS>;
+    const hipError_t e = ensure_dynamic_lds(done, k, (int)cw_lds(PAIRS, THREADS, 2, 32));
+    if (e != hipSuccess) return e;
+  }
   hipLaunchKernelGGL((cache_write_kernel<PAIRS, IN_F32, THREADS>), dim3(grid), dim3(THREADS), cw_lds(PAIRS, THREADS, lph, a.half), st,
                      a, w, lph);
   return hipGetLastError();

@@ -366,3 +366,34 @@ def test_two_streams_and_a_graph():
         assert torch.equal(on[2].cpu(), w[1]) and ref.same(on[0].cpu(), w[0]).all()
         rows = ref.decode(*w)[[s // block for s in slots], :, [s % block for s in slots]].to(torch.bfloat16)
         assert torch.equal(torch.nan_to_num(host(k)), torch.nan_to_num(rows))
+
+
+@pytest.mark.parametrize("D,rot", [(128, 128), (256, 64)])
+def test_a_captured_write_to_long_pages(D, rot):
+    """The wide workgroups, captured first (their LDS passes what a kernel has unasked where all of a head turns): every replay
+    the eager call's codes and scales, from the same cache, with other work between."""
+    H, P, block, T = 2, 12, 80, 600
+    g = torch.Generator().manual_seed(13)
+    slots, pos = runs([(30, T)], block, P, seed=14)
+    xs = [torch.randn(T, H, D, generator=g).to(torch.bfloat16) for _ in range(3)]
+    start = some_cache(P, H, block, D, seed=15)
+    f, i, p = dev(torch.from_numpy(Q.rope_frequencies(rot, 1e5)[0])), ints(slots), ints(pos)
+    x = torch.zeros(T, H, D, dtype=torch.bfloat16, device="cuda")
+    on, eager = ([t.clone().cuda() for t in (start[0], start[0], start[1], start[1])] for _ in range(2))
+    a, qo, q1 = Q.Array.from_torch(x), *(dev(torch.zeros(T, H, D, dtype=torch.bfloat16)) for _ in range(2))
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        Q.rope_cache_fp8(a, a, a, *[Q.Array.from_torch(t) for t in on], p, i, f, q_out=qo, stream=Q.Stream.torch_current())
+    for y in xs:
+        for to in (on, eager):
+            for t, s in zip(to, (start[0], start[0], start[1], start[1])):
+                t.copy_(s)
+        x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        Q.rope_cache_fp8(a, a, a, *[Q.Array.from_torch(t) for t in eager], p, i, f, q_out=q1, stream=Q.Stream.torch_current())
+        torch.cuda.synchronize()
+        assert all(torch.equal(s, t) for s, t in zip(on, eager)) and torch.equal(host(qo), host(q1))
+        codes, scales, _ = ref.store(start[0], start[1], slots, y.double())
+        assert torch.equal(on[3].cpu(), scales) and ref.same(on[1].cpu(), codes).all()
