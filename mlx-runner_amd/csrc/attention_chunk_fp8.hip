@@ -305,7 +305,8 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         if constexpr (WIDE) {
           const uint64_t other = __ballot(vs != __builtin_amdgcn_update_dpp(vs, vs, 0x111, 0xF, 0xF, false)) & 0xFEFEFEFEFEFEFEFEull;
           far = (other | (__ballot(vs - (127 - C8_RANGE) > 2u * C8_RANGE) & valid)) != 0;
-          const int x = __float_as_int((float)(vs - 127)), y = (254 - vs) << 23;
+          // (2^-up is finite for keys that there are not too, at any byte: their weights are zeros, and so is what they add)
+          const int x = __float_as_int((float)(vs - 127)), y = (254 - (vs < 254 ? vs : 254)) << 23;
 #pragma unroll
           for (int v = 0; v < 8; ++v) {
             up[v] = __int_as_float(__builtin_amdgcn_readlane(x, v * 8));
