@@ -318,13 +318,18 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         const uint64_t other = __ballot(vs != __builtin_amdgcn_update_dpp(vs, vs, 0x111, 0xF, 0xF, false)) & 0xFEFEFEFEFEFEFEFEull;
         far = ((uint32_t)other != 0) | ((uint32_t)(other >> 32) != 0) << 1;
         less = 0;
+        int of = vs;  // that of the eight's first key that there is, -1: none
+        if (fine != ~0ull) {
+          const uint32_t in = (uint32_t)(fine >> (ln & 56)) & 0xFFu;
+          of = __builtin_amdgcn_ds_bpermute((int)((ln & 56) + (in ? __builtin_ctz(in) : 0)) * 4, vs);
+          of = in ? of : -1;
+        }
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
           int x[4], most = 0;
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            x[v] = __builtin_amdgcn_readlane(vs, half * 32 + v * 8);
-            x[v] = fine >> (half * 32 + v * 8) & 1 ? x[v] : -1;
+            x[v] = __builtin_amdgcn_readlane(of, half * 32 + v * 8);
             most = x[v] > most ? x[v] : most;
           }
           tv[half] = most;

@@ -69,3 +69,29 @@ def test_the_first_pages_scales_are_nan(D, block, new, window):
     c, there = with_holes(L, 2, D, block, 40 + D, gone)
     assert (c.vs[0] == 255).all() and 0 not in c.table[0]
     check(c, there, gone, new, L, window, 41)
+
+
+@pytest.mark.parametrize("new,window", [(3, 0), (90, 0), (150, 70)])
+@pytest.mark.parametrize("D,block", [(64, 4), (128, 12), (256, 4), (256, 7), (256, 12), (208, 1), (256, 5), (256, 24)])
+@pytest.mark.parametrize("first,others", [(121, (121,)), (119, (119, 125)), (120, (120, 112, 124)), (130, (115, 120)),
+                                          (100, (115, 120)), (255, (119, 125)), (118, (118, 140))])
+def test_eights_that_begin_with_missing_keys(D, block, new, window, first, others):
+    """Every third page or so missing: the keys of a page that is there follow, among eight that go into the products together,
+    keys of a page that is not, whose scale seems to be that of page 0: the same, larger, smaller, or NaN."""
+    L = 400
+    n = -(-L // block)
+    gone = [p for p in range(n - 1) if p % 3 != 1] if block < 24 else [p for p in range(n - 1) if p % 2]
+    c, there = with_holes(L, 2, D, block, 50 + D, gone)
+    for i, p in enumerate(p for p in range(n) if p not in gone):
+        c.vs[int(c.table[0, p])] = others[i % len(others)]
+    c.vs[0] = first
+    check(c, there, gone, new, L, window, 51)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("larger", [125, 127, 140])
+def test_an_eight_after_missing_keys_beside_larger_scales(D, larger):
+    """Pages of 12: none, one with page 0's scale, one with a larger: keys 12 to 15 keep their own, as 16 to 23 do."""
+    c, there = with_holes(36, 2, D, 12, 60, [0])
+    c.vs[int(c.table[0, 1])], c.vs[int(c.table[0, 2])], c.vs[0] = 119, larger, 119
+    check(c, there, [0], 30, 36, 0, 61)
