@@ -108,6 +108,8 @@ class AttentionLayer:
 
     def read(self, slots: torch.Tensor, stream, dtype: torch.dtype = torch.float32):
         """The keys and values in the rows `slots` (int32) of a cache held in 8 bits: two [T, Hkv, D], exact in float32."""
+        if not self.eight:
+            raise ValueError("only a layer of cache='e4m3' is read back")
         k, v = (torch.empty(slots.numel(), self.Hkv, self.D, dtype=dtype, device="cuda") for _ in range(2))
         A = Q.Array.from_torch
         Q.cache_read_fp8(*self.caches, A(slots, Q.INT32), dtype=A(k).dtype, k_out=A(k), v_out=A(v), stream=stream)
