@@ -471,14 +471,17 @@ def rope_cache_fp8(q: Array, k: Array, v: Array, k_cache: Array, v_cache: Array,
     return res
 
 
-def cache_read_fp8(k_cache: Array, v_cache: Array, k_scales: Array, v_scales: Array, slots: Array, *,
+def cache_read_fp8(k_cache: Array | None, v_cache: Array | None, k_scales: Array | None, v_scales: Array | None, slots: Array, *,
                    dtype: int = BFLOAT16, k_out: Array | None = None, v_out: Array | None = None,
-                   stream: Stream | None = None) -> tuple[Array, Array]:
-    """The rows `slots` of such a cache as (k, v) [T, Hkv, D] in dtype; zeros where a slot is none."""
-    ks, vs = (a if a is not None else Array() for a in (k_out, v_out))
+                   stream: Stream | None = None) -> tuple[Array | None, Array | None]:
+    """The rows `slots` of such a cache as (k, v) [T, Hkv, D] in dtype; zeros where a slot is none.  A side without a cache
+    (and a result) is not read: None in its place."""
+    ks, vs = (out if out is not None else Array() if cache is not None else None
+              for cache, out in ((k_cache, k_out), (v_cache, v_out)))
     s = _stream(stream)
-    check(lib.qmm_cache_read_fp8(byref(ks.h), byref(vs.h), k_cache.h, v_cache.h, k_scales.h, v_scales.h, slots.h, dtype,
-                                 s.h), "cache_read_fp8")
+    check(lib.qmm_cache_read_fp8(*(byref(a.h) if a is not None else None for a in (ks, vs)),
+                                 *(a.h if a is not None else _NULL for a in (k_cache, v_cache, k_scales, v_scales)),
+                                 slots.h, dtype, s.h), "cache_read_fp8")
     return ks, vs
 
 

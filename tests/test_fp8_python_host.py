@@ -4,6 +4,7 @@ from pathlib import Path
 
 import pytest
 import torch
+from test_attention_results_host import apart
 
 import qmm as Q
 
@@ -18,3 +19,19 @@ def test_rows_of_a_bfloat16_layer_are_not_read_back():
     layer.eight, layer.Hkv, layer.D, layer.caches = False, 2, 64, ()
     with pytest.raises(ValueError, match="cache='e4m3'"):
         layer.read(torch.zeros(3, dtype=torch.int32), None)
+
+
+def test_cache_read_fp8_of_one_side_needs_that_side():
+    """A side without a cache is not read (the C call's NULL result); one that a result is asked of must be there."""
+    cache, scales = apart(0, (9, 2, 16, 64), Q.UINT8), apart(1, (9, 2), Q.UINT8)
+    slots, out = apart(2, (4,), Q.INT32), apart(3, (4, 2, 64))
+    for args, kw, needle in (((None, None, None, None, slots), {}, "null result pointers"),
+                             ((None, cache, None, scales, slots), dict(k_out=out), "missing k_cache"),
+                             ((cache, None, scales, None, slots), dict(v_out=out), "missing v_cache"),
+                             ((cache, None, None, None, slots), {}, "missing k_scales"),
+                             ((None, cache, None, None, slots), {}, "missing v_scales"),
+                             ((None, cache, None, scales, slots), dict(v_out=scales), "another shape")):
+        Q.lib.qmm_reset_faults_for_test()
+        with pytest.raises(Q.QmmError, match=needle):
+            Q.cache_read_fp8(*args, **kw)
+    Q.lib.qmm_reset_faults_for_test()
