@@ -1,4 +1,5 @@
 """The Python side of a cache held in 8 bits without a GPU."""
+import re
 import sys
 from pathlib import Path
 
@@ -35,3 +36,12 @@ def test_cache_read_fp8_of_one_side_needs_that_side():
         with pytest.raises(Q.QmmError, match=needle):
             Q.cache_read_fp8(*args, **kw)
     Q.lib.qmm_reset_faults_for_test()
+
+
+def test_the_chunk_kernels_are_among_those_looked_at_for_spills():
+    """Six of them, as over a bfloat16 cache: none drops out of the search for spilled vector registers."""
+    found = {}
+    for m in re.finditer(rb"\.symbol[\xa0-\xda](.{1,400}?)\.kd.{0,400}?\.vgpr_spill_count(.)", Path(Q.lib._name).read_bytes(), re.S):
+        found[m.group(1).decode("latin-1")] = m.group(2)[0]
+    chunk = {n: c for n, c in found.items() if "attn_chunk8_kernel" in n}
+    assert len(chunk) == 6 and not any(chunk.values())
