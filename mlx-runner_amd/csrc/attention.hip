@@ -54,6 +54,12 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const AttnShare &s) {
   return c;
 }
 
+// A part's weight beside the largest of its row, 0 where it has no keys of the row.  At least the smallest f32: whatever the
+// scores, a sum that is not finite reaches the row, as it does within a part; 2^-149 of one that is changes nothing.
+__device__ __forceinline__ float part_weight(float m, float top) {
+  return m == -__builtin_inff() ? 0.f : fmaxf(attn_exp2(m - top), __uint_as_float(1u));
+}
+
 // One workgroup per tile, row and COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every
 // wave works out the partials' weights for itself.  MORE: tiles may have more rows than the grid, so a workgroup goes on to
 // every gridDim.y-th (what the compiler forms ahead of such a loop costs 0.2 us where there is one row for each).
@@ -95,7 +101,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
     for (int p = HELD * 64 + lane; p < np; p += 64) top = fmaxf(top, s.ml[place(p) * 2]);
     top = wave_top(top);
     auto weigh = [&](int p, float2 v) __attribute__((always_inline)) {
-      const float f = v.x == -__builtin_inff() ? 0.f : attn_exp2(v.x - top);
+      const float f = part_weight(v.x, top);
       wt[wave][p] = f;
       sum += f * v.y;
     };
@@ -163,7 +169,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
     for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
     for (int p = l; p < np && on; p += 16) {
       if (p >= 16) ml = *(const float2 *)(s.ml + place(p, row) * 2);
-      const float f = ml.x == -__builtin_inff() ? 0.f : attn_exp2(ml.x - top);
+      const float f = part_weight(ml.x, top);
       wt[row][p] = f;
       sum += f * ml.y;
     }
