@@ -397,10 +397,10 @@ int qmm_cache_read_fp8(qmm_array *k_out, qmm_array *v_out, qmm_array k_cache, qm
 
 /* qmm_paged_attention over such a cache, with the same arguments, limits and rules (stale codes and scales of what a row
  * does not see do not reach it).  Keys and values are what qmm_cache_read_fp8 gives in float32.  A query that is not finite
- * gives NaN.  For requests of few rows scores are float32 sums of exact products (of keys as bfloat16, which only underflow can
- * round) and weights go into their products as two bfloat16 parts (2^-16).  For others queries go into their products as two
- * E4M3 parts, which leave 2^-22 of the largest of 64 values; weights rounded to bfloat16 where D is at most 128 (2^-8) and as
- * two E4M3 parts above (2^-8 as well, and 2^-22 of the largest of 32 keys'). */
+ * gives NaN.  Scores are float32 sums of exact products (of keys as bfloat16, which only underflow can round).  Weights go into
+ * their product with v, for requests of few rows, as two bfloat16 parts (2^-16); for others rounded to bfloat16 where D is at
+ * most 128 (2^-8), and as two E4M3 parts above (2^-8 as well, 2^-22 of the largest of 32 keys', and in the product 2^-10 of the
+ * largest of eight keys'). */
 int qmm_paged_attention_fp8(qmm_array *res, qmm_array q, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
                             qmm_array v_scales, qmm_array table, qmm_array q_starts, qmm_array kv_lens, qmm_array gate,
                             float scale, int window, qmm_stream s);

@@ -473,43 +473,7 @@ __device__ __forceinline__ float attn_across(float x, int other) {
   return __int_as_float(__builtin_amdgcn_ds_bpermute(((int)attn_lane() ^ other) * 4, __float_as_int(x)));
 }
 
-// 128 bf16 values of a row, 32 to a lane (of those 16 and 32 apart; PAIR: 64 values, lanes 32 apart), as two E4M3 parts with
-// a scale for all of them each: x = hi 2^t + lo 2^(t - 4).  Two 4-bit significands hold bf16's 8 bits, and what the first part
-// leaves is at most 16 2^t, so what is lost is 2^-22 of those values' largest, if anything.  (The matrix unit takes a scale
-// for every 32 values, but those are 16 of two lanes.)  The scales as bytes of its operand; 255 (NaN) where a value is not finite.
 typedef uint16_t u16x2_t __attribute__((ext_vector_type(2)));
-template <bool PAIR = false>
-__device__ __forceinline__ void attn_split(const u32x4_t (&x)[4], i32x8_t &hi, i32x8_t &lo, int &scale_hi, int &scale_lo) {
-  u16x2_t top = {0, 0};  // of the magnitudes, by their bits: what is not finite is largest
-#pragma unroll
-  for (int i = 0; i < 16; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[i / 4][i % 4] & 0x7FFF7FFFu));
-  uint32_t most = top[0] > top[1] ? top[0] : top[1];
-  if (!PAIR) {
-    const auto r = __builtin_amdgcn_permlane16_swap(most, most, false, false);
-    most = r[0] > r[1] ? r[0] : r[1];
-  }
-  {
-    const auto r = __builtin_amdgcn_permlane32_swap(most, most, false, false);
-    most = r[0] > r[1] ? r[0] : r[1];
-  }
-  const bool odd = most >= 0x7F80u;
-  const int t = odd ? 0 : most ? ceil_scale_exp(__uint_as_float(most << 16)) : -127, u = t - 4 > -127 ? t - 4 : -127;
-  const float sh = e8m0_scale_operand(t), sl = e8m0_scale_operand(u);
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t w0 = x[i / 2][i % 2 * 2], w1 = x[i / 2][i % 2 * 2 + 1];
-    i16x2_t c = {0, 0};
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, w0), sh, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_bf16(c, __builtin_bit_cast(bf16x2_t, w1), sh, true);
-    hi[i] = __builtin_bit_cast(int, c);
-    const f32x2_t a = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi[i], sh, false);
-    const f32x2_t b = __builtin_amdgcn_cvt_scalef32_pk_f32_fp8((uint32_t)hi[i], sh, true);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, __uint_as_float(w0 << 16) - a.x, __uint_as_float(w0 & 0xFFFF0000u) - a.y, sl, false);
-    c = __builtin_amdgcn_cvt_scalef32_pk_fp8_f32(c, __uint_as_float(w1 << 16) - b.x, __uint_as_float(w1 & 0xFFFF0000u) - b.y, sl, true);
-    lo[i] = __builtin_bit_cast(int, c);
-  }
-  scale_hi = odd ? 255 : t + 127, scale_lo = odd ? 255 : u + 127;
-}
 
 // A kernel's arguments (at `offset` of its argument block) read again where they are needed, instead of
 // holding scalar registers through the loop before.

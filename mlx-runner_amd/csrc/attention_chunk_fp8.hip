@@ -1,26 +1,28 @@
 // Paged attention of many rows per key head over a cache of E4M3 codes.
 //
-// S^T = K Q^T on the scaled 32x32x64 MFMA, which takes the codes as they are and a key's scale with them: bf16 queries go in
-// as two E4M3 parts (attn_split: exact but for 2^-22 of a row's largest), two products at twice the rate, so it costs what it
-// costs in bf16.
+// S^T = K Q^T in bf16: every wave widens the keys that it has moved, with their scales (exact), into LDS.  (The scaled
+// 32x32x64 MFMA takes codes as they are, and bf16 queries as two E4M3 parts at the same cost.  But it aligns the products of
+// eight values to the largest and drops what lies below 2^-13 of that one's power of two: beside keys' large channels a score of
+// 1057 came out 0.04 off, and weights by percents.  2048 tokens over 32768 keys, 24 heads on 4 of 256: 1.50-1.55 ms so, 1.65-1.68
+// with bf16, where eight waves' keys take LDS's bandwidth and widening a second barrier; widened by each wave for itself, in
+// registers, 1.68-1.71.  4000 tokens of 32 heads on 8 of 128: 198 and 201 us.)
 //
-// O^T = V^T P^T, where a head has at most 128 values (WIDE): codes are exact in bf16, so every wave widens the rows that it
-// has moved, into LDS, and the weights, rounded to bf16 once, take the values' scales as exponents of two.  With 256 values
-// LDS has no room for that (second parts of the queries 64 KB, tiles 64 KB): the codes go in as they are, and the weights in
-// two E4M3 parts (2^-8 of a weight lost), scaled for each row and 32 keys by a power of two of those keys' own maximum, which
-// the matrix unit takes off again; what E4M3's 18 binades cannot hold is 2^-22 of the largest weight of 32 keys.  A page's
-// scale of values is the other operand's where the tile's keys share it; else it goes into the weights, relative to the
-// tile's largest.  The products cost the same; two parts cost 2.5 instructions a weight, one rounding half of one: 4000
-// tokens of 32 heads on 8 of 128 228 us with two parts, 201 with bf16; chunks of 7 prompts, 16 heads of 64, window 1000, 124
-// and 107.
+// O^T = V^T P^T, where a head has at most 128 values (WIDE): values are widened like keys, and the weights, rounded to bf16
+// once, take the values' scales as exponents of two.  With 256 values LDS has no room for that (half of the queries 64 KB, one
+// tile's keys 32 KB, two tiles' codes of values 32 KB): the codes go into the scaled MFMA as they are, and the weights in two
+// E4M3 parts (2^-8 of a weight lost), scaled for each row and 32 keys by a power of two of those keys' own maximum, which the
+// matrix unit takes off again; what E4M3's 18 binades cannot hold is 2^-22 of the largest weight of 32 keys, what the unit drops
+// of eight products less than 2^-10 of the largest.  A page's scale of values is the other operand's where the tile's keys
+// share it; else it goes into the weights, relative to the tile's largest.  The products cost the same; two parts cost 2.5
+// instructions a weight, one rounding half of one: 4000 tokens of 32 heads on 8 of 128 228 us with two parts, 201 with bf16;
+// chunks of 7 prompts, 16 heads of 64, window 1000, 124 and 107.
 //
 // A tile is 256 rows, 32 for each of eight waves, two a SIMD (D 64: four): one's softmax beside the other's products, with
-// nothing interleaved by hand.  (Codes are half of bf16's bytes: eight waves' operands from LDS take the bandwidth that four
-// waves' of 64 rows take in bf16.)  64 keys at a time in LDS, two buffers, moved by DMA a tile ahead, eight keys by each wave;
-// one barrier a tile.
+// nothing interleaved by hand.  64 keys at a time, eight keys by each wave, moved a tile ahead: by DMA into two buffers, keys of
+// 256 values into registers; one barrier a tile, with 256 values two (one buffer for the widened keys).
 //
-// Bound by the two units in turn: 2048 tokens over 32768 keys, 24 heads on 4 of 256, 1.49-1.56 ms, 1.05 PFLOP/s (bf16 pages
-// 1.43-1.48), the matrix unit busy for 45% of it, the vector unit for most of the rest.
+// Bound by matrix unit, vector unit and LDS in turn: 2048 tokens over 32768 keys, 24 heads on 4 of 256, 1.65-1.68 ms, 0.96
+// PFLOP/s (bf16 pages 1.43-1.48), the matrix unit busy for 41% of it.
 #include <type_traits>
 
 #include "attention.h"
@@ -40,11 +42,11 @@ constexpr int C8_SMALL = C8_SCALES + C8_TAB + C8_VALID + 8 * C8_THREADS;
 constexpr int C8_RANGE = 40;  // weights up to 2^60 times scales up to 2^40 times codes stay far below f32's end
 constexpr int C8_NEAR = 8;  // scales of 32 keys' values that differ by up to 2^8 go in relative to the largest
 
-// Whether the values and their weights go in as bf16
+// Whether keys, values and weights lie in LDS, or go in, as bf16
 constexpr bool c8_wide(int DP) { return DP < 256; }
 constexpr int c8_tile(int DP) { return C8_KT * DP; }
-constexpr int c8_tiles(int DP) { return (c8_wide(DP) ? 8 : 4) * c8_tile(DP); }
-// The queries' second parts, where registers do not hold them
+constexpr int c8_tiles(int DP) { return (c8_wide(DP) ? 12 : 4) * c8_tile(DP); }
+// The queries' upper halves, where registers do not hold them
 constexpr int c8_queries(int DP) { return DP == 128 ? 0 : C8_TR * DP; }
 constexpr int c8_fixed(int DP) {
   const int out = C8_WAVES * 32 * 64 * 4, in = c8_tiles(DP) + c8_queries(DP);  // (rows out: 64 columns of a wave's rows at a time)
@@ -80,14 +82,15 @@ __device__ __forceinline__ float c8_pair_max(float x) {
 template <int DP, bool FULL>
 __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kernel(const AttnArgs args, const AttnShare share) {
   constexpr int CPR = DP / 16;     // 16-byte chunks of a row
-  constexpr int KS = DP / 64;      // k steps of S^T
+  constexpr int KS = DP / 16;      // k steps of S^T
   constexpr int DT = DP / 32;      // 32-column tiles of O^T
   constexpr int RPI = 64 / CPR;    // rows of a DMA operation
   constexpr int OPS = 8 > RPI ? 8 / RPI : 1;  // operations of a wave's 8 rows
   constexpr int TILE = c8_tile(DP), PITCH = DP;
-  constexpr bool LO_LDS = c8_queries(DP) > 0, WIDE = c8_wide(DP);
+  constexpr bool WIDE = c8_wide(DP);
+  constexpr int KR = c8_queries(DP) ? KS / 2 : KS;  // of them with queries in registers
   extern __shared__ __attribute__((aligned(1024))) uint8_t lds[];
-  uint8_t *qlo = lds + c8_tiles(DP);
+  uint8_t *qup = lds + c8_tiles(DP);
   uint8_t *scl = lds + c8_fixed(DP);                 // [2][keys, values][64]
   uint8_t *tab = scl + C8_SCALES;                    // [wave][2][8]
   uint8_t *vm = tab + C8_TAB;                        // [2][8 waves], a byte each
@@ -143,8 +146,7 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
 
     // the lane's row: what it sees, its queries
     float m, l = 0.f;
-    i32x8_t qh[KS], ql[LO_LDS ? 1 : KS];
-    int qs[2] = {0, 0};  // their scales, a byte for each step
+    bf16x8_t q[KR];
     {
       const int ln = (int)attn_lane(), in = wv * 32 + (ln & 31), lh = ln >> 5;
       const bool on = in < t.rows;
@@ -155,28 +157,25 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
       // (a row that sees nothing needs no reference; one past the end has no weights and passes none)
       m = !on ? __builtin_inff() : pos >= 0 ? -__builtin_inff() : 0.f;
       const uint16_t *qp = a.q + attn_row(a, rq.q0, row, head) * a.D;
+      u16x2_t top = {0, 0};  // of the magnitudes, by their bits
+      bf16x8_t *const up = (bf16x8_t *)(qup + wv * 32 * DP) + ln;
 #pragma unroll
       for (int s = 0; s < KS; ++s) {
-        const int at = s * 64 + lh * 32;
-        u32x4_t x[4];
+        const int at = s * 16 + lh * 8;
+        u32x4_t x = {0u, 0u, 0u, 0u};
+        if (at < D) x = *(const u32x4_t *)(qp + at);
+        // a negative scale: -q, so that maxima stay maxima; none: no scores
+        x = a.scale > 0.f ? x : a.scale < 0.f ? x ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          x[i] = u32x4_t{0u, 0u, 0u, 0u};
-          if (at + i * 8 < D) x[i] = *(const u32x4_t *)(qp + at + i * 8);
-          // a negative scale: -q, so that maxima stay maxima; none: no scores
-          x[i] = a.scale > 0.f ? x[i] : a.scale < 0.f ? x[i] ^ 0x80008000u : u32x4_t{0u, 0u, 0u, 0u};
-        }
-        i32x8_t lo;
-        int sh, sl;
-        attn_split<true>(x, qh[s], lo, sh, sl);
-        qs[0] |= sh << 8 * s, qs[1] |= sl << 8 * s;
-        if constexpr (LO_LDS) {
-          i32x4_t *to = (i32x4_t *)(qlo + wv * 32 * DP) + s * 128 + ln;
-          to[0] = __builtin_shufflevector(lo, lo, 0, 1, 2, 3), to[64] = __builtin_shufflevector(lo, lo, 4, 5, 6, 7);
-        } else {
-          ql[s] = lo;
-        }
+        for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2_t, x[i] & 0x7FFF7FFFu));
+        if (s < KR)
+          q[s < KR ? s : 0] = __builtin_bit_cast(bf16x8_t, x);
+        else
+          up[(s - KR) * 64] = __builtin_bit_cast(bf16x8_t, x);
       }
+      // a query that is not finite: NaN
+      const uint32_t nan = top[0] >= 0x7F80u || top[1] >= 0x7F80u ? 0x7FC07FC0u : 0u;
+      q[0] = __builtin_bit_cast(bf16x8_t, __builtin_bit_cast(u32x4_t, q[0]) | nan);
     }
     f32x16_t acc[DT];
 #pragma unroll
@@ -220,13 +219,24 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
             gp_dma16(cache + ((uint64_t)row * (uint32_t)D + c), attn_uniform(la + to + wv * 8 * PITCH + n * 1024));
         }
       };
+      u32x4_t keys[WIDE ? 1 : OPS];  // (not WIDE: on their way in registers; zeros past D)
       auto move_all = [&](int j) __attribute__((always_inline)) {
         const int set = j & 1;
         if (attn_lane() < 8) {
           c8_dma1(ksc + of, attn_uniform(sa + set * 512 + wv * 32));
           c8_dma1(vsc + of, attn_uniform(sa + set * 512 + 256 + wv * 32));
         }
-        move(kc, set * TILE);
+        if constexpr (WIDE) {
+          move(kc, set * TILE);
+        } else {
+          const uint32_t ln = attn_lane();
+#pragma unroll
+          for (int n = 0; n < OPS; ++n) {
+            const uint32_t row = __builtin_amdgcn_ds_bpermute((int)(n * RPI + ln / CPR) * 4, (int)mine), c = ln % CPR * 16;
+            keys[n] = u32x4_t{0u, 0u, 0u, 0u};
+            if (FULL || c < (uint32_t)D) keys[n] = *(const u32x4_t *)(kc + ((uint64_t)row * (uint32_t)D + c));
+          }
+        }
         move(vc, (2 + set) * TILE);
       };
       auto valid_of = [&](int j) __attribute__((always_inline)) -> uint64_t {
@@ -241,54 +251,31 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
       };
 
       f32x16_t sv[2];
-      int kx[2] = {0, 0}, sb = 0, tvv = 0;  // the products' scales
+      int sb = 0, tvv = 0;  // the second product's scales
       i32x8_t ph{}, pl{};
       bf16x8_t pb[4]{};  // (WIDE: the weights of 16 keys each)
+      const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
       // S^T of tile j: 2 x 32 keys
       auto scores = [&](int j) __attribute__((always_inline)) {
-        const int set = j & 1;
-        {
-          const uint32_t ln = attn_lane();
-          const int row = ln & 31, lh = (int)(ln >> 5);
-          const int from = set * TILE + row * PITCH + ((lh * 2) ^ attn_swz8<DP>(row)) * 16;
-          const int *kxl = (const int *)(scl + set * 512) + row;
-          kx[0] = kxl[0], kx[1] = kxl[32];
-          auto load = [&](int s, int half) __attribute__((always_inline)) {
-            const int x = (from ^ s * 64) + half * 32 * PITCH, y = (from ^ (s * 64 + 16)) + half * 32 * PITCH;
-            const i32x4_t lo = *(const i32x4_t *)(lds + x), hi = *(const i32x4_t *)(lds + y);
-            return __builtin_shufflevector(lo, hi, 0, 1, 2, 3, 4, 5, 6, 7);
-          };
-          auto second = [&](int s) __attribute__((always_inline)) {
-            if constexpr (LO_LDS) {
-              const i32x4_t *q = (const i32x4_t *)(qlo + wv * 32 * DP) + s * 128 + ln;
-              return __builtin_shufflevector(q[0], q[64], 0, 1, 2, 3, 4, 5, 6, 7);
-            } else {
-              return ql[s];
-            }
-          };
-          i32x8_t k0 = load(0, 0), k1;
-          auto step = [&](auto s_c) __attribute__((always_inline)) {
-            constexpr int s = decltype(s_c)::value;
-            const f32x16_t z = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
-            i32x8_t k0n;
-            const i32x8_t lo = second(s);
-            k1 = load(s, 1);
-            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0, qh[s], s ? sv[0] : z, 0, 0, 0, kx[0], s, qs[0]);
-            __builtin_amdgcn_sched_barrier(0);
-            sv[0] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k0, lo, sv[0], 0, 0, 0, kx[0], s, qs[1]);
-            if constexpr (s + 1 < KS) k0n = load(s + 1, 0);
-            __builtin_amdgcn_sched_barrier(0);
-            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1, qh[s], s ? sv[1] : z, 0, 0, 0, kx[1], s, qs[0]);
-            __builtin_amdgcn_sched_barrier(0);
-            sv[1] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(k1, lo, sv[1], 0, 0, 0, kx[1], s, qs[1]);
-            __builtin_amdgcn_sched_barrier(0);
-            if constexpr (s + 1 < KS) k0 = k0n;
-          };
-          step(std::integral_constant<int, 0>{});
-          if constexpr (KS > 1) step(std::integral_constant<int, 1>{});
-          if constexpr (KS > 2) step(std::integral_constant<int, 2>{}), step(std::integral_constant<int, 3>{});
-          asm volatile("" : "+v"(sv[0]), "+v"(sv[1]));  // (as after a product)
+        const uint32_t ln = attn_lane();
+        const int row = ln & 31;
+        const int from = (WIDE ? (8 + 2 * (j & 1)) * TILE : 0) + row * 2 * PITCH + ((int)(ln >> 5) ^ attn_swz<DP>(row)) * 16;
+        const bf16x8_t *const up = (const bf16x8_t *)(qup + wv * 32 * DP) + ln;
+        constexpr int N = 2 * KS, AHEAD = 3;
+        auto load = [&](int n) __attribute__((always_inline)) {  // step n / 2 of half n % 2
+          return *(const bf16x8_t *)(lds + (from ^ n / 2 % 8 * 32) + n / 16 * 256 + n % 2 * 32 * 2 * PITCH);
+        };
+        bf16x8_t kf[N], qs = q[0];
+#pragma unroll
+        for (int n = 0; n < AHEAD; ++n) kf[n] = load(n);
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+          if (n + AHEAD < N) kf[n + AHEAD] = load(n + AHEAD);
+          if (n % 2 == 0) qs = n / 2 < KR ? q[n / 2 < KR ? n / 2 : 0] : up[(n / 2 < KR ? 0 : n / 2 - KR) * 64];
+          sv[n % 2] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(kf[n], qs, n < 2 ? z : sv[n % 2], 0, 0, 0);
+          __builtin_amdgcn_sched_barrier(0);
         }
+        asm volatile("" : "+v"(sv[0]), "+v"(sv[1]));  // (as after a product)
       };
       // What the scales of tile j's values do to its weights: of eight keys each (they have one, where pages are multiples of
       // eight), how far it is below the largest of their half, 4 bits each; `far`: the halves where that does not do.
@@ -354,7 +341,7 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         const int k0 = ks + j * C8_KT;
         const uint64_t valid = valid_of(j);
         const bool edge = differ(j) || valid != ~0ull;
-        // (inline assembly reads S^T below: a 16-pass product's results can be read after 19 wait states)
+        // (inline assembly reads S^T below: even a 16-pass product's results can be read after 19 wait states)
         asm volatile("s_nop 15\n\ts_nop 3" : "+v"(sv[0]), "+v"(sv[1]));
         if (edge) {
           const int h4 = (int)attn_lane() >> 5 << 2;
@@ -380,7 +367,6 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
           float top = -__builtin_inff();
 #pragma unroll
           for (int j = 0; j < 32; j += 2) top = c8_max3(top, sv[j >> 4][j & 15], sv[j >> 4][(j & 15) + 1]);
-          asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(top));  // (as below)
           // The reference is the row's first maximum; it follows, and the sums with it, when a score passes it by 2^60.
           if (__any(m == -__builtin_inff() || top * sc > m + 60.f)) {
             const float all = __builtin_ceilf(c8_pair_max(top) * sc);
@@ -436,7 +422,7 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         }
         // (the matrix unit reads its scale operands after the instruction has issued, and the compiler does not know: they
         // stay in their registers until the products are read)
-        asm volatile("" ::"v"(kx[0]), "v"(kx[1]), "v"(sb), "v"(tvv), "v"(top[0]), "v"(top[1]));
+        asm volatile("" ::"v"(sb), "v"(tvv), "v"(top[0]), "v"(top[1]));
         {
           // The reference is the row's first maximum; it follows, and the sums with it, when a score passes it by 2^60.
           const float all = fmaxf(top[0], top[1]);
@@ -541,7 +527,28 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
         }
         if (__any(odd)) *poison = 1;
       };
-      // WIDE: the rows of the values that this wave has moved, as bf16, scales aside (codes are exact there); cleaned as above
+      // The rows that this wave has moved as bf16: keys with their scales, values (WIDE) without (codes are exact there), those
+      // cleaned as above
+      auto wide16 = [&](u32x4_t w, float f, u32x4_t (&o)[2]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+          const bf16x2_t y = k & 1 ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[k >> 1], f, true)
+                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w[k >> 1], f, false);
+          o[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, y);
+        }
+      };
+      auto widen_key = [&](int j, u32x4_t codes, int row, int chunk) __attribute__((always_inline)) {
+        u32x4_t o[2];
+        wide16(codes, __int_as_float(((const int *)(scl + (j & 1) * 512))[row] << 23), o);
+        uint8_t *to = lds + (WIDE ? (8 + 2 * (j & 1)) * TILE : 0) + row * 2 * PITCH;
+        *(u32x4_t *)(to + (chunk ^ attn_swz<DP>(row)) * 16) = o[0];
+        *(u32x4_t *)(to + ((chunk + 1) ^ attn_swz<DP>(row)) * 16) = o[1];
+      };
+      auto widen_keys = [&](int j) __attribute__((always_inline)) {
+        const uint32_t ln = attn_lane();
+#pragma unroll
+        for (int n = 0; n < OPS; ++n) widen_key(j, keys[WIDE ? 0 : n], wv * 8 + n * RPI + (int)(ln / CPR), 2 * (int)(ln % CPR));
+      };
       auto widen = [&](int j) __attribute__((always_inline)) {
         const bool strict = differ(j) || there != 0xFFu;
         bool odd = false;
@@ -549,22 +556,20 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
 #pragma unroll
         for (int n = 0; n < OPS; ++n) {
           if (RPI <= 8 || ln < 8 * CPR) {
-            uint4 x = *(const uint4 *)(lds + (2 + (j & 1)) * TILE + wv * 8 * PITCH + n * 1024 + ln * 16);
+            const int at = wv * 8 * PITCH + n * 1024 + ln * 16;
+            uint4 x = *(const uint4 *)(lds + (2 + (j & 1)) * TILE + at);
             const int own = n * RPI + ln / CPR, row = wv * 8 + own;  // (of the wave's 8, of the tile's)
+            const int chunk = 2 * ((int)(ln % CPR) ^ attn_swz8<DP>(row));
+            u32x4_t o[2];
+            widen_key(j, *(const u32x4_t *)(lds + (j & 1) * TILE + at), row, chunk);
             if (strict) {
               const uint4 y = attn_finite_codes(x);
               const bool in = there >> own & 1;
               odd |= in && (x.x != y.x || x.y != y.y || x.z != y.z || x.w != y.w);
               x = in ? y : attn_zeros();
             }
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            u32x4_t o[2];
-#pragma unroll
-            for (int k = 0; k < 8; ++k) {
-              const bf16x2_t y = k & 1 ? fp8x2_to_bf16x2<true>(w[k >> 1]) : fp8x2_to_bf16x2<false>(w[k >> 1]);
-              o[k >> 2][k & 3] = __builtin_bit_cast(uint32_t, y);
-            }
-            const int c = 2 * ((int)(ln % CPR) ^ attn_swz8<DP>(row)) ^ attn_swz_v<DP>(row);  // (its two chunks stay side by side)
+            wide16(u32x4_t{x.x, x.y, x.z, x.w}, 1.f, o);
+            const int c = chunk ^ attn_swz_v<DP>(row);  // (its two chunks stay side by side)
             u32x4_t *to = (u32x4_t *)(lds + (4 + 2 * (j & 1)) * TILE + row * 2 * PITCH + c * 16);
             to[0] = o[0], to[1] = o[1];
           }
@@ -633,10 +638,13 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
 #pragma unroll 1
       for (int i = 0; i < nt; ++i) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if constexpr (WIDE)
+        if constexpr (WIDE) {
           widen(i);
-        else
+        } else {
+          gp_lds_barrier();  // everyone has done with the last tile's keys (LDS has room for one tile of them)
+          widen_keys(i);
           clean(i);
+        }
         gp_lds_barrier();  // tile i, its valid bits, page ids of tile i + 1; everyone has done with tile i - 1
         if (i + 1 < nt) {
           const int blk = *(const int *)(tab + wv * 64 + ((i + 1) & 1) * 32 + (attn_lane() & 7) * 4);
@@ -654,7 +662,7 @@ __global__ __launch_bounds__(C8_THREADS, DP == 64 ? 4 : 2) void attn_chunk8_kern
           product(i);
       }
       asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-      asm volatile("" ::"v"(sb), "v"(tvv), "v"(kx[0]), "v"(kx[1]));
+      asm volatile("" ::"v"(sb), "v"(tvv));
     }
 
     // Rows out, 64 columns of a wave's 32 rows at a time, through its part of the LDS (16-byte chunks, swizzled by row)

@@ -32,3 +32,14 @@ def test_products_of_all_sizes(kind, D, new):
     q = (q * (1 + 0.1 * torch.rand(new, 4, 1, generator=torch.Generator().manual_seed(new)))).to(torch.bfloat16)
     want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, few=True)
     assert close(attention(c, q, [0, new], [L]), want, bound)
+
+
+@pytest.mark.parametrize("new", [40, 150])
+@pytest.mark.parametrize("D", [16, 64, 96, 128, 208, 256])
+@pytest.mark.parametrize("kind", ["one", "each", "cancel"])
+def test_products_of_all_sizes_for_many_rows(kind, D, new):
+    L = 500
+    c, q = large_channels(L, D, kind, D)
+    q = (q * (1 + 0.1 * torch.rand(new, 4, 1, generator=torch.Generator().manual_seed(new)))).to(torch.bfloat16)
+    want, bound = ref.attend(q.cuda(), c.keys, c.values, [0, new], [L], D ** -0.5, scales=c.scales)
+    assert close(attention(c, q, [0, new], [L]), want, bound)
