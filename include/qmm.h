@@ -390,7 +390,8 @@ int qmm_rope_cache_fp8(qmm_array *q_out, qmm_array k_cache, qmm_array v_cache, q
                        float amplitude, bool interleaved, qmm_array q_norm, qmm_array k_norm, float norm_eps, qmm_stream s);
 
 /* Rows of such a cache read back: k_out[t] = code * 2^(scale - 127) of row slots[t] (int32 [T]; zeros for a slot that is
- * none, as -1), [T, Hkv, D] of `dtype` (bfloat16 or float32, exact but where bfloat16 underflows); v_out likewise.
+ * none, as -1), [T, Hkv, D] of `dtype` (bfloat16 or float32, exact but where bfloat16 underflows or, at scale bytes that
+ * rope_cache_fp8 does not write, a value passes the type's range and becomes infinite); v_out likewise.
  * k_out or v_out may be NULL: that one is not read, and its cache and scales may be null handles. */
 int qmm_cache_read_fp8(qmm_array *k_out, qmm_array *v_out, qmm_array k_cache, qmm_array v_cache, qmm_array k_scales,
                        qmm_array v_scales, qmm_array slots, qmm_dtype dtype, qmm_stream s);

@@ -237,7 +237,6 @@ struct Route {
   size_t bytes;
 };
 
-// ceil(2^(31 + l) / d), l = ceil(log2 d): exact quotients for n < 2^31
 size_t up256(size_t n) { return (n + 255) & ~(size_t)255; }
 
 size_t lay_out(Part &p, const AttnArgs &a, int DP, int g, size_t at) {
@@ -263,8 +262,8 @@ Route route_of(const AttnArgs &a) {
   const bool one = a.R == 1 && (int64_t)a.T * r.g > ROWS_MOST;
   if (!one) {
     r.rows.tr = most <= 16 ? 16 : 32;
-    // (E4M3 pages of up to 128 values: a CU holds three workgroups, with tiles of 4 KB a wave.  Two with 8 KB, and three: 16
-    // heads of 64, 64 requests of 300 keys 23.4 and 20.1 us, 3000 keys 48.9 and 51.2; 32 heads on 8 of 128, one request of 300
+    // (E4M3 pages of up to 128 values: a CU holds three workgroups, with tiles of 4 KB a wave.  Two with 8 KB, and three, when
+    // scores still came from the scaled MFMA (64 requests of 1 to 8192 keys 38.0 us then, 37.0 now): 16 heads of 64, 64 requests of 300 keys 23.4 and 20.1 us, 3000 keys 48.9 and 51.2; 32 heads on 8 of 128, one request of 300
     // keys 12.8 and 11.5, 128 of them 32.7 and 26.5, 64 of 3000 53.3 and 53.8; 12 heads of 96 16 of 3000 28.2 and 24.7)
     r.rows.grid = a.k_scales && r.DP <= 128 ? 3 * cus < AC_MOST ? 3 * cus : AC_MOST : 2 * cus;
     r.rows.min_rows = 0, r.rows.max_rows = few ? INT32_MAX : ROWS_MOST;

@@ -360,8 +360,10 @@ hipError_t launch_rope_fp8(const RopeArgs &a, uint8_t *const (&scales)[ROPE_MAX_
       a.T > 1 << 30 || a.set[0].heads > INT32_MAX / 4 || a.set[1].heads < 1 || a.set[1].heads > 1 << 29 || a.set[1].heads != a.set[2].heads)
     return hipErrorInvalidValue;
   // Pages of more rows than two turns have, and more tokens than decoding requests mostly have together: 1024 threads, q in a
-  // launch of its own.  (2048 tokens, 24 heads on 4 of 256, pages of 64, 128 and 256 rows: with 256 threads 40, 59 and 107 us,
-  // with 1024 27, 34 and 48.  64 requests of 3 tokens, pages of 64: 8.6 and 15.7.)
+  // launch of its own.  What decides is how many rows of a page there are, which only the GPU knows.  (24 heads on 4 of 256, pages
+  // of 64 rows: 2048 tokens of one prompt with 256 threads 35-40 us, with 1024 26; 1024 tokens 24 and 17; 512 17.6 and 13.9; 64 to
+  // 256 16 and 12.  300 decoding requests 8.5 and 16; 600 8.4 and 18; 1000 11.5 and 15.9; 171 of 3 tokens 9.7 and 14.3.  Pages of
+  // 128 and 256: 2048 tokens 51-59 and 26-34, 107 and 48; 512 tokens 32 and 17.6.)
   const int lph = a.D <= 64 ? 2 : a.D <= 128 ? 3 : 4;
   const int threads = a.block > 2 * ROPE_THREADS >> lph && a.T > CW_MANY && a.half % 8 == 0 ? CW_WIDE : ROPE_THREADS, rows = threads >> lph;
   CacheWrite w{};

@@ -191,7 +191,7 @@ struct BlockTableArgs {
 };
 hipError_t launch_block_tables(const BlockTableArgs &a, hipStream_t st);
 
-// n / d for n < 2^31 as the high half of 2 n * mul, shifted.
+// n / d for n < 2^31 as the high half of 2 n * mul, shifted: mul = ceil(2^(31 + l) / d), l = ceil(log2 d), gives exact quotients.
 struct FastDiv {
   uint32_t mul, shift;
 };
