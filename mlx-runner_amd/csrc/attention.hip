@@ -54,10 +54,19 @@ __device__ __forceinline__ Cut cut_of(const AttnArgs &a, const AttnShare &s) {
   return c;
 }
 
-// A part's weight beside the largest of its row, 0 where it has no keys of the row.  At least the smallest f32: whatever the
-// scores, a sum that is not finite reaches the row, as it does within a part; 2^-149 of one that is changes nothing.
+// A part's weight beside the largest of its row: 0 where it has no keys of the row (and no sums), -1 where f32 has no weight
+// for it.
 __device__ __forceinline__ float part_weight(float m, float top) {
-  return m == -__builtin_inff() ? 0.f : fmaxf(attn_exp2(m - top), __uint_as_float(1u));
+  const float f = attn_exp2(m - top);
+  return m == -__builtin_inff() ? 0.f : f == 0.f ? -1.f : f;
+}
+__device__ __forceinline__ void part_add(float4 &o, float f, float4 v) {
+  if (f > 0.f) o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;
+}
+// Of a part without weight, only what is not finite: it reaches the row, whatever the scores, as it does within a part.
+__device__ __forceinline__ void part_add_odd(float4 &o, float f, float4 v) {
+  auto odd = [f](float x) { return f < 0.f && x * 0.f != 0.f ? x : 0.f; };
+  o.x += odd(v.x), o.y += odd(v.y), o.z += odd(v.z), o.w += odd(v.w);
 }
 
 // One workgroup per tile, row and COLS columns.  All that it reads is asked for at once, up to 8 partials a lane; every
@@ -100,10 +109,12 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
     for (int k = 1; k < HELD; ++k) top = fmaxf(top, ml[k].x);
     for (int p = HELD * 64 + lane; p < np; p += 64) top = fmaxf(top, s.ml[place(p) * 2]);
     top = wave_top(top);
+    bool weightless = false;
     auto weigh = [&](int p, float2 v) __attribute__((always_inline)) {
       const float f = part_weight(v.x, top);
       wt[wave][p] = f;
-      sum += f * v.y;
+      weightless |= f < 0.f;
+      sum += fmaxf(f, 0.f) * v.y;
     };
 #pragma unroll
     for (int k = 0; k < HELD; ++k)
@@ -113,15 +124,17 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_kernel(const AttnArgs 
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    auto add = [&](float f, float4 v) __attribute__((always_inline)) {
-      if (f != 0.f) o.x += f * v.x, o.y += f * v.y, o.z += f * v.z, o.w += f * v.w;  // (a part without keys has no sums)
-    };
 #pragma unroll
     for (int i = 0; i < AHEAD; ++i)
-      if (set + i * SETS < np && in) add(wt[wave][set + i * SETS], x[i]);
+      if (set + i * SETS < np && in) part_add(o, wt[wave][set + i * SETS], x[i]);
 #pragma unroll 8
     for (int p = set + AHEAD * SETS; p < np; p += SETS)
-      if (in) add(wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
+      if (in) part_add(o, wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
+    if (__any(weightless)) {
+#pragma unroll 1
+      for (int p = set; p < np; p += SETS)
+        if (in) part_add_odd(o, wt[wave][p], *(const float4 *)(s.acc + place(p) * DP + d0));
+    }
     *(float4 *)&part[set][tid % LPR * 4] = o;
     __syncthreads();
     if (out) {
@@ -144,6 +157,7 @@ template <int DP>
 __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const AttnArgs a, const AttnShare s, int tr) {
   constexpr int LPR = DP / 4, RP = ATTN_THREADS / LPR, TURNS = AJ_ROWS / RP, AHEAD = 2;
   __shared__ float wt[AJ_ROWS][AC_MOST / 2], total[AJ_ROWS];
+  __shared__ int odd[ATTN_THREADS / 64];  // whether a wave's rows have parts without weight
   __shared__ __attribute__((aligned(16))) float part[AJ_ROWS][DP];
   const int tid = threadIdx.x;
   const Cut c = cut_of(a, s);
@@ -164,6 +178,7 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
       if (p < np && row0 + t * RP + r0 < rows && d0 < a.D) x[p][t] = *(const float4 *)(s.acc + place(p, t * RP + r0) * DP + d0);
   {
     float top = ml.x, sum = 0.f;
+    bool weightless = false;
     for (int p = l + 16; p < np && on; p += 16) top = fmaxf(top, s.ml[place(p, row) * 2]);
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) top = fmaxf(top, __shfl_xor(top, off, 16));
@@ -171,25 +186,24 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
       if (p >= 16) ml = *(const float2 *)(s.ml + place(p, row) * 2);
       const float f = part_weight(ml.x, top);
       wt[row][p] = f;
-      sum += f * ml.y;
+      weightless |= f < 0.f;
+      sum += fmaxf(f, 0.f) * ml.y;
     }
 #pragma unroll
     for (int off = 8; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, 16);
     if (l == 0) total[row] = sum;
+    weightless = __any(weightless);
+    if ((tid & 63) == 0) odd[tid >> 6] = weightless;
   }
   __syncthreads();
   float4 o[TURNS];
 #pragma unroll
   for (int t = 0; t < TURNS; ++t) o[t] = make_float4(0.f, 0.f, 0.f, 0.f);
-  auto add = [&](int t, float f, float4 v) __attribute__((always_inline)) {
-    // (a part without keys has no sums)
-    if (f != 0.f) o[t].x += f * v.x, o[t].y += f * v.y, o[t].z += f * v.z, o[t].w += f * v.w;
-  };
 #pragma unroll
   for (int p = 0; p < AHEAD; ++p)
 #pragma unroll
     for (int t = 0; t < TURNS; ++t)
-      if (p < np && row0 + t * RP + r0 < rows && d0 < a.D) add(t, wt[t * RP + r0][p], x[p][t]);
+      if (p < np && row0 + t * RP + r0 < rows && d0 < a.D) part_add(o[t], wt[t * RP + r0][p], x[p][t]);
 #pragma unroll 1
   for (int p = AHEAD; p < np; ++p) {
 #pragma unroll
@@ -197,7 +211,18 @@ __global__ __launch_bounds__(ATTN_THREADS) void attn_join_rows_kernel(const Attn
       if (row0 + t * RP + r0 < rows && d0 < a.D) x[0][t] = *(const float4 *)(s.acc + place(p, t * RP + r0) * DP + d0);
 #pragma unroll
     for (int t = 0; t < TURNS; ++t)
-      if (row0 + t * RP + r0 < rows && d0 < a.D) add(t, wt[t * RP + r0][p], x[0][t]);
+      if (row0 + t * RP + r0 < rows && d0 < a.D) part_add(o[t], wt[t * RP + r0][p], x[0][t]);
+  }
+  int any = 0;
+#pragma unroll
+  for (int w = 0; w < ATTN_THREADS / 64; ++w) any |= odd[w];
+  if (any) {
+#pragma unroll 1
+    for (int p = 0; p < np; ++p)
+#pragma unroll
+      for (int t = 0; t < TURNS; ++t)
+        if (row0 + t * RP + r0 < rows && d0 < a.D)
+          part_add_odd(o[t], wt[t * RP + r0][p], *(const float4 *)(s.acc + place(p, t * RP + r0) * DP + d0));
   }
 #pragma unroll
   for (int t = 0; t < TURNS; ++t) *(float4 *)&part[t * RP + r0][d0] = o[t];

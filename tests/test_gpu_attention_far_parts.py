@@ -49,3 +49,17 @@ def test_values_that_are_not_finite_in_a_part_of_no_weight(D, new):
     fine = torch.ones_like(got, dtype=torch.bool)
     fine[:, :2, 5], fine[:, 2:, 9] = False, False
     assert ((got.double() - want).abs() <= bound)[fine].all()
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [1, 3, 300])
+def test_large_values_in_a_part_of_no_weight(D, new):
+    """Finite values there add nothing, however large: 1e33 beside 1e-11."""
+    c = attention_ref.Cache([L], 2, D, 16, seed=D)
+    c.keys[0][:HALF], c.keys[0][HALF:] = -4, 4
+    c.values[0][:HALF] = 1e33
+    c.values[0][HALF:] *= 1e-11
+    rewrite(c, 0)
+    q = torch.ones(new, 4, D, dtype=torch.bfloat16)
+    want, bound = attention_ref.attend(q, c.keys, c.values, [0, new], [L], 64 / D)
+    assert ((attention(c, q, [0, new], [L], scale=64 / D).double() - want).abs() <= bound).all()
